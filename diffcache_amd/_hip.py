@@ -41,6 +41,7 @@ SYMBOLS = (
     "dc_pq_search_workspace_bytes", "dc_pq_search_bf16", "dc_pq_encode_bf16",
     "dc_data_layer_create", "dc_data_layer_destroy", "dc_data_layer_ctx_len", "dc_data_layer_sizes",
     "dc_data_layer_bind", "dc_data_layer_prefill", "dc_data_layer_insert", "dc_data_layer_query",
+    "dc_mx_ingest_bf16", "dc_mx_append_bf16", "dc_mx_gather_rows_bf16", "dc_mx_attn_workspace_bytes", "dc_mx_attn_bf16",
 )
 
 
@@ -88,6 +89,27 @@ class PrefillArgs(C.Structure):
         ("code_batch_stride", C.c_int64), ("code_head_stride", C.c_int64), ("code_row_stride", C.c_int64),
         ("n_b", C.c_int), ("n_h", C.c_int), ("seq", C.c_int), ("hd", C.c_int),
         ("n_prefix", C.c_int), ("n_suffix", C.c_int),
+    ]
+
+
+class MxStoreArgs(C.Structure):
+    """struct dc_mx_store of include/diffcache_hip.h"""
+    _fields_ = [
+        ("codes", C.c_void_p), ("scale", C.c_void_p),
+        ("code_batch_stride", C.c_int64), ("code_head_stride", C.c_int64), ("code_row_stride", C.c_int64),
+        ("scale_batch_stride", C.c_int64), ("scale_head_stride", C.c_int64), ("scale_row_stride", C.c_int64),
+        ("bits", C.c_int), ("n_rows", C.c_int),
+    ]
+
+
+class MxAttnArgs(C.Structure):
+    """struct dc_mx_attn_args of include/diffcache_hip.h"""
+    _fields_ = [
+        ("q", C.c_void_p), ("new_k", C.c_void_p), ("new_v", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("lens", C.c_void_p), ("k", MxStoreArgs), ("v", MxStoreArgs), ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_size_t),
+        ("n_b", C.c_int), ("n_h", C.c_int), ("group", C.c_int), ("hd", C.c_int), ("n_rows", C.c_int),
+        ("n_sink", C.c_int), ("window", C.c_int), ("scale", C.c_float),
     ]
 
 
@@ -155,6 +177,14 @@ def _load() -> C.CDLL:
         "dc_score_select_sketch_bf16": (i, [p, p, p, p, p, p, i64, i, i, i, i, i64, i64, i64, i64, i64, i64,
                                             i, i, i, i, i, p, sz, p, p, p]),
     }
+    mx = C.POINTER(MxStoreArgs)
+    sigs.update({
+        "dc_mx_ingest_bf16": (i, [mx, mx, p, p, p, i, i, i, i, i, i64, i64, i64, i64, i64, i64, p]),
+        "dc_mx_append_bf16": (i, [mx, mx, p, p, p, i, i, i, p]),
+        "dc_mx_gather_rows_bf16": (i, [mx, mx, p, p, p, i, i, i, i64, i, i64, i64, i64, i64, p]),
+        "dc_mx_attn_workspace_bytes": (sz, [i, i, i, i]),
+        "dc_mx_attn_bf16": (i, [C.POINTER(MxAttnArgs), p]),
+    })
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
         fn.restype = res
@@ -969,3 +999,185 @@ def compose_idx(outer: torch.Tensor, inner: torch.Tensor) -> torch.Tensor:
                               inner.stride(0), _dev(out, "out"), out.stride(0), n_units, n_inner,
                               _stream()))
     return out
+
+
+# ---------------------------------------------------------------------------
+# a cache in blocks of 32 numbers (dc_mx_store)
+# ---------------------------------------------------------------------------
+
+class MxStore:
+    """K or V of a layer, held in 4 or 8 bits with a power of two for every 32 numbers (dc_mx_store in the header):
+    ``codes`` (b, h, n, hd * bits / 8) and ``scale`` (b, h, n, hd / 32), both uint8 with contiguous rows.  Views of larger
+    tensors will do; ``MxStore.zeros`` makes a store of its own, whose rows read as zeros until they are written."""
+
+    def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
+        cs, ss = codes.shape, scale.shape
+        if len(cs) != 4 or len(ss) != 4 or cs[:3] != ss[:3] or codes.dtype != torch.uint8 or scale.dtype != torch.uint8:
+            raise DiffCacheError("codes and scale must be (b, h, n, .) uint8 tensors of the same b, h and n")
+        self.hd = ss[3] * 32
+        if cs[3] not in (self.hd // 2, self.hd) or ss[3] == 0:
+            raise DiffCacheError(f"rows of {cs[3]} code bytes and {ss[3]} scales are neither 4 nor 8 bits to a number")
+        (cb, ch, cr, c1), (sb, sh, sr, s1) = codes.stride(), scale.stride()
+        if c1 != 1 or s1 != 1:
+            raise DiffCacheError("the rows of codes and scale must be contiguous")
+        self.codes, self.scale = codes, scale
+        self.shape = (cs[0], cs[1], cs[2], self.hd)
+        self.bits = 4 if cs[3] * 2 == self.hd else 8
+        self._args = MxStoreArgs(_mx_dev(codes, "codes"), _mx_dev(scale, "scale"), cb, ch, cr, sb, sh, sr, self.bits, cs[2])
+
+    @classmethod
+    def zeros(cls, b: int, h: int, n: int, hd: int, bits: int, device) -> "MxStore":
+        if bits not in (4, 8) or hd not in (64, 128, 256):
+            raise DiffCacheError(f"a store of {bits} bits and head_dim {hd} is not supported (4 or 8; 64, 128 or 256)")
+        return cls(torch.zeros((b, h, n, hd * bits // 8), dtype=torch.uint8, device=device),
+                   torch.zeros((b, h, n, hd // 32), dtype=torch.uint8, device=device))
+
+
+def _mx_dev(t: torch.Tensor, name: str) -> int:
+    """Device pointer of a tensor on the current device, whose stream the call goes to."""
+    if not t.is_cuda:
+        raise DiffCacheError(f"{name} must live in GPU memory (got {t.device}); there is no CPU path")
+    if t.device.index != torch._C._cuda_getDevice():
+        raise DiffCacheError(f"{name} lives on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
+    return t.data_ptr()
+
+
+def _mx_pair(k: MxStore, v: MxStore):
+    if k.shape[:2] != v.shape[:2] or k.hd != v.hd:
+        raise DiffCacheError(f"K store {k.shape} and V store {v.shape} do not belong together")
+    return k.shape[0], k.shape[1], k.hd
+
+
+def _mx_lens(lens: Optional[torch.Tensor], b: int):
+    if lens is None:
+        return None
+    if lens.dtype != torch.int32 or lens.numel() != b or not lens.is_contiguous():
+        raise DiffCacheError(f"lens must be a contiguous int32 tensor of {b} elements")
+    return _mx_dev(lens, "lens")
+
+
+def _mx_src(t: torch.Tensor, shape, name: str) -> torch.Tensor:
+    if t.dtype != torch.bfloat16 or t.shape != shape:
+        raise DiffCacheError(f"{name} must be a {tuple(shape)} bf16 tensor, not {tuple(t.shape)} {t.dtype}")
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(x % 8 for x in t.stride()[:3]):
+        t = t.contiguous()
+    return t
+
+
+def _mx_token(t: torch.Tensor, b: int, h: int, hd: int, name: str) -> torch.Tensor:
+    t = t.contiguous()
+    if t.dtype != torch.bfloat16 or t.numel() != b * h * hd:
+        raise DiffCacheError(f"{name} must hold ({b}, {h}, {hd}) bf16 values")
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def mx_ingest(k: MxStore, v: MxStore, k_src: torch.Tensor, v_src: torch.Tensor, dst_pos: int = 0,
+              lens: Optional[torch.Tensor] = None) -> None:
+    """k_src, v_src (b, seq, h, hd) bf16 into rows [dst_pos, dst_pos + seq) of both stores (dc_mx_ingest_bf16); ``lens``
+    (b) int32 on the device: the first lens[b] tokens of sequence b alone, the rows behind them stay as they are."""
+    b, h, hd = _mx_pair(k, v)
+    if k_src.dim() != 4:
+        raise DiffCacheError("k_src and v_src must be (b, seq, h, hd) bf16 tensors matching the store")
+    seq = k_src.shape[1]
+    k_src, v_src = (_mx_src(t, (b, seq, h, hd), name) for t, name in ((k_src, "k_src"), (v_src, "v_src")))
+    if dst_pos < 0 or dst_pos + seq > min(k.shape[2], v.shape[2]):
+        raise DiffCacheError(f"rows [{dst_pos}, {dst_pos + seq}) outside the store of {min(k.shape[2], v.shape[2])} rows")
+    _check(lib.dc_mx_ingest_bf16(C.byref(k._args), C.byref(v._args), _mx_dev(k_src, "k_src"), _mx_dev(v_src, "v_src"),
+                                 _mx_lens(lens, b), b, seq, h, hd, dst_pos, *k_src.stride()[:3], *v_src.stride()[:3],
+                                 _stream()))
+
+
+def mx_append(k: MxStore, v: MxStore, new_k: torch.Tensor, new_v: torch.Tensor, lens: torch.Tensor) -> None:
+    """One token's (b, h, hd) rows into row lens[b] of every sequence (dc_mx_append_bf16); ``lens`` (b) int32 on the device
+    is not changed, and a row that the stores do not have is not written."""
+    b, h, hd = _mx_pair(k, v)
+    new_k, new_v = _mx_token(new_k, b, h, hd, "new_k"), _mx_token(new_v, b, h, hd, "new_v")
+    _check(lib.dc_mx_append_bf16(C.byref(k._args), C.byref(v._args), _mx_dev(new_k, "new_k"), _mx_dev(new_v, "new_v"),
+                                 _mx_lens(lens, b), b, h, hd, _stream()))
+
+
+def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[torch.Tensor] = None,
+                   out_k: Optional[torch.Tensor] = None, out_v: Optional[torch.Tensor] = None, row_offset: int = 0,
+                   n_idx: Optional[int] = None) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """out[b, h, j, :] = the bf16 numbers of row row_offset + idx[b*H + h, j] for j < n_idx, or of row row_offset + j without
+    ``idx`` (n_idx: up to the store's end).  ``idx`` 32-bit (b*h, >= n_idx); a row that the store does not have reads as
+    zeros.  ``out_k`` / ``out_v`` (b, h, >= n_idx, hd) bf16 are made where they are not given; K or V may be None."""
+    ref = k if k is not None else v
+    if ref is None:
+        raise DiffCacheError("neither K nor V given")
+    b, h, hd = _mx_pair(k, v) if k is not None and v is not None else (ref.shape[0], ref.shape[1], ref.hd)
+    if n_idx is None:
+        n_idx = max(ref.shape[2] - row_offset, 0) if idx is None else idx.shape[1]
+    if n_idx < 0 or row_offset < 0:
+        raise DiffCacheError("n_idx and row_offset must not be negative")
+    if idx is not None:
+        require(idx.dim() == 2 and idx.shape[0] == b * h and idx.shape[1] >= n_idx and idx.element_size() == 4
+                and not idx.is_floating_point() and (idx.shape[1] <= 1 or idx.stride(1) == 1),
+                "idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor with contiguous rows")
+        if idx.stride(0) < n_idx:
+            idx = idx.contiguous()
+    outs = []
+    for s, o, name in ((k, out_k, "out_k"), (v, out_v, "out_v")):
+        if s is not None and o is None:
+            o = torch.empty((b, h, n_idx, hd), dtype=torch.bfloat16, device=s.codes.device)
+        elif o is not None:
+            _store_strides(o)
+            ob, oh, on, od = o.shape
+            require(s is not None and ob == b and oh == h and on >= n_idx and od == hd,
+                    "out_k / out_v must be (bsz, kv_heads, >= n_idx, head_dim), each with its store")
+        outs.append(o)
+    strides = [_store_strides(o) for o in outs if o is not None]
+    if strides[0] != strides[-1]:
+        raise DiffCacheError("out_k and out_v must share their strides")
+    _check(lib.dc_mx_gather_rows_bf16(
+        None if k is None else C.byref(k._args), None if v is None else C.byref(v._args),
+        None if idx is None else _mx_dev(idx, "idx"), *(None if o is None else _mx_dev(o, "out") for o in outs),
+        b, h, n_idx, 0 if idx is None else max(idx.stride(0), n_idx), hd, row_offset, *strides[0], _stream()))
+    return outs[0], outs[1]
+
+
+def mx_attn_workspace_bytes(n_units: int, group: int, hd: int, n_rows: int) -> int:
+    return int(lib.dc_mx_attn_workspace_bytes(n_units, group, hd, n_rows))
+
+
+def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor] = None, n_rows: Optional[int] = None,
+            n_sink: int = 0, window: int = 0, new_k: Optional[torch.Tensor] = None,
+            new_v: Optional[torch.Tensor] = None, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+            lse: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None, want_lse: bool = False):
+    """One token's attention over the cache (dc_mx_attn_bf16): q (b, h*group, hd) bf16 -> out of the same shape, over the
+    first lens[b] rows of every sequence (``lens`` (b) int32 on the device; None: n_rows).  ``n_rows``: the most rows any
+    sequence holds, which sizes the launch (default: the store's).  ``new_k`` / ``new_v`` (b, h, hd): the token's own row, written
+    to row lens[b] and attended to as it is held; lens is not changed.  ``window`` > 0: only the first ``n_sink`` rows and the
+    last ``window``.  With ``lse`` or ``want_lse`` returns (out, lse), lse (b, h*group) fp32 the log of the sum of exponentials."""
+    b, h, hd = _mx_pair(k, v)
+    q = q.contiguous()
+    group = q.numel() // (b * h * hd) if b * h else 1
+    if q.dtype != torch.bfloat16 or q.numel() != b * h * group * hd or (group < 1 and b):
+        raise DiffCacheError("q must be bf16 with (b, h * group, hd) values")
+    if q.data_ptr() % 16:
+        q = q.clone()
+    room = min(k.shape[2], v.shape[2])
+    n_rows = room if n_rows is None else n_rows
+    if not 0 <= n_rows <= room:
+        raise DiffCacheError(f"{n_rows} rows outside the store of {room}")
+    if out is None:
+        out = torch.empty((b, h * group, hd), dtype=torch.bfloat16, device=q.device)
+    elif out.dtype != torch.bfloat16 or out.numel() != q.numel() or not out.is_contiguous():
+        raise DiffCacheError("out must be a contiguous bf16 tensor of the size of q")
+    if lse is None and want_lse:
+        lse = torch.empty((b, h * group), dtype=torch.float32, device=q.device)
+    elif lse is not None and (lse.dtype != torch.float32 or lse.numel() != b * h * group or not lse.is_contiguous()):
+        raise DiffCacheError("lse must be a contiguous fp32 tensor of (b, h * group) elements")
+    if (new_k is None) != (new_v is None):
+        raise DiffCacheError("new_k and new_v must be given together")
+    if new_k is not None:
+        new_k, new_v = _mx_token(new_k, b, h, hd, "new_k"), _mx_token(new_v, b, h, hd, "new_v")
+    if workspace is None:
+        workspace = torch.empty((mx_attn_workspace_bytes(b * h, group, hd, n_rows),), dtype=torch.uint8, device=q.device)
+    a = MxAttnArgs(_mx_dev(q, "q"), None if new_k is None else _mx_dev(new_k, "new_k"),
+                   None if new_v is None else _mx_dev(new_v, "new_v"), _mx_dev(out, "out"),
+                   None if lse is None else _mx_dev(lse, "lse"), _mx_lens(lens, b), k._args, v._args,
+                   _mx_dev(workspace, "workspace"), workspace.numel() * workspace.element_size(), b, h, group, hd, n_rows, n_sink, window,
+                   1.0 / math.sqrt(hd) if scale is None else scale)
+    _check(lib.dc_mx_attn_bf16(C.byref(a), _stream()))
+    return out if lse is None else (out, lse)

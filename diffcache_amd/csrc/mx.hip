@@ -1,0 +1,880 @@
+// A cache held in blocks of 32 numbers: 4-bit (E2M1) or 8-bit (E4M3) codes and one power of two for a block.
+// Writing it (prompts, tokens), reading rows back, and one token's attention over what it holds.
+//
+// A block of numbers x_0 .. x_31 is held as round(x_i / 2^e), rounded to the nearest number of the format, ties to the
+// even code, and the byte e + 127.  e is the least exponent at which the largest |x_i| does not round past the last
+// number of the format (6 in 4 bits, 448 in 8): |x_i - held| <= 2^e in 4 bits, 16 2^e in 8, wherever e is not at its
+// limits.  The limits keep every number that is held a normal bf16 number or zero, so reading back into bf16 is exact.  A
+// block with an infinity or a NaN in it is held as NaN (byte 255).
+//
+// Columns 2 i and 2 i + 1 of a 4-bit row are the low and the high half of byte i.
+#include "dc_common.h"
+#include <math.h>
+#include <type_traits>
+#include <utility>
+
+namespace {
+
+typedef __bf16 mx_bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 mx_bf16x8 __attribute__((ext_vector_type(8)));
+typedef short mx_s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short mx_u16x2 __attribute__((ext_vector_type(2)));
+typedef float mx_f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t mx_u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t mx_u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+
+// A store as the kernels see it; strides in bytes.
+struct View {
+    uint8_t *codes, *scale;
+    int64_t cb, ch, cr, sb, sh, sr;
+};
+inline View view_of(const dc_mx_store &s) {
+    return {(uint8_t *)s.codes,   (uint8_t *)s.scale,   s.code_batch_stride, s.code_head_stride,
+            s.code_row_stride, s.scale_batch_stride, s.scale_head_stride, s.scale_row_stride};
+}
+
+// ---- the format -----------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t mx_bits(mx_bf16x2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// 2^(byte - 127) as the conversions want it: they read the exponent of a float.  Byte 255 gives an infinity, at which
+// they return NaN, and byte 0 zero, at which the codes 0 of a row that is not there give 0.
+__device__ __forceinline__ float mx_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// numbers 2 PAIR and 2 PAIR + 1 of the words w, as two bf16 numbers
+template <int BITS, int PAIR>
+__device__ __forceinline__ uint32_t mx_pair(const uint32_t *w, float scale) {
+    if constexpr (BITS == 4)
+        return mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[PAIR / 4], scale, PAIR % 4));
+    else
+        return mx_bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[PAIR / 2], scale, PAIR % 2 != 0));
+}
+
+template <int BITS>
+struct Coded {
+    uint32_t w[BITS / 4];  // the codes of 8 numbers
+    uint32_t scale;        // the block's byte
+};
+
+// Eight numbers of a block whose others are with the three lanes of the same quad.  On the bits of bf16 numbers, whose
+// magnitudes are ordered as whole numbers.
+template <int BITS>
+__device__ __forceinline__ Coded<BITS> mx_quantise(const uint4 &x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    mx_u16x2 top = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(mx_u16x2, w[i] & 0x7fff7fffu));
+    uint32_t most = top.x > top.y ? top.x : top.y;
+    auto other = [](uint32_t v, auto ctrl) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true);
+    };
+    const uint32_t a = other(most, std::integral_constant<int, 0xB1>{});  // quad_perm [1,0,3,2]
+    most = most > a ? most : a;
+    const uint32_t b = other(most, std::integral_constant<int, 0x4E>{});  // quad_perm [2,3,0,1]
+    most = most > b ? most : b;
+    // the exponent, one more where the fraction would round past the last code: from 7 / 4 on in 4 bits (that tie goes
+    // to the even code, beyond the last), above 29 / 16 in 8 (that one goes down)
+    constexpr int kBump = BITS == 4 ? 0x20 : 0x17, kTop = BITS == 4 ? 2 : 8;
+    constexpr int kLo = BITS == 4 ? 2 : 10, kHi = BITS == 4 ? 252 : 246;
+    int e = (int)((most + kBump) >> 7) - kTop;
+    e = e < kLo ? kLo : (e > kHi ? kHi : e);
+    const bool fine = most < 0x7f80u;
+    const float s = mx_scale((uint32_t)e);
+    Coded<BITS> c;
+    c.scale = fine ? (uint32_t)e : 255u;
+    if constexpr (BITS == 4) {  // (beyond the last code the conversion gives the last one)
+        uint32_t r = 0;
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_bf16x2, w[0]), s, 0);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_bf16x2, w[1]), s, 1);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_bf16x2, w[2]), s, 2);
+        r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(mx_bf16x2, w[3]), s, 3);
+        c.w[0] = fine ? r : 0u;
+    } else {  // (here it gives NaN: numbers beyond 448 2^119, which only the largest scale leaves, are brought back first)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mx_s16x2 r = {0, 0};
+            auto held = [](uint32_t v) {
+                const mx_u16x2 mag = __builtin_elementwise_min(__builtin_bit_cast(mx_u16x2, v & 0x7fff7fffu), mx_u16x2{0x7f60, 0x7f60});
+                return __builtin_bit_cast(mx_bf16x2, __builtin_bit_cast(uint32_t, mag) | (v & 0x80008000u));
+            };
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, held(w[2 * i]), s, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, held(w[2 * i + 1]), s, true);
+            c.w[i] = fine ? __builtin_bit_cast(uint32_t, r) : 0u;
+        }
+    }
+    return c;
+}
+
+// piece p (8 columns) of a row; the scale by the lane with the first piece of a block
+template <int BITS>
+__device__ __forceinline__ void mx_store_piece(uint8_t *codes, uint8_t *scale, int p, const Coded<BITS> &c) {
+    if constexpr (BITS == 4)
+        *reinterpret_cast<uint32_t *>(codes + p * 4) = c.w[0];
+    else
+        *reinterpret_cast<uint2 *>(codes + p * 8) = make_uint2(c.w[0], c.w[1]);
+    if (p % 4 == 0) scale[p / 4] = (uint8_t)c.scale;
+}
+
+// ---- writing --------------------------------------------------------------------------------------------------------
+
+struct IngestArgs {
+    View k, v;
+    const uint16_t *src_k, *src_v;
+    int64_t ksb, kss, ksh, vsb, vss, vsh;  // element strides of the sources: batch, token, head
+    const int32_t *lens;
+    int n_h, seq, dst_pos, chunks;         // chunks: blocks of a unit
+};
+
+constexpr int kIngestBatch = 4;  // pieces of 8 columns a thread takes
+
+// Rows of a prompt.  A thread takes 8 columns (16 bytes), a quad a block of 32, so a wave's piece is 512 / hd whole rows of
+// one unit: it reads segments of 2 hd bytes and writes one contiguous run.
+template <int BITS>
+__device__ __forceinline__ void mx_ingest_rows(const View &st, const uint16_t *src, int64_t ss, const IngestArgs &a, int hd,
+                                               int b, int h, int chunk, int live) {
+    const int ppr = hd / 8, rows_per = kThreads / ppr;  // pieces of a row, rows a block takes at once
+    const int p = threadIdx.x % ppr, r0 = chunk * rows_per * kIngestBatch + threadIdx.x / ppr;
+    uint4 x[kIngestBatch];
+#pragma unroll
+    for (int i = 0; i < kIngestBatch; ++i) {
+        const int r = r0 + i * rows_per;
+        x[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < live) x[i] = dc_load_stream16(src + (int64_t)r * ss + p * 8);
+    }
+    uint8_t *codes = st.codes + b * st.cb + h * st.ch, *scale = st.scale + b * st.sb + h * st.sh;
+#pragma unroll
+    for (int i = 0; i < kIngestBatch; ++i) {
+        const int r = r0 + i * rows_per;
+        const Coded<BITS> c = mx_quantise<BITS>(x[i]);  // (the four lanes of a quad hold one row's: all or none store)
+        const int64_t at = (int64_t)a.dst_pos + r;
+        if (r < live) mx_store_piece<BITS>(codes + at * st.cr, scale + at * st.sr, p, c);
+    }
+}
+
+template <int KB, int VB>
+__global__ __launch_bounds__(kThreads) void mx_ingest_kernel(IngestArgs a, int hd) {
+    const int unit = (int)(blockIdx.x / (unsigned)a.chunks), chunk = (int)(blockIdx.x % (unsigned)a.chunks);
+    const int b = unit / a.n_h, h = unit % a.n_h;
+    int live = a.seq;
+    if (a.lens) {
+        const int n = dc_step_word(a.lens + b);
+        live = n < live ? n : live;
+    }
+    if (blockIdx.y == 0)
+        mx_ingest_rows<KB>(a.k, a.src_k + b * a.ksb + h * a.ksh, a.kss, a, hd, b, h, chunk, live);
+    else
+        mx_ingest_rows<VB>(a.v, a.src_v + b * a.vsb + h * a.vsh, a.vss, a, hd, b, h, chunk, live);
+}
+
+// A token's row of one unit, by hd / 4 lanes: the first half of them K's pieces, the second V's.
+template <int KB, int VB>
+__device__ __forceinline__ void mx_write_token(const View &k, const View &v, const uint16_t *new_k, const uint16_t *new_v, int hd,
+                                               int unit, int b, int h, int64_t at, int lane) {
+    const int ppr = hd / 8;
+    if (lane < ppr) {
+        const Coded<KB> c = mx_quantise<KB>(*reinterpret_cast<const uint4 *>(new_k + (int64_t)unit * hd + lane * 8));
+        mx_store_piece<KB>(k.codes + b * k.cb + h * k.ch + at * k.cr, k.scale + b * k.sb + h * k.sh + at * k.sr, lane, c);
+    } else if (lane < 2 * ppr) {
+        const int p = lane - ppr;
+        const Coded<VB> c = mx_quantise<VB>(*reinterpret_cast<const uint4 *>(new_v + (int64_t)unit * hd + p * 8));
+        mx_store_piece<VB>(v.codes + b * v.cb + h * v.ch + at * v.cr, v.scale + b * v.sb + h * v.sh + at * v.sr, p, c);
+    }
+}
+
+template <int KB, int VB>
+__global__ __launch_bounds__(kThreads) void mx_append_kernel(View k, View v, const uint16_t *new_k, const uint16_t *new_v,
+                                                             const int32_t *lens, int n_units, int n_h, int hd, int cap) {
+    const int unit = (int)blockIdx.x * kWaves + (int)(threadIdx.x >> 6);
+    if (unit >= n_units) return;
+    const int b = unit / n_h, at = lens[b];
+    if (at < 0 || at >= cap) return;
+    mx_write_token<KB, VB>(k, v, new_k, new_v, hd, unit, b, unit % n_h, at, threadIdx.x & 63);
+}
+
+// ---- reading back ---------------------------------------------------------------------------------------------------
+
+struct GatherArgs {
+    View k, v;
+    const uint32_t *idx;
+    int64_t idx_stride, row_offset;
+    uint16_t *out_k, *out_v;
+    int64_t db, dh, dr;  // element strides of the outputs
+    int n_h, n_idx, k_rows, v_rows, chunks;
+};
+
+constexpr int kGatherBatch = 4;
+
+template <int BITS>
+__device__ __forceinline__ void mx_gather(const View &st, uint16_t *out, int n_rows, const GatherArgs &a, int hd, int unit, int chunk) {
+    const int ppr = hd / 8, rows_per = kThreads / ppr, b = unit / a.n_h, h = unit % a.n_h;
+    const int p = threadIdx.x % ppr, j0 = chunk * rows_per * kGatherBatch + threadIdx.x / ppr;
+    const uint8_t *codes = st.codes + b * st.cb + h * st.ch, *scale = st.scale + b * st.sb + h * st.sh;
+    int64_t row[kGatherBatch];
+#pragma unroll
+    for (int i = 0; i < kGatherBatch; ++i) {
+        const int j = j0 + i * rows_per;
+        row[i] = -1;
+        if (j < a.n_idx) row[i] = a.row_offset + (a.idx ? (int64_t)a.idx[(int64_t)unit * a.idx_stride + j] : (int64_t)j);
+        if (row[i] >= n_rows) row[i] = -1;  // (a row that the store does not have reads as zeros)
+    }
+    uint32_t w[kGatherBatch][BITS / 4], s[kGatherBatch];
+#pragma unroll
+    for (int i = 0; i < kGatherBatch; ++i) {
+        s[i] = 0u;
+#pragma unroll
+        for (int t = 0; t < BITS / 4; ++t) w[i][t] = 0u;
+        if (row[i] >= 0) {
+            const uint8_t *src = codes + row[i] * st.cr + p * BITS;
+            if constexpr (BITS == 4) {
+                w[i][0] = *reinterpret_cast<const uint32_t *>(src);
+            } else {
+                const uint2 t = *reinterpret_cast<const uint2 *>(src);
+                w[i][0] = t.x, w[i][1] = t.y;
+            }
+            s[i] = scale[row[i] * st.sr + p / 4];
+        }
+    }
+    uint16_t *dst = out + b * a.db + h * a.dh + p * 8;
+#pragma unroll
+    for (int i = 0; i < kGatherBatch; ++i) {
+        const int j = j0 + i * rows_per;
+        const float f = mx_scale(s[i]);
+        const uint4 x = make_uint4(mx_pair<BITS, 0>(w[i], f), mx_pair<BITS, 1>(w[i], f), mx_pair<BITS, 2>(w[i], f), mx_pair<BITS, 3>(w[i], f));
+        if (j < a.n_idx) dc_store_stream16(dst + (int64_t)j * a.dr, x);
+    }
+}
+
+template <int KB, int VB>
+__global__ __launch_bounds__(kThreads) void mx_gather_kernel(GatherArgs a, int hd, int first) {
+    const int unit = (int)(blockIdx.x / (unsigned)a.chunks), chunk = (int)(blockIdx.x % (unsigned)a.chunks);
+    if ((int)blockIdx.y + first == 0)
+        mx_gather<KB>(a.k, a.out_k, a.k_rows, a, hd, unit, chunk);
+    else
+        mx_gather<VB>(a.v, a.out_v, a.v_rows, a, hd, unit, chunk);
+}
+
+// ---- attention ------------------------------------------------------------------------------------------------------
+//
+// One token's attention, out = sum_r p_r v_r / sum_r p_r with p_r = exp(scale q k_r - m), over the rows of every sequence
+// (all of them, or its first n_sink and its last window).  A unit's rows are cut into steps of 16 TILES rows and its steps
+// into n_splits equal parts, a block each, whose waves take every fourth step; a wave keeps its running maximum, sum and
+// weighted rows in registers, so the codes are read once and nothing is written but the parts' results.
+//
+//   S = K Q^T   v_mfma_f32_16x16x32_bf16 over 16 rows (M), 16 query heads (N) and 32 columns.  Lane (q, c) = (lane / 16,
+//               lane % 16) has the columns hd / 4 q .. of one row in one load, and the codes become bf16 numbers, their scale
+//               included, exactly; instruction j takes its columns 8 j .. + 7.  (The instructions that multiply 4-bit and
+//               8-bit numbers as they are round their sums at some 2^-15 of the largest product: measured, not enough.)
+//   softmax     The heads of a group of up to GP stand in the columns again and again, and lane c keeps the result of tile
+//               c / GP only: 64 rows of 4 heads are then 4 numbers a lane, none of them idle.  The maximum moves
+//               only where a logit passes it by more than 2^8: rare, so nothing crosses lanes from step to step.
+//   O = P V     M = (tile, head) as the lanes have them, N = 16 of the hd columns, K = 32 rows of two tiles; P of the tiles that are not
+//               a lane's is zero.  P is the sum of two bf16 numbers (2^-17 of it is lost: with the fp32 sums the output is
+//               that of an fp32 P to far below its own rounding).  Column n of instruction j is hd / 16 n + j, so that a lane loads
+//               adjacent codes of its own rows.
+//
+// Which row of a tile is which row of M is free as long as K and V agree: M row 4 q + i is the tile's row 4 i + q, so that
+// every load takes whole runs of rows.  Rows behind the end are not asked for: a step's buffers end at its last row, and loads
+// past a buffer's end give zeros.
+struct AttnArgs {
+    const uint16_t *q, *new_k, *new_v;
+    uint16_t *out;
+    float *lse, *ws_acc, *ws_ml;
+    const int32_t *lens;
+    View k, v;
+    int n_h, group, cap, n_sink, window, n_splits;
+    float scale;  // times log2(e)
+};
+
+// What a unit's lengths come to.
+struct Plan {
+    int len, rows;            // rows before the token, and with it
+    int sink, lo;             // rows [0, sink) and [lo, rows) are attended
+    int sink_steps, steps, per, used;
+};
+template <int STEP>
+__device__ __forceinline__ Plan mx_plan(const AttnArgs &a, int b) {
+    Plan p;
+    const int has_new = a.new_k != nullptr;
+    int len = a.lens ? dc_step_word(a.lens + b) : a.cap - has_new;
+    len = len < 0 ? 0 : (len < a.cap ? len : a.cap);
+    p.len = len;
+    p.rows = len + (has_new && len < a.cap ? 1 : 0);
+    p.sink = 0, p.lo = 0;
+    if (a.window > 0 && (int64_t)a.n_sink + a.window < p.rows) p.sink = a.n_sink, p.lo = p.rows - a.window;
+    p.sink_steps = (p.sink + STEP - 1) / STEP;
+    p.steps = p.sink_steps + (int)(((int64_t)p.rows - p.lo + STEP - 1) / STEP);
+    p.per = (p.steps + a.n_splits - 1) / a.n_splits;
+    p.per = p.per < kWaves ? kWaves : p.per;
+    p.used = (p.steps + p.per - 1) / p.per;
+    return p;
+}
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const uint8_t *base, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, (int)bytes, 0x00020000);
+}
+
+// BYTES adjacent bytes at offset off
+template <int BYTES>
+__device__ __forceinline__ void mx_load(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t *dst) {
+    if constexpr (BYTES == 1) {
+        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, 0);
+    } else if constexpr (BYTES == 2) {
+        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, 0);
+    } else if constexpr (BYTES == 4) {
+        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
+    } else if constexpr (BYTES == 8) {
+        const mx_u32x2 t = __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+        dst[0] = t.x, dst[1] = t.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+            const mx_u32x4 t = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 16 * i), 0, 0));
+            dst[4 * i] = t.x, dst[4 * i + 1] = t.y, dst[4 * i + 2] = t.z, dst[4 * i + 3] = t.w;
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t mx_pack_bf16(float lo, float hi) { return mx_bits(mx_bf16x2{(__bf16)lo, (__bf16)hi}); }
+
+template <int HD, int KB, int VB, int GP, int TILES>
+struct Attn {
+    static constexpr int STEP = 16 * TILES;
+    static constexpr int CH = HD / 32;          // products of a tile's S; blocks of a row
+    static constexpr int EPL = HD / 16;         // columns of V of a lane
+    static constexpr int KBYTES = HD / 4 * KB / 8, KW = KBYTES / 4;
+    static constexpr int VBYTES = EPL * VB / 8, VW = VBYTES < 4 ? 1 : VBYTES / 4;
+    static constexpr int SETS = 16 / GP < TILES ? 16 / GP : TILES;  // tiles whose logits share a register
+    static constexpr int REGS = TILES / SETS;   // logit registers of a lane (times 4)
+    static constexpr int KS = HD == 256 ? 2 : 1;  // blocks of a lane's columns of K
+
+    mx_u32x4 bq[CH];
+    uint32_t kw[TILES][KW], ks[TILES];
+    uint32_t vw[TILES * 4][VW], vs[TILES * 4];
+    mx_f32x4 acc[EPL];
+    float m, l;
+    int q, c;
+
+    __device__ __forceinline__ void start(const AttnArgs &a, int unit, int lane) {
+        q = lane >> 4, c = lane & 15;
+        const int head = c % GP;
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+            bq[j] = mx_u32x4{0u, 0u, 0u, 0u};
+            if (head < a.group)
+                bq[j] = *reinterpret_cast<const mx_u32x4 *>(a.q + ((int64_t)unit * a.group + head) * HD + q * (HD / 4) + j * 8);
+        }
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY, l = 0.f;
+    }
+
+    // codes and scales of the rows [row, row + live) of a unit, live <= STEP
+    __device__ __forceinline__ void load_k(const View &k, const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
+        const uint32_t cr = (uint32_t)k.cr, sr = (uint32_t)k.sr;
+        const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * k.cr, (uint32_t)live * cr), rs = mx_rsrc(scale + row * k.sr, (uint32_t)live * sr);
+        const uint32_t r = 4u * (c & 3) + (c >> 2);
+        const uint32_t oc = r * cr + (uint32_t)q * KBYTES, os = r * sr + (uint32_t)(q * HD / 4 / 32);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            mx_load<KBYTES>(rc, oc + 16u * t * cr, kw[t]);
+            mx_load<KS>(rs, os + 16u * t * sr, &ks[t]);
+        }
+    }
+    __device__ __forceinline__ void load_v(const View &v, const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
+        const uint32_t cr = (uint32_t)v.cr, sr = (uint32_t)v.sr;
+        const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * v.cr, (uint32_t)live * cr), rs = mx_rsrc(scale + row * v.sr, (uint32_t)live * sr);
+        const uint32_t oc = (uint32_t)q * cr + (uint32_t)c * VBYTES, os = (uint32_t)q * sr + (uint32_t)(c * EPL / 32);
+#pragma unroll
+        for (int t = 0; t < TILES * 4; ++t) {
+            mx_load<VBYTES>(rc, oc + 4u * t * cr, vw[t]);
+            mx_load<1>(rs, os + 4u * t * sr, &vs[t]);
+        }
+    }
+
+    template <int T>
+    __device__ __forceinline__ mx_f32x4 logits_of() const {
+        mx_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        auto chunk = [&](auto jj) __attribute__((always_inline)) {
+            constexpr int J = decltype(jj)::value;
+            const float f = mx_scale(KS == 1 ? ks[T] : (J < CH / 2 ? ks[T] & 0xffu : ks[T] >> 8));
+            const mx_u32x4 x = {mx_pair<KB, 4 * J>(kw[T], f), mx_pair<KB, 4 * J + 1>(kw[T], f), mx_pair<KB, 4 * J + 2>(kw[T], f),
+                                mx_pair<KB, 4 * J + 3>(kw[T], f)};
+            s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, x), __builtin_bit_cast(mx_bf16x8, bq[J]), s, 0, 0, 0);
+        };
+        each<CH>(chunk);
+        return s;
+    }
+
+    template <int N, typename F>
+    static __device__ __forceinline__ void each(F f) {
+        each_of(f, std::make_integer_sequence<int, N>{});
+    }
+    template <typename F, int... I>
+    static __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+        (f(std::integral_constant<int, I>{}), ...);
+    }
+
+    // the logits of the step that load_k brought, by lane and register: x[r][i] = tile r SETS + c / GP, row 4 i + q, head c % GP
+    __device__ __forceinline__ void logits(float scale, float (&x)[REGS][4]) const {
+        const int set = c / GP;
+        each<TILES>([&](auto tt) __attribute__((always_inline)) {
+            constexpr int T = decltype(tt)::value;
+            const mx_f32x4 s = logits_of<T>();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float y = s[i] * scale;
+                if constexpr (T % SETS == 0)
+                    x[T / SETS][i] = y;
+                else
+                    x[T / SETS][i] = set >= T % SETS ? y : x[T / SETS][i];
+            }
+        });
+    }
+
+    // a new maximum for every head, and what was summed so far brought to it
+    __device__ __forceinline__ void raise(float most) {
+#pragma unroll
+        for (int d = GP; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
+        const float to = fmaxf(m, most);
+        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float g = __shfl(f, 4 * q + i, 64);
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) acc[j][i] *= g;
+        }
+    }
+
+    // weights of the step: p from x; live < STEP where rows are missing
+    __device__ __forceinline__ void weigh(float (&x)[REGS][4], int live) {
+        if (live < STEP) {
+#pragma unroll
+            for (int r = 0; r < REGS; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if ((r * SETS + c / GP) * 16 + 4 * i + q >= live) x[r][i] = -INFINITY;
+        }
+        float most = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, x[r][i]);
+        if (__any(most > m + 8.f)) raise(most);
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[r][i] = __builtin_amdgcn_exp2f(x[r][i] - m);
+        if (live < STEP) {
+#pragma unroll
+            for (int r = 0; r < REGS; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if ((r * SETS + c / GP) * 16 + 4 * i + q >= live) x[r][i] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l += x[r][i];
+    }
+
+    // acc += P V over the step that load_v brought
+    __device__ __forceinline__ void add(const float (&x)[REGS][4]) {
+        uint32_t hi[REGS][2], lo[REGS][2];
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                hi[r][i] = mx_pack_bf16(x[r][2 * i], x[r][2 * i + 1]);
+                lo[r][i] = mx_pack_bf16(x[r][2 * i] - dc_bf16_lo(hi[r][i]), x[r][2 * i + 1] - dc_bf16_hi(hi[r][i]));
+            }
+        const int set = c / GP;
+        each<TILES / 2>([&](auto uu) __attribute__((always_inline)) {
+            constexpr int U = decltype(uu)::value, T0 = 2 * U, T1 = 2 * U + 1;
+            auto of = [&](const uint32_t(&w)[REGS][2], int tile, int i) __attribute__((always_inline)) {
+                return set == tile % SETS ? w[tile / SETS][i] : 0u;
+            };
+            const mx_u32x4 ah = {of(hi, T0, 0), of(hi, T0, 1), of(hi, T1, 0), of(hi, T1, 1)};
+            const mx_u32x4 al = {of(lo, T0, 0), of(lo, T0, 1), of(lo, T1, 0), of(lo, T1, 1)};
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) f[i] = mx_scale(vs[8 * U + i]);
+            each<EPL / 2>([&](auto jj) __attribute__((always_inline)) {
+                constexpr int J = decltype(jj)::value;
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = mx_pair<VB, J>(vw[8 * U + i], f[i]);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t sel = half ? 0x07060302u : 0x05040100u;  // the high or the low halves of two words
+                    const mx_u32x4 b = {__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
+                                        __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel)};
+                    mx_f32x4 &o = acc[2 * J + half];
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, al), __builtin_bit_cast(mx_bf16x8, b), o, 0, 0, 0);
+                    o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, ah), __builtin_bit_cast(mx_bf16x8, b), o, 0, 0, 0);
+                }
+            });
+        });
+    }
+};
+
+inline size_t attn_shared_bytes(int hd, int group) { return (size_t)(2 * kWaves * 16 + kWaves * group * hd) * sizeof(float); }
+
+template <int HD, int KB, int VB, int GP, int TILES>
+__global__ __launch_bounds__(kThreads, 2) void mx_attn_kernel(AttnArgs a) {
+    using T = Attn<HD, KB, VB, GP, TILES>;
+    constexpr int STEP = T::STEP;
+    extern __shared__ float s_dyn[];
+    float *s_m = s_dyn, *s_l = s_dyn + kWaves * 16, *s_acc = s_dyn + 2 * kWaves * 16;  // [wave][16], [wave][16], [wave][group * HD]
+    const int unit = blockIdx.x, split = dc_chunk(), tid = threadIdx.x, lane = tid & 63;
+    if (split >= a.n_splits) return;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int b = unit / a.n_h, h = unit % a.n_h, G = a.group;
+    const Plan p = mx_plan<STEP>(a, b);
+    const int begin = split * p.per, end = begin + p.per < p.steps ? begin + p.per : p.steps;
+    if (begin >= end && a.n_splits > 1) return;  // (the merge knows which parts there are)
+    const uint8_t *kc = a.k.codes + b * a.k.cb + h * a.k.ch, *ksc = a.k.scale + b * a.k.sb + h * a.k.sh;
+    const uint8_t *vc = a.v.codes + b * a.v.cb + h * a.v.ch, *vsc = a.v.scale + b * a.v.sb + h * a.v.sh;
+
+    // The token's row is the unit's last: the block that attends to it writes it, and reads it when all its waves see it.
+    if (p.rows > p.len && end == p.steps) {
+        if (wave == 0) mx_write_token<KB, VB>(a.k, a.v, a.new_k, a.new_v, HD, unit, b, h, p.len, lane);
+        __syncthreads();
+    }
+
+    T w;
+    w.start(a, unit, lane);
+    // step s: rows [row, row + live)
+    auto place = [&](int s, int64_t &row, int &live) __attribute__((always_inline)) {
+        const bool in_sink = s < p.sink_steps;
+        row = in_sink ? (int64_t)s * STEP : p.lo + (int64_t)(s - p.sink_steps) * STEP;
+        const int64_t left = (in_sink ? p.sink : p.rows) - row;
+        live = left < STEP ? (int)left : STEP;
+    };
+    int64_t row;
+    int live = 0, s = begin + wave;
+    if (s < end) {
+        place(s, row, live);
+        w.load_k(a.k, kc, ksc, row, live);
+        w.load_v(a.v, vc, vsc, row, live);
+    }
+    while (s < end) {
+        float x[T::REGS][4];
+        w.logits(a.scale, x);
+        const int next = s + kWaves, now = live;
+        if (next < end) {
+            place(next, row, live);
+            w.load_k(a.k, kc, ksc, row, live);
+        }
+        w.weigh(x, now);
+        w.add(x);
+        if (next < end) w.load_v(a.v, vc, vsc, row, live);
+        s = next;
+    }
+
+    // the wave's heads: over the lanes that had other rows, and over the tiles
+    float l = w.l;
+#pragma unroll
+    for (int d = GP; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+    if (lane < GP) s_m[wave * 16 + lane] = w.m, s_l[wave * 16 + lane] = l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // M row 4 q + i is head (4 q + i) % GP of a tile
+        const int head = (4 * w.q + i) % GP;
+        float *dst = s_acc + (wave * G + head) * HD + w.c * T::EPL;
+        const bool mine = 4 * w.q + i < GP && head < G;
+#pragma unroll
+        for (int j = 0; j < T::EPL; ++j) {
+            float o = w.acc[j][i];
+#pragma unroll
+            for (int d = GP * 4; d < 64; d <<= 1) o += __shfl_xor(o, d, 64);
+            if (mine) dst[j] = o;
+        }
+    }
+    __syncthreads();
+    auto weight = [](float m, float top) __attribute__((always_inline)) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f; };
+    auto top_of = [&](int head) __attribute__((always_inline)) {
+        float top = s_m[head];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i * 16 + head]);
+        return top;
+    };
+    const int64_t slot = (int64_t)unit * a.n_splits + split;
+    for (int o = tid; o < G * HD; o += kThreads) {
+        const int head = o / HD;
+        const float top = top_of(head);
+        float sum = 0.f, total = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            const float f = weight(s_m[i * 16 + head], top), li = s_l[i * 16 + head];
+            sum = fmaf(f, s_acc[i * G * HD + o], sum);
+            total += li == li ? f * li : li;  // (a sum that is no number stays none, whatever its maximum)
+        }
+        if (a.n_splits > 1) {
+            a.ws_acc[slot * (G * HD) + o] = sum;
+            if (o % HD == 0) {
+                float *ml = a.ws_ml + (slot * G + head) * 2;
+                ml[0] = top, ml[1] = total;
+            }
+        } else {
+            a.out[(int64_t)unit * G * HD + o] = dc_f32_to_bf16(total == 0.f ? 0.f : sum / total);
+            if (a.lse && o % HD == 0) a.lse[(int64_t)unit * G + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f;
+        }
+    }
+}
+
+// The parts of one query head joined: one block per (unit, head).
+template <int HD, int STEP>
+__global__ __launch_bounds__(kThreads) void mx_merge_kernel(AttnArgs a) {
+    constexpr int kLanes = HD / 4, kParts = kThreads / kLanes;
+    __shared__ float4 s_acc[kThreads];
+    const int unit = blockIdx.x / a.group, g = blockIdx.x % a.group, tid = threadIdx.x, lane = tid & 63;
+    const Plan p = mx_plan<STEP>(a, unit / a.n_h);
+    const int64_t slot0 = (int64_t)unit * a.n_splits;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0 * a.group + g;
+    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + (slot0 * a.group + g) * kLanes + tid % kLanes;
+    float top = -INFINITY;
+    for (int s = lane; s < p.used; s += 64) top = fmaxf(top, ml[(int64_t)s * a.group].x);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    auto weight = [&](float m) __attribute__((always_inline)) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f; };
+    float total = 0.f;
+    for (int s = lane; s < p.used; s += 64) {
+        const float2 o = ml[(int64_t)s * a.group];
+        total += o.y == o.y ? weight(o.x) * o.y : o.y;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d, 64);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = tid / kLanes; s < p.used; s += kParts) {
+        const float f = weight(ml[(int64_t)s * a.group].x);
+        const float4 v = pa[(int64_t)s * a.group * kLanes];
+        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    }
+    s_acc[tid] = acc;
+    __syncthreads();
+    if (tid < HD) {
+        const float *v = reinterpret_cast<const float *>(s_acc) + tid;
+        float sum = v[0];
+#pragma unroll
+        for (int i = 1; i < kParts; ++i) sum += v[i * HD];
+        a.out[(int64_t)blockIdx.x * HD + tid] = dc_f32_to_bf16(total == 0.f ? 0.f : sum / total);
+    }
+    if (a.lse && tid == 0) a.lse[blockIdx.x] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f;
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+
+int check_store(const char *who, const char *which, const dc_mx_store &s, int n_b, int n_h, int hd, bool written) {
+    DC_REQUIRE(s.bits == 4 || s.bits == 8, "%s: %s holds %d bits, not 4 or 8", who, which, s.bits);
+    DC_REQUIRE(s.n_rows >= 0, "%s: %s has a negative number of rows", who, which);
+    DC_REQUIRE((s.codes && s.scale) || s.n_rows == 0, "%s: null pointer in %s", who, which);
+    const int64_t row = (int64_t)hd * s.bits / 8, blocks = hd / 32;
+    DC_REQUIRE(dc_aligned16(s.codes) && s.code_batch_stride % 16 == 0 && s.code_head_stride % 16 == 0 && s.code_row_stride % 16 == 0,
+               "%s: %s's codes must be 16-byte aligned, its strides multiples of 16 bytes", who, which);
+    DC_REQUIRE((uintptr_t)s.scale % blocks == 0 && s.scale_batch_stride % blocks == 0 && s.scale_head_stride % blocks == 0 &&
+                   s.scale_row_stride % blocks == 0,
+               "%s: %s's scales and their strides must be multiples of %lld bytes", who, which, (long long)blocks);
+    DC_REQUIRE(s.code_row_stride >= row && s.scale_row_stride >= blocks, "%s: rows of %s overlap", who, which);
+    DC_REQUIRE(s.code_row_stride < (1 << 24) && s.scale_row_stride < (1 << 24), "%s: rows of %s are too far apart", who, which);
+    DC_REQUIRE(s.code_batch_stride >= 0 && s.code_head_stride >= 0 && s.scale_batch_stride >= 0 && s.scale_head_stride >= 0,
+               "%s: negative stride in %s", who, which);
+    if (written) {
+        DC_REQUIRE((n_b <= 1 || (s.code_batch_stride > 0 && s.scale_batch_stride > 0)) &&
+                       (n_h <= 1 || (s.code_head_stride > 0 && s.scale_head_stride > 0)),
+                   "%s: units of %s share their rows", who, which);
+    }
+    return DC_OK;
+}
+
+int check_units(const char *who, int n_b, int n_h, int hd) {
+    DC_REQUIRE(n_b >= 0 && n_h >= 1, "%s: bad sizes", who);
+    DC_REQUIRE((int64_t)n_b * n_h < (1 << 24), "%s: too many units", who);
+    DC_REQUIRE(hd == 64 || hd == 128 || hd == 256, "%s: head_dim %d unsupported", who, hd);
+    return DC_OK;
+}
+
+// blocks of a unit in a grid of (unit, chunk) by n_units * chunks
+int check_grid(const char *who, int64_t n_units, int64_t chunks) {
+    DC_REQUIRE(n_units * chunks < (1ll << 31), "%s: grid too large", who);
+    return DC_OK;
+}
+
+#define DC_TRY(x)                 \
+    do {                          \
+        const int rc_ = (x);      \
+        if (rc_ != DC_OK) return rc_; \
+    } while (0)
+
+#define DC_MX_BY_BITS(KERNEL, KBITS, VBITS, ...)                                              \
+    do {                                                                                      \
+        if ((KBITS) == 4 && (VBITS) == 4) hipLaunchKernelGGL((KERNEL<4, 4>), __VA_ARGS__);    \
+        else if ((KBITS) == 4) hipLaunchKernelGGL((KERNEL<4, 8>), __VA_ARGS__);               \
+        else if ((VBITS) == 4) hipLaunchKernelGGL((KERNEL<8, 4>), __VA_ARGS__);               \
+        else hipLaunchKernelGGL((KERNEL<8, 8>), __VA_ARGS__);                                 \
+    } while (0)
+
+// Blocks that the attention's splits come to, at most: two for a CU.
+constexpr int kBlocks = 512;
+constexpr int attn_tiles(int hd) { return hd == 256 ? 2 : 4; }
+
+// parts of a unit of up to n_rows attended rows that are worth a block: a step to each of its waves
+int64_t attn_parts(int hd, int64_t n_rows, int n_sink) {
+    const int64_t step = 16 * attn_tiles(hd);
+    const int64_t steps = (n_rows + step - 1) / step + (n_sink > 0 ? (n_sink + step - 1) / step : 0);
+    const int64_t parts = (steps + kWaves - 1) / kWaves;
+    return parts > 0 ? parts : 1;
+}
+
+template <int HD, int KB, int VB>
+void launch_attn(const AttnArgs &a, int n_units, hipStream_t st) {
+    constexpr int TILES = attn_tiles(HD);
+    const dim3 grid = dc_unit_grid(n_units, a.n_splits);
+    const size_t lds = attn_shared_bytes(HD, a.group);
+#define DC_LAUNCH_MX(GP) hipLaunchKernelGGL((mx_attn_kernel<HD, KB, VB, GP, TILES>), grid, dim3(kThreads), lds, st, a)
+    if (a.group > 8) DC_LAUNCH_MX(16);
+    else if (a.group > 4 || TILES == 2) DC_LAUNCH_MX(8);
+    else if constexpr (TILES == 4) DC_LAUNCH_MX(4);
+#undef DC_LAUNCH_MX
+    if (a.n_splits > 1)
+        hipLaunchKernelGGL((mx_merge_kernel<HD, 16 * TILES>), dim3((unsigned)(n_units * a.group)), dim3(kThreads), 0, st, a);
+}
+
+template <int HD>
+void launch_attn_bits(int kbits, int vbits, const AttnArgs &a, int n_units, hipStream_t st) {
+    if (kbits == 4 && vbits == 4) launch_attn<HD, 4, 4>(a, n_units, st);
+    else if (kbits == 4) launch_attn<HD, 4, 8>(a, n_units, st);
+    else if (vbits == 4) launch_attn<HD, 8, 4>(a, n_units, st);
+    else launch_attn<HD, 8, 8>(a, n_units, st);
+}
+
+}  // namespace
+
+extern "C" int dc_mx_ingest_bf16(const dc_mx_store *k, const dc_mx_store *v, const void *k_src, const void *v_src,
+                                 const int32_t *lens, int n_b, int seq, int n_h, int hd, int dst_pos, int64_t ksb, int64_t kss,
+                                 int64_t ksh, int64_t vsb, int64_t vss, int64_t vsh, void *stream) {
+    const char *who = "dc_mx_ingest_bf16";
+    DC_TRY(check_units(who, n_b, n_h, hd));
+    DC_REQUIRE(seq >= 0 && dst_pos >= 0, "%s: bad sizes", who);
+    const int64_t n_units = (int64_t)n_b * n_h;
+    if (n_units == 0 || seq == 0) return DC_OK;
+    DC_REQUIRE(k && v && k_src && v_src, "%s: null pointer", who);
+    DC_TRY(check_store(who, "k", *k, n_b, n_h, hd, true));
+    DC_TRY(check_store(who, "v", *v, n_b, n_h, hd, true));
+    DC_REQUIRE((int64_t)dst_pos + seq <= k->n_rows && (int64_t)dst_pos + seq <= v->n_rows,
+               "%s: rows [%d, %lld) outside the store", who, dst_pos, (long long)dst_pos + seq);
+    DC_REQUIRE(dc_aligned16(k_src) && dc_aligned16(v_src), "%s: pointers must be 16-byte aligned", who);
+    DC_REQUIRE(ksb % 8 == 0 && kss % 8 == 0 && ksh % 8 == 0 && vsb % 8 == 0 && vss % 8 == 0 && vsh % 8 == 0,
+               "%s: strides must be multiples of 8 elements", who);
+    const int rows_per = kThreads / (hd / 8) * kIngestBatch;
+    const int64_t chunks = (seq + rows_per - 1) / rows_per;
+    DC_TRY(check_grid(who, n_units, chunks));
+    IngestArgs a = {view_of(*k), view_of(*v), (const uint16_t *)k_src, (const uint16_t *)v_src, ksb, kss, ksh, vsb, vss, vsh,
+                    lens, n_h, seq, dst_pos, (int)chunks};
+    DC_MX_BY_BITS(mx_ingest_kernel, k->bits, v->bits, dim3((unsigned)(n_units * chunks), 2), dim3(kThreads), 0, (hipStream_t)stream, a, hd);
+    DC_CHECK_LAUNCH(who);
+    return DC_OK;
+}
+
+extern "C" int dc_mx_append_bf16(const dc_mx_store *k, const dc_mx_store *v, const void *new_k, const void *new_v, const int32_t *lens,
+                                 int n_b, int n_h, int hd, void *stream) {
+    const char *who = "dc_mx_append_bf16";
+    DC_TRY(check_units(who, n_b, n_h, hd));
+    const int n_units = n_b * n_h;
+    if (n_units == 0) return DC_OK;
+    DC_REQUIRE(k && v && new_k && new_v && lens, "%s: null pointer", who);
+    DC_TRY(check_store(who, "k", *k, n_b, n_h, hd, true));
+    DC_TRY(check_store(who, "v", *v, n_b, n_h, hd, true));
+    DC_REQUIRE(dc_aligned16(new_k) && dc_aligned16(new_v), "%s: pointers must be 16-byte aligned", who);
+    const int cap = k->n_rows < v->n_rows ? k->n_rows : v->n_rows;
+    DC_MX_BY_BITS(mx_append_kernel, k->bits, v->bits, dim3((unsigned)((n_units + kWaves - 1) / kWaves)), dim3(kThreads), 0,
+                  (hipStream_t)stream, view_of(*k), view_of(*v), (const uint16_t *)new_k, (const uint16_t *)new_v, lens, n_units, n_h, hd, cap);
+    DC_CHECK_LAUNCH(who);
+    return DC_OK;
+}
+
+extern "C" int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v, const uint32_t *idx, void *out_k, void *out_v, int n_b,
+                                      int n_h, int n_idx, int64_t idx_unit_stride, int hd, int64_t row_offset, int64_t dsb, int64_t dsh,
+                                      int64_t dsr, void *stream) {
+    const char *who = "dc_mx_gather_rows_bf16";
+    DC_TRY(check_units(who, n_b, n_h, hd));
+    DC_REQUIRE(n_idx >= 0 && row_offset >= 0, "%s: bad sizes", who);
+    const int64_t n_units = (int64_t)n_b * n_h;
+    if (n_units == 0 || n_idx == 0) return DC_OK;
+    DC_REQUIRE(out_k || out_v, "%s: null pointer", who);
+    DC_REQUIRE((!out_k || k) && (!out_v || v), "%s: source missing for an output", who);
+    if (out_k) DC_TRY(check_store(who, "k", *k, n_b, n_h, hd, false));
+    if (out_v) DC_TRY(check_store(who, "v", *v, n_b, n_h, hd, false));
+    DC_REQUIRE(!idx || idx_unit_stride >= n_idx, "%s: idx_unit_stride < n_idx", who);
+    DC_REQUIRE((!out_k || dc_aligned16(out_k)) && (!out_v || dc_aligned16(out_v)), "%s: pointers must be 16-byte aligned", who);
+    DC_REQUIRE(dsb % 8 == 0 && dsh % 8 == 0 && dsr % 8 == 0, "%s: strides must be multiples of 8 elements", who);
+    const int rows_per = kThreads / (hd / 8) * kGatherBatch;
+    const int64_t chunks = ((int64_t)n_idx + rows_per - 1) / rows_per;
+    DC_TRY(check_grid(who, n_units, chunks));
+    const dc_mx_store &ks = out_k ? *k : *v, &vs = out_v ? *v : *k;
+    GatherArgs a = {view_of(ks), view_of(vs), idx, idx_unit_stride, row_offset, (uint16_t *)out_k, (uint16_t *)out_v, dsb, dsh, dsr,
+                    n_h, n_idx, ks.n_rows, vs.n_rows, (int)chunks};
+    DC_MX_BY_BITS(mx_gather_kernel, ks.bits, vs.bits, dim3((unsigned)(n_units * chunks), out_k && out_v ? 2 : 1), dim3(kThreads), 0,
+                  (hipStream_t)stream, a, hd, out_k ? 0 : 1);
+    DC_CHECK_LAUNCH(who);
+    return DC_OK;
+}
+
+extern "C" size_t dc_mx_attn_workspace_bytes(int n_units, int group, int hd, int n_rows) {
+    if (n_units <= 0 || group <= 0 || hd < 64 || n_rows < 0) return 256;
+    // (as many parts as the grid has blocks, or as there are: never less for more units or rows)
+    const int64_t parts = n_units * (attn_parts(hd, n_rows, 0) + 1);
+    const size_t slots = (size_t)(parts < kBlocks ? parts : kBlocks);
+    return dc_align_up(slots * group * hd * 4, 256) + dc_align_up(slots * group * 2 * 4, 256);
+}
+
+extern "C" int dc_mx_attn_bf16(const dc_mx_attn_args *x, void *stream) {
+    const char *who = "dc_mx_attn_bf16";
+    DC_REQUIRE(x, "%s: null pointer", who);
+    DC_TRY(check_units(who, x->n_b, x->n_h, x->hd));
+    const int n_units = x->n_b * x->n_h;
+    if (n_units == 0) return DC_OK;
+    DC_REQUIRE(x->q && x->out, "%s: null pointer", who);
+    DC_REQUIRE((x->new_k == nullptr) == (x->new_v == nullptr), "%s: new_k and new_v must both be set or both be null", who);
+    DC_TRY(check_store(who, "k", x->k, x->n_b, x->n_h, x->hd, x->new_k != nullptr));
+    DC_TRY(check_store(who, "v", x->v, x->n_b, x->n_h, x->hd, x->new_k != nullptr));
+    DC_REQUIRE(x->group >= 1 && x->group <= 16, "%s: group %d not in [1,16]", who, x->group);
+    DC_REQUIRE(x->n_rows >= 0 && x->n_rows <= x->k.n_rows && x->n_rows <= x->v.n_rows, "%s: %d rows outside the store", who, x->n_rows);
+    DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
+    DC_REQUIRE(dc_aligned16(x->q) && (!x->new_k || (dc_aligned16(x->new_k) && dc_aligned16(x->new_v))),
+               "%s: pointers must be 16-byte aligned", who);
+    DC_REQUIRE((int64_t)n_units * x->group < (1ll << 31), "%s: grid too large", who);
+    const int64_t attended = x->window > 0 && (int64_t)x->n_sink + x->window < x->n_rows ? x->window : x->n_rows;
+    const int64_t parts = attn_parts(x->hd, attended, attended < x->n_rows ? x->n_sink : 0);
+    const int64_t most = kBlocks / n_units > 1 ? kBlocks / n_units : 1;
+    AttnArgs a;
+    a.n_splits = (int)(parts < most ? parts : most);
+    if (a.n_splits > 1) {
+        const size_t slots = (size_t)n_units * a.n_splits;
+        const size_t acc_bytes = dc_align_up(slots * x->group * x->hd * 4, 256), need = acc_bytes + dc_align_up(slots * x->group * 2 * 4, 256);
+        DC_REQUIRE(x->workspace && ((uintptr_t)x->workspace & 255u) == 0, "%s: workspace must be non-null and 256-byte aligned", who);
+        if (x->workspace_bytes < need) {
+            dc_set_error("%s: workspace %zu bytes < %zu needed", who, x->workspace_bytes, need);
+            return DC_ENOMEM;
+        }
+        a.ws_acc = (float *)x->workspace;
+        a.ws_ml = (float *)((char *)x->workspace + acc_bytes);
+    } else {
+        a.ws_acc = a.ws_ml = nullptr;
+    }
+    a.q = (const uint16_t *)x->q, a.new_k = (const uint16_t *)x->new_k, a.new_v = (const uint16_t *)x->new_v;
+    a.out = (uint16_t *)x->out, a.lse = x->lse, a.lens = x->lens;
+    a.k = view_of(x->k), a.v = view_of(x->v);
+    a.n_h = x->n_h, a.group = x->group, a.cap = x->n_rows, a.n_sink = x->n_sink, a.window = x->window;
+    a.scale = x->scale * 1.44269504088896341f;
+    hipStream_t st = (hipStream_t)stream;
+    if (x->hd == 64) launch_attn_bits<64>(x->k.bits, x->v.bits, a, n_units, st);
+    else if (x->hd == 128) launch_attn_bits<128>(x->k.bits, x->v.bits, a, n_units, st);
+    else launch_attn_bits<256>(x->k.bits, x->v.bits, a, n_units, st);
+    DC_CHECK_LAUNCH(who);
+    return DC_OK;
+}

@@ -1,3 +1,4 @@
 from .diffcache import DiffCache
+from .mxcache import MxCache
 
-__all__ = ["DiffCache"]
+__all__ = ["DiffCache", "MxCache"]

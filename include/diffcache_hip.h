@@ -628,6 +628,86 @@ int dc_data_layer_insert(dc_data_layer *dl, const void *keys, const void *vals, 
 int dc_data_layer_query(dc_data_layer *dl, void *out_keys, void *out_vals, int64_t out_rows,
                         const void *queries, int ef, int *n_out, void *stream);
 
+/*
+ * A cache held in blocks of 32 numbers, 4.25 or 8.25 bits to a number instead of bf16's 16, for callers that attend
+ * to the whole of a long context.  The reference has no such cache: it takes the place of the assembled bf16 buffer and
+ * of flash_attn_with_kvcache over it (src/diffcache/kvcache/diffcache.py:48-66, src/diffcache/base.py:134-142).
+ *
+ * A block of a row (columns 32 i .. + 31) is held as a code for every number and one byte e: number = code's 2^(e - 127).
+ *   bits 4   E2M1: 0, 0.5, 1, 1.5, 2, 3, 4, 6 for codes 0 .. 7, negative with bit 3; column 2 i in the low half of byte i
+ *   bits 8   E4M3 (largest number 448, codes 0x7f and 0xff NaN)
+ * Numbers are rounded to the nearest, ties to the even code; e is the least at which the block's largest number does not
+ * round past the last code, from 2 to 252 (bits 4) or 10 to 246 (bits 8), so that every number held is a normal bf16 number
+ * or zero: reading back into bf16 is exact.  A block with an infinity or a NaN in it is held as NaN (e = 255).
+ *
+ * dc_mx_store names one tensor (K or V) of a layer: row r of unit (b, h) has its hd * bits / 8 bytes of codes at
+ *   codes + b * code_batch_stride + h * code_head_stride + r * code_row_stride
+ * and its hd / 32 scales, contiguous, likewise; strides in bytes.  Codes are 16-byte aligned with strides multiples of 16, scales
+ * and their strides multiples of hd / 32; rows may be up to 16 MiB apart.  n_rows: the rows there is room for.  Units that share
+ * rows (a stride of 0) may be read, not written.  K and V may be held in different bits.  hd: 64, 128 or 256.
+ */
+typedef struct dc_mx_store {
+    void *codes, *scale;
+    int64_t code_batch_stride, code_head_stride, code_row_stride;
+    int64_t scale_batch_stride, scale_head_stride, scale_row_stride;
+    int bits, n_rows;
+} dc_mx_store;
+
+/*
+ * Rows of a prompt: k_src, v_src (n_b, seq, n_h, hd) bf16 by element strides (batch, token, head; hd contiguous) into rows
+ * [dst_pos, dst_pos + seq) of the stores.  lens: NULL, or (n_b) int32 on the device: only the first lens[b] tokens of sequence b
+ * are written, the rows behind them are left as they were.  The counterpart of dc_ingest_kv_bf16
+ * (diffcache.py:142-147, nsw.rs:503-508).
+ */
+int dc_mx_ingest_bf16(const dc_mx_store *k, const dc_mx_store *v, const void *k_src, const void *v_src,
+                      const int32_t *lens, int n_b, int seq, int n_h, int hd, int dst_pos,
+                      int64_t k_batch_stride, int64_t k_token_stride, int64_t k_head_stride,
+                      int64_t v_batch_stride, int64_t v_token_stride, int64_t v_head_stride, void *stream);
+
+/*
+ * One token of every sequence: new_k, new_v (n_b, n_h, hd) bf16 into row lens[b] (int32 on the device) of sequence b.  A row
+ * that the stores do not have is not written.  The counterpart of dc_append_kv_bf16 (lib.rs:352-369).
+ */
+int dc_mx_append_bf16(const dc_mx_store *k, const dc_mx_store *v, const void *new_k, const void *new_v,
+                      const int32_t *lens, int n_b, int n_h, int hd, void *stream);
+
+/*
+ * out[b, h, j, :] = the bf16 numbers of row row_offset + idx[u * idx_unit_stride + j], j < n_idx (row_offset + j where idx is
+ * NULL); a row that the store does not have reads as zeros.  out_k or out_v may be NULL, and its store with it.  The
+ * counterpart of dc_gather_rows_bf16 (nsw.rs:621-629).
+ */
+int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v, const uint32_t *idx, void *out_k, void *out_v,
+                           int n_b, int n_h, int n_idx, int64_t idx_unit_stride, int hd, int64_t row_offset,
+                           int64_t dst_batch_stride, int64_t dst_head_stride, int64_t dst_row_stride, void *stream);
+
+/*
+ * One token's attention over the cache: out (n_b, n_h * group, hd) bf16, softmax(scale q k^T) v over the rows of each sequence.
+ *   lens     (n_b) int32 on the device, the rows that sequence b holds; NULL: n_rows, less one with a token of its own
+ *   n_rows   the most rows any sequence holds, the token's among them (at most the stores' rows): sizes the launch; rows
+ *            at or beyond it are neither attended to nor written
+ *   new_k, new_v  NULL, or (n_b, n_h, hd) bf16: the token's own row, written to row lens[b] as dc_mx_append_bf16 does and
+ *            attended to as it is held.  lens is not changed
+ *   window   0: all rows; else the first n_sink and the last `window` (the token's own among them)
+ *   lse      NULL, or (n_b, n_h * group) fp32: log of the sum of exp(scale q k^T)
+ * A sequence without rows has out 0 and lse -inf.  Rows that are not attended to may hold anything; one that is and holds a NaN
+ * makes its unit's outputs NaN.  group: up to 16 query heads.  Sums and statistics are fp32.  The workspace
+ * (dc_mx_attn_workspace_bytes, 256-byte aligned; enough for more units or rows is enough for fewer) holds nothing between calls;
+ * calls that may overlap need one each.  Replaces flash_attn_with_kvcache (base.py:134-142) over such a cache.
+ */
+typedef struct dc_mx_attn_args {
+    const void *q, *new_k, *new_v;
+    void *out;
+    float *lse;
+    const int32_t *lens;
+    dc_mx_store k, v;
+    void *workspace;
+    size_t workspace_bytes;
+    int n_b, n_h, group, hd, n_rows, n_sink, window;
+    float scale;
+} dc_mx_attn_args;
+size_t dc_mx_attn_workspace_bytes(int n_units, int group, int hd, int n_rows);
+int dc_mx_attn_bf16(const dc_mx_attn_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
