@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -177,13 +178,13 @@ def _load() -> C.CDLL:
         "dc_score_select_sketch_bf16": (i, [p, p, p, p, p, p, i64, i, i, i, i, i64, i64, i64, i64, i64, i64,
                                             i, i, i, i, i, p, sz, p, p, p]),
     }
-    mx = C.POINTER(MxStoreArgs)
+    mx = C.c_char_p   # a struct's bytes (MxStore keeps its own): packing them costs a fifth of filling in a ctypes structure
     sigs.update({
         "dc_mx_ingest_bf16": (i, [mx, mx, p, p, p, i, i, i, i, i, i64, i64, i64, i64, i64, i64, p]),
         "dc_mx_append_bf16": (i, [mx, mx, p, p, p, i, i, i, p]),
         "dc_mx_gather_rows_bf16": (i, [mx, mx, p, p, p, i, i, i, i64, i, i64, i64, i64, i64, p]),
         "dc_mx_attn_workspace_bytes": (sz, [i, i, i, i]),
-        "dc_mx_attn_bf16": (i, [C.POINTER(MxAttnArgs), p]),
+        "dc_mx_attn_bf16": (i, [mx, p]),
     })
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -1005,25 +1006,49 @@ def compose_idx(outer: torch.Tensor, inner: torch.Tensor) -> torch.Tensor:
 # a cache in blocks of 32 numbers (dc_mx_store)
 # ---------------------------------------------------------------------------
 
+# The two structs' bytes.  (A call of these wrappers costs a few microseconds, as much as the kernels of a short context:
+# every attribute is read once and every tensor made in the cheapest way.)
+_MX_STORE = struct.Struct("@2P6q2i")
+_MX_ATTN = struct.Struct("@6P%ds%dsPN7if" % (_MX_STORE.size, _MX_STORE.size))
+_device = torch._C._cuda_getDevice
+_U8, _BF16, _F32, _I32 = torch.uint8, torch.bfloat16, torch.float32, torch.int32
+
+
+def _mx_dev(t: torch.Tensor, name: str) -> int:
+    """Device pointer of a tensor on the current device, whose stream the call goes to."""
+    at = t.get_device()
+    if at < 0:
+        raise DiffCacheError(f"{name} must live in GPU memory (got {t.device}); there is no CPU path")
+    if at != _device():
+        raise DiffCacheError(f"{name} lives on {t.device}, the current device is cuda:{_device()}")
+    return t.data_ptr()
+
+
 class MxStore:
     """K or V of a layer, held in 4 or 8 bits with a power of two for every 32 numbers (dc_mx_store in the header):
     ``codes`` (b, h, n, hd * bits / 8) and ``scale`` (b, h, n, hd / 32), both uint8 with contiguous rows.  Views of larger
     tensors will do; ``MxStore.zeros`` makes a store of its own, whose rows read as zeros until they are written."""
 
+    __slots__ = ("codes", "scale", "shape", "units", "hd", "bits", "args")
+
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
-        cs, ss = codes.shape, scale.shape
-        if len(cs) != 4 or len(ss) != 4 or cs[:3] != ss[:3] or codes.dtype != torch.uint8 or scale.dtype != torch.uint8:
+        if codes.dim() != 4 or scale.dim() != 4 or codes.dtype is not _U8 or scale.dtype is not _U8:
             raise DiffCacheError("codes and scale must be (b, h, n, .) uint8 tensors of the same b, h and n")
-        self.hd = ss[3] * 32
-        if cs[3] not in (self.hd // 2, self.hd) or ss[3] == 0:
-            raise DiffCacheError(f"rows of {cs[3]} code bytes and {ss[3]} scales are neither 4 nor 8 bits to a number")
-        (cb, ch, cr, c1), (sb, sh, sr, s1) = codes.stride(), scale.stride()
-        if c1 != 1 or s1 != 1:
+        b, h, n, row = codes.shape
+        sb, sh, sn, blocks = scale.shape
+        if sb != b or sh != h or sn != n:
+            raise DiffCacheError("codes and scale must be (b, h, n, .) uint8 tensors of the same b, h and n")
+        hd = blocks * 32
+        bits = 4 if row * 2 == hd else 8
+        if row * 8 != hd * bits or hd == 0:
+            raise DiffCacheError(f"rows of {row} code bytes and {blocks} scales are neither 4 nor 8 bits to a number")
+        cb, ch, cr, c1 = codes.stride()
+        sb, sh, sr, s1 = scale.stride()
+        if c1 != 1 or (s1 != 1 and blocks > 1):
             raise DiffCacheError("the rows of codes and scale must be contiguous")
         self.codes, self.scale = codes, scale
-        self.shape = (cs[0], cs[1], cs[2], self.hd)
-        self.bits = 4 if cs[3] * 2 == self.hd else 8
-        self._args = MxStoreArgs(_mx_dev(codes, "codes"), _mx_dev(scale, "scale"), cb, ch, cr, sb, sh, sr, self.bits, cs[2])
+        self.shape, self.units, self.hd, self.bits = (b, h, n, hd), (b, h, hd), hd, bits
+        self.args = _MX_STORE.pack(_mx_dev(codes, "codes"), _mx_dev(scale, "scale"), cb, ch, cr, sb, sh, sr, bits, n)
 
     @classmethod
     def zeros(cls, b: int, h: int, n: int, hd: int, bits: int, device) -> "MxStore":
@@ -1033,42 +1058,34 @@ class MxStore:
                    torch.zeros((b, h, n, hd // 32), dtype=torch.uint8, device=device))
 
 
-def _mx_dev(t: torch.Tensor, name: str) -> int:
-    """Device pointer of a tensor on the current device, whose stream the call goes to."""
-    if not t.is_cuda:
-        raise DiffCacheError(f"{name} must live in GPU memory (got {t.device}); there is no CPU path")
-    if t.device.index != torch._C._cuda_getDevice():
-        raise DiffCacheError(f"{name} lives on {t.device}, the current device is cuda:{torch._C._cuda_getDevice()}")
-    return t.data_ptr()
-
-
-def _mx_pair(k: MxStore, v: MxStore):
-    if k.shape[:2] != v.shape[:2] or k.hd != v.hd:
+def _mx_pair(k: MxStore, v: MxStore) -> Tuple[int, int, int]:
+    if k.units != v.units:
         raise DiffCacheError(f"K store {k.shape} and V store {v.shape} do not belong together")
-    return k.shape[0], k.shape[1], k.hd
+    return k.units
 
 
-def _mx_lens(lens: Optional[torch.Tensor], b: int):
+def _mx_lens(lens: Optional[torch.Tensor], b: int) -> int:
     if lens is None:
-        return None
-    if lens.dtype != torch.int32 or lens.numel() != b or not lens.is_contiguous():
+        return 0
+    if lens.dtype is not _I32 or lens.numel() != b or not lens.is_contiguous():
         raise DiffCacheError(f"lens must be a contiguous int32 tensor of {b} elements")
     return _mx_dev(lens, "lens")
 
 
-def _mx_src(t: torch.Tensor, shape, name: str) -> torch.Tensor:
+def _mx_src(t: torch.Tensor, shape, name: str):
     if t.dtype != torch.bfloat16 or t.shape != shape:
-        raise DiffCacheError(f"{name} must be a {tuple(shape)} bf16 tensor, not {tuple(t.shape)} {t.dtype}")
-    if t.stride(3) != 1 or t.data_ptr() % 16 or any(x % 8 for x in t.stride()[:3]):
-        t = t.contiguous()
-    return t
+        raise DiffCacheError(f"{name} must be a {shape} bf16 tensor, not {tuple(t.shape)} {t.dtype}")
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or s0 & 7 or s1 & 7 or s2 & 7 or t.data_ptr() & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        s0, s1, s2, s3 = t.stride()
+    return t, s0, s1, s2
 
 
 def _mx_token(t: torch.Tensor, b: int, h: int, hd: int, name: str) -> torch.Tensor:
-    t = t.contiguous()
     if t.dtype != torch.bfloat16 or t.numel() != b * h * hd:
         raise DiffCacheError(f"{name} must hold ({b}, {h}, {hd}) bf16 values")
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.is_contiguous() and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def mx_ingest(k: MxStore, v: MxStore, k_src: torch.Tensor, v_src: torch.Tensor, dst_pos: int = 0,
@@ -1079,12 +1096,21 @@ def mx_ingest(k: MxStore, v: MxStore, k_src: torch.Tensor, v_src: torch.Tensor, 
     if k_src.dim() != 4:
         raise DiffCacheError("k_src and v_src must be (b, seq, h, hd) bf16 tensors matching the store")
     seq = k_src.shape[1]
-    k_src, v_src = (_mx_src(t, (b, seq, h, hd), name) for t, name in ((k_src, "k_src"), (v_src, "v_src")))
-    if dst_pos < 0 or dst_pos + seq > min(k.shape[2], v.shape[2]):
-        raise DiffCacheError(f"rows [{dst_pos}, {dst_pos + seq}) outside the store of {min(k.shape[2], v.shape[2])} rows")
-    _check(lib.dc_mx_ingest_bf16(C.byref(k._args), C.byref(v._args), _mx_dev(k_src, "k_src"), _mx_dev(v_src, "v_src"),
-                                 _mx_lens(lens, b), b, seq, h, hd, dst_pos, *k_src.stride()[:3], *v_src.stride()[:3],
-                                 _stream()))
+    k_src, k0, k1, k2 = _mx_src(k_src, (b, seq, h, hd), "k_src")
+    v_src, v0, v1, v2 = _mx_src(v_src, (b, seq, h, hd), "v_src")
+    room = min(k.shape[2], v.shape[2])
+    if dst_pos < 0 or dst_pos + seq > room:
+        raise DiffCacheError(f"rows [{dst_pos}, {dst_pos + seq}) outside the store of {room} rows")
+    _check(lib.dc_mx_ingest_bf16(k.args, v.args, _mx_dev(k_src, "k_src"), _mx_dev(v_src, "v_src"), _mx_lens(lens, b) or None, b, seq,
+                                 h, hd, dst_pos, k0, k1, k2, v0, v1, v2, _mx_stream(k)))
+
+
+def _mx_stream(s: MxStore) -> int:
+    """The current stream, for a store on the current device (which may have changed since the store was made)."""
+    at = _device()
+    if s.codes.get_device() != at:
+        raise DiffCacheError(f"the store lives on {s.codes.device}, the current device is cuda:{at}")
+    return torch._C._cuda_getCurrentRawStream(at)
 
 
 def mx_append(k: MxStore, v: MxStore, new_k: torch.Tensor, new_v: torch.Tensor, lens: torch.Tensor) -> None:
@@ -1092,8 +1118,8 @@ def mx_append(k: MxStore, v: MxStore, new_k: torch.Tensor, new_v: torch.Tensor, 
     is not changed, and a row that the stores do not have is not written."""
     b, h, hd = _mx_pair(k, v)
     new_k, new_v = _mx_token(new_k, b, h, hd, "new_k"), _mx_token(new_v, b, h, hd, "new_v")
-    _check(lib.dc_mx_append_bf16(C.byref(k._args), C.byref(v._args), _mx_dev(new_k, "new_k"), _mx_dev(new_v, "new_v"),
-                                 _mx_lens(lens, b), b, h, hd, _stream()))
+    _check(lib.dc_mx_append_bf16(k.args, v.args, _mx_dev(new_k, "new_k"), _mx_dev(new_v, "new_v"), _mx_lens(lens, b) or None, b, h, hd,
+                                 _mx_stream(k)))
 
 
 def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[torch.Tensor] = None,
@@ -1105,35 +1131,48 @@ def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[tor
     ref = k if k is not None else v
     if ref is None:
         raise DiffCacheError("neither K nor V given")
-    b, h, hd = _mx_pair(k, v) if k is not None and v is not None else (ref.shape[0], ref.shape[1], ref.hd)
-    if n_idx is None:
-        n_idx = max(ref.shape[2] - row_offset, 0) if idx is None else idx.shape[1]
+    b, h, hd = ref.units if v is None else _mx_pair(ref, v)
+    idx_ptr = idx_stride = 0
+    if idx is None:
+        if n_idx is None:
+            n_idx = max(ref.shape[2] - row_offset, 0)
+    else:
+        require(idx.dim() == 2 and idx.shape[0] == b * h and idx.element_size() == 4 and not idx.is_floating_point(),
+                "idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor")
+        wide = idx.shape[1]
+        if n_idx is None:
+            n_idx = wide
+        require(wide >= n_idx, "idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor")
+        idx_stride, one = idx.stride()
+        if idx_stride < wide or (one != 1 and wide > 1):
+            idx = idx.clone(memory_format=torch.contiguous_format)
+            idx_stride = wide
+        idx_ptr = _mx_dev(idx, "idx")
     if n_idx < 0 or row_offset < 0:
         raise DiffCacheError("n_idx and row_offset must not be negative")
-    if idx is not None:
-        require(idx.dim() == 2 and idx.shape[0] == b * h and idx.shape[1] >= n_idx and idx.element_size() == 4
-                and not idx.is_floating_point() and (idx.shape[1] <= 1 or idx.stride(1) == 1),
-                "idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor with contiguous rows")
-        if idx.stride(0) < n_idx:
-            idx = idx.contiguous()
-    outs = []
-    for s, o, name in ((k, out_k, "out_k"), (v, out_v, "out_v")):
-        if s is not None and o is None:
-            o = torch.empty((b, h, n_idx, hd), dtype=torch.bfloat16, device=s.codes.device)
-        elif o is not None:
-            _store_strides(o)
+    strides = None
+    ptrs = [None, None]
+    for i, (s, o, name) in enumerate(((k, out_k, "out_k"), (v, out_v, "out_v"))):
+        if o is not None:
+            st = _store_strides(o)
             ob, oh, on, od = o.shape
             require(s is not None and ob == b and oh == h and on >= n_idx and od == hd,
                     "out_k / out_v must be (bsz, kv_heads, >= n_idx, head_dim), each with its store")
-        outs.append(o)
-    strides = [_store_strides(o) for o in outs if o is not None]
-    if strides[0] != strides[-1]:
-        raise DiffCacheError("out_k and out_v must share their strides")
-    _check(lib.dc_mx_gather_rows_bf16(
-        None if k is None else C.byref(k._args), None if v is None else C.byref(v._args),
-        None if idx is None else _mx_dev(idx, "idx"), *(None if o is None else _mx_dev(o, "out") for o in outs),
-        b, h, n_idx, 0 if idx is None else max(idx.stride(0), n_idx), hd, row_offset, *strides[0], _stream()))
-    return outs[0], outs[1]
+        elif s is not None:
+            st = (h * n_idx * hd, n_idx * hd, hd)
+            o = torch.empty_strided((b, h, n_idx, hd), st + (1,), dtype=torch.bfloat16, device=s.codes.device)
+            if i:
+                out_v = o
+            else:
+                out_k = o
+        else:
+            continue
+        if strides is not None and strides != st:
+            raise DiffCacheError("out_k and out_v must share their strides")
+        strides, ptrs[i] = st, _mx_dev(o, name)
+    _check(lib.dc_mx_gather_rows_bf16(None if k is None else k.args, None if v is None else v.args, idx_ptr or None, *ptrs,
+                                      b, h, n_idx, idx_stride, hd, row_offset, *strides, _mx_stream(ref)))
+    return out_k, out_v
 
 
 def mx_attn_workspace_bytes(n_units: int, group: int, hd: int, n_rows: int) -> int:
@@ -1150,34 +1189,49 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
     to row lens[b] and attended to as it is held; lens is not changed.  ``window`` > 0: only the first ``n_sink`` rows and the
     last ``window``.  With ``lse`` or ``want_lse`` returns (out, lse), lse (b, h*group) fp32 the log of the sum of exponentials."""
     b, h, hd = _mx_pair(k, v)
-    q = q.contiguous()
-    group = q.numel() // (b * h * hd) if b * h else 1
-    if q.dtype != torch.bfloat16 or q.numel() != b * h * group * hd or (group < 1 and b):
+    numel = q.numel()
+    hq = numel // (b * hd) if b else h
+    group = hq // h
+    if q.dtype is not _BF16 or numel != b * h * group * hd or group < 1:
         raise DiffCacheError("q must be bf16 with (b, h * group, hd) values")
-    if q.data_ptr() % 16:
-        q = q.clone()
-    room = min(k.shape[2], v.shape[2])
-    n_rows = room if n_rows is None else n_rows
-    if not 0 <= n_rows <= room:
+    if not q.is_contiguous() or q.data_ptr() & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+    room = k.shape[2]
+    if v.shape[2] < room:
+        room = v.shape[2]
+    if n_rows is None:
+        n_rows = room
+    elif not 0 <= n_rows <= room:
         raise DiffCacheError(f"{n_rows} rows outside the store of {room}")
+    if n_sink < 0 or window < 0:
+        raise DiffCacheError("n_sink and window must not be negative")
+    dev = q.device
     if out is None:
-        out = torch.empty((b, h * group, hd), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.numel() != q.numel() or not out.is_contiguous():
+        out = torch.empty_strided((b, hq, hd), (hq * hd, hd, 1), dtype=_BF16, device=dev)
+    elif out.dtype is not _BF16 or out.numel() != numel or not out.is_contiguous():
         raise DiffCacheError("out must be a contiguous bf16 tensor of the size of q")
-    if lse is None and want_lse:
-        lse = torch.empty((b, h * group), dtype=torch.float32, device=q.device)
-    elif lse is not None and (lse.dtype != torch.float32 or lse.numel() != b * h * group or not lse.is_contiguous()):
+    lse_ptr = new_k_ptr = new_v_ptr = ws_ptr = ws_bytes = 0
+    if lse is None:
+        if want_lse:
+            lse = torch.empty_strided((b, hq), (hq, 1), dtype=_F32, device=dev)
+            lse_ptr = lse.data_ptr()
+    elif lse.dtype is not _F32 or lse.numel() != b * hq or not lse.is_contiguous():
         raise DiffCacheError("lse must be a contiguous fp32 tensor of (b, h * group) elements")
-    if (new_k is None) != (new_v is None):
-        raise DiffCacheError("new_k and new_v must be given together")
-    if new_k is not None:
+    else:
+        lse_ptr = _mx_dev(lse, "lse")
+    if new_k is not None and new_v is not None:
         new_k, new_v = _mx_token(new_k, b, h, hd, "new_k"), _mx_token(new_v, b, h, hd, "new_v")
-    if workspace is None:
-        workspace = torch.empty((mx_attn_workspace_bytes(b * h, group, hd, n_rows),), dtype=torch.uint8, device=q.device)
-    a = MxAttnArgs(_mx_dev(q, "q"), None if new_k is None else _mx_dev(new_k, "new_k"),
-                   None if new_v is None else _mx_dev(new_v, "new_v"), _mx_dev(out, "out"),
-                   None if lse is None else _mx_dev(lse, "lse"), _mx_lens(lens, b), k._args, v._args,
-                   _mx_dev(workspace, "workspace"), workspace.numel() * workspace.element_size(), b, h, group, hd, n_rows, n_sink, window,
-                   1.0 / math.sqrt(hd) if scale is None else scale)
-    _check(lib.dc_mx_attn_bf16(C.byref(a), _stream()))
+        new_k_ptr, new_v_ptr = _mx_dev(new_k, "new_k"), _mx_dev(new_v, "new_v")
+    elif new_k is not new_v:
+        raise DiffCacheError("new_k and new_v must be given together")
+    if workspace is not None:
+        ws_ptr, ws_bytes = _mx_dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
+    else:
+        ws_bytes = lib.dc_mx_attn_workspace_bytes(b * h, group, hd, n_rows)
+        if ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=_U8, device=dev)
+            ws_ptr = workspace.data_ptr()
+    args = _MX_ATTN.pack(_mx_dev(q, "q"), new_k_ptr, new_v_ptr, _mx_dev(out, "out"), lse_ptr, _mx_lens(lens, b), k.args, v.args,
+                         ws_ptr, ws_bytes, b, h, group, hd, n_rows, n_sink, window, hd ** -0.5 if scale is None else scale)
+    _check(lib.dc_mx_attn_bf16(args, _mx_stream(k)))
     return out if lse is None else (out, lse)

@@ -24,6 +24,7 @@ typedef uint32_t mx_u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t mx_u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kMostWaves = 8;  // of a block of the attention
 
 // A store as the kernels see it; strides in bytes.
 struct View {
@@ -260,7 +261,7 @@ __global__ __launch_bounds__(kThreads) void mx_gather_kernel(GatherArgs a, int h
 //
 // One token's attention, out = sum_r p_r v_r / sum_r p_r with p_r = exp(scale q k_r - m), over the rows of every sequence
 // (all of them, or its first n_sink and its last window).  A unit's rows are cut into steps of 16 TILES rows and its steps
-// into n_splits equal parts, a block each, whose waves take every fourth step; a wave keeps its running maximum, sum and
+// into n_splits equal parts, a block each, whose waves take every eighth step; a wave keeps its running maximum, sum and
 // weighted rows in registers, so the codes are read once and nothing is written but the parts' results.
 //
 //   S = K Q^T   v_mfma_f32_16x16x32_bf16 over 16 rows (M), 16 query heads (N) and 32 columns.  Lane (q, c) = (lane / 16,
@@ -284,7 +285,8 @@ struct AttnArgs {
     float *lse, *ws_acc, *ws_ml;
     const int32_t *lens;
     View k, v;
-    int n_h, group, cap, n_sink, window, n_splits;
+    int n_h, group, cap, n_sink, window, n_splits, waves;  // waves of a block
+    uint32_t per_split;  // 2^32 / n_splits, rounded up
     float scale;  // times log2(e)
 };
 
@@ -292,7 +294,7 @@ struct AttnArgs {
 struct Plan {
     int len, rows;            // rows before the token, and with it
     int sink, lo;             // rows [0, sink) and [lo, rows) are attended
-    int sink_steps, steps, per, used;
+    int sink_steps, steps, per;
 };
 template <int STEP>
 __device__ __forceinline__ Plan mx_plan(const AttnArgs &a, int b) {
@@ -306,9 +308,9 @@ __device__ __forceinline__ Plan mx_plan(const AttnArgs &a, int b) {
     if (a.window > 0 && (int64_t)a.n_sink + a.window < p.rows) p.sink = a.n_sink, p.lo = p.rows - a.window;
     p.sink_steps = (p.sink + STEP - 1) / STEP;
     p.steps = p.sink_steps + (int)(((int64_t)p.rows - p.lo + STEP - 1) / STEP);
-    p.per = (p.steps + a.n_splits - 1) / a.n_splits;
-    p.per = p.per < kWaves ? kWaves : p.per;
-    p.used = (p.steps + p.per - 1) / p.per;
+    // steps / n_splits, rounded up; now and then one more, which leaves a last part shorter
+    p.per = a.n_splits == 1 ? p.steps : (int)__umulhi((uint32_t)(p.steps + a.n_splits - 1), a.per_split);
+    p.per = p.per < a.waves ? a.waves : p.per;
     return p;
 }
 
@@ -316,28 +318,56 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const uint8_t *base, u
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, (int)bytes, 0x00020000);
 }
 
-// BYTES adjacent bytes at offset off
-template <int BYTES>
+// BYTES adjacent bytes at offset off.  AUX 2: read once (non-temporal)
+constexpr int kOnce = 2;
+template <int BYTES, int AUX>
 __device__ __forceinline__ void mx_load(__amdgpu_buffer_rsrc_t r, uint32_t off, uint32_t *dst) {
     if constexpr (BYTES == 1) {
-        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, 0);
+        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(r, (int)off, 0, AUX);
     } else if constexpr (BYTES == 2) {
-        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, 0);
+        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(r, (int)off, 0, AUX);
     } else if constexpr (BYTES == 4) {
-        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, 0);
+        dst[0] = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)off, 0, AUX);
     } else if constexpr (BYTES == 8) {
-        const mx_u32x2 t = __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, 0));
+        const mx_u32x2 t = __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, AUX));
         dst[0] = t.x, dst[1] = t.y;
     } else {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
-            const mx_u32x4 t = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 16 * i), 0, 0));
+            const mx_u32x4 t = __builtin_bit_cast(mx_u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)(off + 16 * i), 0, AUX));
             dst[4 * i] = t.x, dst[4 * i + 1] = t.y, dst[4 * i + 2] = t.z, dst[4 * i + 3] = t.w;
         }
     }
 }
 
 __device__ __forceinline__ uint32_t mx_pack_bf16(float lo, float hi) { return mx_bits(mx_bf16x2{(__bf16)lo, (__bf16)hi}); }
+
+// a over the lanes' halves in the low half, b over them in the high one
+__device__ __forceinline__ float mx_fold32(float a, float b) {
+    const mx_u32x2 r = __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false));
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+// a over the rows 0 and 1 (2 and 3) of 16 lanes in row 0 (2), b over them in row 1 (3)
+__device__ __forceinline__ float mx_fold16(float a, float b) {
+    const mx_u32x2 r = __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false));
+    return __uint_as_float(r.x) + __uint_as_float(r.y);
+}
+
+// f over the lanes whose number is the same modulo GP (4, 8 or 16), in every one of them
+template <int GP, typename F>
+__device__ __forceinline__ float mx_over_lanes(float x, F f) {
+    auto turned = [](float v, auto ctrl) __attribute__((always_inline)) {  // by 4 or 8 lanes of 16
+        return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    if constexpr (GP <= 4) x = f(x, turned(x, std::integral_constant<int, 0x124>{}));  // row_ror:4
+    if constexpr (GP <= 8) x = f(x, turned(x, std::integral_constant<int, 0x128>{}));  // row_ror:8
+    const uint32_t u = __float_as_uint(x);
+    const mx_u32x2 r = __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+    x = f(__uint_as_float(r.x), __uint_as_float(r.y));
+    const uint32_t w = __float_as_uint(x);
+    const mx_u32x2 s = __builtin_bit_cast(mx_u32x2, __builtin_amdgcn_permlane32_swap(w, w, false, false));
+    return f(__uint_as_float(s.x), __uint_as_float(s.y));
+}
 
 template <int HD, int KB, int VB, int GP, int TILES>
 struct Attn {
@@ -359,38 +389,41 @@ struct Attn {
 
     __device__ __forceinline__ void start(const AttnArgs &a, int unit, int lane) {
         q = lane >> 4, c = lane & 15;
-        const int head = c % GP;
+        const int head = c % GP < a.group ? c % GP : a.group - 1;  // (the last head again in the place of one that does not exist)
+        const uint16_t *src = a.q + ((int64_t)unit * a.group + head) * HD + q * (HD / 4);
 #pragma unroll
-        for (int j = 0; j < CH; ++j) {
-            bq[j] = mx_u32x4{0u, 0u, 0u, 0u};
-            if (head < a.group)
-                bq[j] = *reinterpret_cast<const mx_u32x4 *>(a.q + ((int64_t)unit * a.group + head) * HD + q * (HD / 4) + j * 8);
-        }
+        for (int j = 0; j < CH; ++j) bq[j] = *reinterpret_cast<const mx_u32x4 *>(src + j * 8);
 #pragma unroll
         for (int j = 0; j < EPL; ++j) acc[j] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
         m = -INFINITY, l = 0.f;
     }
 
-    // codes and scales of the rows [row, row + live) of a unit, live <= STEP
+    // Codes and scales of the rows [row, row + live) of a unit, live <= STEP.  A tile has buffers of its own, which the scalar
+    // unit moves along: one offset for all of them, and an end of their own.
     __device__ __forceinline__ void load_k(const View &k, const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
-        const uint32_t cr = (uint32_t)k.cr, sr = (uint32_t)k.sr;
-        const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * k.cr, (uint32_t)live * cr), rs = mx_rsrc(scale + row * k.sr, (uint32_t)live * sr);
+        const uint8_t *pc = codes + row * k.cr, *ps = scale + row * k.sr;
         const uint32_t r = 4u * (c & 3) + (c >> 2);
-        const uint32_t oc = r * cr + (uint32_t)q * KBYTES, os = r * sr + (uint32_t)(q * HD / 4 / 32);
+        const uint32_t oc = r * (uint32_t)k.cr + (uint32_t)q * KBYTES, os = r * (uint32_t)k.sr + (uint32_t)(q * HD / 4 / 32);
 #pragma unroll
         for (int t = 0; t < TILES; ++t) {
-            mx_load<KBYTES>(rc, oc + 16u * t * cr, kw[t]);
-            mx_load<KS>(rs, os + 16u * t * sr, &ks[t]);
+            const uint32_t rows = (uint32_t)(live > 16 * t ? live - 16 * t : 0);
+            mx_load<KBYTES, kOnce>(mx_rsrc(pc + 16 * t * k.cr, rows * (uint32_t)k.cr), oc, kw[t]);
+            mx_load<KS, 0>(mx_rsrc(ps + 16 * t * k.sr, rows * (uint32_t)k.sr), os, &ks[t]);
         }
     }
     __device__ __forceinline__ void load_v(const View &v, const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
+        const uint8_t *pc = codes + row * v.cr, *ps = scale + row * v.sr;
         const uint32_t cr = (uint32_t)v.cr, sr = (uint32_t)v.sr;
-        const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * v.cr, (uint32_t)live * cr), rs = mx_rsrc(scale + row * v.sr, (uint32_t)live * sr);
         const uint32_t oc = (uint32_t)q * cr + (uint32_t)c * VBYTES, os = (uint32_t)q * sr + (uint32_t)(c * EPL / 32);
 #pragma unroll
-        for (int t = 0; t < TILES * 4; ++t) {
-            mx_load<VBYTES>(rc, oc + 4u * t * cr, vw[t]);
-            mx_load<1>(rs, os + 4u * t * sr, &vs[t]);
+        for (int t = 0; t < TILES; ++t) {
+            const uint32_t rows = (uint32_t)(live > 16 * t ? live - 16 * t : 0);
+            const __amdgpu_buffer_rsrc_t rc = mx_rsrc(pc + 16 * t * v.cr, rows * cr), rs = mx_rsrc(ps + 16 * t * v.sr, rows * sr);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                mx_load<VBYTES, kOnce>(rc, oc + 4u * i * cr, vw[4 * t + i]);
+                mx_load<1, 0>(rs, os + 4u * i * sr, &vs[4 * t + i]);
+            }
         }
     }
 
@@ -425,29 +458,32 @@ struct Attn {
             const mx_f32x4 s = logits_of<T>();
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float y = s[i] * scale;
                 if constexpr (T % SETS == 0)
-                    x[T / SETS][i] = y;
+                    x[T / SETS][i] = s[i];
                 else
-                    x[T / SETS][i] = set >= T % SETS ? y : x[T / SETS][i];
+                    x[T / SETS][i] = set >= T % SETS ? s[i] : x[T / SETS][i];
             }
         });
+#pragma unroll
+        for (int r = 0; r < REGS; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[r][i] *= scale;
     }
 
     // a new maximum for every head, and what was summed so far brought to it
     __device__ __forceinline__ void raise(float most) {
+        const float to = fmaxf(m, mx_over_lanes<GP>(most, [](float a, float b) { return fmaxf(a, b); }));
+        if (__any(m > -INFINITY)) {
+            const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
+            l *= f;
 #pragma unroll
-        for (int d = GP; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d, 64));
-        const float to = fmaxf(m, most);
-        const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
-        m = to;
-        l *= f;
+            for (int i = 0; i < 4; ++i) {
+                const float g = __shfl(f, 4 * q + i, 64);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float g = __shfl(f, 4 * q + i, 64);
-#pragma unroll
-            for (int j = 0; j < EPL; ++j) acc[j][i] *= g;
+                for (int j = 0; j < EPL; ++j) acc[j][i] *= g;
+            }
         }
+        m = to;
     }
 
     // weights of the step: p from x; live < STEP where rows are missing
@@ -480,6 +516,32 @@ struct Attn {
         for (int r = 0; r < REGS; ++r)
 #pragma unroll
             for (int i = 0; i < 4; ++i) l += x[r][i];
+    }
+
+    // dst[head][column] = the wave's sums over all tiles: M row 4 q + i is head (4 q + i) % GP of a tile.  Rows of 16 lanes trade
+    // halves of what they hold, so that each ends with the sums of its own heads.
+    __device__ __forceinline__ void finish(float *dst, int G) const {
+        float o[GP / 4][EPL];  // the heads of this row of lanes
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) {
+            if constexpr (GP == 4) {
+                o[0][j] = mx_fold16(mx_fold32(acc[j][0], acc[j][2]), mx_fold32(acc[j][1], acc[j][3]));
+            } else if constexpr (GP == 8) {
+                o[0][j] = mx_fold32(acc[j][0], acc[j][2]), o[1][j] = mx_fold32(acc[j][1], acc[j][3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[i][j] = acc[j][i];
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < GP / 4; ++r) {
+            const int head = GP == 4 ? q : GP == 8 ? 4 * (q & 1) + (q >> 1) * 2 + r : 4 * q + r;
+            if (head < G) {
+#pragma unroll
+                for (int j = 0; j < EPL; j += 4)
+                    *reinterpret_cast<float4 *>(dst + head * HD + c * EPL + j) = make_float4(o[r][j], o[r][j + 1], o[r][j + 2], o[r][j + 3]);
+            }
+        }
     }
 
     // acc += P V over the step that load_v brought
@@ -522,21 +584,29 @@ struct Attn {
     }
 };
 
-inline size_t attn_shared_bytes(int hd, int group) { return (size_t)(2 * kWaves * 16 + kWaves * group * hd) * sizeof(float); }
+inline size_t attn_shared_bytes(int hd, int group, int waves) { return (size_t)waves * (32 + group * hd) * sizeof(float); }
 
 template <int HD, int KB, int VB, int GP, int TILES>
-__global__ __launch_bounds__(kThreads, 2) void mx_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a) {
     using T = Attn<HD, KB, VB, GP, TILES>;
     constexpr int STEP = T::STEP;
     extern __shared__ float s_dyn[];
-    float *s_m = s_dyn, *s_l = s_dyn + kWaves * 16, *s_acc = s_dyn + 2 * kWaves * 16;  // [wave][16], [wave][16], [wave][group * HD]
-    const int unit = blockIdx.x, split = dc_chunk(), tid = threadIdx.x, lane = tid & 63;
-    if (split >= a.n_splits) return;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int b = unit / a.n_h, h = unit % a.n_h, G = a.group;
+    // (all arguments at once: read where they are first used, they are half a dozen round trips in a row)
+    asm volatile("" ::"s"(a.q), "s"(a.new_k), "s"(a.lens), "s"(a.k.codes), "s"(a.k.scale), "s"(a.k.cb), "s"(a.k.ch), "s"(a.k.cr), "s"(a.k.sb),
+                 "s"(a.k.sh), "s"(a.k.sr), "s"(a.v.codes), "s"(a.v.scale), "s"(a.v.cb), "s"(a.v.ch), "s"(a.v.cr), "s"(a.v.sb), "s"(a.v.sh),
+                 "s"(a.v.sr), "s"(a.n_h), "s"(a.group), "s"(a.cap), "s"(a.n_sink), "s"(a.window), "s"(a.n_splits), "s"(a.waves));
+    const int waves = a.waves;
+    float *s_m = s_dyn, *s_l = s_dyn + waves * 16, *s_acc = s_dyn + 2 * waves * 16;  // [wave][16], [wave][16], [wave][group * HD]
+    const int b = blockIdx.x, h = blockIdx.y, split = blockIdx.z, unit = b * a.n_h + h, G = a.group;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    T w;
+    w.start(a, unit, lane);
     const Plan p = mx_plan<STEP>(a, b);
     const int begin = split * p.per, end = begin + p.per < p.steps ? begin + p.per : p.steps;
-    if (begin >= end && a.n_splits > 1) return;  // (the merge knows which parts there are)
+    if (begin >= end && a.n_splits > 1) {  // a part without rows: the merge takes nothing of it
+        if (tid < G) reinterpret_cast<float2 *>(a.ws_ml)[((int64_t)unit * a.n_splits + split) * G + tid] = make_float2(-INFINITY, 0.f);
+        return;
+    }
     const uint8_t *kc = a.k.codes + b * a.k.cb + h * a.k.ch, *ksc = a.k.scale + b * a.k.sb + h * a.k.sh;
     const uint8_t *vc = a.v.codes + b * a.v.cb + h * a.v.ch, *vsc = a.v.scale + b * a.v.sb + h * a.v.sh;
 
@@ -546,8 +616,6 @@ __global__ __launch_bounds__(kThreads, 2) void mx_attn_kernel(AttnArgs a) {
         __syncthreads();
     }
 
-    T w;
-    w.start(a, unit, lane);
     // step s: rows [row, row + live)
     auto place = [&](int s, int64_t &row, int &live) __attribute__((always_inline)) {
         const bool in_sink = s < p.sink_steps;
@@ -555,64 +623,57 @@ __global__ __launch_bounds__(kThreads, 2) void mx_attn_kernel(AttnArgs a) {
         const int64_t left = (in_sink ? p.sink : p.rows) - row;
         live = left < STEP ? (int)left : STEP;
     };
+    // a wave's steps are every waves-th of the block's, from a start of its block's own on
+    const int mine = end > begin + wave ? (end - begin - wave + waves - 1) / waves : 0;
+    const uint32_t turn = (uint32_t)(unit * a.n_splits + split) * 0x9e3779b9u;
+    int at = (int)(((uint64_t)turn * (uint32_t)mine) >> 32);
     int64_t row;
-    int live = 0, s = begin + wave;
-    if (s < end) {
-        place(s, row, live);
+    int live = 0;
+    if (mine > 0) {
+        place(begin + wave + at * waves, row, live);
         w.load_k(a.k, kc, ksc, row, live);
         w.load_v(a.v, vc, vsc, row, live);
     }
-    while (s < end) {
+    for (int i = 0; i < mine; ++i) {
         float x[T::REGS][4];
         w.logits(a.scale, x);
-        const int next = s + kWaves, now = live;
-        if (next < end) {
-            place(next, row, live);
+        const int now = live;
+        const bool more = i + 1 < mine;
+        if (more) {
+            at = at + 1 < mine ? at + 1 : 0;
+            place(begin + wave + at * waves, row, live);
             w.load_k(a.k, kc, ksc, row, live);
         }
         w.weigh(x, now);
         w.add(x);
-        if (next < end) w.load_v(a.v, vc, vsc, row, live);
-        s = next;
+        if (more) w.load_v(a.v, vc, vsc, row, live);
     }
 
     // the wave's heads: over the lanes that had other rows, and over the tiles
-    float l = w.l;
-#pragma unroll
-    for (int d = GP; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+    const float l = mx_over_lanes<GP>(w.l, [](float a, float b) { return a + b; });
     if (lane < GP) s_m[wave * 16 + lane] = w.m, s_l[wave * 16 + lane] = l;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        // M row 4 q + i is head (4 q + i) % GP of a tile
-        const int head = (4 * w.q + i) % GP;
-        float *dst = s_acc + (wave * G + head) * HD + w.c * T::EPL;
-        const bool mine = 4 * w.q + i < GP && head < G;
-#pragma unroll
-        for (int j = 0; j < T::EPL; ++j) {
-            float o = w.acc[j][i];
-#pragma unroll
-            for (int d = GP * 4; d < 64; d <<= 1) o += __shfl_xor(o, d, 64);
-            if (mine) dst[j] = o;
-        }
-    }
+    w.finish(s_acc + wave * G * HD, G);
     __syncthreads();
     auto weight = [](float m, float top) __attribute__((always_inline)) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f; };
-    auto top_of = [&](int head) __attribute__((always_inline)) {
-        float top = s_m[head];
-#pragma unroll
-        for (int i = 1; i < kWaves; ++i) top = fmaxf(top, s_m[i * 16 + head]);
-        return top;
-    };
     const int64_t slot = (int64_t)unit * a.n_splits + split;
-    for (int o = tid; o < G * HD; o += kThreads) {
+    for (int o = tid; o < G * HD; o += waves * 64) {
         const int head = o / HD;
-        const float top = top_of(head);
+        // (without a branch to a wave: the first one again in the place of those that a block of four does not have)
+        float m[kMostWaves], l[kMostWaves], part[kMostWaves];
+#pragma unroll
+        for (int i = 0; i < kMostWaves; ++i) {
+            const int at = i < waves ? i : 0;
+            m[i] = s_m[at * 16 + head], l[i] = s_l[at * 16 + head], part[i] = s_acc[at * G * HD + o];
+        }
+        float top = m[0];
+#pragma unroll
+        for (int i = 1; i < kMostWaves; ++i) top = fmaxf(top, m[i]);
         float sum = 0.f, total = 0.f;
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-            const float f = weight(s_m[i * 16 + head], top), li = s_l[i * 16 + head];
-            sum = fmaf(f, s_acc[i * G * HD + o], sum);
-            total += li == li ? f * li : li;  // (a sum that is no number stays none, whatever its maximum)
+        for (int i = 0; i < kMostWaves; ++i) {
+            const float f = i < waves ? weight(m[i], top) : 0.f;
+            sum = fmaf(f, i < waves ? part[i] : 0.f, sum);
+            total += i >= waves ? 0.f : l[i] == l[i] ? f * l[i] : l[i];  // (a sum that is no number stays none, whatever its maximum)
         }
         if (a.n_splits > 1) {
             a.ws_acc[slot * (G * HD) + o] = sum;
@@ -627,41 +688,61 @@ __global__ __launch_bounds__(kThreads, 2) void mx_attn_kernel(AttnArgs a) {
     }
 }
 
-// The parts of one query head joined: one block per (unit, head).
-template <int HD, int STEP>
+// The parts of one query head joined: one block per (unit, head).  What it reads is asked for at once, before any weight is
+// known: rounds of kBatch kParts parts (32 at 128 columns), HD / 4 threads to a part.
+constexpr int kBatch = 4;
+template <int HD>
 __global__ __launch_bounds__(kThreads) void mx_merge_kernel(AttnArgs a) {
     constexpr int kLanes = HD / 4, kParts = kThreads / kLanes;
     __shared__ float4 s_acc[kThreads];
-    const int unit = blockIdx.x / a.group, g = blockIdx.x % a.group, tid = threadIdx.x, lane = tid & 63;
-    const Plan p = mx_plan<STEP>(a, unit / a.n_h);
-    const int64_t slot0 = (int64_t)unit * a.n_splits;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0 * a.group + g;
-    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + (slot0 * a.group + g) * kLanes + tid % kLanes;
-    float top = -INFINITY;
-    for (int s = lane; s < p.used; s += 64) top = fmaxf(top, ml[(int64_t)s * a.group].x);
+    const int unit = blockIdx.x / a.group, g = blockIdx.x % a.group, tid = threadIdx.x, lane = tid & 63, n = a.n_splits;
+    const int64_t slot0 = (int64_t)unit * n * a.group + g;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0;
+    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + slot0 * kLanes + tid % kLanes;
+    float4 v[kBatch];
+    float2 o[kBatch];
+    auto load = [&](int s0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+        for (int i = 0; i < kBatch; ++i) {  // (the last part again where there are no more)
+            const int s = s0 + i * kParts, at = (s < n ? s : n - 1) * a.group;
+            o[i] = ml[at], v[i] = pa[(int64_t)at * kLanes];
+        }
+    };
+    const float2 own = lane < n ? ml[lane * a.group] : make_float2(-INFINITY, 0.f);
+    load(tid / kLanes);
+    float top = own.x;
+    for (int s = lane + 64; s < n; s += 64) top = fmaxf(top, ml[s * a.group].x);
+    top = mx_over_lanes<4>(top, [](float x, float y) { return fmaxf(x, y); });
+#pragma unroll
+    for (int d = 2; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
     auto weight = [&](float m) __attribute__((always_inline)) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f; };
-    float total = 0.f;
-    for (int s = lane; s < p.used; s += 64) {
-        const float2 o = ml[(int64_t)s * a.group];
-        total += o.y == o.y ? weight(o.x) * o.y : o.y;
-    }
+    auto share = [&](float2 x) __attribute__((always_inline)) { return x.y == x.y ? weight(x.x) * x.y : x.y; };
+    float total = share(own);
+    for (int s = lane + 64; s < n; s += 64) total += share(ml[s * a.group]);
+    total = mx_over_lanes<4>(total, [](float x, float y) { return x + y; });
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) total += __shfl_xor(total, d, 64);
+    for (int d = 2; d > 0; d >>= 1) total += __shfl_xor(total, d, 64);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = tid / kLanes; s < p.used; s += kParts) {
-        const float f = weight(ml[(int64_t)s * a.group].x);
-        const float4 v = pa[(int64_t)s * a.group * kLanes];
-        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    for (int s0 = tid / kLanes;;) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            // (a part without rows has no sums in the workspace)
+            const bool in = s0 + i * kParts < n && o[i].x > -INFINITY;
+            const float f = in ? weight(o[i].x) : 0.f;
+            acc.x = fmaf(f, in ? v[i].x : 0.f, acc.x), acc.y = fmaf(f, in ? v[i].y : 0.f, acc.y);
+            acc.z = fmaf(f, in ? v[i].z : 0.f, acc.z), acc.w = fmaf(f, in ? v[i].w : 0.f, acc.w);
+        }
+        s0 += kBatch * kParts;
+        if (s0 - tid / kLanes >= n) break;
+        load(s0);
     }
     s_acc[tid] = acc;
     __syncthreads();
     if (tid < HD) {
-        const float *v = reinterpret_cast<const float *>(s_acc) + tid;
-        float sum = v[0];
+        const float *x = reinterpret_cast<const float *>(s_acc) + tid;
+        float sum = x[0];
 #pragma unroll
-        for (int i = 1; i < kParts; ++i) sum += v[i * HD];
+        for (int i = 1; i < kParts; ++i) sum += x[i * HD];
         a.out[(int64_t)blockIdx.x * HD + tid] = dc_f32_to_bf16(total == 0.f ? 0.f : sum / total);
     }
     if (a.lse && tid == 0) a.lse[blockIdx.x] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f;
@@ -718,30 +799,35 @@ int check_grid(const char *who, int64_t n_units, int64_t chunks) {
         else hipLaunchKernelGGL((KERNEL<8, 8>), __VA_ARGS__);                                 \
     } while (0)
 
-// Blocks that the attention's splits come to, at most: two for a CU.
-constexpr int kBlocks = 512;
 constexpr int attn_tiles(int hd) { return hd == 256 ? 2 : 4; }
 
-// parts of a unit of up to n_rows attended rows that are worth a block: a step to each of its waves
-int64_t attn_parts(int hd, int64_t n_rows, int n_sink) {
+// How a unit's rows are dealt out.
+struct AttnCut {
+    int n_splits, waves;
+};
+constexpr int kBlocks = 512;  // of four waves, two to a CU
+constexpr int kAlone = 2;     // steps of a wave up to which a unit is one block of eight waves: less than a second kernel that joins parts
+constexpr int kWide = 8;
+AttnCut attn_cut(int64_t n_units, int hd, int64_t n_rows, int n_sink) {
     const int64_t step = 16 * attn_tiles(hd);
-    const int64_t steps = (n_rows + step - 1) / step + (n_sink > 0 ? (n_sink + step - 1) / step : 0);
-    const int64_t parts = (steps + kWaves - 1) / kWaves;
-    return parts > 0 ? parts : 1;
+    const int64_t steps = (n_rows + step - 1) / step + (n_sink + step - 1) / step;
+    if (steps <= kAlone * kWide) return {1, steps <= kWaves ? kWaves : kWide};
+    const int64_t parts = (steps + kWaves - 1) / kWaves, most = kBlocks / n_units > 1 ? kBlocks / n_units : 1;
+    return {(int)(parts < most ? parts : most), kWaves};
 }
 
 template <int HD, int KB, int VB>
 void launch_attn(const AttnArgs &a, int n_units, hipStream_t st) {
     constexpr int TILES = attn_tiles(HD);
-    const dim3 grid = dc_unit_grid(n_units, a.n_splits);
-    const size_t lds = attn_shared_bytes(HD, a.group);
-#define DC_LAUNCH_MX(GP) hipLaunchKernelGGL((mx_attn_kernel<HD, KB, VB, GP, TILES>), grid, dim3(kThreads), lds, st, a)
+    const dim3 grid((unsigned)(n_units / a.n_h), (unsigned)a.n_h, (unsigned)a.n_splits);
+    const size_t lds = attn_shared_bytes(HD, a.group, a.waves);
+#define DC_LAUNCH_MX(GP) hipLaunchKernelGGL((mx_attn_kernel<HD, KB, VB, GP, TILES>), grid, dim3(a.waves * 64), lds, st, a)
     if (a.group > 8) DC_LAUNCH_MX(16);
     else if (a.group > 4 || TILES == 2) DC_LAUNCH_MX(8);
     else if constexpr (TILES == 4) DC_LAUNCH_MX(4);
 #undef DC_LAUNCH_MX
     if (a.n_splits > 1)
-        hipLaunchKernelGGL((mx_merge_kernel<HD, 16 * TILES>), dim3((unsigned)(n_units * a.group)), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(mx_merge_kernel<HD>, dim3((unsigned)(n_units * a.group)), dim3(kThreads), 0, st, a);
 }
 
 template <int HD>
@@ -825,9 +911,12 @@ extern "C" int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v
 }
 
 extern "C" size_t dc_mx_attn_workspace_bytes(int n_units, int group, int hd, int n_rows) {
-    if (n_units <= 0 || group <= 0 || hd < 64 || n_rows < 0) return 256;
-    // (as many parts as the grid has blocks, or as there are: never less for more units or rows)
-    const int64_t parts = n_units * (attn_parts(hd, n_rows, 0) + 1);
+    if (n_units <= 0 || group <= 0 || hd < 64 || n_rows < 0) return 0;
+    // none where every unit is one block; else as many parts as the grid has blocks, or as there are: never less for more
+    // units or rows.  (Sinks may make one step more of the rows.)
+    const int64_t step = 16 * attn_tiles(hd), steps = (n_rows + step - 1) / step + 1;
+    if (steps <= kAlone * kWide) return 0;
+    const int64_t parts = n_units * ((steps + kWaves - 1) / kWaves);
     const size_t slots = (size_t)(parts < kBlocks ? parts : kBlocks);
     return dc_align_up(slots * group * hd * 4, 256) + dc_align_up(slots * group * 2 * 4, 256);
 }
@@ -847,12 +936,12 @@ extern "C" int dc_mx_attn_bf16(const dc_mx_attn_args *x, void *stream) {
     DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
     DC_REQUIRE(dc_aligned16(x->q) && (!x->new_k || (dc_aligned16(x->new_k) && dc_aligned16(x->new_v))),
                "%s: pointers must be 16-byte aligned", who);
-    DC_REQUIRE((int64_t)n_units * x->group < (1ll << 31), "%s: grid too large", who);
+    DC_REQUIRE(x->n_h < (1 << 16), "%s: too many heads", who);
     const int64_t attended = x->window > 0 && (int64_t)x->n_sink + x->window < x->n_rows ? x->window : x->n_rows;
-    const int64_t parts = attn_parts(x->hd, attended, attended < x->n_rows ? x->n_sink : 0);
-    const int64_t most = kBlocks / n_units > 1 ? kBlocks / n_units : 1;
+    const AttnCut cut = attn_cut(n_units, x->hd, attended, attended < x->n_rows ? x->n_sink : 0);
     AttnArgs a;
-    a.n_splits = (int)(parts < most ? parts : most);
+    a.n_splits = cut.n_splits, a.waves = cut.waves;
+    a.per_split = (uint32_t)((0xffffffffull + a.n_splits) / a.n_splits);
     if (a.n_splits > 1) {
         const size_t slots = (size_t)n_units * a.n_splits;
         const size_t acc_bytes = dc_align_up(slots * x->group * x->hd * 4, 256), need = acc_bytes + dc_align_up(slots * x->group * 2 * 4, 256);

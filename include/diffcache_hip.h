@@ -691,7 +691,7 @@ int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v, const uin
  *   lse      NULL, or (n_b, n_h * group) fp32: log of the sum of exp(scale q k^T)
  * A sequence without rows has out 0 and lse -inf.  Rows that are not attended to may hold anything; one that is and holds a NaN
  * makes its unit's outputs NaN.  group: up to 16 query heads.  Sums and statistics are fp32.  The workspace
- * (dc_mx_attn_workspace_bytes, 256-byte aligned; enough for more units or rows is enough for fewer) holds nothing between calls;
+ * (dc_mx_attn_workspace_bytes, 256-byte aligned; 0: none; enough for more units or rows is enough for fewer) holds nothing between calls;
  * calls that may overlap need one each.  Replaces flash_attn_with_kvcache (base.py:134-142) over such a cache.
  */
 typedef struct dc_mx_attn_args {

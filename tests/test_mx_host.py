@@ -1,5 +1,5 @@
 """The block-scaled cache without a GPU: the plain form's own properties, struct layouts, and every refusal."""
-import ctypes as C
+import ctypes
 import os
 import re
 
@@ -50,6 +50,18 @@ def test_structs_match_the_header(name, cls):
     names = [re.sub(r"[^A-Za-z0-9_]", "", n.split()[-1]) for decl in body.split(";") if decl.strip()
              for n in decl.replace("*", " ").split(",")]
     assert names == [n for n, _ in cls._fields_]
+    packed = hip._MX_STORE if cls is hip.MxStoreArgs else hip._MX_ATTN
+    assert packed.size == ctypes.sizeof(cls)
+
+
+def test_packed_bytes_are_the_structs():
+    store = hip._MX_STORE.pack(*range(1, 9), 4, 99)
+    assert store == bytes(hip.MxStoreArgs(*range(1, 9), 4, 99))
+    other = hip._MX_STORE.pack(*range(11, 19), 8, 98)
+    args = hip._MX_ATTN.pack(*range(21, 27), store, other, 31, 32, *range(41, 48), 0.25)
+    want = hip.MxAttnArgs(*range(21, 27), hip.MxStoreArgs.from_buffer_copy(store), hip.MxStoreArgs.from_buffer_copy(other), 31,
+                          32, *range(41, 48), 0.25)
+    assert args == bytes(want)
 
 
 def fake(bits=4, n_rows=64, hd=128, **more):
@@ -59,6 +71,11 @@ def fake(bits=4, n_rows=64, hd=128, **more):
     for name, x in more.items():
         setattr(s, name, x)
     return s
+
+
+def ref_of(x):
+    """A struct as the library's calls take it."""
+    return bytes(x)
 
 
 def refused(rc, message):
@@ -79,11 +96,11 @@ def test_bad_stores_are_refused_everywhere(change, message):
     good, bad = fake(), fake(**change)
     p = 1 << 22
     for k, v in ((good, bad), (bad, good)):
-        refused(hip.lib.dc_mx_ingest_bf16(C.byref(k), C.byref(v), p, p, None, 2, 8, 2, 128, 0, *[1024] * 6, None), message)
-        refused(hip.lib.dc_mx_append_bf16(C.byref(k), C.byref(v), p, p, p, 2, 2, 128, None), message)
-        refused(hip.lib.dc_mx_gather_rows_bf16(C.byref(k), C.byref(v), None, p, p, 2, 2, 8, 0, 128, 0, 1024, 1024, 128, None), message)
+        refused(hip.lib.dc_mx_ingest_bf16(ref_of(k), ref_of(v), p, p, None, 2, 8, 2, 128, 0, *[1024] * 6, None), message)
+        refused(hip.lib.dc_mx_append_bf16(ref_of(k), ref_of(v), p, p, p, 2, 2, 128, None), message)
+        refused(hip.lib.dc_mx_gather_rows_bf16(ref_of(k), ref_of(v), None, p, p, 2, 2, 8, 0, 128, 0, 1024, 1024, 128, None), message)
         a = attn_args(k=k, v=v)
-        refused(hip.lib.dc_mx_attn_bf16(C.byref(a), None), message)
+        refused(hip.lib.dc_mx_attn_bf16(ref_of(a), None), message)
 
 
 def attn_args(**change):
@@ -106,12 +123,12 @@ def attn_args(**change):
 ])
 def test_bad_attention_is_refused(change, message):
     a = attn_args(**change)
-    refused(hip.lib.dc_mx_attn_bf16(C.byref(a), None), message)
+    refused(hip.lib.dc_mx_attn_bf16(ref_of(a), None), message)
 
 
 def test_a_small_workspace_is_refused():
     a = attn_args(k=fake(n_rows=4096), v=fake(n_rows=4096), n_rows=4096, workspace_bytes=1024)
-    assert hip.lib.dc_mx_attn_bf16(C.byref(a), None) == -12
+    assert hip.lib.dc_mx_attn_bf16(ref_of(a), None) == -12
     assert "needed" in hip.lib.dc_last_error().decode()
     refused(hip.lib.dc_mx_attn_bf16(None, None), "null")
 
@@ -123,12 +140,12 @@ def test_enough_workspace_for_more_is_enough_for_fewer():
             sizes = [hip.mx_attn_workspace_bytes(units, 4, hd, n) for n in (0, 1, 64, 65, 1000, 100000, 2**31 - 1)]
             assert sizes == sorted(sizes) and sizes[-1] >= last
             last = sizes[-1]
-    assert hip.mx_attn_workspace_bytes(0, 4, 128, 100) == hip.mx_attn_workspace_bytes(4, 4, 128, -1) == 256
+    assert hip.mx_attn_workspace_bytes(0, 4, 128, 100) == hip.mx_attn_workspace_bytes(4, 4, 128, -1) == 0
 
 
 def test_bad_rows_are_refused():
     s, p = fake(), 1 << 22
-    call = lambda **c: hip.lib.dc_mx_ingest_bf16(*{**dict(k=C.byref(s), v=C.byref(s), ks=p, vs=p, lens=None, b=2, seq=8, h=2, hd=128, at=0, s0=1024, s1=1024,  # noqa: E731
+    call = lambda **c: hip.lib.dc_mx_ingest_bf16(*{**dict(k=ref_of(s), v=ref_of(s), ks=p, vs=p, lens=None, b=2, seq=8, h=2, hd=128, at=0, s0=1024, s1=1024,  # noqa: E731
                                                           s2=1024, s3=1024, s4=1024, s5=1024, st=None), **c}.values())
     refused(call(k=None), "null")
     refused(call(ks=None), "null")
@@ -140,7 +157,7 @@ def test_bad_rows_are_refused():
     refused(call(s5=4), "multiples of 8")
     refused(call(hd=32), "head_dim")
     assert call(seq=0) == 0 and call(b=0) == 0
-    call = lambda **c: hip.lib.dc_mx_gather_rows_bf16(*{**dict(k=C.byref(s), v=C.byref(s), idx=None, ok=p, ov=p, b=2, h=2, n=8, ist=8, hd=128, off=0,  # noqa: E731
+    call = lambda **c: hip.lib.dc_mx_gather_rows_bf16(*{**dict(k=ref_of(s), v=ref_of(s), idx=None, ok=p, ov=p, b=2, h=2, n=8, ist=8, hd=128, off=0,  # noqa: E731
                                                                d0=1024, d1=1024, d2=128, st=None), **c}.values())
     refused(call(ok=None, ov=None), "null")
     refused(call(k=None), "source missing")
@@ -150,8 +167,8 @@ def test_bad_rows_are_refused():
     refused(call(off=-1), "bad sizes")
     refused(call(n=-1), "bad sizes")
     assert call(n=0) == 0 and call(b=0) == 0
-    refused(hip.lib.dc_mx_append_bf16(C.byref(s), C.byref(s), p, p, None, 2, 2, 128, None), "null")
-    refused(hip.lib.dc_mx_append_bf16(C.byref(s), C.byref(s), p + 8, p, p, 2, 2, 128, None), "aligned")
+    refused(hip.lib.dc_mx_append_bf16(ref_of(s), ref_of(s), p, p, None, 2, 2, 128, None), "null")
+    refused(hip.lib.dc_mx_append_bf16(ref_of(s), ref_of(s), p + 8, p, p, 2, 2, 128, None), "aligned")
 
 
 def test_wrappers_refuse_what_does_not_fit():
