@@ -610,12 +610,6 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
     const uint8_t *kc = a.k.codes + b * a.k.cb + h * a.k.ch, *ksc = a.k.scale + b * a.k.sb + h * a.k.sh;
     const uint8_t *vc = a.v.codes + b * a.v.cb + h * a.v.ch, *vsc = a.v.scale + b * a.v.sb + h * a.v.sh;
 
-    // The token's row is the unit's last: the block that attends to it writes it, and reads it when all its waves see it.
-    if (p.rows > p.len && end == p.steps) {
-        if (wave == 0) mx_write_token<KB, VB>(a.k, a.v, a.new_k, a.new_v, HD, unit, b, h, p.len, lane);
-        __syncthreads();
-    }
-
     // step s: rows [row, row + live)
     auto place = [&](int s, int64_t &row, int &live) __attribute__((always_inline)) {
         const bool in_sink = s < p.sink_steps;
@@ -626,12 +620,20 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
     // a wave's steps are every waves-th of the block's, from a start of its block's own on
     const int mine = end > begin + wave ? (end - begin - wave + waves - 1) / waves : 0;
     const uint32_t turn = (uint32_t)(unit * a.n_splits + split) * 0x9e3779b9u;
-    int at = (int)(((uint64_t)turn * (uint32_t)mine) >> 32);
+    // The token's row is the unit's last: the wave with the last step writes it first and takes that step last, token or not (so
+    // that a row written beforehand gives the same sums).
+    const bool last = mine > 0 && begin + wave + (mine - 1) * waves == p.steps - 1, writes = last && p.rows > p.len;
+    int at = last ? 0 : (int)(((uint64_t)turn * (uint32_t)mine) >> 32);
+    if (writes) mx_write_token<KB, VB>(a.k, a.v, a.new_k, a.new_v, HD, unit, b, h, p.len, lane);
     int64_t row;
     int live = 0;
-    if (mine > 0) {
+    auto load_k = [&]() __attribute__((always_inline)) {
+        if (writes && at == mine - 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // (its lanes see each other's stores)
         place(begin + wave + at * waves, row, live);
         w.load_k(a.k, kc, ksc, row, live);
+    };
+    if (mine > 0) {
+        load_k();
         w.load_v(a.v, vc, vsc, row, live);
     }
     for (int i = 0; i < mine; ++i) {
@@ -641,8 +643,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
         const bool more = i + 1 < mine;
         if (more) {
             at = at + 1 < mine ? at + 1 : 0;
-            place(begin + wave + at * waves, row, live);
-            w.load_k(a.k, kc, ksc, row, live);
+            load_k();
         }
         w.weigh(x, now);
         w.add(x);
@@ -806,7 +807,7 @@ struct AttnCut {
     int n_splits, waves;
 };
 constexpr int kBlocks = 512;  // of four waves, two to a CU
-constexpr int kAlone = 2;     // steps of a wave up to which a unit is one block of eight waves: less than a second kernel that joins parts
+constexpr int kAlone = 3;     // steps of a wave up to which a unit is one block of eight waves: less than a second kernel that joins parts
 constexpr int kWide = 8;
 AttnCut attn_cut(int64_t n_units, int hd, int64_t n_rows, int n_sink) {
     const int64_t step = 16 * attn_tiles(hd);
