@@ -97,8 +97,8 @@ class MxStoreArgs(C.Structure):
     """struct dc_mx_store of include/diffcache_hip.h"""
     _fields_ = [
         ("codes", C.c_void_p), ("scale", C.c_void_p),
-        ("code_batch_stride", C.c_int64), ("code_head_stride", C.c_int64), ("code_row_stride", C.c_int64),
-        ("scale_batch_stride", C.c_int64), ("scale_head_stride", C.c_int64), ("scale_row_stride", C.c_int64),
+        ("code_batch_stride", C.c_int64), ("code_head_stride", C.c_int64),
+        ("scale_batch_stride", C.c_int64), ("scale_head_stride", C.c_int64),
         ("bits", C.c_int), ("n_rows", C.c_int),
     ]
 
@@ -1008,7 +1008,7 @@ def compose_idx(outer: torch.Tensor, inner: torch.Tensor) -> torch.Tensor:
 
 # The two structs' bytes.  (A call of these wrappers costs a few microseconds, as much as the kernels of a short context:
 # every attribute is read once and every tensor made in the cheapest way.)
-_MX_STORE = struct.Struct("@2P6q2i")
+_MX_STORE = struct.Struct("@2P4q2i")
 _MX_ATTN = struct.Struct("@6P%ds%dsPN7if" % (_MX_STORE.size, _MX_STORE.size))
 _device = torch._C._cuda_getDevice
 _U8, _BF16, _F32, _I32 = torch.uint8, torch.bfloat16, torch.float32, torch.int32
@@ -1026,8 +1026,8 @@ def _mx_dev(t: torch.Tensor, name: str) -> int:
 
 class MxStore:
     """K or V of a layer, held in 4 or 8 bits with a power of two for every 32 numbers (dc_mx_store in the header):
-    ``codes`` (b, h, n, hd * bits / 8) and ``scale`` (b, h, n, hd / 32), both uint8 with contiguous rows.  Views of larger
-    tensors will do; ``MxStore.zeros`` makes a store of its own, whose rows read as zeros until they are written."""
+    ``codes`` (b, h, n, hd * bits / 8) and ``scale`` (b, h, n, hd / 32), both uint8, a unit's rows one after another.  Views of
+    larger tensors will do; ``MxStore.zeros`` makes a store of its own, whose rows read as zeros until they are written."""
 
     __slots__ = ("codes", "scale", "shape", "units", "hd", "bits", "args")
 
@@ -1044,11 +1044,11 @@ class MxStore:
             raise DiffCacheError(f"rows of {row} code bytes and {blocks} scales are neither 4 nor 8 bits to a number")
         cb, ch, cr, c1 = codes.stride()
         sb, sh, sr, s1 = scale.stride()
-        if c1 != 1 or (s1 != 1 and blocks > 1):
-            raise DiffCacheError("the rows of codes and scale must be contiguous")
+        if c1 != 1 or (s1 != 1 and blocks > 1) or (n > 1 and (cr != row or sr != blocks)):
+            raise DiffCacheError("a unit's rows must lie one after another in codes and in scale")
         self.codes, self.scale = codes, scale
         self.shape, self.units, self.hd, self.bits = (b, h, n, hd), (b, h, hd), hd, bits
-        self.args = _MX_STORE.pack(_mx_dev(codes, "codes"), _mx_dev(scale, "scale"), cb, ch, cr, sb, sh, sr, bits, n)
+        self.args = _MX_STORE.pack(_mx_dev(codes, "codes"), _mx_dev(scale, "scale"), cb, ch, sb, sh, bits, n)
 
     @classmethod
     def zeros(cls, b: int, h: int, n: int, hd: int, bits: int, device) -> "MxStore":

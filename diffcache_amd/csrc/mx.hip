@@ -29,11 +29,10 @@ constexpr int kMostWaves = 8;  // of a block of the attention
 // A store as the kernels see it; strides in bytes.
 struct View {
     uint8_t *codes, *scale;
-    int64_t cb, ch, cr, sb, sh, sr;
+    int64_t cb, ch, sb, sh;
 };
 inline View view_of(const dc_mx_store &s) {
-    return {(uint8_t *)s.codes,   (uint8_t *)s.scale,   s.code_batch_stride, s.code_head_stride,
-            s.code_row_stride, s.scale_batch_stride, s.scale_head_stride, s.scale_row_stride};
+    return {(uint8_t *)s.codes, (uint8_t *)s.scale, s.code_batch_stride, s.code_head_stride, s.scale_batch_stride, s.scale_head_stride};
 }
 
 // ---- the format -----------------------------------------------------------------------------------------------------
@@ -151,7 +150,7 @@ __device__ __forceinline__ void mx_ingest_rows(const View &st, const uint16_t *s
         const int r = r0 + i * rows_per;
         const Coded<BITS> c = mx_quantise<BITS>(x[i]);  // (the four lanes of a quad hold one row's: all or none store)
         const int64_t at = (int64_t)a.dst_pos + r;
-        if (r < live) mx_store_piece<BITS>(codes + at * st.cr, scale + at * st.sr, p, c);
+        if (r < live) mx_store_piece<BITS>(codes + at * (ppr * BITS), scale + at * (ppr / 4), p, c);
     }
 }
 
@@ -177,11 +176,11 @@ __device__ __forceinline__ void mx_write_token(const View &k, const View &v, con
     const int ppr = hd / 8;
     if (lane < ppr) {
         const Coded<KB> c = mx_quantise<KB>(*reinterpret_cast<const uint4 *>(new_k + (int64_t)unit * hd + lane * 8));
-        mx_store_piece<KB>(k.codes + b * k.cb + h * k.ch + at * k.cr, k.scale + b * k.sb + h * k.sh + at * k.sr, lane, c);
+        mx_store_piece<KB>(k.codes + b * k.cb + h * k.ch + at * (ppr * KB), k.scale + b * k.sb + h * k.sh + at * (ppr / 4), lane, c);
     } else if (lane < 2 * ppr) {
         const int p = lane - ppr;
         const Coded<VB> c = mx_quantise<VB>(*reinterpret_cast<const uint4 *>(new_v + (int64_t)unit * hd + p * 8));
-        mx_store_piece<VB>(v.codes + b * v.cb + h * v.ch + at * v.cr, v.scale + b * v.sb + h * v.sh + at * v.sr, p, c);
+        mx_store_piece<VB>(v.codes + b * v.cb + h * v.ch + at * (ppr * VB), v.scale + b * v.sb + h * v.sh + at * (ppr / 4), p, c);
     }
 }
 
@@ -228,14 +227,14 @@ __device__ __forceinline__ void mx_gather(const View &st, uint16_t *out, int n_r
 #pragma unroll
         for (int t = 0; t < BITS / 4; ++t) w[i][t] = 0u;
         if (row[i] >= 0) {
-            const uint8_t *src = codes + row[i] * st.cr + p * BITS;
+            const uint8_t *src = codes + row[i] * (ppr * BITS) + p * BITS;
             if constexpr (BITS == 4) {
                 w[i][0] = *reinterpret_cast<const uint32_t *>(src);
             } else {
                 const uint2 t = *reinterpret_cast<const uint2 *>(src);
                 w[i][0] = t.x, w[i][1] = t.y;
             }
-            s[i] = scale[row[i] * st.sr + p / 4];
+            s[i] = scale[row[i] * (ppr / 4) + p / 4];
         }
     }
     uint16_t *dst = out + b * a.db + h * a.dh + p * 8;
@@ -277,8 +276,10 @@ __global__ __launch_bounds__(kThreads) void mx_gather_kernel(GatherArgs a, int h
 //               adjacent codes of its own rows.
 //
 // Which row of a tile is which row of M is free as long as K and V agree: M row 4 q + i is the tile's row 4 i + q, so that
-// every load takes whole runs of rows.  Rows behind the end are not asked for: a step's buffers end at its last row, and loads
-// past a buffer's end give zeros.
+// every load takes whole runs of rows (with row 4 q + i, lines are asked for in pieces, which non-temporal loads do not
+// find in the nearest cache: 2.4 times the requests of the next, 183 us for 177 at 8 x 131072 tokens).
+// Rows behind the end are not asked for: a step's buffers end at its last row, and what a load asks of the words past a buffer's
+// end is zero.
 struct AttnArgs {
     const uint16_t *q, *new_k, *new_v;
     uint16_t *out;
@@ -316,6 +317,13 @@ __device__ __forceinline__ Plan mx_plan(const AttnArgs &a, int b) {
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const uint8_t *base, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, (int)bytes, 0x00020000);
+}
+
+// An offset whose bits the compiler does not know: it would make an or of a constant added to it, which the loads cannot take
+// into their own constant, and spend a register and an instruction on every one of them.
+__device__ __forceinline__ uint32_t mx_opaque(int x) {
+    asm("" : "+v"(x));
+    return (uint32_t)x;
 }
 
 // BYTES adjacent bytes at offset off.  AUX 2: read once (non-temporal)
@@ -374,14 +382,17 @@ struct Attn {
     static constexpr int STEP = 16 * TILES;
     static constexpr int CH = HD / 32;          // products of a tile's S; blocks of a row
     static constexpr int EPL = HD / 16;         // columns of V of a lane
-    static constexpr int KBYTES = HD / 4 * KB / 8, KW = KBYTES / 4;
+    // K: KN loads of KBYTES, those of a row's four lanes side by side; a load is KCOLS columns, in KS blocks a lane has a part of
+    static constexpr int KCOLS = HD == 64 ? 16 : 128 / KB, KN = HD / 4 / KCOLS, KBYTES = KCOLS * KB / 8, KW = KN * KBYTES / 4;
+    static constexpr int kcol(int j) { return j * 8 / KCOLS * 4 * KCOLS + j * 8 % KCOLS; }  // first column of chunk j, of lanes q = 0
     static constexpr int VBYTES = EPL * VB / 8, VW = VBYTES < 4 ? 1 : VBYTES / 4;
+    static constexpr int KROW = HD * KB / 8, VROW = HD * VB / 8;
     static constexpr int SETS = 16 / GP < TILES ? 16 / GP : TILES;  // tiles whose logits share a register
     static constexpr int REGS = TILES / SETS;   // logit registers of a lane (times 4)
-    static constexpr int KS = HD == 256 ? 2 : 1;  // blocks of a lane's columns of K
+    static constexpr int KS = KN;
 
     mx_u32x4 bq[CH];
-    uint32_t kw[TILES][KW], ks[TILES];
+    uint32_t kw[TILES][KW], ks[TILES][KS];
     uint32_t vw[TILES * 4][VW], vs[TILES * 4];
     mx_f32x4 acc[EPL];
     float m, l;
@@ -390,40 +401,35 @@ struct Attn {
     __device__ __forceinline__ void start(const AttnArgs &a, int unit, int lane) {
         q = lane >> 4, c = lane & 15;
         const int head = c % GP < a.group ? c % GP : a.group - 1;  // (the last head again in the place of one that does not exist)
-        const uint16_t *src = a.q + ((int64_t)unit * a.group + head) * HD + q * (HD / 4);
+        const uint16_t *src = a.q + ((int64_t)unit * a.group + head) * HD + q * KCOLS;
 #pragma unroll
-        for (int j = 0; j < CH; ++j) bq[j] = *reinterpret_cast<const mx_u32x4 *>(src + j * 8);
+        for (int j = 0; j < CH; ++j) bq[j] = *reinterpret_cast<const mx_u32x4 *>(src + kcol(j));
 #pragma unroll
         for (int j = 0; j < EPL; ++j) acc[j] = mx_f32x4{0.f, 0.f, 0.f, 0.f};
         m = -INFINITY, l = 0.f;
     }
 
-    // Codes and scales of the rows [row, row + live) of a unit, live <= STEP.  A tile has buffers of its own, which the scalar
-    // unit moves along: one offset for all of them, and an end of their own.
-    __device__ __forceinline__ void load_k(const View &k, const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
-        const uint8_t *pc = codes + row * k.cr, *ps = scale + row * k.sr;
-        const uint32_t r = 4u * (c & 3) + (c >> 2);
-        const uint32_t oc = r * (uint32_t)k.cr + (uint32_t)q * KBYTES, os = r * (uint32_t)k.sr + (uint32_t)(q * HD / 4 / 32);
+    // Codes and scales of the rows [row, row + live) of a unit, live <= STEP; lane (q, c) has row 4 (c % 4) + c / 4 of every tile.
+    __device__ __forceinline__ void load_k(const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
+        const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * KROW, (uint32_t)live * KROW), rs = mx_rsrc(scale + row * CH, (uint32_t)live * CH);
+        const int r = 4 * (c & 3) + (c >> 2);
+        const uint32_t oc = mx_opaque(r * KROW + q * KBYTES), os = mx_opaque(r * CH + q * KCOLS / 32);
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const uint32_t rows = (uint32_t)(live > 16 * t ? live - 16 * t : 0);
-            mx_load<KBYTES, kOnce>(mx_rsrc(pc + 16 * t * k.cr, rows * (uint32_t)k.cr), oc, kw[t]);
-            mx_load<KS, 0>(mx_rsrc(ps + 16 * t * k.sr, rows * (uint32_t)k.sr), os, &ks[t]);
-        }
-    }
-    __device__ __forceinline__ void load_v(const View &v, const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
-        const uint8_t *pc = codes + row * v.cr, *ps = scale + row * v.sr;
-        const uint32_t cr = (uint32_t)v.cr, sr = (uint32_t)v.sr;
-        const uint32_t oc = (uint32_t)q * cr + (uint32_t)c * VBYTES, os = (uint32_t)q * sr + (uint32_t)(c * EPL / 32);
+        for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            const uint32_t rows = (uint32_t)(live > 16 * t ? live - 16 * t : 0);
-            const __amdgpu_buffer_rsrc_t rc = mx_rsrc(pc + 16 * t * v.cr, rows * cr), rs = mx_rsrc(ps + 16 * t * v.sr, rows * sr);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                mx_load<VBYTES, kOnce>(rc, oc + 4u * i * cr, vw[4 * t + i]);
-                mx_load<1, 0>(rs, os + 4u * i * sr, &vs[4 * t + i]);
+            for (int n = 0; n < KN; ++n) {
+                mx_load<KBYTES, kOnce>(rc, oc + 16 * KROW * t + 4 * KBYTES * n, &kw[t][KBYTES / 4 * n]);
+                mx_load<1, 0>(rs, os + 16 * CH * t + 4 * KCOLS / 32 * n, &ks[t][n]);
             }
+    }
+    // lane (q, c) has columns EPL c .. of the rows 4 i + q of every tile
+    __device__ __forceinline__ void load_v(const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
+        const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * VROW, (uint32_t)live * VROW), rs = mx_rsrc(scale + row * CH, (uint32_t)live * CH);
+        const uint32_t oc = mx_opaque(q * VROW + c * VBYTES), os = mx_opaque(q * CH + c * EPL / 32);
+#pragma unroll
+        for (int t = 0; t < TILES * 4; ++t) {
+            mx_load<VBYTES, kOnce>(rc, oc + 4 * VROW * t, vw[t]);
+            mx_load<1, 0>(rs, os + 4 * CH * t, &vs[t]);
         }
     }
 
@@ -432,7 +438,7 @@ struct Attn {
         mx_f32x4 s = {0.f, 0.f, 0.f, 0.f};
         auto chunk = [&](auto jj) __attribute__((always_inline)) {
             constexpr int J = decltype(jj)::value;
-            const float f = mx_scale(KS == 1 ? ks[T] : (J < CH / 2 ? ks[T] & 0xffu : ks[T] >> 8));
+            const float f = mx_scale(ks[T][J * 8 / KCOLS]);
             const mx_u32x4 x = {mx_pair<KB, 4 * J>(kw[T], f), mx_pair<KB, 4 * J + 1>(kw[T], f), mx_pair<KB, 4 * J + 2>(kw[T], f),
                                 mx_pair<KB, 4 * J + 3>(kw[T], f)};
             s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, x), __builtin_bit_cast(mx_bf16x8, bq[J]), s, 0, 0, 0);
@@ -592,9 +598,9 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
     constexpr int STEP = T::STEP;
     extern __shared__ float s_dyn[];
     // (all arguments at once: read where they are first used, they are half a dozen round trips in a row)
-    asm volatile("" ::"s"(a.q), "s"(a.new_k), "s"(a.lens), "s"(a.k.codes), "s"(a.k.scale), "s"(a.k.cb), "s"(a.k.ch), "s"(a.k.cr), "s"(a.k.sb),
-                 "s"(a.k.sh), "s"(a.k.sr), "s"(a.v.codes), "s"(a.v.scale), "s"(a.v.cb), "s"(a.v.ch), "s"(a.v.cr), "s"(a.v.sb), "s"(a.v.sh),
-                 "s"(a.v.sr), "s"(a.n_h), "s"(a.group), "s"(a.cap), "s"(a.n_sink), "s"(a.window), "s"(a.n_splits), "s"(a.waves));
+    asm volatile("" ::"s"(a.q), "s"(a.new_k), "s"(a.lens), "s"(a.k.codes), "s"(a.k.scale), "s"(a.k.cb), "s"(a.k.ch), "s"(a.k.sb),
+                 "s"(a.k.sh), "s"(a.v.codes), "s"(a.v.scale), "s"(a.v.cb), "s"(a.v.ch), "s"(a.v.sb), "s"(a.v.sh),
+                 "s"(a.n_h), "s"(a.group), "s"(a.cap), "s"(a.n_sink), "s"(a.window), "s"(a.n_splits), "s"(a.waves));
     const int waves = a.waves;
     float *s_m = s_dyn, *s_l = s_dyn + waves * 16, *s_acc = s_dyn + 2 * waves * 16;  // [wave][16], [wave][16], [wave][group * HD]
     const int b = blockIdx.x, h = blockIdx.y, split = blockIdx.z, unit = b * a.n_h + h, G = a.group;
@@ -630,11 +636,11 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
     auto load_k = [&]() __attribute__((always_inline)) {
         if (writes && at == mine - 1) __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");  // (its lanes see each other's stores)
         place(begin + wave + at * waves, row, live);
-        w.load_k(a.k, kc, ksc, row, live);
+        w.load_k(kc, ksc, row, live);
     };
     if (mine > 0) {
         load_k();
-        w.load_v(a.v, vc, vsc, row, live);
+        w.load_v(vc, vsc, row, live);
     }
     for (int i = 0; i < mine; ++i) {
         float x[T::REGS][4];
@@ -647,7 +653,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
         }
         w.weigh(x, now);
         w.add(x);
-        if (more) w.load_v(a.v, vc, vsc, row, live);
+        if (more) w.load_v(vc, vsc, row, live);
     }
 
     // the wave's heads: over the lanes that had other rows, and over the tiles
@@ -755,14 +761,11 @@ int check_store(const char *who, const char *which, const dc_mx_store &s, int n_
     DC_REQUIRE(s.bits == 4 || s.bits == 8, "%s: %s holds %d bits, not 4 or 8", who, which, s.bits);
     DC_REQUIRE(s.n_rows >= 0, "%s: %s has a negative number of rows", who, which);
     DC_REQUIRE((s.codes && s.scale) || s.n_rows == 0, "%s: null pointer in %s", who, which);
-    const int64_t row = (int64_t)hd * s.bits / 8, blocks = hd / 32;
-    DC_REQUIRE(dc_aligned16(s.codes) && s.code_batch_stride % 16 == 0 && s.code_head_stride % 16 == 0 && s.code_row_stride % 16 == 0,
-               "%s: %s's codes must be 16-byte aligned, its strides multiples of 16 bytes", who, which);
-    DC_REQUIRE((uintptr_t)s.scale % blocks == 0 && s.scale_batch_stride % blocks == 0 && s.scale_head_stride % blocks == 0 &&
-                   s.scale_row_stride % blocks == 0,
+    const int64_t blocks = hd / 32;
+    DC_REQUIRE(dc_aligned16(s.codes) && s.code_batch_stride % 16 == 0 && s.code_head_stride % 16 == 0,
+               "%s: %s's codes must be 16-byte aligned, their strides multiples of 16 bytes", who, which);
+    DC_REQUIRE((uintptr_t)s.scale % blocks == 0 && s.scale_batch_stride % blocks == 0 && s.scale_head_stride % blocks == 0,
                "%s: %s's scales and their strides must be multiples of %lld bytes", who, which, (long long)blocks);
-    DC_REQUIRE(s.code_row_stride >= row && s.scale_row_stride >= blocks, "%s: rows of %s overlap", who, which);
-    DC_REQUIRE(s.code_row_stride < (1 << 24) && s.scale_row_stride < (1 << 24), "%s: rows of %s are too far apart", who, which);
     DC_REQUIRE(s.code_batch_stride >= 0 && s.code_head_stride >= 0 && s.scale_batch_stride >= 0 && s.scale_head_stride >= 0,
                "%s: negative stride in %s", who, which);
     if (written) {

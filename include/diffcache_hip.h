@@ -640,16 +640,15 @@ int dc_data_layer_query(dc_data_layer *dl, void *out_keys, void *out_vals, int64
  * round past the last code, from 2 to 252 (bits 4) or 10 to 246 (bits 8), so that every number held is a normal bf16 number
  * or zero: reading back into bf16 is exact.  A block with an infinity or a NaN in it is held as NaN (e = 255).
  *
- * dc_mx_store names one tensor (K or V) of a layer: row r of unit (b, h) has its hd * bits / 8 bytes of codes at
- *   codes + b * code_batch_stride + h * code_head_stride + r * code_row_stride
- * and its hd / 32 scales, contiguous, likewise; strides in bytes.  Codes are 16-byte aligned with strides multiples of 16, scales
- * and their strides multiples of hd / 32; rows may be up to 16 MiB apart.  n_rows: the rows there is room for.  Units that share
- * rows (a stride of 0) may be read, not written.  K and V may be held in different bits.  hd: 64, 128 or 256.
+ * dc_mx_store names one tensor (K or V) of a layer: unit (b, h) has its rows' codes, hd * bits / 8 bytes each, one after another at
+ *   codes + b * code_batch_stride + h * code_head_stride
+ * and its rows' hd / 32 scales likewise; strides in bytes.  Codes are 16-byte aligned with strides multiples of 16, scales and
+ * their strides multiples of hd / 32.  n_rows: the rows that a unit has room for.  Units that share rows (a stride of 0) may be
+ * read, not written.  K and V may be held in different bits.  hd: 64, 128 or 256.
  */
 typedef struct dc_mx_store {
     void *codes, *scale;
-    int64_t code_batch_stride, code_head_stride, code_row_stride;
-    int64_t scale_batch_stride, scale_head_stride, scale_row_stride;
+    int64_t code_batch_stride, code_head_stride, scale_batch_stride, scale_head_stride;
     int bits, n_rows;
 } dc_mx_store;
 

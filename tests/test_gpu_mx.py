@@ -134,15 +134,16 @@ def test_prompts_of_unequal_lengths(lens):
 
 
 def test_sources_and_stores_of_other_layouts():
-    """Sources (b, h, s, d) transposed and cut out of a fused projection; stores that are views of (layers, b, n, h, .) tensors."""
+    """Sources (b, h, s, d) transposed and cut out of a fused projection; stores that are views of
+    (b, layers, h, rows, .) tensors."""
     rng = np.random.default_rng(4)
     b, h, seq, hd = 2, 3, 37, 128
     k_t, kx = bf16(rng.standard_normal((b, h, seq, hd)))
     qkv, x = bf16(rng.standard_normal((b, seq, 4 * h * hd)))
     v = qkv[..., 2 * h * hd:3 * h * hd].view(b, seq, h, hd)
     vx = x[..., 2 * h * hd:3 * h * hd].reshape(b, seq, h, hd)
-    ks, vs = (hip().MxStore(torch.zeros((4, b, 50, h, hd * n // 8), dtype=torch.uint8, device=DEV)[2].transpose(1, 2),
-                            torch.zeros((4, b, 50, h, hd // 32), dtype=torch.uint8, device=DEV)[2].transpose(1, 2)) for n in (4, 8))
+    ks, vs = (hip().MxStore(torch.zeros((b, 4, h, 60, hd * n // 8), dtype=torch.uint8, device=DEV)[:, 2, :, 7:57],
+                            torch.zeros((b, 4, h, 60, hd // 32), dtype=torch.uint8, device=DEV)[:, 2, :, 7:57]) for n in (4, 8))
     hip().mx_ingest(ks, vs, k_t.transpose(1, 2), v, dst_pos=5)
     for s, want, bits in ((ks, kx, 4), (vs, vx.transpose(0, 2, 1, 3), 8)):
         codes, scale = ref.encode(want, bits)
@@ -371,29 +372,51 @@ def test_a_token_without_lens_takes_the_last_row():
     assert np.array_equal(ks.codes.cpu().numpy()[:, :, 49], codes) and np.array_equal(vs.scale.cpu().numpy()[:, :, 49], scale)
 
 
-def test_units_far_apart_and_rows_far_apart():
-    """Offsets beyond 32 bits: between units, and between the rows of one."""
+def test_units_far_apart():
+    """Offsets beyond 32 bits between the units."""
     rng = np.random.default_rng(14)
     n, hd = 600, 128
-    room = torch.zeros((9 << 30,), dtype=torch.uint8, device=DEV)
-    far = (4 << 30) + 64
-    x, y = keys(rng, (2, 1, n, hd)), rng.standard_normal((2, 1, n, hd))
-    for unit_stride, row_stride in ((far, 64), (64, 8 << 20)):
-        stores = []
-        for i, z in enumerate((x, y)):
-            base = room[i * (64 << 10) * (1 if unit_stride == far else 0) + (0 if unit_stride == far else 256 * i):]
-            codes = torch.as_strided(base, (2, 1, n, 64), (unit_stride, 64, row_stride, 1))
-            small = store_of(z, 4)
-            codes.copy_(small.codes)
-            stores.append(hip().MxStore(codes, small.scale))
-        q, qx = bf16(rng.standard_normal((2, 4, hd)))
-        check_attention(q, qx, *stores, [n, n - 1])
-        back = hip().mx_gather_rows(stores[0], None)[0]
-        assert np.array_equal(f64(back), held(stores[0]))
-        nk, _ = bf16(rng.standard_normal((2, 1, hd)))
-        at = torch.tensor([n - 1, n - 2], dtype=torch.int32, device=DEV)
-        hip().mx_append(*stores, nk, nk, at)
-        check_attention(q, qx, *stores, [n, n - 1])
+    room = torch.zeros((5 << 30,), dtype=torch.uint8, device=DEV)
+    stores = []
+    for i, z in enumerate((keys(rng, (2, 1, n, hd)), rng.standard_normal((2, 1, n, hd)))):
+        small = store_of(z, 4)
+        codes = torch.as_strided(room[i << 16:], (2, 1, n, 64), ((4 << 30) + 64, 64, 64, 1))
+        scale = torch.as_strided(room[(i << 16) + (1 << 20):], (2, 1, n, 4), ((4 << 30) + 8, 4, 4, 1))
+        codes.copy_(small.codes)
+        scale.copy_(small.scale)
+        stores.append(hip().MxStore(codes, scale))
+    q, qx = bf16(rng.standard_normal((2, 4, hd)))
+    check_attention(q, qx, *stores, [n, n - 1])
+    back = hip().mx_gather_rows(stores[0], None)[0]
+    assert np.array_equal(f64(back), held(stores[0]))
+    nk, _ = bf16(rng.standard_normal((2, 1, hd)))
+    hip().mx_append(*stores, nk, nk, torch.tensor([n - 1, n - 2], dtype=torch.int32, device=DEV))
+    check_attention(q, qx, *stores, [n, n - 1])
+
+
+def test_rows_beyond_four_gib_of_a_unit():
+    """One unit of 17 million rows of 256 bytes: prompts, tokens, rows and a window at its end."""
+    rng = np.random.default_rng(24)
+    n, hd, last = 17 << 20, 256, 300
+    s = hip().MxStore.zeros(1, 1, n, hd, 8, DEV)
+    (k, kx), (v, vx) = bf16(rng.standard_normal((1, last, 1, hd))), bf16(rng.standard_normal((1, last, 1, hd)))
+    other = hip().MxStore.zeros(1, 1, n, hd, 8, DEV)
+    hip().mx_ingest(s, other, k, v, dst_pos=n - last)
+    nk, _ = bf16(rng.standard_normal((1, 1, hd)))
+    q, qx = bf16(rng.standard_normal((1, 2, hd)))
+    at = torch.tensor([n - 1], dtype=torch.int32, device=DEV)
+    out = hip().mx_attn(q, s, other, at, new_k=nk, new_v=nk, n_sink=3, window=last)
+    back_k, back_v = hip().mx_gather_rows(s, other, row_offset=n - last)
+    want = ref.decode(*ref.encode(kx[:, :last - 1].transpose(0, 2, 1, 3), 8))
+    assert np.array_equal(f64(back_k)[:, :, :last - 1], want)
+    token = ref.decode(*ref.encode(f64(nk), 8))
+    assert np.array_equal(f64(back_k)[:, :, last - 1], token) and np.array_equal(f64(back_v)[:, :, last - 1], token)
+    zeros = np.zeros((3, hd))
+    want, _, weight, _ = ref.attention(qx[0], np.concatenate([zeros, f64(back_k)[0, 0]]), np.concatenate([zeros, f64(back_v)[0, 0]]), hd ** -0.5)
+    assert (np.abs(f64(out)[0] - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -14 * weight).all()
+    idx = torch.tensor([[n - 1, 0, n - last]], dtype=torch.int32, device=DEV)
+    got = hip().mx_gather_rows(s, None, idx)[0]
+    assert torch.equal(got[0, 0], torch.stack([back_k[0, 0, -1], torch.zeros_like(back_k[0, 0, 0]), back_k[0, 0, 0]]))
 
 
 def test_shared_units_may_be_read():

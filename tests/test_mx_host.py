@@ -55,9 +55,9 @@ def test_structs_match_the_header(name, cls):
 
 
 def test_packed_bytes_are_the_structs():
-    store = hip._MX_STORE.pack(*range(1, 9), 4, 99)
-    assert store == bytes(hip.MxStoreArgs(*range(1, 9), 4, 99))
-    other = hip._MX_STORE.pack(*range(11, 19), 8, 98)
+    store = hip._MX_STORE.pack(*range(1, 7), 4, 99)
+    assert store == bytes(hip.MxStoreArgs(*range(1, 7), 4, 99))
+    other = hip._MX_STORE.pack(*range(11, 17), 8, 98)
     args = hip._MX_ATTN.pack(*range(21, 27), store, other, 31, 32, *range(41, 48), 0.25)
     want = hip.MxAttnArgs(*range(21, 27), hip.MxStoreArgs.from_buffer_copy(store), hip.MxStoreArgs.from_buffer_copy(other), 31,
                           32, *range(41, 48), 0.25)
@@ -66,8 +66,8 @@ def test_packed_bytes_are_the_structs():
 
 def fake(bits=4, n_rows=64, hd=128, **more):
     """A store that no kernel is launched on: every call below is refused first."""
-    s = hip.MxStoreArgs(1 << 20, 1 << 21, 2 * n_rows * hd * bits // 8, n_rows * hd * bits // 8, hd * bits // 8,
-                        2 * n_rows * (hd // 32), n_rows * (hd // 32), hd // 32, bits, n_rows)
+    s = hip.MxStoreArgs(1 << 20, 1 << 21, 2 * n_rows * hd * bits // 8, n_rows * hd * bits // 8, 2 * n_rows * (hd // 32),
+                        n_rows * (hd // 32), bits, n_rows)
     for name, x in more.items():
         setattr(s, name, x)
     return s
@@ -84,10 +84,9 @@ def refused(rc, message):
 
 BAD_STORES = [
     (dict(bits=5), "5 bits"), (dict(bits=0), "0 bits"), (dict(codes=None), "null"), (dict(scale=None), "null"),
-    (dict(codes=(1 << 20) + 8), "16-byte"), (dict(code_row_stride=72), "16 bytes"), (dict(code_head_stride=8), "16 bytes"),
-    (dict(scale=(1 << 21) + 2), "multiples of 4"), (dict(scale_row_stride=6), "multiples of 4"), (dict(code_row_stride=48), "overlap"),
-    (dict(scale_row_stride=0), "overlap"), (dict(code_row_stride=1 << 24), "too far apart"), (dict(code_batch_stride=-64), "negative"),
-    (dict(n_rows=-1), "negative"),
+    (dict(codes=(1 << 20) + 8), "16-byte"), (dict(code_batch_stride=72), "16 bytes"), (dict(code_head_stride=8), "16 bytes"),
+    (dict(scale=(1 << 21) + 2), "multiples of 4"), (dict(scale_head_stride=6), "multiples of 4"), (dict(code_batch_stride=-64), "negative"),
+    (dict(scale_head_stride=-4), "negative"), (dict(n_rows=-1), "negative"),
 ]
 
 
@@ -182,8 +181,10 @@ def test_wrappers_refuse_what_does_not_fit():
             hip.MxStore(codes, scale)
     with pytest.raises(hip.DiffCacheError, match="neither 4 nor 8 bits"):
         hip.MxStore(u8(1, 2, 8, 96), u8(1, 2, 8, 4))
-    with pytest.raises(hip.DiffCacheError, match="contiguous"):
-        hip.MxStore(u8(1, 2, 64, 8).transpose(2, 3), u8(1, 2, 8, 4))
+    for codes, scale in ((u8(1, 2, 64, 8).transpose(2, 3), u8(1, 2, 8, 4)), (u8(1, 8, 2, 64).transpose(1, 2), u8(1, 2, 8, 4)),
+                         (u8(1, 2, 8, 64), u8(1, 8, 2, 4).transpose(1, 2)), (u8(1, 2, 8, 64), u8(1, 2, 8, 8)[..., :4])):
+        with pytest.raises(hip.DiffCacheError, match="one after another"):
+            hip.MxStore(codes, scale)
     for bits, hd in ((5, 128), (4, 96)):
         with pytest.raises(hip.DiffCacheError, match="not supported"):
             hip.MxStore.zeros(1, 1, 1, hd, bits, "cpu")
