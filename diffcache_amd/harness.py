@@ -9,7 +9,10 @@ offline), so that the retrieval path can be timed inside a whole decode step:
 tokens per second with the dense parts of the model in the loop.
 
     python -m diffcache_amd.harness --layers 32 --batch 8 --ctx 131072 --steps 20
+    python -m diffcache_amd.harness --layers 32 --batch 8 --ctx 131072 --cache mx4
 
+``--cache mx4``, ``mx8`` and ``mx84`` (8-bit keys, 4-bit values) attend to the whole context in an ``MxCache`` instead of a
+selection of it in a ``DiffCache``.
 Everything dense is plain PyTorch (hipBLASLt GEMMs); only the cache calls go to
 the HIP library.
 """
@@ -19,11 +22,15 @@ import argparse
 import json
 import math
 import time
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import torch
 
 from .kvcache.diffcache import DiffCache
+from .kvcache.mxcache import MxCache
+
+Cache = Union[DiffCache, MxCache]
+MX_BITS = {"mx4": (4, 4), "mx8": (8, 8), "mx84": (8, 4)}
 
 
 class SyntheticLlama:
@@ -90,7 +97,7 @@ class SyntheticLlama:
         gate, up = gu[:, :self.inter], gu[:, self.inter:]
         return x + (torch.nn.functional.silu(gate) * up) @ self.wd[layer].t()
 
-    def decode_step(self, cache: DiffCache, x: torch.Tensor) -> torch.Tensor:
+    def decode_step(self, cache: Cache, x: torch.Tensor) -> torch.Tensor:
         """One token for every sequence of the batch: x (b, hidden) -> (b, hidden)."""
         pos = cache.seq_len(0)
         for layer in range(self.num_layers):
@@ -105,7 +112,7 @@ class GraphedDecoder:
     precedes the cache query (norm, QKV, RoPE) and one for what follows the attention
     (o_proj, MLP), with the cache call in between, which only enqueues kernels."""
 
-    def __init__(self, model: SyntheticLlama, cache: DiffCache, batch: int) -> None:
+    def __init__(self, model: SyntheticLlama, cache: Cache, batch: int) -> None:
         self.model, self.cache = model, cache
         dev, dt = model.device, torch.bfloat16
         self.x = torch.zeros((batch, model.hidden), device=dev, dtype=dt)
@@ -153,7 +160,7 @@ class GraphedDecoder:
         return self.x
 
 
-def synthetic_prompt_cache(cache: DiffCache, ctx: int, seed: int = 1) -> None:
+def synthetic_prompt_cache(cache: Cache, ctx: int, seed: int = 1) -> None:
     """Fill every layer of the cache with a random prompt of ``ctx`` tokens (keys with
     per-channel log-normal scales, as in the benchmark's configuration 3)."""
     dev = cache.device
@@ -169,15 +176,19 @@ def synthetic_prompt_cache(cache: DiffCache, ctx: int, seed: int = 1) -> None:
 
 def run(layers: int, batch: int, ctx: int, budget: int, steps: int, warmup: int, key_sketch: bool,
         graphs: bool = True, hidden: int = 4096, hq: int = 32, hkv: int = 8, hd: int = 128, inter: int = 14336,
-        sink: int = 4, recent: int = 64) -> dict:
+        sink: int = 4, recent: int = 64, cache_kind: str = "diffcache") -> dict:
     dev = "cuda"
     model = SyntheticLlama(layers, hidden, hq, hkv, hd, inter, device=dev)
     room = warmup + steps + 8
-    cache = DiffCache(num_layers=layers, batch_size=batch, max_length=ctx + room, num_kv_heads=hkv,
-                      num_q_heads=hq, head_dim=hd, retrieval_budget=budget, nsw_m=16, nsw_ef_cons=200,
-                      kvbuf_prefix_len=sink, kvbuf_suffix_len=recent, kvbuf_suffix_maxlen=recent + room,
-                      attn_mass_threshold=0.9, k_check_seq=[1 << 30],
-                      r_sq=[[4.0] * hkv for _ in range(layers)], key_sketch=key_sketch)
+    if cache_kind in MX_BITS:
+        bits = MX_BITS[cache_kind]
+        cache: Cache = MxCache(layers, batch, ctx + room, hkv, hq, hd, key_bits=bits[0], value_bits=bits[1])
+    else:
+        cache = DiffCache(num_layers=layers, batch_size=batch, max_length=ctx + room, num_kv_heads=hkv,
+                          num_q_heads=hq, head_dim=hd, retrieval_budget=budget, nsw_m=16, nsw_ef_cons=200,
+                          kvbuf_prefix_len=sink, kvbuf_suffix_len=recent, kvbuf_suffix_maxlen=recent + room,
+                          attn_mass_threshold=0.9, k_check_seq=[1 << 30],
+                          r_sq=[[4.0] * hkv for _ in range(layers)], key_sketch=key_sketch)
     synthetic_prompt_cache(cache, ctx)
     x = torch.randn((batch, hidden), device=dev, dtype=torch.bfloat16)
     dec = GraphedDecoder(model, cache, batch) if graphs else None
@@ -201,7 +212,7 @@ def run(layers: int, batch: int, ctx: int, budget: int, steps: int, warmup: int,
         "ms_per_step": dt * 1e3,
         "config": {"layers": layers, "batch": batch, "ctx": ctx, "budget": budget, "hidden": hidden,
                    "q_heads": hq, "kv_heads": hkv, "head_dim": hd, "intermediate": inter,
-                   "key_sketch": key_sketch, "graphs": graphs, "weights": "random bf16",
+                   "key_sketch": key_sketch, "graphs": graphs, "weights": "random bf16", "cache": cache_kind,
                    "prompt": "synthetic K/V"},
         "weight_bytes": model.weight_bytes(),
         "finite": bool(torch.isfinite(x.float()).all()),
@@ -218,12 +229,14 @@ def main(argv: Optional[List[str]] = None) -> int:
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--no-sketch", action="store_true", help="stream the bf16 keys instead of the 8-bit sketch")
     ap.add_argument("--eager", action="store_true", help="no captured graphs around the dense halves")
+    ap.add_argument("--cache", choices=["diffcache", *MX_BITS], default="diffcache",
+                    help="attend to a selection of bf16 rows, or to all rows held in 4 or 8 bits")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
         print("harness: no GPU visible")
         return 2
     print(json.dumps(run(args.layers, args.batch, args.ctx, args.budget, args.steps, args.warmup,
-                         not args.no_sketch, graphs=not args.eager)))
+                         not args.no_sketch, graphs=not args.eager, cache_kind=args.cache)))
     return 0
 
 
