@@ -1046,6 +1046,8 @@ class MxStore:
         sb, sh, sr, s1 = scale.stride()
         if c1 != 1 or (s1 != 1 and blocks > 1) or (n > 1 and (cr != row or sr != blocks)):
             raise DiffCacheError("a unit's rows must lie one after another in codes and in scale")
+        if codes.get_device() != scale.get_device():
+            raise DiffCacheError(f"codes live on {codes.device}, scale on {scale.device}")
         self.codes, self.scale = codes, scale
         self.shape, self.units, self.hd, self.bits = (b, h, n, hd), (b, h, hd), hd, bits
         self.args = _MX_STORE.pack(_mx_dev(codes, "codes"), _mx_dev(scale, "scale"), cb, ch, sb, sh, bits, n)
@@ -1102,14 +1104,14 @@ def mx_ingest(k: MxStore, v: MxStore, k_src: torch.Tensor, v_src: torch.Tensor, 
     if dst_pos < 0 or dst_pos + seq > room:
         raise DiffCacheError(f"rows [{dst_pos}, {dst_pos + seq}) outside the store of {room} rows")
     _check(lib.dc_mx_ingest_bf16(k.args, v.args, _mx_dev(k_src, "k_src"), _mx_dev(v_src, "v_src"), _mx_lens(lens, b) or None, b, seq,
-                                 h, hd, dst_pos, k0, k1, k2, v0, v1, v2, _mx_stream(k)))
+                                 h, hd, dst_pos, k0, k1, k2, v0, v1, v2, _mx_stream(k, v)))
 
 
-def _mx_stream(s: MxStore) -> int:
-    """The current stream, for a store on the current device (which may have changed since the store was made)."""
+def _mx_stream(k: MxStore, v: MxStore) -> int:
+    """The current stream, for stores on the current device (which may have changed since they were made)."""
     at = _device()
-    if s.codes.get_device() != at:
-        raise DiffCacheError(f"the store lives on {s.codes.device}, the current device is cuda:{at}")
+    if k.codes.get_device() != at or v.codes.get_device() != at:
+        raise DiffCacheError(f"the stores live on {k.codes.device} and {v.codes.device}, the current device is cuda:{at}")
     return torch._C._cuda_getCurrentRawStream(at)
 
 
@@ -1119,7 +1121,7 @@ def mx_append(k: MxStore, v: MxStore, new_k: torch.Tensor, new_v: torch.Tensor, 
     b, h, hd = _mx_pair(k, v)
     new_k, new_v = _mx_token(new_k, b, h, hd, "new_k"), _mx_token(new_v, b, h, hd, "new_v")
     _check(lib.dc_mx_append_bf16(k.args, v.args, _mx_dev(new_k, "new_k"), _mx_dev(new_v, "new_v"), _mx_lens(lens, b) or None, b, h, hd,
-                                 _mx_stream(k)))
+                                 _mx_stream(k, v)))
 
 
 def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[torch.Tensor] = None,
@@ -1171,7 +1173,8 @@ def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[tor
             raise DiffCacheError("out_k and out_v must share their strides")
         strides, ptrs[i] = st, _mx_dev(o, name)
     _check(lib.dc_mx_gather_rows_bf16(None if k is None else k.args, None if v is None else v.args, idx_ptr or None, *ptrs,
-                                      b, h, n_idx, idx_stride, hd, row_offset, *strides, _mx_stream(ref)))
+                                      b, h, n_idx, idx_stride, hd, row_offset, *strides,
+                                      _mx_stream(ref, ref if v is None else v)))
     return out_k, out_v
 
 
@@ -1233,5 +1236,5 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
             ws_ptr = workspace.data_ptr()
     args = _MX_ATTN.pack(_mx_dev(q, "q"), new_k_ptr, new_v_ptr, _mx_dev(out, "out"), lse_ptr, _mx_lens(lens, b), k.args, v.args,
                          ws_ptr, ws_bytes, b, h, group, hd, n_rows, n_sink, window, hd ** -0.5 if scale is None else scale)
-    _check(lib.dc_mx_attn_bf16(args, _mx_stream(k)))
+    _check(lib.dc_mx_attn_bf16(args, _mx_stream(k, v)))
     return out if lse is None else (out, lse)

@@ -307,7 +307,7 @@ __device__ __forceinline__ Plan mx_plan(const AttnArgs &a, int b) {
     p.rows = len + (has_new && len < a.cap ? 1 : 0);
     p.sink = 0, p.lo = 0;
     if (a.window > 0 && (int64_t)a.n_sink + a.window < p.rows) p.sink = a.n_sink, p.lo = p.rows - a.window;
-    p.sink_steps = (p.sink + STEP - 1) / STEP;
+    p.sink_steps = (int)(((uint32_t)p.sink + STEP - 1) / STEP);
     p.steps = p.sink_steps + (int)(((int64_t)p.rows - p.lo + STEP - 1) / STEP);
     // steps / n_splits, rounded up; now and then one more, which leaves a last part shorter
     p.per = a.n_splits == 1 ? p.steps : (int)__umulhi((uint32_t)(p.steps + a.n_splits - 1), a.per_split);
@@ -783,9 +783,9 @@ int check_units(const char *who, int n_b, int n_h, int hd) {
     return DC_OK;
 }
 
-// blocks of a unit in a grid of (unit, chunk) by n_units * chunks
-int check_grid(const char *who, int64_t n_units, int64_t chunks) {
-    DC_REQUIRE(n_units * chunks < (1ll << 31), "%s: grid too large", who);
+// blocks of a unit in a grid of (unit, chunk) by n_units * chunks; the last one's rows, those beyond the end too, are ints
+int check_grid(const char *who, int64_t n_units, int64_t chunks, int rows_per) {
+    DC_REQUIRE(n_units * chunks < (1ll << 31) && chunks * rows_per < (1ll << 31), "%s: grid too large", who);
     return DC_OK;
 }
 
@@ -862,7 +862,7 @@ extern "C" int dc_mx_ingest_bf16(const dc_mx_store *k, const dc_mx_store *v, con
                "%s: strides must be multiples of 8 elements", who);
     const int rows_per = kThreads / (hd / 8) * kIngestBatch;
     const int64_t chunks = (seq + rows_per - 1) / rows_per;
-    DC_TRY(check_grid(who, n_units, chunks));
+    DC_TRY(check_grid(who, n_units, chunks, rows_per));
     IngestArgs a = {view_of(*k), view_of(*v), (const uint16_t *)k_src, (const uint16_t *)v_src, ksb, kss, ksh, vsb, vss, vsh,
                     lens, n_h, seq, dst_pos, (int)chunks};
     DC_MX_BY_BITS(mx_ingest_kernel, k->bits, v->bits, dim3((unsigned)(n_units * chunks), 2), dim3(kThreads), 0, (hipStream_t)stream, a, hd);
@@ -904,7 +904,7 @@ extern "C" int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v
     DC_REQUIRE(dsb % 8 == 0 && dsh % 8 == 0 && dsr % 8 == 0, "%s: strides must be multiples of 8 elements", who);
     const int rows_per = kThreads / (hd / 8) * kGatherBatch;
     const int64_t chunks = ((int64_t)n_idx + rows_per - 1) / rows_per;
-    DC_TRY(check_grid(who, n_units, chunks));
+    DC_TRY(check_grid(who, n_units, chunks, rows_per));
     const dc_mx_store &ks = out_k ? *k : *v, &vs = out_v ? *v : *k;
     GatherArgs a = {view_of(ks), view_of(vs), idx, idx_unit_stride, row_offset, (uint16_t *)out_k, (uint16_t *)out_v, dsb, dsh, dsr,
                     n_h, n_idx, ks.n_rows, vs.n_rows, (int)chunks};

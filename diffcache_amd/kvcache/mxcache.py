@@ -65,7 +65,8 @@ class MxCache:
         else:
             lens = [int(x) for x in lens]
             hip.require(len(lens) == self.batch_size and all(0 <= x <= seq for x in lens), "lens does not fit the prompts")
-            self.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+            # (from pinned memory: nothing waits for the device)
+            self.lens.copy_(torch.tensor(lens, dtype=torch.int32, pin_memory=True), non_blocking=True)
             self._longest = max(lens)
         hip.mx_ingest(self.kstore[layer_idx], self.vstore[layer_idx], key_states, value_states,
                       lens=None if lens is None else self.lens)
