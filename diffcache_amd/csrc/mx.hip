@@ -387,13 +387,13 @@ struct Attn {
     static constexpr int kcol(int j) { return j * 8 / KCOLS * 4 * KCOLS + j * 8 % KCOLS; }  // first column of chunk j, of lanes q = 0
     static constexpr int VBYTES = EPL * VB / 8, VW = VBYTES < 4 ? 1 : VBYTES / 4;
     static constexpr int KROW = HD * KB / 8, VROW = HD * VB / 8;
+    static constexpr int SBYTES = STEP * CH;    // a step's scales
     static constexpr int SETS = 16 / GP < TILES ? 16 / GP : TILES;  // tiles whose logits share a register
     static constexpr int REGS = TILES / SETS;   // logit registers of a lane (times 4)
-    static constexpr int KS = KN;
 
     mx_u32x4 bq[CH];
-    uint32_t kw[TILES][KW], ks[TILES][KS];
-    uint32_t vw[TILES * 4][VW], vs[TILES * 4];
+    uint32_t kw[TILES][KW], ks[CH > 4 ? 2 : 1];
+    uint32_t vw[TILES * 4][VW], vs[CH > 4 ? 2 : 1];
     mx_f32x4 acc[EPL];
     float m, l;
     int q, c;
@@ -410,35 +410,62 @@ struct Attn {
     }
 
     // Codes and scales of the rows [row, row + live) of a unit, live <= STEP; lane (q, c) has row 4 (c % 4) + c / 4 of every tile.
+    // The scales of the whole step are one load: lane l has row l's.
     __device__ __forceinline__ void load_k(const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
         const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * KROW, (uint32_t)live * KROW), rs = mx_rsrc(scale + row * CH, (uint32_t)live * CH);
-        const int r = 4 * (c & 3) + (c >> 2);
-        const uint32_t oc = mx_opaque(r * KROW + q * KBYTES), os = mx_opaque(r * CH + q * KCOLS / 32);
+        const uint32_t oc = mx_opaque((4 * (c & 3) + (c >> 2)) * KROW + q * KBYTES);
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
-            for (int n = 0; n < KN; ++n) {
-                mx_load<KBYTES, kOnce>(rc, oc + 16 * KROW * t + 4 * KBYTES * n, &kw[t][KBYTES / 4 * n]);
-                mx_load<1, 0>(rs, os + 16 * CH * t + 4 * KCOLS / 32 * n, &ks[t][n]);
-            }
+            for (int n = 0; n < KN; ++n) mx_load<KBYTES, kOnce>(rc, oc + 16 * KROW * t + 4 * KBYTES * n, &kw[t][KBYTES / 4 * n]);
+        mx_load<CH, 0>(rs, (uint32_t)(16 * q + c) * CH, ks);
     }
     // lane (q, c) has columns EPL c .. of the rows 4 i + q of every tile
     __device__ __forceinline__ void load_v(const uint8_t *codes, const uint8_t *scale, int64_t row, int live) {
         const __amdgpu_buffer_rsrc_t rc = mx_rsrc(codes + row * VROW, (uint32_t)live * VROW), rs = mx_rsrc(scale + row * CH, (uint32_t)live * CH);
-        const uint32_t oc = mx_opaque(q * VROW + c * VBYTES), os = mx_opaque(q * CH + c * EPL / 32);
+        const uint32_t oc = mx_opaque(q * VROW + c * VBYTES);
 #pragma unroll
-        for (int t = 0; t < TILES * 4; ++t) {
-            mx_load<VBYTES, kOnce>(rc, oc + 4 * VROW * t, vw[t]);
-            mx_load<1, 0>(rs, os + 4 * CH * t, &vs[t]);
+        for (int t = 0; t < TILES * 4; ++t) mx_load<VBYTES, kOnce>(rc, oc + 4 * VROW * t, vw[t]);
+        mx_load<CH, 0>(rs, (uint32_t)(16 * q + c) * CH, vs);
+    }
+
+    // A step's scales go through the wave's own bytes of LDS, from a row to a lane to what the lanes use: block by block, the rows
+    // in the order of the lanes that have them.  (Byte by byte from memory they are 20 of a step's 40 loads.)
+    __device__ __forceinline__ void spread(uint8_t *lds, const uint32_t *w, int slot) const {
+        if (16 * q + c < STEP) {
+#pragma unroll
+            for (int j = 0; j < CH; ++j) lds[j * STEP + slot] = (uint8_t)(w[j / 4] >> (8 * (j % 4)));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // (what is read back is other lanes')
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ void spread_k(uint8_t *lds, uint32_t (&f)[KN]) const {
+        spread(lds, ks, (4 * (c & 3) + (c >> 2)) * TILES + q);  // row 16 q + c of the step is tile q's, of the lanes 4 (c % 4) + c / 4
+#pragma unroll
+        for (int n = 0; n < KN; ++n) {
+            const uint8_t *src = lds + (4 * KCOLS * n + q * KCOLS) / 32 * STEP + c * TILES;
+            if constexpr (TILES == 4) f[n] = *reinterpret_cast<const uint32_t *>(src);
+            else f[n] = *reinterpret_cast<const uint16_t *>(src);
+        }
+    }
+    __device__ __forceinline__ void spread_v(uint8_t *lds, uint32_t (&f)[TILES]) const {
+        spread(lds, vs, (c & 3) * 4 * TILES + 4 * q + (c >> 2));  // row 16 q + c is row 4 i + c % 4 of tile q, i = c / 4
+        const uint8_t *src = lds + c * EPL / 32 * STEP + q * 4 * TILES;
+        if constexpr (TILES == 4) {
+            const uint4 t = *reinterpret_cast<const uint4 *>(src);
+            f[0] = t.x, f[1] = t.y, f[2] = t.z, f[3] = t.w;
+        } else {
+            const uint2 t = *reinterpret_cast<const uint2 *>(src);
+            f[0] = t.x, f[1] = t.y;
         }
     }
 
     template <int T>
-    __device__ __forceinline__ mx_f32x4 logits_of() const {
+    __device__ __forceinline__ mx_f32x4 logits_of(const uint32_t (&ksc)[KN]) const {
         mx_f32x4 s = {0.f, 0.f, 0.f, 0.f};
         auto chunk = [&](auto jj) __attribute__((always_inline)) {
             constexpr int J = decltype(jj)::value;
-            const float f = mx_scale(ks[T][J * 8 / KCOLS]);
+            const float f = mx_scale((ksc[J * 8 / KCOLS] >> (8 * T)) & 0xffu);
             const mx_u32x4 x = {mx_pair<KB, 4 * J>(kw[T], f), mx_pair<KB, 4 * J + 1>(kw[T], f), mx_pair<KB, 4 * J + 2>(kw[T], f),
                                 mx_pair<KB, 4 * J + 3>(kw[T], f)};
             s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(mx_bf16x8, x), __builtin_bit_cast(mx_bf16x8, bq[J]), s, 0, 0, 0);
@@ -457,11 +484,13 @@ struct Attn {
     }
 
     // the logits of the step that load_k brought, by lane and register: x[r][i] = tile r SETS + c / GP, row 4 i + q, head c % GP
-    __device__ __forceinline__ void logits(float scale, float (&x)[REGS][4]) const {
+    __device__ __forceinline__ void logits(uint8_t *lds, float scale, float (&x)[REGS][4]) const {
         const int set = c / GP;
+        uint32_t ksc[KN];
+        spread_k(lds, ksc);
         each<TILES>([&](auto tt) __attribute__((always_inline)) {
             constexpr int T = decltype(tt)::value;
-            const mx_f32x4 s = logits_of<T>();
+            const mx_f32x4 s = logits_of<T>(ksc);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if constexpr (T % SETS == 0)
@@ -551,7 +580,9 @@ struct Attn {
     }
 
     // acc += P V over the step that load_v brought
-    __device__ __forceinline__ void add(const float (&x)[REGS][4]) {
+    __device__ __forceinline__ void add(uint8_t *lds, const float (&x)[REGS][4]) {
+        uint32_t vsc[TILES];
+        spread_v(lds, vsc);
         uint32_t hi[REGS][2], lo[REGS][2];
 #pragma unroll
         for (int r = 0; r < REGS; ++r)
@@ -570,7 +601,7 @@ struct Attn {
             const mx_u32x4 al = {of(lo, T0, 0), of(lo, T0, 1), of(lo, T1, 0), of(lo, T1, 1)};
             float f[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = mx_scale(vs[8 * U + i]);
+            for (int i = 0; i < 8; ++i) f[i] = mx_scale((vsc[2 * U + i / 4] >> (8 * (i % 4))) & 0xffu);
             each<EPL / 2>([&](auto jj) __attribute__((always_inline)) {
                 constexpr int J = decltype(jj)::value;
                 uint32_t w[8];
@@ -590,7 +621,10 @@ struct Attn {
     }
 };
 
-inline size_t attn_shared_bytes(int hd, int group, int waves) { return (size_t)waves * (32 + group * hd) * sizeof(float); }
+inline size_t attn_shared_bytes(int hd, int group, int waves) {
+    const size_t sums = (size_t)group * hd * sizeof(float), scales = 2 * (hd == 256 ? 32 : 64) * (hd / 32);
+    return waves * (32 * sizeof(float) + (sums > scales ? sums : scales));
+}
 
 template <int HD, int KB, int VB, int GP, int TILES>
 __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a) {
@@ -607,6 +641,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     T w;
     w.start(a, unit, lane);
+    uint8_t *lds = reinterpret_cast<uint8_t *>(s_acc) + wave * 2 * T::SBYTES;  // (the sums come when all scales were used)
     const Plan p = mx_plan<STEP>(a, b);
     const int begin = split * p.per, end = begin + p.per < p.steps ? begin + p.per : p.steps;
     if (begin >= end && a.n_splits > 1) {  // a part without rows: the merge takes nothing of it
@@ -644,7 +679,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
     }
     for (int i = 0; i < mine; ++i) {
         float x[T::REGS][4];
-        w.logits(a.scale, x);
+        w.logits(lds, a.scale, x);
         const int now = live;
         const bool more = i + 1 < mine;
         if (more) {
@@ -652,11 +687,12 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
             load_k();
         }
         w.weigh(x, now);
-        w.add(x);
+        w.add(lds + T::SBYTES, x);
         if (more) w.load_v(vc, vsc, row, live);
     }
 
     // the wave's heads: over the lanes that had other rows, and over the tiles
+    __syncthreads();
     const float l = mx_over_lanes<GP>(w.l, [](float a, float b) { return a + b; });
     if (lane < GP) s_m[wave * 16 + lane] = w.m, s_l[wave * 16 + lane] = l;
     w.finish(s_acc + wave * G * HD, G);
@@ -809,14 +845,20 @@ constexpr int attn_tiles(int hd) { return hd == 256 ? 2 : 4; }
 struct AttnCut {
     int n_splits, waves;
 };
-constexpr int kBlocks = 512;  // of four waves, two to a CU
-constexpr int kAlone = 3;     // steps of a wave up to which a unit is one block of eight waves: less than a second kernel that joins parts
-constexpr int kWide = 8;
-AttnCut attn_cut(int64_t n_units, int hd, int64_t n_rows, int n_sink) {
+// Blocks of four waves: two to a CU, which the loads in flight of 64 rows to a wave keep busy (8 x 131072 tokens of 8 heads x
+// 128 in 4 bits: 174 us, with 768 blocks 176, with 1024 183; a document of 32601 12.5 / 13.7 / 14.0).  Rows of 32 bytes are half
+// of that in flight: four to a CU once every wave has six steps or more (64 columns, 4 bits: 16 x 32000 tokens 60.6 -> 50.8 us, a
+// million of one 112 -> 92.5, but 2 x 32000 12.3 -> 12.6).
+constexpr int kBlocks = 512, kLeanBlocks = 2 * kBlocks, kLeanSteps = 6 * kWaves;
+// Steps of a wave up to which a unit is one block of eight waves, which writes the output itself: less than a second kernel
+// that joins parts (1024 tokens: 9.3 us, in parts 6.5 + 2.7 and a launch; 1500: 11.5, 8.7 + 2.9; 2048: 13.6, 7.5 + 2.8).
+constexpr int kAlone = 3, kWide = 8;
+AttnCut attn_cut(int64_t n_units, int hd, int64_t n_rows, int n_sink, int bits) {
     const int64_t step = 16 * attn_tiles(hd);
     const int64_t steps = (n_rows + step - 1) / step + (n_sink + step - 1) / step;
     if (steps <= kAlone * kWide) return {1, steps <= kWaves ? kWaves : kWide};
-    const int64_t parts = (steps + kWaves - 1) / kWaves, most = kBlocks / n_units > 1 ? kBlocks / n_units : 1;
+    const bool lean = hd == 64 && bits == 8 && n_units * steps >= (int64_t)kLeanSteps * kBlocks;
+    const int64_t parts = (steps + kWaves - 1) / kWaves, blocks = lean ? kLeanBlocks : kBlocks, most = blocks / n_units > 1 ? blocks / n_units : 1;
     return {(int)(parts < most ? parts : most), kWaves};
 }
 
@@ -921,7 +963,8 @@ extern "C" size_t dc_mx_attn_workspace_bytes(int n_units, int group, int hd, int
     const int64_t step = 16 * attn_tiles(hd), steps = (n_rows + step - 1) / step + 1;
     if (steps <= kAlone * kWide) return 0;
     const int64_t parts = n_units * ((steps + kWaves - 1) / kWaves);
-    const size_t slots = (size_t)(parts < kBlocks ? parts : kBlocks);
+    const int64_t blocks = hd == 64 ? kLeanBlocks : kBlocks;
+    const size_t slots = (size_t)(parts < blocks ? parts : blocks);
     return dc_align_up(slots * group * hd * 4, 256) + dc_align_up(slots * group * 2 * 4, 256);
 }
 
@@ -942,7 +985,7 @@ extern "C" int dc_mx_attn_bf16(const dc_mx_attn_args *x, void *stream) {
                "%s: pointers must be 16-byte aligned", who);
     DC_REQUIRE(x->n_h < (1 << 16), "%s: too many heads", who);
     const int64_t attended = x->window > 0 && (int64_t)x->n_sink + x->window < x->n_rows ? x->window : x->n_rows;
-    const AttnCut cut = attn_cut(n_units, x->hd, attended, attended < x->n_rows ? x->n_sink : 0);
+    const AttnCut cut = attn_cut(n_units, x->hd, attended, attended < x->n_rows ? x->n_sink : 0, x->k.bits + x->v.bits);
     AttnArgs a;
     a.n_splits = cut.n_splits, a.waves = cut.waves;
     a.per_split = (uint32_t)((0xffffffffull + a.n_splits) / a.n_splits);
