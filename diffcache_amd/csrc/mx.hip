@@ -128,10 +128,12 @@ struct IngestArgs {
     int n_h, seq, dst_pos, chunks;         // chunks: blocks of a unit
 };
 
-constexpr int kIngestBatch = 4;  // pieces of 8 columns a thread takes
-
 // Rows of a prompt.  A thread takes 8 columns (16 bytes), a quad a block of 32, so a wave's piece is 512 / hd whole rows of
-// one unit: it reads segments of 2 hd bytes and writes one contiguous run.
+// one unit: it reads segments of 2 hd bytes and writes one contiguous run.  The largest number of a block is two DPP steps
+// away and the conversions do the rounding, so what bounds it is HBM: 2 + 17/32 bytes a number in 4 bits (K and V of 8 x
+// 32768 tokens of 8 heads x 128: 208 us = 6.5 TB/s; of 32601 of one sequence 28 us = 6.0).  Four pieces to a thread,
+// requested together: 208 us, with eight 208, with two 214, with one 290.
+constexpr int kIngestBatch = 4;
 template <int BITS>
 __device__ __forceinline__ void mx_ingest_rows(const View &st, const uint16_t *src, int64_t ss, const IngestArgs &a, int hd,
                                                int b, int h, int chunk, int live) {
@@ -184,6 +186,7 @@ __device__ __forceinline__ void mx_write_token(const View &k, const View &v, con
     }
 }
 
+// A token's rows alone, a wave to a unit: one round trip to the length, one to the numbers, and the launch.
 template <int KB, int VB>
 __global__ __launch_bounds__(kThreads) void mx_append_kernel(View k, View v, const uint16_t *new_k, const uint16_t *new_v,
                                                              const int32_t *lens, int n_units, int n_h, int hd, int cap) {
@@ -205,7 +208,11 @@ struct GatherArgs {
     int n_h, n_idx, k_rows, v_rows, chunks;
 };
 
-constexpr int kGatherBatch = 4;
+// Rows back into bf16: a thread makes 8 columns of a row, 4 or 8 bytes of codes and one of scales into 16.  All rows of K and V
+// of 32601 tokens of 8 heads x 128: 26 us = 6.5 TB/s, written mostly.  Rows in any order touch a line for their codes and one
+// for their scales and are bound by that and by the id in front: 2117 of 131072 rows of 64 units 25 us, 1092 of 8 units 4.1 us.
+// Two rows to a thread; with four 29 and 5.1 us, with one 28 and 4.2 (and all rows 37).
+constexpr int kGatherBatch = 2;
 
 template <int BITS>
 __device__ __forceinline__ void mx_gather(const View &st, uint16_t *out, int n_rows, const GatherArgs &a, int hd, int unit, int chunk) {
@@ -260,26 +267,36 @@ __global__ __launch_bounds__(kThreads) void mx_gather_kernel(GatherArgs a, int h
 //
 // One token's attention, out = sum_r p_r v_r / sum_r p_r with p_r = exp(scale q k_r - m), over the rows of every sequence
 // (all of them, or its first n_sink and its last window).  A unit's rows are cut into steps of 16 TILES rows and its steps
-// into n_splits equal parts, a block each, whose waves take every eighth step; a wave keeps its running maximum, sum and
+// into n_splits equal parts, a block each, whose waves take them in turn; a wave keeps its running maximum, sum and
 // weighted rows in registers, so the codes are read once and nothing is written but the parts' results.
 //
-//   S = K Q^T   v_mfma_f32_16x16x32_bf16 over 16 rows (M), 16 query heads (N) and 32 columns.  Lane (q, c) = (lane / 16,
-//               lane % 16) has the columns hd / 4 q .. of one row in one load, and the codes become bf16 numbers, their scale
-//               included, exactly; instruction j takes its columns 8 j .. + 7.  (The instructions that multiply 4-bit and
-//               8-bit numbers as they are round their sums at some 2^-15 of the largest product: measured, not enough.)
+//   S = K Q^T   v_mfma_f32_16x16x32_bf16 over 16 rows (M), 16 query heads (N) and 32 columns.  The codes become bf16 numbers, their
+//               scale included, exactly (one conversion for two numbers), and are operands as they come: which columns an
+//               instruction takes is free as long as Q's are the same, so lane (q, c) = (lane / 16, lane % 16) has 16 bytes (8
+//               of 64 columns in 4 bits) of one row, the row's four lanes side by side.  (The instructions that multiply
+//               4-bit and 8-bit numbers as they are round their sums at some 2^-15 of the largest product: measured, and not
+//               enough for logits.)
 //   softmax     The heads of a group of up to GP stand in the columns again and again, and lane c keeps the result of tile
-//               c / GP only: 64 rows of 4 heads are then 4 numbers a lane, none of them idle.  The maximum moves
-//               only where a logit passes it by more than 2^8: rare, so nothing crosses lanes from step to step.
+//               c / GP only: 64 rows of 4 heads are then 4 numbers a lane, none of them idle.  In powers of two.  The maximum
+//               moves only where a logit passes it by more than 8: rare, so nothing crosses lanes from step to step, and a
+//               weight is at most 2^8 of fp32 sums.
 //   O = P V     M = (tile, head) as the lanes have them, N = 16 of the hd columns, K = 32 rows of two tiles; P of the tiles that are not
-//               a lane's is zero.  P is the sum of two bf16 numbers (2^-17 of it is lost: with the fp32 sums the output is
-//               that of an fp32 P to far below its own rounding).  Column n of instruction j is hd / 16 n + j, so that a lane loads
-//               adjacent codes of its own rows.
+//               a lane's is zero.  P is the sum of two bf16 numbers: 2^-16 of a weight is lost at most, which the output's own
+//               2^-8 covers (a third instruction of every three would buy the rest).  Column n of instruction j is hd / 16 n + j,
+//               so that a lane loads adjacent codes of its own rows and pairs of rows are put together by byte permutes.
 //
 // Which row of a tile is which row of M is free as long as K and V agree: M row 4 q + i is the tile's row 4 i + q, so that
-// every load takes whole runs of rows (with row 4 q + i, lines are asked for in pieces, which non-temporal loads do not
-// find in the nearest cache: 2.4 times the requests of the next, 183 us for 177 at 8 x 131072 tokens).
+// every load takes whole lines (with row 4 q + i they are asked for in pieces, which non-temporal loads do not find in the
+// nearest cache: 2.4 times the requests of the next, 183 us for 174 at 8 x 131072 tokens).
 // Rows behind the end are not asked for: a step's buffers end at its last row, and what a load asks of the words past a buffer's
-// end is zero.
+// end is zero.  Every offset inside a step is a constant of the load.
+//
+// What bounds it: HBM from some 100 MB on.  8 x 131072 tokens of 8 heads x 128 with groups of 4, in 4 bits, 1.14 GB: 174 us = 6.5
+// TB/s; a million of one sequence 170 us; 8 x 65536 of 4 heads x 256 94 us = 6.1 TB/s; 8 x 131072 of 8 heads x 64 97 us = 5.9 TB/s.  64
+// rows of 128 columns are some 370 vector, 48 matrix and 22 load instructions of a wave, 55 % of the time the bytes take.
+// Below, the chain of length, rows, products and the join: 32601 tokens of 8 units 12.5 + 3.9 us (the bytes 5.4), 517 tokens
+// 7.5 us in one kernel.  Starts of their own for the blocks' steps: without them a million tokens take 200 us for 177, the
+// blocks' places being a power of two apart.  Loads without the non-temporal hint: 198 us for 180.
 struct AttnArgs {
     const uint16_t *q, *new_k, *new_v;
     uint16_t *out;
@@ -732,7 +749,8 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
 }
 
 // The parts of one query head joined: one block per (unit, head).  What it reads is asked for at once, before any weight is
-// known: rounds of kBatch kParts parts (32 at 128 columns), HD / 4 threads to a part.
+// known: rounds of kBatch kParts parts (32 at 128 columns), HD / 4 threads to a part.  A kernel's start and two round trips: 64
+// parts of 32 heads 3.9 us (5.5 part by part), 8 parts of 256 heads 4.8.
 constexpr int kBatch = 4;
 template <int HD>
 __global__ __launch_bounds__(kThreads) void mx_merge_kernel(AttnArgs a) {
