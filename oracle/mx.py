@@ -38,8 +38,8 @@ def _nearest(a: np.ndarray, bits: int) -> np.ndarray:
 
 
 def encode(x: np.ndarray, bits: int):
-    """x (..., hd) -> codes (..., hd * bits / 8), scale (..., hd / 32), both uint8.  The scale is found by trying: the least
-    exponent at which the block's largest number does not round past the last code."""
+    """x (..., hd) -> codes (..., hd * bits / 8), scale (..., hd / 32), both uint8.  The scale is the least exponent at which the
+    block's largest number does not round past the last code, found by trying."""
     x = np.asarray(x, dtype=np.float64)
     blocks = x.reshape(-1, 32)
     lo, hi = LIMITS[bits]
@@ -47,11 +47,11 @@ def encode(x: np.ndarray, bits: int):
         most = np.max(np.abs(blocks), axis=1)
     fine = np.isfinite(most)
     safe = np.where(fine, most, 0.0)
-    e = np.full(len(blocks), hi)
-    for byte in range(hi - 1, lo - 1, -1):
-        # (scales only fit from some exponent on, so the walk down may stop caring where one no longer does)
-        fits = _nearest(np.ldexp(safe, 127 - byte), bits) <= LAST[bits]
-        e = np.where(fits & (e == byte + 1), byte, e)
+    # (one less than what brings the largest number's leading bit to the last code's never fits: try that one, then one more)
+    first = np.frexp(safe)[1] - 1 - EMAX[bits] + 127
+    fits = _nearest(np.ldexp(safe, 127 - first), bits) <= LAST[bits]
+    e = np.where(safe > 0, np.where(fits, first, first + 1), lo)
+    e = np.clip(e, lo, hi)
     y = np.where(fine[:, None], blocks, 0.0) * np.ldexp(1.0, 127 - e)[:, None]
     code = np.minimum(_nearest(np.abs(y), bits), LAST[bits]) | (np.signbit(y).astype(int) << (bits - 1))
     code = code.astype(np.uint8).reshape(x.shape)
