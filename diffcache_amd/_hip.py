@@ -1032,11 +1032,12 @@ class MxStore:
     __slots__ = ("codes", "scale", "shape", "units", "hd", "bits", "args")
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
-        if codes.dim() != 4 or scale.dim() != 4 or codes.dtype is not _U8 or scale.dtype is not _U8:
-            raise DiffCacheError("codes and scale must be (b, h, n, .) uint8 tensors of the same b, h and n")
-        b, h, n, row = codes.shape
-        sb, sh, sn, blocks = scale.shape
-        if sb != b or sh != h or sn != n:
+        try:
+            b, h, n, row = codes.shape
+            b2, h2, n2, blocks = scale.shape
+        except ValueError:
+            b2 = b = -1
+        if b < 0 or b2 != b or h2 != h or n2 != n or codes.dtype is not _U8 or scale.dtype is not _U8:
             raise DiffCacheError("codes and scale must be (b, h, n, .) uint8 tensors of the same b, h and n")
         hd = blocks * 32
         bits = 4 if row * 2 == hd else 8
@@ -1046,11 +1047,13 @@ class MxStore:
         sb, sh, sr, s1 = scale.stride()
         if c1 != 1 or (s1 != 1 and blocks > 1) or (n > 1 and (cr != row or sr != blocks)):
             raise DiffCacheError("a unit's rows must lie one after another in codes and in scale")
-        if codes.get_device() != scale.get_device():
-            raise DiffCacheError(f"codes live on {codes.device}, scale on {scale.device}")
+        at = codes.get_device()
+        if at < 0 or scale.get_device() != at or at != _device():
+            _mx_dev(codes, "codes")
+            _mx_dev(scale, "scale")
         self.codes, self.scale = codes, scale
         self.shape, self.units, self.hd, self.bits = (b, h, n, hd), (b, h, hd), hd, bits
-        self.args = _MX_STORE.pack(_mx_dev(codes, "codes"), _mx_dev(scale, "scale"), cb, ch, sb, sh, bits, n)
+        self.args = _MX_STORE.pack(codes.data_ptr(), scale.data_ptr(), cb, ch, sb, sh, bits, n)
 
     @classmethod
     def zeros(cls, b: int, h: int, n: int, hd: int, bits: int, device) -> "MxStore":
@@ -1134,17 +1137,19 @@ def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[tor
     if ref is None:
         raise DiffCacheError("neither K nor V given")
     b, h, hd = ref.units if v is None else _mx_pair(ref, v)
-    idx_ptr = idx_stride = 0
+    idx_ptr = None
+    idx_stride = 0
     if idx is None:
         if n_idx is None:
             n_idx = max(ref.shape[2] - row_offset, 0)
     else:
-        require(idx.dim() == 2 and idx.shape[0] == b * h and idx.element_size() == 4 and not idx.is_floating_point(),
-                "idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor")
+        if idx.dim() != 2 or idx.shape[0] != b * h or idx.element_size() != 4 or idx.is_floating_point():
+            raise DiffCacheError("idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor")
         wide = idx.shape[1]
         if n_idx is None:
             n_idx = wide
-        require(wide >= n_idx, "idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor")
+        elif wide < n_idx:
+            raise DiffCacheError("idx must be a 32-bit (bsz * kv_heads, >= n_idx) tensor")
         idx_stride, one = idx.stride()
         if idx_stride < wide or (one != 1 and wide > 1):
             idx = idx.clone(memory_format=torch.contiguous_format)
@@ -1152,30 +1157,40 @@ def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[tor
         idx_ptr = _mx_dev(idx, "idx")
     if n_idx < 0 or row_offset < 0:
         raise DiffCacheError("n_idx and row_offset must not be negative")
+    shape, own = (b, h, n_idx, hd), (h * n_idx * hd, n_idx * hd, hd, 1)
+    k_ptr = v_ptr = None
     strides = None
-    ptrs = [None, None]
-    for i, (s, o, name) in enumerate(((k, out_k, "out_k"), (v, out_v, "out_v"))):
-        if o is not None:
-            st = _store_strides(o)
-            ob, oh, on, od = o.shape
-            require(s is not None and ob == b and oh == h and on >= n_idx and od == hd,
-                    "out_k / out_v must be (bsz, kv_heads, >= n_idx, head_dim), each with its store")
-        elif s is not None:
-            st = (h * n_idx * hd, n_idx * hd, hd)
-            o = torch.empty_strided((b, h, n_idx, hd), st + (1,), dtype=torch.bfloat16, device=s.codes.device)
-            if i:
-                out_v = o
-            else:
-                out_k = o
-        else:
-            continue
-        if strides is not None and strides != st:
-            raise DiffCacheError("out_k and out_v must share their strides")
-        strides, ptrs[i] = st, _mx_dev(o, name)
-    _check(lib.dc_mx_gather_rows_bf16(None if k is None else k.args, None if v is None else v.args, idx_ptr or None, *ptrs,
-                                      b, h, n_idx, idx_stride, hd, row_offset, *strides,
+    if out_k is not None:
+        strides = _mx_out(out_k, k, shape)
+        k_ptr = _mx_dev(out_k, "out_k")
+    elif k is not None:
+        out_k = torch.empty_strided(shape, own, dtype=_BF16, device=k.codes.device)
+        k_ptr, strides = out_k.data_ptr(), own
+    if out_v is not None:
+        v_strides = _mx_out(out_v, v, shape)
+        v_ptr = _mx_dev(out_v, "out_v")
+    elif v is not None:
+        out_v = torch.empty_strided(shape, own, dtype=_BF16, device=v.codes.device)
+        v_ptr, v_strides = out_v.data_ptr(), own
+    else:
+        v_strides = strides
+    if strides is None:
+        strides = v_strides
+    elif strides[:3] != v_strides[:3]:
+        raise DiffCacheError("out_k and out_v must share their strides")
+    _check(lib.dc_mx_gather_rows_bf16(None if k is None else k.args, None if v is None else v.args, idx_ptr, k_ptr, v_ptr, b, h,
+                                      n_idx, idx_stride, hd, row_offset, strides[0], strides[1], strides[2],
                                       _mx_stream(ref, ref if v is None else v)))
     return out_k, out_v
+
+
+def _mx_out(o: torch.Tensor, s: Optional[MxStore], shape) -> Tuple[int, int, int]:
+    """Strides of an output (b, h, >= n, hd) of rows of the store s."""
+    strides = _store_strides(o)
+    b, h, n, hd = o.shape
+    if s is None or b != shape[0] or h != shape[1] or n < shape[2] or hd != shape[3]:
+        raise DiffCacheError("out_k / out_v must be (bsz, kv_heads, >= n_idx, head_dim), each with its store")
+    return strides
 
 
 def mx_attn_workspace_bytes(n_units: int, group: int, hd: int, n_rows: int) -> int:
@@ -1208,11 +1223,14 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
         raise DiffCacheError(f"{n_rows} rows outside the store of {room}")
     if n_sink < 0 or window < 0:
         raise DiffCacheError("n_sink and window must not be negative")
-    dev = q.device
+    q_ptr, dev = _mx_dev(q, "q"), q.device
     if out is None:
         out = torch.empty_strided((b, hq, hd), (hq * hd, hd, 1), dtype=_BF16, device=dev)
+        out_ptr = out.data_ptr()
     elif out.dtype is not _BF16 or out.numel() != numel or not out.is_contiguous():
         raise DiffCacheError("out must be a contiguous bf16 tensor of the size of q")
+    else:
+        out_ptr = _mx_dev(out, "out")
     lse_ptr = new_k_ptr = new_v_ptr = ws_ptr = ws_bytes = 0
     if lse is None:
         if want_lse:
@@ -1234,7 +1252,7 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
         if ws_bytes:
             workspace = torch.empty(ws_bytes, dtype=_U8, device=dev)
             ws_ptr = workspace.data_ptr()
-    args = _MX_ATTN.pack(_mx_dev(q, "q"), new_k_ptr, new_v_ptr, _mx_dev(out, "out"), lse_ptr, _mx_lens(lens, b), k.args, v.args,
+    args = _MX_ATTN.pack(q_ptr, new_k_ptr, new_v_ptr, out_ptr, lse_ptr, _mx_lens(lens, b), k.args, v.args,
                          ws_ptr, ws_bytes, b, h, group, hd, n_rows, n_sink, window, hd ** -0.5 if scale is None else scale)
     _check(lib.dc_mx_attn_bf16(args, _mx_stream(k, v)))
     return out if lse is None else (out, lse)
