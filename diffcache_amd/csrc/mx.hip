@@ -274,15 +274,15 @@ __global__ __launch_bounds__(kThreads) void mx_gather_kernel(GatherArgs a, int h
 //               scale included, exactly (one conversion for two numbers), and are operands as they come: which columns an
 //               instruction takes is free as long as Q's are the same, so lane (q, c) = (lane / 16, lane % 16) has 16 bytes (8
 //               of 64 columns in 4 bits) of one row, the row's four lanes side by side.  (The instructions that multiply
-//               4-bit and 8-bit numbers as they are round their sums at some 2^-15 of the largest product: measured, and not
-//               enough for logits.)
+//               4-bit and 8-bit numbers as they are gave sums off by up to 2^-13 of that of the products' magnitudes: not
+//               enough for logits of a few tens.)
 //   softmax     The heads of a group of up to GP stand in the columns again and again, and lane c keeps the result of tile
 //               c / GP only: 64 rows of 4 heads are then 4 numbers a lane, none of them idle.  In powers of two.  The maximum
 //               moves only where a logit passes it by more than 8: rare, so nothing crosses lanes from step to step, and a
 //               weight is at most 2^8 of fp32 sums.
 //   O = P V     M = (tile, head) as the lanes have them, N = 16 of the hd columns, K = 32 rows of two tiles; P of the tiles that are not
-//               a lane's is zero.  P is the sum of two bf16 numbers: 2^-16 of a weight is lost at most, which the output's own
-//               2^-8 covers (a third instruction of every three would buy the rest).  Column n of instruction j is hd / 16 n + j,
+//               a lane's is zero.  P is the sum of two bf16 numbers: 2^-16 of a weight is lost at most, far below the output's own
+//               2^-8.  Column n of instruction j is hd / 16 n + j,
 //               so that a lane loads adjacent codes of its own rows and pairs of rows are put together by byte permutes.
 //
 // Which row of a tile is which row of M is free as long as K and V agree: M row 4 q + i is the tile's row 4 i + q, so that

@@ -528,3 +528,95 @@ def test_sizes_of_nothing():
     none = hip().MxStore.zeros(0, 2, 5, 64, 4, DEV)
     assert hip().mx_attn(q[:0], none, none).shape[0] == 0
     assert hip().mx_gather_rows(none, none)[0].shape == (0, 2, 5, 64)
+
+
+def test_arguments_in_other_forms():
+    """q as one row a sequence, strided, off its alignment and as the output; stores of unequal room; out and lse given."""
+    rng = np.random.default_rng(25)
+    b, h, g, hd, n = 3, 2, 4, 128, 700
+    ks, vs = store_of(keys(rng, (b, h, n, hd)), 4), store_of(rng.standard_normal((b, h, n + 9, hd)), 8)
+    q, qx = bf16(rng.standard_normal((b, h * g, hd)))
+    want, want_lse = check_attention(q, qx, ks, vs, [700, 650, 1])
+    lens = torch.tensor([700, 650, 1], dtype=torch.int32, device=DEV)
+    assert torch.equal(hip().mx_attn(q.view(b, 1, h * g * hd), ks, vs, lens), want)
+    wide = torch.zeros((b, h * g, 2 * hd + 1), dtype=torch.bfloat16, device=DEV)
+    wide[..., 1:hd + 1] = q
+    assert torch.equal(hip().mx_attn(wide[..., 1:hd + 1], ks, vs, lens), want)
+    flat = torch.zeros(q.numel() + 3, dtype=torch.bfloat16, device=DEV)
+    flat[3:] = q.flatten()
+    assert torch.equal(hip().mx_attn(flat[3:].view(q.shape), ks, vs, lens), want)
+    lse = torch.empty((b, h * g), device=DEV)
+    same = q.clone()
+    out, got = hip().mx_attn(same, ks, vs, lens, out=same, lse=lse)
+    assert out is same and got is lse and torch.equal(out, want) and torch.equal(lse, want_lse)
+    ws = torch.full((hip().mx_attn_workspace_bytes(b * h * 7, g, hd, 9 * n),), 0xff, dtype=torch.uint8, device=DEV)
+    long_k, long_v = store_of(keys(rng, (b, h, 5000, hd)), 4), store_of(rng.standard_normal((b, h, 5000, hd)), 4)
+    check_attention(q, qx, long_k, long_v, [4999, 3, 0], workspace=ws)          # whatever it held, and more of it than needed
+    check_attention(q, qx, long_k, long_v, [0, 0, 0], workspace=ws)
+    # the token's rows in the shape of a model's projection, cut out of it
+    fused = torch.randn((b, 1, 3 * h, hd), device=DEV).to(torch.bfloat16)
+    nk, nv = fused[:, :, h:2 * h], fused[:, :, 2 * h:]
+    one, two = store_of(held(ks)[:, :, :650], 4, 701), store_of(held(vs)[:, :, :650], 8, 701)
+    hip().mx_attn(q, one, two, lens.clamp(max=650), new_k=nk, new_v=nv)
+    back_k, back_v = hip().mx_gather_rows(one, two, lens.clamp(max=650).view(b, 1).expand(b, h).reshape(b * h, 1))
+    for got, new, bits in ((back_k, nk, 4), (back_v, nv, 8)):
+        assert np.array_equal(f64(got)[:, :, 0], ref.decode(*ref.encode(f64(new)[:, 0], bits)))
+
+
+def test_very_many_sequences():
+    rng = np.random.default_rng(26)
+    b, n, hd = 70001, 2, 64
+    x = np.zeros((b, 1, n, hd))
+    x[:, 0, :, :4] = rng.integers(-6, 7, (b, n, 4)) / 2
+    x[:, 0, :, 32] = 6
+    ks = vs = store_of(x, 4)
+    q = torch.zeros((b, 2, hd), dtype=torch.bfloat16, device=DEV)
+    q[:, :, 0] = 1
+    lens = torch.arange(b, dtype=torch.int32, device=DEV) % 3
+    out, lse = hip().mx_attn(q, ks, vs, lens, scale=1.0, want_lse=True)
+    live = np.arange(n)[None] < (np.arange(b) % 3)[:, None]
+    e = np.where(live, np.exp(held(ks)[:, 0, :, 0]), 0.0)
+    total = e.sum(1)
+    want = np.where(total[:, None] > 0, (e[:, :, None] * held(vs)[:, 0]).sum(1) / np.maximum(total, 1e-30)[:, None], 0.0)
+    assert (np.abs(f64(out) - want[:, None]) <= 2.0 ** -8 * np.abs(want)[:, None] + 2.0 ** -13 * 6).all()
+    assert np.array_equal(np.isinf(f64(lse)[:, 0]), total == 0)
+
+
+def test_wrappers_refuse_on_the_gpu():
+    m = hip()
+    ks, vs = m.MxStore.zeros(2, 2, 40, 128, 4, DEV), m.MxStore.zeros(2, 2, 40, 128, 8, DEV)
+    q = torch.zeros((2, 8, 128), dtype=torch.bfloat16, device=DEV)
+    nk = torch.zeros((2, 2, 128), dtype=torch.bfloat16, device=DEV)
+    lens = torch.zeros(2, dtype=torch.int32, device=DEV)
+    src = torch.zeros((2, 10, 2, 128), dtype=torch.bfloat16, device=DEV)
+    bad = [
+        (lambda: m.mx_attn(q.half(), ks, vs, lens), "bf16"), (lambda: m.mx_attn(q[:, :7], ks, vs, lens), "values"),
+        (lambda: m.mx_attn(q.cpu(), ks, vs, lens), "GPU memory"), (lambda: m.mx_attn(q, ks, vs, lens.long()), "int32"),
+        (lambda: m.mx_attn(q, ks, vs, lens[:1]), "2 elements"), (lambda: m.mx_attn(q, ks, vs, lens.cpu()), "GPU memory"),
+        (lambda: m.mx_attn(q, ks, vs, lens, n_rows=41), "outside"), (lambda: m.mx_attn(q, ks, vs, lens, window=-1), "negative"),
+        (lambda: m.mx_attn(q, ks, vs, lens, new_k=nk), "together"), (lambda: m.mx_attn(q, ks, vs, lens, new_k=nk, new_v=nk[:1]), "new_v"),
+        (lambda: m.mx_attn(q, ks, vs, lens, out=q.float()), "out"), (lambda: m.mx_attn(q, ks, vs, lens, out=q[:, :4]), "out"),
+        (lambda: m.mx_attn(q, ks, vs, lens, lse=q.float()), "lse"), (lambda: m.mx_attn(q.repeat(1, 5, 1), ks, vs, lens), "group"),
+        (lambda: m.mx_attn(q, ks, m.MxStore.zeros(2, 1, 40, 128, 4, DEV), lens), "belong"),
+        (lambda: m.mx_attn(q, ks, m.MxStore.zeros(2, 2, 40, 64, 4, DEV), lens), "belong"),
+        (lambda: m.mx_ingest(ks, vs, src, src, dst_pos=31), "outside"), (lambda: m.mx_ingest(ks, vs, src, src[:, :9]), "v_src"),
+        (lambda: m.mx_ingest(ks, vs, src.float(), src), "k_src"), (lambda: m.mx_ingest(ks, vs, src[0], src[0]), "k_src"),
+        (lambda: m.mx_ingest(ks, vs, src, src, dst_pos=-1), "outside"), (lambda: m.mx_ingest(ks, vs, src, src, lens=lens.float()), "int32"),
+        (lambda: m.mx_append(ks, vs, nk, nk[:, :1], lens), "new_v"), (lambda: m.mx_append(ks, vs, nk, nk, None), "null"),
+        (lambda: m.mx_gather_rows(None, None), "neither"), (lambda: m.mx_gather_rows(ks, vs, lens), "idx"),
+        (lambda: m.mx_gather_rows(ks, vs, lens.view(1, 2).expand(4, 2), n_idx=3), "idx"),
+        (lambda: m.mx_gather_rows(ks, vs, torch.zeros((4, 2), device=DEV)), "idx"), (lambda: m.mx_gather_rows(ks, vs, row_offset=-1), "negative"),
+        (lambda: m.mx_gather_rows(ks, vs, n_idx=10, out_k=nk.view(2, 2, 1, 128)), "out_k"),
+        (lambda: m.mx_gather_rows(ks, None, n_idx=1, out_v=nk.view(2, 2, 1, 128)), "each with its store"),
+        (lambda: m.mx_gather_rows(ks, vs, n_idx=5, out_k=src[:, :5].transpose(1, 2)), "share"),
+        (lambda: m.MxStore(ks.codes, vs.scale.cpu()), "GPU memory"),
+    ]
+    before = ks.codes.clone()
+    for call, message in bad:
+        with pytest.raises(m.DiffCacheError, match=message):
+            call()
+    small = torch.empty(256, dtype=torch.uint8, device=DEV)
+    big = [m.MxStore.zeros(2, 2, 5000, 128, 4, DEV) for _ in range(2)]
+    with pytest.raises(m.DiffCacheError, match="needed"):
+        m.mx_attn(q, *big, lens, workspace=small)
+    assert torch.equal(ks.codes, before) and not torch.isnan(m.mx_attn(q, ks, vs, lens).float()).any()
