@@ -749,12 +749,11 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
 }
 
 // The parts of one query head joined: one block per (unit, head).  What it reads is asked for at once, before any weight is
-// known: rounds of kBatch kParts parts (32 at 128 columns), HD / 4 threads to a part.  A kernel's start and two round trips: 64
-// parts of 32 heads 3.9 us (5.5 part by part), 8 parts of 256 heads 4.8.
-constexpr int kBatch = 4;
+// known: rounds of kBatch kParts parts (32 at 128 and at 256 columns, 64 at 64), HD / 4 threads to a part.  A kernel's start and two round trips: 64
+// parts of 32 heads 3.9 us (5.5 part by part), 8 parts of 256 heads 4.8, 128 parts of 16 heads of 256 columns 5.0 (6.2 in rounds of 16).
 template <int HD>
 __global__ __launch_bounds__(kThreads) void mx_merge_kernel(AttnArgs a) {
-    constexpr int kLanes = HD / 4, kParts = kThreads / kLanes;
+    constexpr int kLanes = HD / 4, kParts = kThreads / kLanes, kBatch = HD == 256 ? 8 : 4;
     __shared__ float4 s_acc[kThreads];
     const int unit = blockIdx.x / a.group, g = blockIdx.x % a.group, tid = threadIdx.x, lane = tid & 63, n = a.n_splits;
     const int64_t slot0 = (int64_t)unit * n * a.group + g;
