@@ -399,7 +399,7 @@ struct Attn {
     static constexpr int STEP = 16 * TILES;
     static constexpr int CH = HD / 32;          // products of a tile's S; blocks of a row
     static constexpr int EPL = HD / 16;         // columns of V of a lane
-    // K: KN loads of KBYTES, those of a row's four lanes side by side; a load is KCOLS columns, in KS blocks a lane has a part of
+    // K: KN loads of KBYTES, KCOLS columns of one block each, those of a row's four lanes side by side
     static constexpr int KCOLS = HD == 64 ? 16 : 128 / KB, KN = HD / 4 / KCOLS, KBYTES = KCOLS * KB / 8, KW = KN * KBYTES / 4;
     static constexpr int kcol(int j) { return j * 8 / KCOLS * 4 * KCOLS + j * 8 % KCOLS; }  // first column of chunk j, of lanes q = 0
     static constexpr int VBYTES = EPL * VB / 8, VW = VBYTES < 4 ? 1 : VBYTES / 4;
