@@ -474,6 +474,39 @@ def test_captured_steps_follow_the_lengths():
             assert torch.equal(c["ks"].codes, c["eager"][0].codes) and torch.equal(c["lens"], lens + 1)
 
 
+def test_writing_and_reading_back_captured():
+    """Prompts, a token and rows read back in one graph, replayed on other inputs among eager work: every replay against eager calls."""
+    b, h, seq, hd = 2, 3, 150, 128
+    src = [torch.zeros((b, seq, h, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    new = [torch.zeros((b, h, hd), dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    lens = torch.tensor([seq, 20], dtype=torch.int32, device=DEV)
+    idx = torch.zeros((b * h, 9), dtype=torch.int32, device=DEV)
+    stores = [[m.zeros(b, h, seq + 1, hd, bits, DEV) for bits in (4, 8)] for m in (hip().MxStore, hip().MxStore)]
+
+    def work(k, v):
+        hip().mx_ingest(k, v, *src, lens=lens)
+        hip().mx_append(k, v, *new, lens)
+        return hip().mx_gather_rows(k, v) + hip().mx_gather_rows(k, v, idx, row_offset=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured = work(*stores[0])
+    for i in range(5):
+        for t in src + new:
+            t.copy_(torch.randn(t.shape, device=DEV) * 2.0 ** (10 * i - 20))
+        lens.copy_(torch.tensor([seq - i, 20 + 25 * i], dtype=torch.int32))
+        idx.copy_(torch.randint(0, seq, idx.shape, device=DEV))
+        graph.replay()
+        eager = work(*stores[1])
+        if i % 2:
+            torch.cuda.synchronize()
+        for x, y in zip(captured, eager):
+            assert torch.equal(x, y), i
+        for x, y in zip(*stores):
+            assert torch.equal(x.codes, y.codes) and torch.equal(x.scale, y.scale)
+
+
 def test_two_streams_at_once():
     rng = np.random.default_rng(17)
     ks, vs = store_of(keys(rng, (2, 4, 9000, 128)), 4), store_of(rng.standard_normal((2, 4, 9000, 128)), 4)
