@@ -1055,12 +1055,21 @@ class MxStore:
         self.shape, self.units, self.hd, self.bits = (b, h, n, hd), (b, h, hd), hd, bits
         self.args = _MX_STORE.pack(codes.data_ptr(), scale.data_ptr(), cb, ch, sb, sh, bits, n)
 
+    def __reduce__(self):
+        return _mx_store_again, (self.codes, self.scale)    # args holds addresses of this store's tensors, not of a copy's
+
     @classmethod
     def zeros(cls, b: int, h: int, n: int, hd: int, bits: int, device) -> "MxStore":
         if bits not in (4, 8) or hd not in (64, 128, 256):
             raise DiffCacheError(f"a store of {bits} bits and head_dim {hd} is not supported (4 or 8; 64, 128 or 256)")
         return cls(torch.zeros((b, h, n, hd * bits // 8), dtype=torch.uint8, device=device),
                    torch.zeros((b, h, n, hd // 32), dtype=torch.uint8, device=device))
+
+
+def _mx_store_again(codes: torch.Tensor, scale: torch.Tensor) -> MxStore:
+    """A copied or unpickled store: over the copied tensors, on their device whichever is current."""
+    with torch.cuda.device(codes.get_device()):
+        return MxStore(codes, scale)
 
 
 def _mx_pair(k: MxStore, v: MxStore) -> Tuple[int, int, int]:
