@@ -408,6 +408,10 @@ struct Attn {
     static constexpr int SETS = 16 / GP < TILES ? 16 / GP : TILES;  // tiles whose logits share a register
     static constexpr int REGS = TILES / SETS;   // logit registers of a lane (times 4)
 
+    // A head's maximum before any logit passed it, in a wave with rows (-inf stands for no rows): finite, so that a row whose logit is
+    // -inf has the weight 0 then too, where -inf - -inf would be NaN.
+    static constexpr float kLowest = -3.402823466e+38f;
+
     mx_u32x4 bq[CH];
     uint32_t kw[TILES][KW], ks[CH > 4 ? 2 : 1];
     uint32_t vw[TILES * 4][VW], vs[CH > 4 ? 2 : 1];
@@ -525,8 +529,8 @@ struct Attn {
     // a new maximum for every head, and what was summed so far brought to it
     __device__ __forceinline__ void raise(float most) {
         const float to = fmaxf(m, mx_over_lanes<GP>(most, [](float a, float b) { return fmaxf(a, b); }));
-        if (__any(m > -INFINITY)) {
-            const float f = m > -INFINITY ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
+        if (__any(m > kLowest)) {
+            const float f = m > kLowest ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
             l *= f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -681,6 +685,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
     // The token's row is the unit's last: the wave with the last step writes it first and takes that step last, token or not (so
     // that a row written beforehand gives the same sums).
     const bool last = mine > 0 && begin + wave + (mine - 1) * waves == p.steps - 1, writes = last && p.rows > p.len;
+    if (mine > 0) w.m = T::kLowest;
     int at = last ? 0 : (int)(((uint64_t)turn * (uint32_t)mine) >> 32);
     if (writes) mx_write_token<KB, VB>(a.k, a.v, a.new_k, a.new_v, HD, unit, b, h, p.len, lane);
     int64_t row;
@@ -742,7 +747,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
                 ml[0] = top, ml[1] = total;
             }
         } else {
-            a.out[(int64_t)unit * G * HD + o] = dc_f32_to_bf16(total == 0.f ? 0.f : sum / total);
+            a.out[(int64_t)unit * G * HD + o] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
             if (a.lse && o % HD == 0) a.lse[(int64_t)unit * G + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f;
         }
     }
@@ -803,7 +808,7 @@ __global__ __launch_bounds__(kThreads) void mx_merge_kernel(AttnArgs a) {
         float sum = x[0];
 #pragma unroll
         for (int i = 1; i < kParts; ++i) sum += x[i * HD];
-        a.out[(int64_t)blockIdx.x * HD + tid] = dc_f32_to_bf16(total == 0.f ? 0.f : sum / total);
+        a.out[(int64_t)blockIdx.x * HD + tid] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
     }
     if (a.lse && tid == 0) a.lse[blockIdx.x] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f;
 }
