@@ -59,17 +59,20 @@ class MxCache:
         hip.require(0 < seq <= self.max_length, "the prompt is empty or longer than max_length")
         # a replay would move the rows and leave the host's length as it is
         hip.require(not torch.cuda.is_current_stream_capturing(), "a prefill cannot be captured in a graph")
-        if lens is None:
-            self.lens.fill_(seq)
-            self._longest = seq
-        else:
+        at, longest = None, seq
+        if lens is not None:
             lens = [int(x) for x in lens]
             hip.require(len(lens) == self.batch_size and all(0 <= x <= seq for x in lens), "lens does not fit the prompts")
             # (from pinned memory: nothing waits for the device)
-            self.lens.copy_(torch.tensor(lens, dtype=torch.int32, pin_memory=True), non_blocking=True)
-            self._longest = max(lens)
-        hip.mx_ingest(self.kstore[layer_idx], self.vstore[layer_idx], key_states, value_states,
-                      lens=None if lens is None else self.lens)
+            at = torch.tensor(lens, dtype=torch.int32, pin_memory=True).to(self.device, non_blocking=True)
+            longest = max(lens)
+        hip.mx_ingest(self.kstore[layer_idx], self.vstore[layer_idx], key_states, value_states, lens=at)
+        # only now: a call that was refused leaves the lengths of what the cache holds
+        if at is None:
+            self.lens.fill_(seq)
+        else:
+            self.lens.copy_(at)
+        self._longest = longest
         return key_states, value_states
 
     def decode_attention(self, layer_idx: int, queries: torch.Tensor, key_states: torch.Tensor,
