@@ -1006,6 +1006,8 @@ def compose_idx(outer: torch.Tensor, inner: torch.Tensor) -> torch.Tensor:
 # a cache in blocks of 32 numbers (dc_mx_store)
 # ---------------------------------------------------------------------------
 
+MX_MAX_GROUP = 16   # query heads to a KV head, at most
+
 # The two structs' bytes.  (A call of these wrappers costs a few microseconds, as much as the kernels of a short context:
 # every attribute is read once and every tensor made in the cheapest way.)
 _MX_STORE = struct.Struct("@2P4q2i")

@@ -32,7 +32,10 @@ class MxCache:
                  head_dim: int, key_bits: int = 4, value_bits: int = 4, sink_len: int = 0, window: int = 0,
                  device: str = "cuda") -> None:
         hip.require(num_layers >= 1 and batch_size >= 1 and max_length >= 1, "a cache needs layers, sequences and rows")
-        hip.require(num_q_heads % num_kv_heads == 0, "num_q_heads must be a multiple of num_kv_heads")
+        hip.require(num_kv_heads >= 1 and num_q_heads >= 1 and num_q_heads % num_kv_heads == 0,
+                    "num_q_heads must be a multiple of num_kv_heads")
+        hip.require(num_q_heads // num_kv_heads <= hip.MX_MAX_GROUP,
+                    f"more than {hip.MX_MAX_GROUP} query heads to a KV head are not supported")
         hip.require(sink_len >= 0 and window >= 0, "sink_len and window must not be negative")
         self.num_layers, self.batch_size, self.max_length = num_layers, batch_size, max_length
         self.num_kv_heads, self.num_q_heads, self.head_dim = num_kv_heads, num_q_heads, head_dim

@@ -31,3 +31,19 @@ def test_a_copied_store_names_its_own_memory(on_cpu, again):
     assert (other.shape, other.units, other.hd, other.bits) == (store.shape, store.units, store.hd, store.bits)
     # strides, room and bits go along
     assert struct.unpack("@2P4q2i", other.args)[2:] == struct.unpack("@2P4q2i", store.args)[2:]
+
+
+@pytest.mark.parametrize("hkv,hq,message", [(2, 34, "query heads"), (1, 32, "query heads"), (2, 7, "multiple"), (0, 4, "multiple"),
+                                            (2, 0, "multiple"), (-1, 4, "multiple")])
+def test_heads_that_no_step_could_attend_with_are_refused_at_once(hkv, hq, message):
+    """Before any memory is taken: where there is no GPU, anything later fails otherwise."""
+    from diffcache_amd import MxCache
+    with pytest.raises(AssertionError, match=message):
+        MxCache(1, 1, 64, hkv, hq, 128)
+
+
+def test_the_largest_group_is_the_library_s():
+    store = hip.MxStoreArgs(1 << 20, 1 << 21, 4096, 4096, 256, 256, 4, 64)
+    p = 1 << 22
+    args = hip.MxAttnArgs(p, None, None, p, None, p, store, store, p, 1 << 30, 2, 2, hip.MX_MAX_GROUP + 1, 128, 64, 0, 0, 0.1)
+    assert hip.lib.dc_mx_attn_bf16(bytes(args), None) == -22 and f"not in [1,{hip.MX_MAX_GROUP}]" in hip.lib.dc_last_error().decode()
