@@ -925,7 +925,7 @@ extern "C" int dc_mx_ingest_bf16(const dc_mx_store *k, const dc_mx_store *v, con
     DC_REQUIRE(ksb % 8 == 0 && kss % 8 == 0 && ksh % 8 == 0 && vsb % 8 == 0 && vss % 8 == 0 && vsh % 8 == 0,
                "%s: strides must be multiples of 8 elements", who);
     const int rows_per = kThreads / (hd / 8) * kIngestBatch;
-    const int64_t chunks = (seq + rows_per - 1) / rows_per;
+    const int64_t chunks = ((int64_t)seq + rows_per - 1) / rows_per;
     DC_TRY(check_grid(who, n_units, chunks, rows_per));
     IngestArgs a = {view_of(*k), view_of(*v), (const uint16_t *)k_src, (const uint16_t *)v_src, ksb, kss, ksh, vsb, vss, vsh,
                     lens, n_h, seq, dst_pos, (int)chunks};

@@ -47,3 +47,23 @@ def test_the_largest_group_is_the_library_s():
     p = 1 << 22
     args = hip.MxAttnArgs(p, None, None, p, None, p, store, store, p, 1 << 30, 2, 2, hip.MX_MAX_GROUP + 1, 128, 64, 0, 0, 0.1)
     assert hip.lib.dc_mx_attn_bf16(bytes(args), None) == -22 and f"not in [1,{hip.MX_MAX_GROUP}]" in hip.lib.dc_last_error().decode()
+
+
+def refused(rc, message):
+    assert rc == -22 and message in hip.lib.dc_last_error().decode(), (rc, hip.lib.dc_last_error())
+
+
+def long_store(n_rows, hd, bits=4):
+    """A store of one unit that no kernel is launched on."""
+    return bytes(hip.MxStoreArgs(1 << 20, 1 << 21, 0, 0, 0, 0, bits, n_rows))
+
+
+@pytest.mark.parametrize("hd,rows_per", [(64, 128), (128, 64), (256, 32)])
+def test_prompts_near_the_end_of_32_bits_are_refused(hd, rows_per):
+    """A thread's row numbers, those past the end too, are ints: of the last block all have to be."""
+    last, p = 2**31 - 1, 1 << 22
+    s = long_store(last, hd)
+    for seq, dst in ((last, 0), (last - 1, 1), (last - rows_per + 2, 0)):   # (the sum of seq and rows_per - 1 passes 2^31)
+        refused(hip.lib.dc_mx_ingest_bf16(s, s, p, p, None, 1, seq, 1, hd, dst, 0, 0, 0, 0, 0, 0, None), "grid too large")
+    for n in (last, last - 1):
+        refused(hip.lib.dc_mx_gather_rows_bf16(s, s, None, p, p, 1, 1, n, 0, hd, 0, 0, 0, 0, None), "grid too large")
