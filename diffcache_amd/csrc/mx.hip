@@ -841,9 +841,12 @@ int check_units(const char *who, int n_b, int n_h, int hd) {
     return DC_OK;
 }
 
-// blocks of a unit in a grid of (unit, chunk) by n_units * chunks; the last one's rows, those beyond the end too, are ints
+// A launch has less than 2^32 threads in a dimension.
+bool grid_fits(int64_t blocks, int threads) { return blocks * threads < (1ll << 32); }
+
+// chunks: blocks of a unit in a grid of (unit, chunk) in one dimension; the last one's rows, those beyond the end too, are ints
 int check_grid(const char *who, int64_t n_units, int64_t chunks, int rows_per) {
-    DC_REQUIRE(n_units * chunks < (1ll << 31) && chunks * rows_per < (1ll << 31), "%s: grid too large", who);
+    DC_REQUIRE(grid_fits(n_units * chunks, kThreads) && chunks * rows_per < (1ll << 31), "%s: grid too large", who);
     return DC_OK;
 }
 
@@ -1007,7 +1010,8 @@ extern "C" int dc_mx_attn_bf16(const dc_mx_attn_args *x, void *stream) {
                "%s: pointers must be 16-byte aligned", who);
     DC_REQUIRE(x->n_h < (1 << 16), "%s: too many heads", who);
     const int64_t attended = x->window > 0 && (int64_t)x->n_sink + x->window < x->n_rows ? x->window : x->n_rows;
-    const AttnCut cut = attn_cut(n_units, x->hd, attended, attended < x->n_rows ? x->n_sink : 0, x->k.bits + x->v.bits);
+    AttnCut cut = attn_cut(n_units, x->hd, attended, attended < x->n_rows ? x->n_sink : 0, x->k.bits + x->v.bits);
+    if (!grid_fits(x->n_b, cut.waves * 64)) cut.waves = kWaves;  // (of four waves all units fit that check_units lets through)
     AttnArgs a;
     a.n_splits = cut.n_splits, a.waves = cut.waves;
     a.per_split = (uint32_t)((0xffffffffull + a.n_splits) / a.n_splits);

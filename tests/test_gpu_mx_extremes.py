@@ -110,3 +110,27 @@ def test_logits_above_fp32(n):
     bad = torch.isnan(out[0])
     assert bad[1].all() and bad.sum() == 128
     assert torch.isnan(lse[0, 1]) and torch.isfinite(lse[0, [0, 2, 3]]).all()
+
+
+def test_eight_million_sequences():
+    """Units of eight waves would be more threads than a launch takes: they are of four."""
+    b, n, hd = 1 << 23, 257, 64
+    rng = np.random.default_rng(3)
+    k, v = rng.integers(-2, 3, (1, 1, n, hd)) / 2, rng.choice([-6.0, -3, -1, 0, 1, 2, 4], (1, 1, n, hd))
+    m = hip()
+    ks, vs = (m.MxStore(s.codes.expand(b, -1, -1, -1), s.scale.expand(b, -1, -1, -1)) for s in (store_of(k, 4), store_of(v, 4)))
+    q = torch.from_numpy(rng.integers(-4, 5, (1, 1, hd)) / 4).to(torch.bfloat16).to(DEV)
+    lens = torch.arange(b, dtype=torch.int32, device=DEV) % (n + 1)
+    out, lse = m.mx_attn(q.expand(b, 1, hd), ks, vs, lens, scale=0.125, want_lse=True)
+    qx = q.double().cpu().numpy()[0]
+    want = [ref.attention(qx, k[0, 0, :i], v[0, 0, :i], 0.125) for i in range(n + 1)]
+    # logits are exact; weights, their sums and P as in check()
+    rel = 2.0 ** -15 + (4 + n) * 2.0 ** -23
+    o = torch.from_numpy(np.concatenate([x[0] for x in want])).to(DEV)
+    tol = 2.0 ** -8 * o.abs() + torch.from_numpy(np.concatenate([x[2] for x in want])).to(DEV) * rel * (1 + 2.0 ** -7)
+    e = torch.from_numpy(np.concatenate([x[1] for x in want])).to(DEV)
+    for lo in range(0, b, 1 << 20):
+        at = lens[lo:lo + (1 << 20)].long()
+        assert ((out[lo:lo + (1 << 20), 0].double() - o[at]).abs() <= tol[at]).all()
+        got = lse[lo:lo + (1 << 20), 0].double()
+        assert (got[at == 0] == -math.inf).all() and ((got - e[at])[at > 0].abs() <= rel + 2.0 ** -20).all()

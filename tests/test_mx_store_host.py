@@ -67,3 +67,11 @@ def test_prompts_near_the_end_of_32_bits_are_refused(hd, rows_per):
         refused(hip.lib.dc_mx_ingest_bf16(s, s, p, p, None, 1, seq, 1, hd, dst, 0, 0, 0, 0, 0, 0, None), "grid too large")
     for n in (last, last - 1):
         refused(hip.lib.dc_mx_gather_rows_bf16(s, s, None, p, p, 1, 1, n, 0, hd, 0, 0, 0, 0, None), "grid too large")
+
+
+def test_more_blocks_than_a_launch_takes_are_refused():
+    """2^24 blocks of 256 threads: one more thread than a launch counts."""
+    p, b, h, hd = 1 << 22, 1 << 12, 1 << 11, 64
+    s = bytes(hip.MxStoreArgs(1 << 20, 1 << 30, h * 160 * 32, 160 * 32, h * 160 * 2, 160 * 2, 4, 160))
+    refused(hip.lib.dc_mx_ingest_bf16(s, s, p, p, None, b, 129, h, hd, 0, 0, 0, 0, 0, 0, 0, None), "grid too large")
+    refused(hip.lib.dc_mx_gather_rows_bf16(s, s, None, p, p, b, h, 65, 0, hd, 0, 0, 0, 0, None), "grid too large")
