@@ -815,6 +815,25 @@ __global__ __launch_bounds__(kThreads) void mx_merge_kernel(AttnArgs a) {
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
+// Whether no two of n_b x n_h units, size bytes each, have a byte in common: every pair is an offset of i sb and one of j sh apart.
+bool units_apart(int64_t n_b, int64_t n_h, uint64_t sb, uint64_t sh, uint64_t size) {
+    if ((n_h <= 1 || sh >= size) && (n_b <= 1 || sb >= (uint64_t)(n_h - 1) * sh + size)) return true;  // (a sequence behind the other)
+    if (n_b > n_h) {
+        const int64_t n = n_b;
+        const uint64_t s = sb;
+        n_b = n_h, sb = sh, n_h = n, sh = s;
+    }
+    // n_b is the smaller count: for every i sb the multiples of sh next to it
+    for (int64_t i = 0; i < n_b; ++i) {
+        const uint64_t x = (uint64_t)i * sb;
+        uint64_t j = sh ? x / sh : 0;
+        if (j > (uint64_t)(n_h - 1)) j = (uint64_t)(n_h - 1);
+        if ((i || j) && x - j * sh < size) return false;
+        if (j + 1 < (uint64_t)n_h && (j + 1) * sh - x < size) return false;
+    }
+    return true;
+}
+
 int check_store(const char *who, const char *which, const dc_mx_store &s, int n_b, int n_h, int hd, bool written) {
     DC_REQUIRE(s.bits == 4 || s.bits == 8, "%s: %s holds %d bits, not 4 or 8", who, which, s.bits);
     DC_REQUIRE(s.n_rows >= 0, "%s: %s has a negative number of rows", who, which);
@@ -827,8 +846,8 @@ int check_store(const char *who, const char *which, const dc_mx_store &s, int n_
     DC_REQUIRE(s.code_batch_stride >= 0 && s.code_head_stride >= 0 && s.scale_batch_stride >= 0 && s.scale_head_stride >= 0,
                "%s: negative stride in %s", who, which);
     if (written) {
-        DC_REQUIRE((n_b <= 1 || (s.code_batch_stride > 0 && s.scale_batch_stride > 0)) &&
-                       (n_h <= 1 || (s.code_head_stride > 0 && s.scale_head_stride > 0)),
+        DC_REQUIRE(units_apart(n_b, n_h, (uint64_t)s.code_batch_stride, (uint64_t)s.code_head_stride, (uint64_t)s.n_rows * (hd * s.bits / 8)) &&
+                       units_apart(n_b, n_h, (uint64_t)s.scale_batch_stride, (uint64_t)s.scale_head_stride, (uint64_t)s.n_rows * blocks),
                    "%s: units of %s share their rows", who, which);
     }
     return DC_OK;

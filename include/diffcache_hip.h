@@ -643,8 +643,8 @@ int dc_data_layer_query(dc_data_layer *dl, void *out_keys, void *out_vals, int64
  * dc_mx_store names one tensor (K or V) of a layer: unit (b, h) has its rows' codes, hd * bits / 8 bytes each, one after another at
  *   codes + b * code_batch_stride + h * code_head_stride
  * and its rows' hd / 32 scales likewise; strides in bytes.  Codes are 16-byte aligned with strides multiples of 16, scales and
- * their strides multiples of hd / 32.  n_rows: the rows that a unit has room for.  Units that share rows (a stride of 0) may be
- * read, not written.  K and V may be held in different bits.  hd: 64, 128 or 256.
+ * their strides multiples of hd / 32.  n_rows: the rows that a unit has room for.  Units that share any of them (a stride of 0, or one
+ * shorter than the rows) may be read, not written.  K and V may be held in different bits.  hd: 64, 128 or 256.
  */
 typedef struct dc_mx_store {
     void *codes, *scale;

@@ -1,5 +1,6 @@
 """Stores and caches of the block-scaled kind without a GPU: copies, and calls that are refused before anything is launched."""
 import copy
+import itertools
 import pickle
 import struct
 
@@ -75,3 +76,57 @@ def test_more_blocks_than_a_launch_takes_are_refused():
     s = bytes(hip.MxStoreArgs(1 << 20, 1 << 30, h * 160 * 32, 160 * 32, h * 160 * 2, 160 * 2, 4, 160))
     refused(hip.lib.dc_mx_ingest_bf16(s, s, p, p, None, b, 129, h, hd, 0, 0, 0, 0, 0, 0, 0, None), "grid too large")
     refused(hip.lib.dc_mx_gather_rows_bf16(s, s, None, p, p, b, h, 65, 0, hd, 0, 0, 0, 0, None), "grid too large")
+
+
+def every_call(k, v, b, h, hd=128):
+    """The calls that write, each with stores that nothing else is wrong with."""
+    p = 1 << 22
+    yield lambda: hip.lib.dc_mx_ingest_bf16(k, v, p, p, None, b, 1, h, hd, 0, 0, 0, 0, 0, 0, 0, None)
+    yield lambda: hip.lib.dc_mx_append_bf16(k, v, p, p, p, b, h, hd, None)
+    args = hip.MxAttnArgs(p, p, p, p, None, p, hip.MxStoreArgs.from_buffer_copy(k), hip.MxStoreArgs.from_buffer_copy(v), None, 0, b, h, 1,
+                          hd, 1, 0, 0, 0.1)
+    yield lambda: hip.lib.dc_mx_attn_bf16(bytes(args), None)
+
+
+def store(b, h, n, cb, ch, sb, sh, bits=4):
+    return bytes(hip.MxStoreArgs(1 << 20, 1 << 21, cb, ch, sb, sh, bits, n))
+
+
+# strides in rows (64 and 4 bytes): batch, head; of units of 10 rows
+@pytest.mark.parametrize("b,h,code,scale", [
+    (3, 2, (20, 9), (20, 10)), (3, 2, (20, 10), (20, 9)), (3, 2, (19, 10), (20, 10)), (3, 2, (20, 10), (19, 10)), (3, 2, (10, 10), (20, 10)),
+    (3, 2, (1, 30), (20, 10)), (5, 1, (9, 0), (10, 0)), (1, 4, (0, 10), (0, 3)), (2, 2, (15, 10), (20, 10)), (2, 3, (25, 10), (30, 10)),
+    (3, 3, (10, 20), (30, 10)), (3, 1, (0, 0), (10, 0)), (1, 3, (0, 10), (0, 0)), (4, 7, (30, 45), (70, 10)),
+])
+def test_units_that_overlap_are_not_written(b, h, code, scale):
+    good = store(b, h, 10, h * 640, 640, h * 40, 40)
+    bad = store(b, h, 10, 64 * code[0], 64 * code[1], 4 * scale[0], 4 * scale[1])
+    for k, v in ((good, bad), (bad, good)):
+        for call in every_call(k, v, b, h):
+            refused(call(), "share their rows")
+
+
+@pytest.mark.parametrize("b,h,code,scale", [
+    (3, 2, (20, 10), (20, 10)), (3, 2, (10, 30), (10, 30)), (3, 2, (100, 10), (25, 12)), (1, 4, (0, 10), (0, 10)), (1, 4, (3, 10), (1, 10)),
+    (5, 1, (10, 0), (10, 1)), (2, 2, (15, 30), (10, 20)), (2, 3, (10, 20), (30, 10)), (1, 1, (0, 0), (0, 0)),
+])
+def test_units_that_lie_apart_are(b, h, code, scale):
+    """Apart also where the units of one sequence lie between another's: refused nowhere (without a GPU the launch fails)."""
+    s = store(b, h, 10, 64 * code[0], 64 * code[1], 4 * scale[0], 4 * scale[1])
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are made up")
+    for call in every_call(s, s, b, h):
+        assert call() == -5
+
+
+def test_overlap_against_every_pair_of_units():
+    """The rule against a comparison of all pairs, over small strides."""
+    if torch.cuda.is_available():
+        pytest.skip("the addresses are made up")
+    for b, h, n in ((2, 3, 2), (3, 2, 3), (4, 4, 1)):
+        for cb, ch in itertools.product(range(0, 9), repeat=2):
+            rows = [i * cb + j * ch for i in range(b) for j in range(h)]
+            apart = all(abs(x - y) >= n for x, y in itertools.combinations(rows, 2))
+            s = store(b, h, n, 64 * cb, 64 * ch, 4 * h * n, 4 * n)
+            rc = hip.lib.dc_mx_append_bf16(s, s, 1 << 22, 1 << 22, 1 << 22, b, h, 128, None)
+            assert rc == (-5 if apart else -22), (b, h, n, cb, ch)
