@@ -1257,6 +1257,8 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
     elif new_k is not new_v:
         raise DiffCacheError("new_k and new_v must be given together")
     if workspace is not None:
+        if not workspace.is_contiguous():
+            raise DiffCacheError("workspace must be contiguous")
         ws_ptr, ws_bytes = _mx_dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
     else:
         ws_bytes = lib.dc_mx_attn_workspace_bytes(b * h, group, hd, n_rows)

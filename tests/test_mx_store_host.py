@@ -130,3 +130,33 @@ def test_overlap_against_every_pair_of_units():
             s = store(b, h, n, 64 * cb, 64 * ch, 4 * h * n, 4 * n)
             rc = hip.lib.dc_mx_append_bf16(s, s, 1 << 22, 1 << 22, 1 << 22, b, h, 128, None)
             assert rc == (-5 if apart else -22), (b, h, n, cb, ch)
+
+
+class NotReached:
+    def __getattr__(self, name):
+        if name == "dc_mx_attn_workspace_bytes":
+            return lambda *a: 0
+        raise AssertionError(f"{name} was called")
+
+
+@pytest.fixture
+def no_library(on_cpu, monkeypatch):
+    """What a wrapper refuses by itself: a call that gets further fails."""
+    monkeypatch.setattr(hip, "lib", NotReached())
+    monkeypatch.setattr(hip, "_mx_stream", lambda k, v: 0)
+
+
+def cpu_store(b=1, h=2, n=2000, hd=128, bits=4):
+    return hip.MxStore(torch.zeros((b, h, n, hd * bits // 8), dtype=torch.uint8), torch.zeros((b, h, n, hd // 32), dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(1, dtype=torch.uint8).expand(1 << 24), torch.zeros(1 << 12, dtype=torch.uint8)[::2],
+                                       torch.zeros((2, 64), dtype=torch.float32).t()])
+def test_a_workspace_with_gaps_or_overlaps_is_refused(no_library, workspace):
+    """Its elements say nothing about the memory behind it."""
+    s = cpu_store()
+    q = torch.zeros((1, 8, 128), dtype=torch.bfloat16)
+    with pytest.raises(hip.DiffCacheError, match="workspace must be contiguous"):
+        hip.mx_attn(q, s, s, workspace=workspace)
+    with pytest.raises(AssertionError, match="dc_mx_attn_bf16"):    # a plain one goes on
+        hip.mx_attn(q, s, s, workspace=torch.zeros(1 << 12, dtype=torch.uint8))
