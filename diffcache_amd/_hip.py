@@ -1055,7 +1055,10 @@ class MxStore:
             _mx_dev(scale, "scale")
         self.codes, self.scale = codes, scale
         self.shape, self.units, self.hd, self.bits = (b, h, n, hd), (b, h, hd), hd, bits
-        self.args = _MX_STORE.pack(codes.data_ptr(), scale.data_ptr(), cb, ch, sb, sh, bits, n)
+        try:
+            self.args = _MX_STORE.pack(codes.data_ptr(), scale.data_ptr(), cb, ch, sb, sh, bits, n)
+        except struct.error as e:
+            raise DiffCacheError(f"a store of {n} rows does not fit the library's types: {e}") from None
 
     def __reduce__(self):
         return _mx_store_again, (self.codes, self.scale)    # args holds addresses of this store's tensors, not of a copy's
@@ -1168,6 +1171,8 @@ def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[tor
         idx_ptr = _mx_dev(idx, "idx")
     if n_idx < 0 or row_offset < 0:
         raise DiffCacheError("n_idx and row_offset must not be negative")
+    if n_idx >> 31 or row_offset >> 62:
+        raise DiffCacheError("n_idx or row_offset is too large")
     shape, own = (b, h, n_idx, hd), (h * n_idx * hd, n_idx * hd, hd, 1)
     k_ptr = v_ptr = None
     strides = None
@@ -1220,7 +1225,7 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
     b, h, hd = _mx_pair(k, v)
     numel = q.numel()
     hq = numel // (b * hd) if b else h
-    group = hq // h
+    group = hq // h if h else 0
     if q.dtype is not _BF16 or numel != b * h * group * hd or group < 1:
         raise DiffCacheError("q must be bf16 with (b, h * group, hd) values")
     if not q.is_contiguous() or q.data_ptr() & 15:
@@ -1265,7 +1270,11 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
         if ws_bytes:
             workspace = torch.empty(ws_bytes, dtype=_U8, device=dev)
             ws_ptr = workspace.data_ptr()
-    args = _MX_ATTN.pack(q_ptr, new_k_ptr, new_v_ptr, out_ptr, lse_ptr, _mx_lens(lens, b), k.args, v.args,
-                         ws_ptr, ws_bytes, b, h, group, hd, n_rows, n_sink, window, hd ** -0.5 if scale is None else scale)
+    lens_ptr = _mx_lens(lens, b)
+    try:
+        args = _MX_ATTN.pack(q_ptr, new_k_ptr, new_v_ptr, out_ptr, lse_ptr, lens_ptr, k.args, v.args,
+                             ws_ptr, ws_bytes, b, h, group, hd, n_rows, n_sink, window, hd ** -0.5 if scale is None else scale)
+    except struct.error as e:
+        raise DiffCacheError(f"n_rows, n_sink, window or scale does not fit its type: {e}") from None
     _check(lib.dc_mx_attn_bf16(args, _mx_stream(k, v)))
     return out if lse is None else (out, lse)

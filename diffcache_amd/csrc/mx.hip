@@ -978,7 +978,7 @@ extern "C" int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v
                                       int64_t dsr, void *stream) {
     const char *who = "dc_mx_gather_rows_bf16";
     DC_TRY(check_units(who, n_b, n_h, hd));
-    DC_REQUIRE(n_idx >= 0 && row_offset >= 0, "%s: bad sizes", who);
+    DC_REQUIRE(n_idx >= 0 && row_offset >= 0 && row_offset < (1ll << 62), "%s: bad sizes", who);  // (an id is added to it)
     const int64_t n_units = (int64_t)n_b * n_h;
     if (n_units == 0 || n_idx == 0) return DC_OK;
     DC_REQUIRE(out_k || out_v, "%s: null pointer", who);

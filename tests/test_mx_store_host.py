@@ -160,3 +160,30 @@ def test_a_workspace_with_gaps_or_overlaps_is_refused(no_library, workspace):
         hip.mx_attn(q, s, s, workspace=workspace)
     with pytest.raises(AssertionError, match="dc_mx_attn_bf16"):    # a plain one goes on
         hip.mx_attn(q, s, s, workspace=torch.zeros(1 << 12, dtype=torch.uint8))
+
+
+def test_numbers_that_no_c_type_holds_are_refused(no_library):
+    s = cpu_store()
+    q = torch.zeros((1, 8, 128), dtype=torch.bfloat16)
+    for bad in (dict(window=1 << 31), dict(n_sink=1 << 40), dict(n_sink=1.5), dict(window=1 << 64)):
+        with pytest.raises(hip.DiffCacheError, match="does not fit"):
+            hip.mx_attn(q, s, s, **bad)
+    out = torch.zeros((1, 1, 1, 128), dtype=torch.bfloat16).expand(1, 2, (1 << 32) + 3, 128)
+    for bad in (dict(n_idx=1 << 31), dict(n_idx=(1 << 32) + 3), dict(row_offset=1 << 63, n_idx=3), dict(row_offset=1 << 64, n_idx=3)):
+        with pytest.raises(hip.DiffCacheError, match="too large"):   # (ctypes would take the low bits)
+            hip.mx_gather_rows(s, None, out_k=out, **bad)
+    long = [torch.empty((1, 1, 1 << 31, row), dtype=torch.uint8, device="meta") for row in (64, 4)]
+    with pytest.raises(hip.DiffCacheError, match="does not fit"):
+        hip.MxStore(*long)
+
+
+def test_rows_past_any_row_are_refused_where_their_number_would_wrap():
+    s = long_store(64, 128)
+    for off in (1 << 62, 2**63 - 1):
+        refused(hip.lib.dc_mx_gather_rows_bf16(s, s, 1 << 22, 1 << 22, 1 << 22, 1, 1, 1, 1, 128, off, 128, 128, 128, None), "bad sizes")
+
+
+def test_a_store_without_heads_is_refused(no_library):
+    s = cpu_store(h=0)
+    with pytest.raises(hip.DiffCacheError, match="q must be"):
+        hip.mx_attn(torch.zeros((1, 0, 128), dtype=torch.bfloat16), s, s)
