@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import operator
 import os
 import struct
 from typing import Optional, Tuple
@@ -1031,7 +1032,9 @@ class MxStore:
     ``codes`` (b, h, n, hd * bits / 8) and ``scale`` (b, h, n, hd / 32), both uint8, a unit's rows one after another.  Views of
     larger tensors will do; ``MxStore.zeros`` makes a store of its own, whose rows read as zeros until they are written."""
 
-    __slots__ = ("codes", "scale", "shape", "units", "hd", "bits", "args")
+    __slots__ = ("_codes", "_scale", "shape", "units", "hd", "bits", "args")
+    codes = property(operator.attrgetter("_codes"))    # (not to be exchanged: args holds their addresses)
+    scale = property(operator.attrgetter("_scale"))
 
     def __init__(self, codes: torch.Tensor, scale: torch.Tensor):
         try:
@@ -1053,7 +1056,7 @@ class MxStore:
         if at < 0 or scale.get_device() != at or at != _device():
             _mx_dev(codes, "codes")
             _mx_dev(scale, "scale")
-        self.codes, self.scale = codes, scale
+        self._codes, self._scale = codes, scale
         self.shape, self.units, self.hd, self.bits = (b, h, n, hd), (b, h, hd), hd, bits
         try:
             self.args = _MX_STORE.pack(codes.data_ptr(), scale.data_ptr(), cb, ch, sb, sh, bits, n)
@@ -1127,7 +1130,7 @@ def mx_ingest(k: MxStore, v: MxStore, k_src: torch.Tensor, v_src: torch.Tensor, 
 def _mx_stream(k: MxStore, v: MxStore) -> int:
     """The current stream, for stores on the current device (which may have changed since they were made)."""
     at = _device()
-    if k.codes.get_device() != at or v.codes.get_device() != at:
+    if k._codes.get_device() != at or v._codes.get_device() != at:
         raise DiffCacheError(f"the stores live on {k.codes.device} and {v.codes.device}, the current device is cuda:{at}")
     return torch._C._cuda_getCurrentRawStream(at)
 

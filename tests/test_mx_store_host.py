@@ -187,3 +187,15 @@ def test_a_store_without_heads_is_refused(no_library):
     s = cpu_store(h=0)
     with pytest.raises(hip.DiffCacheError, match="q must be"):
         hip.mx_attn(torch.zeros((1, 0, 128), dtype=torch.bfloat16), s, s)
+
+
+def test_a_store_s_tensors_cannot_be_exchanged(on_cpu):
+    """Its calls go to the memory that it was made of."""
+    s = cpu_store(n=8)
+    for name in ("codes", "scale"):
+        t = getattr(s, name)
+        with pytest.raises(AttributeError):
+            setattr(s, name, t.clone())
+        assert getattr(s, name) is t
+    s.codes[:] = 3       # what they hold can be
+    assert addresses(s) == (s.codes.data_ptr(), s.scale.data_ptr()) and (s.codes == 3).all()
