@@ -1223,7 +1223,8 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
     """One token's attention over the cache (dc_mx_attn_bf16): q (b, h*group, hd) bf16 -> out of the same shape, over the
     first lens[b] rows of every sequence (``lens`` (b) int32 on the device; None: n_rows).  ``n_rows``: the most rows any
     sequence holds, which sizes the launch (default: the store's).  ``new_k`` / ``new_v`` (b, h, hd): the token's own row, written
-    to row lens[b] and attended to as it is held; lens is not changed.  ``window`` > 0: only the first ``n_sink`` rows and the
+    to row lens[b] and attended to as it is held; lens is not changed.  A negative length counts as 0 (the token's row is row 0 then,
+    unlike mx_append's); a sequence of n_rows or more has no row for it and keeps what it holds.  ``window`` > 0: only the first ``n_sink`` rows and the
     last ``window``.  With ``lse`` or ``want_lse`` returns (out, lse), lse (b, h*group) fp32 the log of the sum of exponentials."""
     b, h, hd = _mx_pair(k, v)
     numel = q.numel()

@@ -681,11 +681,13 @@ int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v, const uin
 
 /*
  * One token's attention over the cache: out (n_b, n_h * group, hd) bf16, softmax(scale q k^T) v over the rows of each sequence.
- *   lens     (n_b) int32 on the device, the rows that sequence b holds; NULL: n_rows, less one with a token of its own
+ *   lens     (n_b) int32 on the device, the rows that sequence b holds; NULL: n_rows, less one with a token of its own.  A negative
+ *            length counts as 0, so a token's row is row 0 then (dc_mx_append_bf16 skips it): an idle sequence whose rows
+ *            are to stay as they are is given n_rows or more
  *   n_rows   the most rows any sequence holds, the token's among them (at most the stores' rows): sizes the launch; rows
  *            at or beyond it are neither attended to nor written
- *   new_k, new_v  NULL, or (n_b, n_h, hd) bf16: the token's own row, written to row lens[b] as dc_mx_append_bf16 does and
- *            attended to as it is held.  lens is not changed
+ *   new_k, new_v  NULL, or (n_b, n_h, hd) bf16: the token's own row, written to row lens[b] and attended to as it is held.  lens
+ *            is not changed
  *   window   0: all rows; else the first n_sink and the last `window` (the token's own among them)
  *   lse      NULL, or (n_b, n_h * group) fp32: log of the sum of exp(scale q k^T)
  * A sequence without rows has out 0 and lse -inf.  Rows that are not attended to may hold anything; one that is and holds a NaN
