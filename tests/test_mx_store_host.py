@@ -199,3 +199,9 @@ def test_a_store_s_tensors_cannot_be_exchanged(on_cpu):
         assert getattr(s, name) is t
     s.codes[:] = 3       # what they hold can be
     assert addresses(s) == (s.codes.data_ptr(), s.scale.data_ptr()) and (s.codes == 3).all()
+
+
+def test_kernels_do_not_spill():
+    """The 256-column kernels stand close to the 256 registers that two waves to a SIMD leave."""
+    from test_host_logic import test_scan_kernels_do_not_spill as check
+    check("mx.hip", ["mx_ingest_kernel", "mx_append_kernel", "mx_gather_kernel", "mx_attn_kernel", "mx_merge_kernel"])
