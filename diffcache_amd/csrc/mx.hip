@@ -186,7 +186,8 @@ __device__ __forceinline__ void mx_write_token(const View &k, const View &v, con
     }
 }
 
-// A token's rows alone, a wave to a unit: one round trip to the length, one to the numbers, and the launch.
+// A token's rows alone, a wave to a unit: one round trip to the length, one to the numbers, and the launch: 2.3 us for 8 units of 128
+// columns, 3.5 for 4096.
 template <int KB, int VB>
 __global__ __launch_bounds__(kThreads) void mx_append_kernel(View k, View v, const uint16_t *new_k, const uint16_t *new_v,
                                                              const int32_t *lens, int n_units, int n_h, int hd, int cap) {
@@ -289,12 +290,14 @@ __global__ __launch_bounds__(kThreads) void mx_gather_kernel(GatherArgs a, int h
 // every load takes whole lines (with row 4 q + i they are asked for in pieces, which non-temporal loads do not find in the
 // nearest cache: 2.4 times the requests of the next, 183 us for 174 at 8 x 131072 tokens).
 // Rows behind the end are not asked for: a step's buffers end at its last row, and what a load asks of the words past a buffer's
-// end is zero.  Every offset inside a step is a constant of the load.
+// end is zero.  Offsets inside a step are constants of the load up to its 4095; the last rows of a step of 8 bits a number lie past that at 128
+// columns and at 256, and add to a register.
 //
-// What bounds it: HBM from some 100 MB on.  8 x 131072 tokens of 8 heads x 128 with groups of 4, in 4 bits, 1.14 GB: 174 us = 6.5
-// TB/s; a million of one sequence 170 us; 8 x 65536 of 4 heads x 256 94 us = 6.1 TB/s; 8 x 131072 of 8 heads x 64 97 us = 5.9 TB/s.  64
+// What bounds it: HBM from some 100 MB on.  8 x 131072 tokens of 8 heads x 128 with groups of 4, in 4 bits, 1.14 GB: 173-181 us =
+// 6.3-6.6 TB/s (medians of seven runs of 20 launches); a million of one sequence 170-180 us; 8 x 65536 of 4 heads x 256 97 us = 5.9 TB/s;
+// 8 x 131072 of 8 heads x 64 98 us = 5.8 TB/s.  64
 // rows of 128 columns are some 370 vector, 48 matrix and 22 load instructions of a wave, 55 % of the time the bytes take.
-// Below, the chain of length, rows, products and the join: 32601 tokens of 8 units 12.5 + 3.9 us (the bytes 5.4), 517 tokens
+// Below, the chain of length, rows, products and the join: 32601 tokens of 8 units 12.1 + 3.9 us (the bytes 5.4), 517 tokens
 // 7.5 us in one kernel.  Starts of their own for the blocks' steps: without them a million tokens take 200 us for 177, the
 // blocks' places being a power of two apart.  Loads without the non-temporal hint: 198 us for 180.
 struct AttnArgs {
@@ -756,6 +759,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void mx_attn_kernel(AttnArgs a)
 // The parts of one query head joined: one block per (unit, head).  What it reads is asked for at once, before any weight is
 // known: rounds of kBatch kParts parts (32 at 128 and at 256 columns, 64 at 64), HD / 4 threads to a part.  A kernel's start and two round trips: 64
 // parts of 32 heads 3.9 us (5.5 part by part), 8 parts of 256 heads 4.8, 128 parts of 16 heads of 256 columns 5.0 (6.2 in rounds of 16).
+// A unit alone has its rounds one after the other: 512 parts of 4 heads of 128 columns 13.4, 1024 of 64 columns 17.7.
 template <int HD>
 __global__ __launch_bounds__(kThreads) void mx_merge_kernel(AttnArgs a) {
     constexpr int kLanes = HD / 4, kParts = kThreads / kLanes, kBatch = HD == 256 ? 8 : 4;
@@ -892,7 +896,9 @@ struct AttnCut {
 // Blocks of four waves: two to a CU, which the loads in flight of 64 rows to a wave keep busy (8 x 131072 tokens of 8 heads x
 // 128 in 4 bits: 174 us, with 768 blocks 176, with 1024 183; a document of 32601 12.5 / 13.7 / 14.0).  Rows of 32 bytes are half
 // of that in flight: four to a CU once every wave has six steps or more (64 columns, 4 bits: 16 x 32000 tokens 60.6 -> 50.8 us, a
-// million of one 112 -> 92.5, but 2 x 32000 12.3 -> 12.6).
+// million of one 112 -> 92.5, but 2 x 32000 12.3 -> 12.6).  Every unit gets the same number of blocks, rounded down: with 8192 rows of 128
+// columns 256 units take 47 us, 384 79, 512 89, 640 121; of 64 units whose lengths differ the longest's blocks end last (8 of 131072
+// rows and 56 of 8192: 152 us, 64 of their mean length 36).
 constexpr int kBlocks = 512, kLeanBlocks = 2 * kBlocks, kLeanSteps = 6 * kWaves;
 // Steps of a wave up to which a unit is one block of eight waves, which writes the output itself: less than a second kernel
 // that joins parts (1024 tokens: 9.3 us, in parts 6.5 + 2.7 and a launch; 1500: 11.5, 8.7 + 2.9; 2048: 13.6, 7.5 + 2.8).

@@ -16,7 +16,8 @@ The lengths of the sequences live in ``lens``, an int32 tensor on the device (th
 ``base.py:134-142``): a captured ``decode_attention`` writes to and attends over the rows that it names and counts it
 up after the last layer, so a captured step stays right on every replay; ``advance_host_step`` brings the host's mirror
 up to date.  Sequences of one batch may have prompts of different lengths.  ``window`` > 0 attends to the first
-``sink_len`` and the last ``window`` rows alone.
+``sink_len`` and the last ``window`` rows alone.  All layers share one workspace: calls and replays of one cache go one after another
+(two caches may run side by side).  A copied or saved cache has memory of its own.
 """
 from __future__ import annotations
 
