@@ -1149,7 +1149,8 @@ def mx_gather_rows(k: Optional[MxStore], v: Optional[MxStore], idx: Optional[tor
                    n_idx: Optional[int] = None) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
     """out[b, h, j, :] = the bf16 numbers of row row_offset + idx[b*H + h, j] for j < n_idx, or of row row_offset + j without
     ``idx`` (n_idx: up to the store's end).  ``idx`` 32-bit (b*h, >= n_idx); a row that the store does not have reads as
-    zeros.  ``out_k`` / ``out_v`` (b, h, >= n_idx, hd) bf16 are made where they are not given; K or V may be None."""
+    zeros.  ``out_k`` / ``out_v`` (b, h, >= n_idx, hd) bf16 share their strides and are made where they are not given (contiguous,
+    for n_idx rows: one of another layout needs the other given too); K or V may be None."""
     ref = k if k is not None else v
     if ref is None:
         raise DiffCacheError("neither K nor V given")

@@ -290,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void mx_gather_kernel(GatherArgs a, int h
 // every load takes whole lines (with row 4 q + i they are asked for in pieces, which non-temporal loads do not find in the
 // nearest cache: 2.4 times the requests of the next, 183 us for 174 at 8 x 131072 tokens).
 // Rows behind the end are not asked for: a step's buffers end at its last row, and what a load asks of the words past a buffer's
-// end is zero.  Offsets inside a step are constants of the load up to its 4095; the last rows of a step of 8 bits a number lie past that at 128
+// end is zero.  Offsets inside a step are constants of the load up to its 4095; the later rows of a step of 8 bits a number lie past that at 128
 // columns and at 256, and add to a register.
 //
 // What bounds it: HBM from some 100 MB on.  8 x 131072 tokens of 8 heads x 128 with groups of 4, in 4 bits, 1.14 GB: 173-181 us =

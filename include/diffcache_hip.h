@@ -691,8 +691,9 @@ int dc_mx_gather_rows_bf16(const dc_mx_store *k, const dc_mx_store *v, const uin
  *   window   0: all rows; else the first n_sink and the last `window` (the token's own among them)
  *   lse      NULL, or (n_b, n_h * group) fp32: log of the sum of exp(scale q k^T)
  * A sequence without rows has out 0 and lse -inf.  Rows that are not attended to may hold anything.  Of those that are, a NaN in
- * a block of K makes its unit's outputs and lse NaN, one in a block of V the unit's outputs in these 32 columns.  Logits are fp32: one that
- * falls below its range is -inf, a weight of 0 (with no other logits out is 0, lse -inf); one above it makes its head NaN.
+ * a block of K makes its unit's outputs and lse NaN, one in a block of V the unit's outputs in these 32 columns.  Logits are fp32, before
+ * the scale too: one that falls below its range is -inf, a weight of 0 (with no other logits out is 0, lse -inf); one above it makes its
+ * head NaN.
  * group: up to 16 query heads.  Sums and statistics are fp32.  The workspace
  * (dc_mx_attn_workspace_bytes, 256-byte aligned; 0: none; enough for more units or rows is enough for fewer) holds nothing between calls;
  * calls that may overlap need one each.  Replaces flash_attn_with_kvcache (base.py:134-142) over such a cache.
