@@ -44,6 +44,7 @@ SYMBOLS = (
     "dc_data_layer_create", "dc_data_layer_destroy", "dc_data_layer_ctx_len", "dc_data_layer_sizes",
     "dc_data_layer_bind", "dc_data_layer_prefill", "dc_data_layer_insert", "dc_data_layer_query",
     "dc_mx_ingest_bf16", "dc_mx_append_bf16", "dc_mx_gather_rows_bf16", "dc_mx_attn_workspace_bytes", "dc_mx_attn_bf16",
+    "dc_paged_append_bf16", "dc_paged_attn_workspace_bytes", "dc_paged_attn_bf16",
 )
 
 
@@ -112,6 +113,48 @@ class MxAttnArgs(C.Structure):
         ("workspace_bytes", C.c_size_t),
         ("n_b", C.c_int), ("n_h", C.c_int), ("group", C.c_int), ("hd", C.c_int), ("n_rows", C.c_int),
         ("n_sink", C.c_int), ("window", C.c_int), ("scale", C.c_float),
+    ]
+
+
+class PagedStoreArgs(C.Structure):
+    """struct dc_paged_store of include/diffcache_hip.h"""
+    _fields_ = [
+        ("k", C.c_void_p), ("v", C.c_void_p),
+        ("k_page_stride", C.c_int64), ("k_head_stride", C.c_int64), ("v_page_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("n_pages", C.c_int), ("page", C.c_int),
+    ]
+
+
+class PagedTokensArgs(C.Structure):
+    """struct dc_paged_tokens of include/diffcache_hip.h"""
+    _fields_ = [
+        ("table", C.c_void_p), ("start", C.c_void_p), ("cu", C.c_void_p), ("counts", C.c_void_p),
+        ("table_stride", C.c_int64),
+        ("n_b", C.c_int), ("max_new", C.c_int), ("n_tokens", C.c_int), ("table_pages", C.c_int),
+    ]
+
+
+class PagedAppendArgs(C.Structure):
+    """struct dc_paged_append_args of include/diffcache_hip.h"""
+    _fields_ = [
+        ("k_src", C.c_void_p), ("v_src", C.c_void_p), ("q_src", C.c_void_p), ("q_out", C.c_void_p), ("inv_freq", C.c_void_p),
+        ("pos", C.c_void_p), ("store", PagedStoreArgs), ("tokens", PagedTokensArgs),
+        ("k_batch_stride", C.c_int64), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v_batch_stride", C.c_int64), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("q_batch_stride", C.c_int64), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("n_h", C.c_int), ("n_q", C.c_int), ("hd", C.c_int), ("rot", C.c_int), ("interleaved", C.c_int), ("n_axes", C.c_int),
+        ("section", C.c_int * 4),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    """struct dc_paged_attn_args of include/diffcache_hip.h"""
+    _fields_ = [
+        ("q", C.c_void_p), ("out", C.c_void_p), ("lse", C.c_void_p), ("store", PagedStoreArgs), ("tokens", PagedTokensArgs),
+        ("q_batch_stride", C.c_int64), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("n_h", C.c_int), ("group", C.c_int), ("hd", C.c_int), ("n_rows", C.c_int), ("n_sink", C.c_int), ("window", C.c_int),
+        ("scale", C.c_float),
     ]
 
 
@@ -186,6 +229,9 @@ def _load() -> C.CDLL:
         "dc_mx_gather_rows_bf16": (i, [mx, mx, p, p, p, i, i, i, i64, i, i64, i64, i64, i64, p]),
         "dc_mx_attn_workspace_bytes": (sz, [i, i, i, i]),
         "dc_mx_attn_bf16": (i, [mx, p]),
+        "dc_paged_append_bf16": (i, [mx, p]),
+        "dc_paged_attn_workspace_bytes": (sz, [i, i, i, i, i]),
+        "dc_paged_attn_bf16": (i, [mx, p]),
     })
     for name, (res, args) in sigs.items():
         fn = getattr(lib, name)
@@ -1282,4 +1328,203 @@ def mx_attn(q: torch.Tensor, k: MxStore, v: MxStore, lens: Optional[torch.Tensor
     except struct.error as e:
         raise DiffCacheError(f"n_rows, n_sink, window or scale does not fit its type: {e}") from None
     _check(lib.dc_mx_attn_bf16(args, _mx_stream(k, v)))
+    return out if lse is None else (out, lse)
+
+
+# ---------------------------------------------------------------------------
+# K and V in pages (dc_paged_store)
+# ---------------------------------------------------------------------------
+
+PAGED_MAX_GROUP = 16   # query heads to a KV head, at most
+# the structs' bytes, those inside them in their places (all of them are aligned to 8)
+_PAGED_APPEND = struct.Struct("@6P2P4q2i4Pq4i9q10i")
+_PAGED_ATTN = struct.Struct("@3P2P4q2i4Pq4i3qPN6if0q")
+
+
+def _paged_store(k_pages: torch.Tensor, v_pages: torch.Tensor):
+    """The fields of a dc_paged_store, and (h, hd)."""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype is not _BF16 or v_pages.dtype is not _BF16:
+        raise DiffCacheError("k_pages and v_pages must be (n_pages, h, page, hd) bf16 tensors of one shape")
+    n, h, page, hd = shape
+    k0, k1, k2, k3 = k_pages.stride()
+    v0, v1, v2, v3 = v_pages.stride()
+    if k3 != 1 or v3 != 1 or (page > 1 and (k2 != hd or v2 != hd)):
+        raise DiffCacheError("a page's rows must lie one after another")
+    if n == 0 or h == 0:
+        raise DiffCacheError("a store needs a page and a head")
+    return (_mx_dev(k_pages, "k_pages"), _mx_dev(v_pages, "v_pages"), k0, k1, v0, v1, n, page), h, hd
+
+
+def _paged_tokens(x: torch.Tensor, table: torch.Tensor, start: Optional[torch.Tensor], cu: Optional[torch.Tensor],
+                  counts: Optional[torch.Tensor], max_new: Optional[int], name: str):
+    """The fields of a dc_paged_tokens, and the leading dimensions of the tokens' tensors."""
+    if table.dim() != 2 or table.dtype is not _I32:
+        raise DiffCacheError("table must be an int32 tensor (b, pages)")
+    b, pages = table.shape
+    t0, t1 = table.stride()
+    if pages == 0 or (t1 != 1 and pages > 1) or (t0 < pages and b > 1):
+        raise DiffCacheError("table must have contiguous rows")
+    if cu is not None:
+        if x.dim() != 3 or counts is not None:
+            raise DiffCacheError(f"with cu, {name} holds packed tokens (tokens, heads, hd), and counts are not given")
+        if cu.dtype is not _I32 or cu.numel() != b + 1 or not cu.is_contiguous():
+            raise DiffCacheError(f"cu must be a contiguous int32 tensor of {b + 1} elements")
+        tokens = x.shape[0]
+        lead = (tokens,)
+        if max_new is None:
+            max_new = tokens
+        cu_ptr, counts_ptr = _mx_dev(cu, "cu"), 0
+    else:
+        lead = tuple(x.shape[:-2])
+        if len(lead) not in (1, 2) or lead[0] != b:
+            raise DiffCacheError(f"{name} must be ({b}, heads, hd), or ({b}, tokens, heads, hd), or packed with cu")
+        tokens = lead[1] if len(lead) == 2 else 1
+        if max_new is not None and max_new != tokens:
+            raise DiffCacheError(f"max_new is {max_new}, and {name} has {tokens} tokens to a sequence")
+        max_new, tokens = tokens, b * tokens
+        cu_ptr, counts_ptr = 0, _mx_lens(counts, b) if counts is not None else 0
+    start_ptr = 0
+    if start is not None:
+        if start.dtype is not _I32 or start.numel() != b or not start.is_contiguous():
+            raise DiffCacheError(f"start must be a contiguous int32 tensor of {b} elements")
+        start_ptr = _mx_dev(start, "start")
+    return (_mx_dev(table, "table"), start_ptr, cu_ptr, counts_ptr, t0 if b > 1 else pages, b, max_new, tokens, pages), lead
+
+
+def _paged_src(t: torch.Tensor, lead, heads: Optional[int], hd: int, name: str):
+    """A tensor of tokens: itself or an aligned copy, and its (batch, token, head) strides."""
+    n = len(lead)
+    shape = t.shape
+    if t.dtype is not _BF16 or len(shape) != n + 2 or shape[:n] != lead or shape[n + 1] != hd or (heads is not None and shape[n] != heads):
+        raise DiffCacheError(f"{name} must be bf16 of {(*lead, 'heads' if heads is None else heads, hd)}, not {tuple(shape)} {t.dtype}")
+    strides = t.stride()
+    if strides[-1] != 1 or t.data_ptr() & 15 or any(s & 7 for s in strides[:-1]):
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = t.stride()
+    return t, strides[0], strides[-3], strides[-2]
+
+
+def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                 start: Optional[torch.Tensor] = None, *, cu: Optional[torch.Tensor] = None,
+                 counts: Optional[torch.Tensor] = None, max_new: Optional[int] = None, q: Optional[torch.Tensor] = None,
+                 q_out: Optional[torch.Tensor] = None, inv_freq: Optional[torch.Tensor] = None, interleaved: bool = False,
+                 pos: Optional[torch.Tensor] = None, sections: Optional[Tuple[int, ...]] = None) -> Optional[torch.Tensor]:
+    """New tokens' K and V into their pages, K and ``q`` rotated on the way (dc_paged_append_bf16); returns the rotated queries.
+
+    ``k_pages``, ``v_pages`` (n_pages, h, page, hd) bf16; ``table`` (b, pages) int32 names the page of every ``page`` rows of a
+    sequence (an id that the store does not have: no page, its rows are not written); ``start`` (b) int32: the rows that the
+    sequences hold already (None: none), which is not changed.  Tokens come as ``k``, ``v`` (b, h, hd), one to a sequence; as (b,
+    tokens, h, hd), of which ``counts`` (b) int32 may name the first ones that count; or packed, (tokens, h, hd) with ``cu``
+    (b + 1) int32, where ``max_new`` is the most of a sequence.  ``inv_freq`` (rot / 2) fp32 turns on the rotation of the first rot
+    columns by position * inv_freq: of columns f and f + rot / 2, or of 2 f and 2 f + 1 with ``interleaved``.  A token's
+    position is its row, or ``pos`` (int32, as many as there are tokens); with ``sections``, up to four numbers of frequencies that add up to
+    rot / 2, ``pos`` has a last dimension of as many and a section's frequencies go by its own.  ``q_out`` (contiguous, of q's
+    shape) may be a contiguous ``q`` itself."""
+    store, h, hd = _paged_store(k_pages, v_pages)
+    tokens, lead = _paged_tokens(k, table, start, cu, counts, max_new, "k")
+    k, k0, k1, k2 = _paged_src(k, lead, h, hd, "k")
+    v, v0, v1, v2 = _paged_src(v, lead, h, hd, "v")
+    rot = n_q = q0 = q1 = q2 = inv_ptr = pos_ptr = q_ptr = out_ptr = 0
+    if inv_freq is not None:
+        if inv_freq.dtype is not _F32 or not inv_freq.is_contiguous():
+            raise DiffCacheError("inv_freq must be a contiguous fp32 tensor")
+        rot, inv_ptr = 2 * inv_freq.numel(), _mx_dev(inv_freq, "inv_freq")
+    elif q is not None or pos is not None or sections is not None:
+        raise DiffCacheError("q, pos and sections are for a rotation: inv_freq is missing")
+    n_axes, section = 1, (0, 0, 0, 0)
+    if sections is not None:
+        n_axes = len(sections)
+        if not 1 <= n_axes <= 4 or pos is None:
+            raise DiffCacheError("sections are one to four numbers of frequencies, and need pos")
+        section = tuple(sections) + (0,) * (4 - n_axes)
+    if pos is not None:
+        want = (*lead, n_axes) if sections is not None else lead
+        if pos.dtype is not _I32 or pos.shape != want or not pos.is_contiguous():
+            raise DiffCacheError(f"pos must be a contiguous int32 tensor of {tuple(want)}")
+        pos_ptr = _mx_dev(pos, "pos")
+    if q is not None:
+        given = q
+        q, q0, q1, q2 = _paged_src(q, lead, None, hd, "q")
+        n_q, q_ptr = q.shape[-2], _mx_dev(q, "q")
+        if q_out is None:
+            q_out = torch.empty(q.shape, dtype=_BF16, device=q.device)
+            out_ptr = q_out.data_ptr()
+        elif q_out.dtype is not _BF16 or q_out.shape != given.shape or not q_out.is_contiguous():
+            raise DiffCacheError("q_out must be a contiguous bf16 tensor of q's shape")
+        else:
+            out_ptr = _mx_dev(q_out, "q_out")
+    elif q_out is not None:
+        raise DiffCacheError("q_out is given without q")
+    try:
+        args = _PAGED_APPEND.pack(_mx_dev(k, "k"), _mx_dev(v, "v"), q_ptr, out_ptr, inv_ptr, pos_ptr, *store, *tokens,
+                                  k0, k1, k2, v0, v1, v2, q0, q1, q2, h, n_q, hd, rot, bool(interleaved), n_axes, *section)
+    except struct.error as e:
+        raise DiffCacheError(f"a size or a section does not fit its type: {e}") from None
+    _check(lib.dc_paged_append_bf16(args, _stream()))
+    return q_out
+
+
+def paged_attn_workspace_bytes(n_units: int, group: int, hd: int, n_rows: int, max_new: int = 1) -> int:
+    return int(lib.dc_paged_attn_workspace_bytes(n_units, group, hd, n_rows, max_new))
+
+
+def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+               start: Optional[torch.Tensor] = None, *, cu: Optional[torch.Tensor] = None, counts: Optional[torch.Tensor] = None,
+               max_new: Optional[int] = None, n_rows: Optional[int] = None, n_sink: int = 0, window: int = 0,
+               scale: Optional[float] = None, out: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+               want_lse: bool = False, workspace: Optional[torch.Tensor] = None):
+    """Attention of new tokens over the rows of their sequences (dc_paged_attn_bf16), whose own rows ``paged_append`` wrote: token i
+    of sequence b attends to rows 0 .. start[b] + i, with ``window`` > 0 to the first ``n_sink`` and the last ``window`` of these.
+    ``q`` (b, h * group, hd), (b, tokens, h * group, hd) or packed (tokens, h * group, hd), with ``start``, ``counts``, ``cu``, ``max_new`` and the
+    pages as in ``paged_append``.  ``n_rows``: no sequence has more rows, those of its new tokens among them (default: the table's); sizes the
+    launch.  Returns out of q's shape, whose tokens that do not count stay as they were; with ``lse`` or ``want_lse`` (out, lse), lse
+    (..., h * group) fp32 the log of the sum of exponentials.  A token without rows has out 0 and lse -inf."""
+    store, h, hd = _paged_store(k_pages, v_pages)
+    tokens, lead = _paged_tokens(q, table, start, cu, counts, max_new, "q")
+    q, q0, q1, q2 = _paged_src(q, lead, None, hd, "q")
+    hq = q.shape[-2]
+    group = hq // h
+    if group * h != hq or group < 1:
+        raise DiffCacheError(f"q has {hq} heads, the store {h}")
+    if group > PAGED_MAX_GROUP:
+        raise DiffCacheError(f"more than {PAGED_MAX_GROUP} query heads to a KV head are not supported")
+    b, max_new, _, pages = tokens[5:]
+    room = pages * store[7]
+    if n_rows is None:
+        n_rows = room
+    elif not 1 <= n_rows <= room:
+        raise DiffCacheError(f"{n_rows} rows outside the table of {room}")
+    dev = q.device
+    if out is None:
+        out = torch.empty(q.shape, dtype=_BF16, device=dev)
+        out_ptr = out.data_ptr()
+    elif out.dtype is not _BF16 or out.numel() != q.numel() or not out.is_contiguous():
+        raise DiffCacheError("out must be a contiguous bf16 tensor of the size of q")
+    else:
+        out_ptr = _mx_dev(out, "out")
+    lse_ptr = ws_ptr = 0
+    if lse is None:
+        if want_lse:
+            lse = torch.empty(q.shape[:-1], dtype=_F32, device=dev)
+            lse_ptr = lse.data_ptr()
+    elif lse.dtype is not _F32 or lse.numel() * hd != q.numel() or not lse.is_contiguous():
+        raise DiffCacheError("lse must be a contiguous fp32 tensor of (..., h * group) elements")
+    else:
+        lse_ptr = _mx_dev(lse, "lse")
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise DiffCacheError("workspace must be contiguous")
+        ws_ptr, ws_bytes = _mx_dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
+    else:
+        ws_bytes = lib.dc_paged_attn_workspace_bytes(b * h, group, hd, n_rows, max_new)
+        if ws_bytes:
+            workspace = torch.empty(ws_bytes, dtype=_U8, device=dev)
+            ws_ptr = workspace.data_ptr()
+    try:
+        args = _PAGED_ATTN.pack(_mx_dev(q, "q"), out_ptr, lse_ptr, *store, *tokens, q0, q1, q2, ws_ptr, ws_bytes, h, group, hd,
+                                n_rows, n_sink, window, hd ** -0.5 if scale is None else scale)
+    except struct.error as e:
+        raise DiffCacheError(f"n_sink, window, max_new or scale does not fit its type: {e}") from None
+    _check(lib.dc_paged_attn_bf16(args, _stream()))
     return out if lse is None else (out, lse)

@@ -1,0 +1,498 @@
+// Attention over keys and values in pages: the entry point, the kernel for up to 16 rows of queries of a KV head (one token, or
+// a few drafted ones), and the join of the parts of a long axis.
+#include "dc_paged.h"
+#include <math.h>
+
+namespace {
+
+constexpr int kThreads = 256, kWaves = 4, kMostWaves = 8, kRows = 16;
+
+// out = sum_r p_r v_r / sum_r p_r with p_r = exp(scale q k_r - m), over the rows that a token attends to.  A unit's (one sequence's, one KV
+// head's) rows are cut into steps of 16 TILES, its steps into n_splits parts, a block each, whose waves take them in turn; a wave
+// keeps its running maximum, sum and weighted rows in registers, so K and V are read once and nothing is written but the parts' results.
+//
+//   S = K Q^T   v_mfma_f32_16x16x32_bf16 over 16 rows (M), 16 (token, head) pairs (N) and 32 columns.  Lane (q, c) = (lane / 16, lane % 16)
+//               loads 16 bytes of one row, its four lanes side by side.
+//   softmax     in powers of two, fp32.  Lane c keeps pair c's maximum, which moves only where a logit passes it by more than 8: nothing
+//               crosses lanes from step to step, and a weight is at most 2^8 of fp32 sums.
+//   O = P V     M = 16 pairs, N = 16 of the hd columns, K = 32 rows of two tiles, P as it stands in the lanes.  P is the sum of two bf16
+//               numbers: 2^-16 of a weight is lost at most, far below the output's own 2^-8; the matrix unit has the time.  Lane (q, c) loads
+//               adjacent columns of its own rows; byte permutes put the rows of a column together.
+//
+// Which row of a tile is which row of M is free as long as K and V agree: M row 4 q + i is the tile's row 4 i + q, so that every
+// load takes whole lines.  A tile of 16 rows lies in one page, so its address is the scalar unit's; page ids are read a step ahead.
+template <int HD, int TILES>
+struct Rows {
+    static constexpr int STEP = 16 * TILES, CH = HD / 32, EPL = HD / 16, VW = EPL / 2;
+
+    dc_u32x4 bq[CH];
+    dc_u32x4 kw[TILES][CH];
+    uint32_t vw[TILES * 4][VW];
+    dc_f32x4 acc[EPL];
+    float m, l;
+    int q, c;
+
+    __device__ __forceinline__ void start(int lane) {
+        q = lane >> 4, c = lane & 15;
+#pragma unroll
+        for (int j = 0; j < EPL; ++j) acc[j] = dc_f32x4{0.f, 0.f, 0.f, 0.f};
+        m = -INFINITY, l = 0.f;
+    }
+    __device__ __forceinline__ void load_q(const uint16_t *src) {
+#pragma unroll
+        for (int s = 0; s < CH; ++s) bq[s] = *reinterpret_cast<const dc_u32x4 *>(src + 32 * s + 8 * q);
+    }
+    // lane (q, c) has columns 32 s + 8 q .. of row 4 (c % 4) + c / 4 of every tile
+    __device__ __forceinline__ void load_k(const uint16_t *const (&tile)[TILES]) {
+        const int off = (4 * (c & 3) + (c >> 2)) * HD + 8 * q;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int s = 0; s < CH; ++s) kw[t][s] = __builtin_nontemporal_load(reinterpret_cast<const dc_u32x4 *>(tile[t] + off + 32 * s));
+    }
+    // column j of lane c's
+    static __device__ __forceinline__ int column(int c, int j) { return HD == 64 ? 4 * c + j : 128 * (j / 8) + 8 * c + j % 8; }
+    // lane (q, c) has its columns of the rows 4 i + q of every tile
+    __device__ __forceinline__ void load_v(const uint16_t *const (&tile)[TILES]) {
+        const int off = q * HD + column(c, 0);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint16_t *src = tile[t] + off + 4 * i * HD;
+                if constexpr (HD == 64) {
+                    const dc_u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const dc_u32x2 *>(src));
+                    vw[4 * t + i][0] = w.x, vw[4 * t + i][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int u = 0; u < HD / 128; ++u) {
+                        const dc_u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const dc_u32x4 *>(src + 128 * u));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) vw[4 * t + i][4 * u + e] = w[e];
+                    }
+                }
+            }
+    }
+
+    // x[t][i]: tile t, row 4 i + q, pair c
+    __device__ __forceinline__ void logits(float scale, float (&x)[TILES][4]) const {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            dc_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < CH; ++j)
+                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, kw[t][j]), __builtin_bit_cast(dc_bf16x8, bq[j]), s, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t][i] = s[i] * scale;
+        }
+    }
+
+    // a new maximum for every pair, and what was summed so far brought to it
+    __device__ __forceinline__ void raise(float most) {
+        const float to = fmaxf(m, dc_over16(most, [](float a, float b) { return fmaxf(a, b); }));
+        if (__any(m > kNoLogit)) {
+            const float f = m > kNoLogit ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
+            l *= f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float g = __shfl(f, 4 * q + i, 64);
+#pragma unroll
+                for (int j = 0; j < EPL; ++j) acc[j][i] *= g;
+            }
+        }
+        m = to;
+    }
+    __device__ __forceinline__ void weigh(float (&x)[TILES][4]) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, x[t][i]);
+        if (__any(most > m + 8.f)) raise(most);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - m);
+                l += x[t][i];
+            }
+    }
+
+    // acc += P V over the step that load_v brought; whole: every row is attended to by every pair
+    __device__ __forceinline__ void add(const float (&x)[TILES][4], bool whole) {
+#pragma unroll
+        for (int u = 0; u < TILES / 2; ++u) {
+            dc_u32x4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x0 = x[2 * u + i / 2][2 * (i % 2)], x1 = x[2 * u + i / 2][2 * (i % 2) + 1];
+                hi[i] = dc_pack_bf16(x0, x1);
+                lo[i] = dc_pack_bf16(x0 - dc_bf16_lo(hi[i]), x1 - dc_bf16_hi(hi[i]));
+            }
+            auto both = [&](dc_u32x4 w, dc_f32x4 o) __attribute__((always_inline)) {
+                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, lo), __builtin_bit_cast(dc_bf16x8, w), o, 0, 0, 0);
+                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, hi), __builtin_bit_cast(dc_bf16x8, w), o, 0, 0, 0);
+            };
+#pragma unroll
+            for (int j = 0; j < EPL; ++j) {
+                const uint32_t sel = j % 2 ? 0x07060302u : 0x05040100u;  // the high or the low halves of two words
+                dc_u32x4 w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(vw[8 * u + 2 * i + 1][j / 2], vw[8 * u + 2 * i][j / 2], sel);
+                if (whole) acc[j] = both(w, acc[j]);
+                else dc_careful<4>(w, acc[j], both);
+            }
+        }
+    }
+
+    // dst[pair][column] = the wave's sums
+    __device__ __forceinline__ void finish(float *dst, int pairs) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (4 * q + i < pairs) {
+#pragma unroll
+                for (int j = 0; j < EPL; j += 4)
+                    *reinterpret_cast<float4 *>(dst + (4 * q + i) * HD + column(c, j)) = make_float4(acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]);
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ float weight(float m, float top) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f; }
+// a part's share of the sum (one that is no number stays none, whatever its maximum)
+__device__ __forceinline__ float share(float m, float l, float top) { return l == l ? weight(m, top) * l : l; }
+__device__ __forceinline__ float log_sum(float top, float total) { return total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f; }
+
+template <int HD, int TILES>
+__global__ __launch_bounds__(kMostWaves * 64, 2) void paged_rows_kernel(DcPagedAttn a) {
+    using T = Rows<HD, TILES>;
+    constexpr int STEP = T::STEP;
+    extern __shared__ float s_dyn[];
+    const int waves = a.waves;
+    float *s_m = s_dyn, *s_l = s_dyn + waves * kRows, *s_acc = s_dyn + 2 * waves * kRows;  // [wave][16], [wave][16], [wave][pairs * HD]
+    const int b = blockIdx.x, h = blockIdx.y, split = blockIdx.z, unit = b * a.n_h + h, G = a.group;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const DcSpan span = dc_span(a.t, b);
+    if (span.count == 0) return;
+    const int pairs = span.count * G, p_lo = span.start, p_hi = span.start + span.count - 1;
+    const DcSteps st = dc_steps<STEP>(a, p_lo, p_hi);
+    const int64_t slot = (int64_t)unit * a.n_splits + split;
+    int per = a.n_splits == 1 ? st.steps : (int)((uint32_t)(st.steps + a.n_splits - 1) / (uint32_t)a.n_splits);
+    per = per < waves ? waves : per;
+    const int begin = split * per, end = begin + per < st.steps ? begin + per : st.steps;
+    if (begin >= end && a.n_splits > 1) {  // a part without rows: the join takes nothing of it
+        if (tid < pairs) reinterpret_cast<float2 *>(a.ws_ml)[slot * a.tile_rows + tid] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+    T w;
+    w.start(lane);
+    const int pair = w.c < pairs ? w.c : pairs - 1, token = pair / G;  // (the last pair again in the place of one that does not exist)
+    w.load_q(a.q + dc_token_at(a.t, a.qs, span, b, token) + (int64_t)(h * G + pair % G) * a.qs.h);
+    const int p = span.start + token;
+
+    const uint16_t *kh = a.p.k + h * a.p.kh, *vh = a.p.v + h * a.p.vh;
+    const int32_t *table = a.p.table + (int64_t)b * a.p.table_stride;
+    const int last_page = (a.n_rows - 1) >> a.p.shift, mask = (1 << a.p.shift) - 1;
+    // a wave's steps are every waves-th of the block's, from a start of its block's own on
+    const int mine = end > begin + wave ? (end - begin - wave + waves - 1) / waves : 0;
+    int at = (int)(((uint64_t)((uint32_t)slot * 0x9e3779b9u) * (uint32_t)mine) >> 32);
+    int id[TILES], row = 0;
+    auto look = [&]() __attribute__((always_inline)) {
+        row = st.row(begin + wave + at * waves, STEP);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int page = (row + 16 * t) >> a.p.shift;
+            id[t] = dc_page_id(a.p, table, page < last_page ? page : last_page);
+        }
+    };
+    const uint16_t *kt[TILES], *vt[TILES];
+    int held_row = 0, live = 0;  // of the step in the registers: its first row, and a bit for each tile that has a page
+    auto place = [&]() __attribute__((always_inline)) {
+        held_row = row, live = 0;
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+            const int64_t page = id[t] < 0 ? 0 : id[t];
+            live |= id[t] < 0 ? 0 : 1 << t;
+            const int64_t in = (int64_t)((row + 16 * t) & mask) * HD;
+            kt[t] = kh + page * a.p.kp + in, vt[t] = vh + page * a.p.vp + in;
+        }
+    };
+    if (mine > 0) {
+        w.m = kNoLogit;
+        look();
+        place();
+        w.load_k(kt);
+        w.load_v(vt);
+        at = at + 1 < mine ? at + 1 : 0;
+        look();
+    }
+    for (int n = 0; n < mine; ++n) {
+        float x[TILES][4];
+        w.logits(a.scale, x);
+        const bool more = n + 1 < mine;
+        const int r0 = held_row, have = live;
+        if (more) {
+            place();
+            w.load_k(kt);
+            at = at + 1 < mine ? at + 1 : 0;
+            look();
+        }
+        // every row for every pair?
+        const bool whole = have == (1 << TILES) - 1 && r0 + STEP - 1 <= p_lo && r0 + STEP <= a.n_rows &&
+                           (a.window == 0 || r0 > p_hi - a.window || r0 + STEP <= a.n_sink);
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!((have >> t) & 1) || !dc_attends(a, p, r0 + 16 * t + 4 * i + w.q)) x[t][i] = -INFINITY;
+        }
+        w.weigh(x);
+        w.add(x, whole);
+        if (more) w.load_v(vt);
+    }
+
+    // the pairs' statistics and sums over the block's waves
+    const float l = dc_over16(w.l, [](float a, float b) { return a + b; });
+    if (lane < kRows) s_m[wave * kRows + lane] = w.m, s_l[wave * kRows + lane] = l;
+    w.finish(s_acc + wave * pairs * HD, pairs);
+    __syncthreads();
+    for (int o = tid; o < pairs * HD; o += waves * 64) {
+        const int r = o / HD;
+        // (without a branch to a wave: the first one again in the place of those that a block of four does not have)
+        float m[kMostWaves], ls[kMostWaves], part[kMostWaves];
+#pragma unroll
+        for (int i = 0; i < kMostWaves; ++i) {
+            const int x = i < waves ? i : 0;
+            m[i] = s_m[x * kRows + r], ls[i] = s_l[x * kRows + r], part[i] = s_acc[x * pairs * HD + o];
+        }
+        float top = m[0];
+#pragma unroll
+        for (int i = 1; i < kMostWaves; ++i) top = fmaxf(top, m[i]);
+        float sum = 0.f, total = 0.f;
+#pragma unroll
+        for (int i = 0; i < kMostWaves; ++i) {
+            sum = fmaf(i < waves ? weight(m[i], top) : 0.f, i < waves ? part[i] : 0.f, sum);
+            total += i < waves ? share(m[i], ls[i], top) : 0.f;
+        }
+        if (a.n_splits > 1) {
+            a.ws_acc[(slot * a.tile_rows + r) * HD + o % HD] = sum;
+            if (o % HD == 0) reinterpret_cast<float2 *>(a.ws_ml)[slot * a.tile_rows + r] = make_float2(top, total);
+        } else {
+            const int64_t dst = (int64_t)(span.first + r / G) * a.n_h * G + h * G + r % G;
+            a.out[dst * HD + o % HD] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
+            if (a.lse && o % HD == 0) a.lse[dst] = log_sum(top, total);
+        }
+    }
+}
+
+// What a join's block has to know of its row of a unit: where the parts are, and where the result goes.
+struct Row {
+    int64_t slot0, dst;  // the row's place in part 0; the (token, head) of the outputs
+    bool live;
+};
+__device__ __forceinline__ Row row_of(const DcPagedAttn &a, int group, int r) {
+    const int unit = group / a.tiles, b = unit / a.n_h, h = unit % a.n_h;
+    const int pair = (group % a.tiles) * a.tile_rows + r, token = pair / a.group;
+    const DcSpan span = dc_span(a.t, b);
+    return {(int64_t)group * a.n_splits * a.tile_rows + r, (int64_t)(span.first + token) * a.n_h * a.group + h * a.group + pair % a.group,
+            token < span.count};
+}
+
+// The parts of one row joined by a block: HD / 4 threads to a part, all of a round's parts asked for before any weight is known.
+template <int HD>
+__global__ __launch_bounds__(kThreads) void paged_join_kernel(DcPagedAttn a) {
+    constexpr int kLanes = HD / 4, kParts = kThreads / kLanes, kBatch = HD == 256 ? 8 : 4;
+    __shared__ float4 s_acc[kThreads];
+    const int tid = threadIdx.x, lane = tid & 63, n = a.n_splits;
+    const Row row = row_of(a, (int)(blockIdx.x / (unsigned)a.tile_rows), (int)(blockIdx.x % (unsigned)a.tile_rows));
+    if (!row.live) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + row.slot0;
+    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + row.slot0 * kLanes + tid % kLanes;
+    const int64_t step = a.tile_rows;
+    float4 v[kBatch];
+    float2 o[kBatch];
+    auto load = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {  // (the last part again where there are no more)
+            const int s = s0 + i * kParts;
+            const int64_t at = (s < n ? s : n - 1) * step;
+            o[i] = ml[at], v[i] = pa[at * kLanes];
+        }
+    };
+    const float2 own = lane < n ? ml[lane * step] : make_float2(-INFINITY, 0.f);
+    load(tid / kLanes);
+    auto all = [&](float x, auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) x = f(x, __shfl_xor(x, d, 64));
+        return dc_over16(x, f);
+    };
+    float top = own.x;
+    for (int s = lane + 64; s < n; s += 64) top = fmaxf(top, ml[s * step].x);
+    top = all(top, [](float x, float y) { return fmaxf(x, y); });
+    float total = share(own.x, own.y, top);
+    for (int s = lane + 64; s < n; s += 64) total += share(ml[s * step].x, ml[s * step].y, top);
+    total = all(total, [](float x, float y) { return x + y; });
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = tid / kLanes;;) {
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            // (a part without rows has no sums in the workspace)
+            const bool in = s0 + i * kParts < n && o[i].x > -INFINITY;
+            const float f = in ? weight(o[i].x, top) : 0.f;
+            acc.x = fmaf(f, in ? v[i].x : 0.f, acc.x), acc.y = fmaf(f, in ? v[i].y : 0.f, acc.y);
+            acc.z = fmaf(f, in ? v[i].z : 0.f, acc.z), acc.w = fmaf(f, in ? v[i].w : 0.f, acc.w);
+        }
+        s0 += kBatch * kParts;
+        if (s0 - tid / kLanes >= n) break;
+        load(s0);
+    }
+    s_acc[tid] = acc;
+    __syncthreads();
+    if (tid < HD) {
+        const float *x = reinterpret_cast<const float *>(s_acc) + tid;
+        float sum = x[0];
+#pragma unroll
+        for (int i = 1; i < kParts; ++i) sum += x[i * HD];
+        a.out[row.dst * HD + tid] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
+    }
+    if (a.lse && tid == 0) a.lse[row.dst] = log_sum(top, total);
+}
+
+// The same for many rows of few parts: HD / 4 threads to a row, its parts one after another.
+template <int HD>
+__global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(DcPagedAttn a) {
+    constexpr int kLanes = HD / 4, kPer = kThreads / kLanes;
+    const int at = (int)(blockIdx.x * kPer) + (int)threadIdx.x / kLanes, c = threadIdx.x % kLanes;  // (tile_rows is a multiple of kPer)
+    const Row row = row_of(a, at / a.tile_rows, at % a.tile_rows);
+    if (!row.live) return;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + row.slot0;
+    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + row.slot0 * kLanes + c;
+    float top = -INFINITY, total = 0.f;
+    for (int s = 0; s < a.n_splits; ++s) top = fmaxf(top, ml[s * (int64_t)a.tile_rows].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.n_splits; ++s) {
+        const float2 o = ml[s * (int64_t)a.tile_rows];
+        total += share(o.x, o.y, top);
+        if (!(o.x > -INFINITY)) continue;
+        const float4 v = pa[s * (int64_t)a.tile_rows * kLanes];
+        const float f = weight(o.x, top);
+        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    }
+    const float d = total == 0.f ? 1.f : total;
+    *reinterpret_cast<uint2 *>(a.out + row.dst * HD + 4 * c) = make_uint2(dc_pack_bf16(acc.x / d, acc.y / d), dc_pack_bf16(acc.z / d, acc.w / d));
+    if (a.lse && c == 0) a.lse[row.dst] = log_sum(top, total);
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+
+constexpr int row_tiles(int hd) { return hd == 256 ? 2 : 4; }
+constexpr int kBlocks = 512;  // two to a CU
+// Steps of a wave up to which a unit is one block of eight waves, which writes the output itself.
+constexpr int kAlone = 2;
+
+struct Cut {
+    bool chunk;
+    int n_splits, waves, tiles, tile_rows;
+};
+Cut cut_of(int64_t n_units, int group, int hd, int64_t rows, int max_new) {
+    Cut c;
+    c.chunk = (int64_t)max_new * group > kRows;
+    if (c.chunk) {
+        c.tile_rows = kChunkRows, c.waves = 4;
+        c.tiles = (int)(((int64_t)max_new * group + kChunkRows - 1) / kChunkRows);
+        c.n_splits = dc_paged_chunk_splits(n_units, c.tiles, hd, rows);
+        return c;
+    }
+    c.tiles = 1, c.tile_rows = max_new * group;
+    const int64_t step = 16 * row_tiles(hd), steps = (rows + step - 1) / step;
+    if (steps <= kAlone * kMostWaves) {
+        c.n_splits = 1, c.waves = steps <= kWaves ? kWaves : kMostWaves;
+        return c;
+    }
+    const int64_t parts = (steps + kWaves - 1) / kWaves, most = kBlocks / n_units > 1 ? kBlocks / n_units : 1;
+    c.n_splits = (int)(parts < most ? parts : most), c.waves = kWaves;
+    return c;
+}
+size_t acc_bytes(int64_t slots, int rows, int hd) { return dc_align_up((size_t)slots * rows * hd * 4, 256); }
+size_t ml_bytes(int64_t slots, int rows) { return dc_align_up((size_t)slots * rows * 8, 256); }
+
+template <int HD>
+void launch_rows(const DcPagedAttn &a, int n_units, hipStream_t st) {
+    const size_t lds = (size_t)a.waves * (2 * kRows + a.tile_rows * HD) * sizeof(float);
+    hipLaunchKernelGGL((paged_rows_kernel<HD, row_tiles(HD)>), dim3((unsigned)(n_units / a.n_h), (unsigned)a.n_h, (unsigned)a.n_splits),
+                       dim3(a.waves * 64), lds, st, a);
+}
+
+}  // namespace
+
+extern "C" size_t dc_paged_attn_workspace_bytes(int n_units, int group, int hd, int n_rows, int max_new) {
+    if (n_units <= 0 || n_units >= (1 << 24) || group <= 0 || group > 16 || hd < 64 || n_rows < 0 || max_new <= 0) return 0;
+    const Cut c = cut_of(n_units, group, hd, n_rows, max_new);
+    if (c.n_splits == 1) return 0;
+    const int64_t slots = (int64_t)n_units * c.tiles * c.n_splits;
+    return acc_bytes(slots, c.tile_rows, hd) + ml_bytes(slots, c.tile_rows);
+}
+
+extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
+    const char *who = "dc_paged_attn_bf16";
+    DC_REQUIRE(x, "%s: null pointer", who);
+    const dc_paged_tokens &t = x->tokens;
+    DC_REQUIRE(t.n_b >= 0 && t.max_new >= 0 && t.n_tokens >= 0, "%s: bad sizes", who);
+    if (t.n_b == 0 || t.max_new == 0) return DC_OK;
+    if (const int rc = dc_check_paged(who, x->store, t, x->n_h, x->hd, false)) return rc;
+    DC_REQUIRE(x->q && x->out, "%s: null pointer", who);
+    DC_REQUIRE(dc_aligned16(x->q) && dc_aligned16(x->out) && x->q_batch_stride % 8 == 0 && x->q_token_stride % 8 == 0 && x->q_head_stride % 8 == 0,
+               "%s: pointers must be 16-byte aligned, strides multiples of 8 elements", who);
+    DC_REQUIRE(x->group >= 1 && x->group <= 16, "%s: group %d not in [1,16]", who, x->group);
+    DC_REQUIRE(x->n_rows >= 1 && x->n_rows <= (int64_t)t.table_pages * x->store.page, "%s: %d rows outside the table", who, x->n_rows);
+    DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
+    DC_REQUIRE(x->scale > 0.f && x->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
+    DC_REQUIRE((int64_t)t.max_new * x->group < (1ll << 30), "%s: too many tokens", who);
+    const int n_units = t.n_b * x->n_h;
+    const Cut c = cut_of(n_units, x->group, x->hd, x->n_rows, t.max_new);
+    const int64_t slots = (int64_t)n_units * c.tiles * c.n_splits;
+    DC_REQUIRE(dc_grid_fits(c.chunk ? slots : t.n_b, c.waves * 64), "%s: grid too large", who);
+    DcPagedAttn a;
+    a.ws_acc = a.ws_ml = nullptr;
+    if (c.n_splits > 1) {
+        const size_t acc = acc_bytes(slots, c.tile_rows, x->hd), need = acc + ml_bytes(slots, c.tile_rows);
+        DC_REQUIRE(x->workspace && ((uintptr_t)x->workspace & 255u) == 0, "%s: workspace must be non-null and 256-byte aligned", who);
+        if (x->workspace_bytes < need) {
+            dc_set_error("%s: workspace %zu bytes < %zu needed", who, x->workspace_bytes, need);
+            return DC_ENOMEM;
+        }
+        a.ws_acc = (float *)x->workspace, a.ws_ml = (float *)((char *)x->workspace + acc);
+    }
+    a.q = (const uint16_t *)x->q, a.out = (uint16_t *)x->out, a.lse = x->lse;
+    a.p = dc_pages_of(x->store, t), a.t = dc_new_of(t);
+    a.qs = {x->q_batch_stride, x->q_token_stride, x->q_head_stride};
+    a.n_h = x->n_h, a.group = x->group, a.n_rows = x->n_rows, a.n_sink = x->n_sink, a.window = x->window;
+    a.n_splits = c.n_splits, a.waves = c.waves, a.tiles = c.tiles, a.tile_rows = c.tile_rows;
+    a.scale = x->scale * 1.44269504088896341f;
+    hipStream_t st = (hipStream_t)stream;
+    if (c.chunk) {
+        if (const int rc = dc_paged_chunk_launch(a, x->hd, n_units, st)) return rc;
+    } else if (x->hd == 64) {
+        launch_rows<64>(a, n_units, st);
+    } else if (x->hd == 128) {
+        launch_rows<128>(a, n_units, st);
+    } else {
+        launch_rows<256>(a, n_units, st);
+    }
+    DC_CHECK_LAUNCH(who);
+    if (c.n_splits > 1) {
+        const int64_t rows = (int64_t)n_units * c.tiles * c.tile_rows;
+#define DC_JOIN(HD)                                                                                                                        \
+    do {                                                                                                                                   \
+        if (c.chunk) hipLaunchKernelGGL(paged_join_rows_kernel<HD>, dim3((unsigned)(rows / (kThreads / (HD / 4)))), dim3(kThreads), 0, st, a); \
+        else hipLaunchKernelGGL(paged_join_kernel<HD>, dim3((unsigned)rows), dim3(kThreads), 0, st, a);                                    \
+    } while (0)
+        if (x->hd == 64) DC_JOIN(64);
+        else if (x->hd == 128) DC_JOIN(128);
+        else DC_JOIN(256);
+#undef DC_JOIN
+        DC_CHECK_LAUNCH(who);
+    }
+    return DC_OK;
+}

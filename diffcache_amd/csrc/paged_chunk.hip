@@ -1,0 +1,247 @@
+// Attention of many new tokens over keys and values in pages, each over the rows up to its own.
+//
+// A unit (one sequence, one KV head) has count * group (token, head) pairs, its heads side by side so that they share K and V.  A block
+// of four waves takes 128 of them and goes over the rows that they attend to in steps of KT, staged through LDS; a wave has 32 pairs.
+//
+//   S^T = K Q^T   v_mfma_f32_32x32x16_bf16, M = 32 rows, N = the wave's 32 pairs.  A lane then has one pair's logits of half the rows, so that
+//                 maximum and sum stay inside it but for one exchange between the wave's halves where the maximum moves.
+//   O^T = V^T P^T M = 32 of the hd columns, N = the pairs, K = 16 rows: P^T stands in the lanes as the operand wants it, and V^T comes out of
+//                 LDS by the transposing reads, rows in the order that P^T has them.  Rescaling O is a factor of the lane's own.
+//
+// P is rounded to bf16 (2^-8 of a weight at most; the sum is that of the weights before): a second product for the rest would be half as
+// much matrix work again, for an error no larger than that of the output's own rounding (against 64 bits 2.1e-3 of the result with both,
+// 1.7e-3 is the output's alone).  Softmax in powers of two, fp32; the maximum moves where a
+// logit passes it by more than 8.
+#include "dc_paged.h"
+
+namespace {
+
+constexpr int kThreads = 256, kRowsOfWave = 32;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) dc_u32x4 lds_u32x4;
+typedef __attribute__((address_space(3))) uint8_t lds_u8;
+
+template <int HD, int KT>
+struct Tile {
+    static constexpr int ROW = HD * 2, CHUNKS = HD / 8;          // bytes and 16-byte chunks of a row
+    static constexpr int PER = 64 / CHUNKS;                      // rows of a wave's load
+    static constexpr int LOADS = KT / PER / 4;                   // loads of a wave for K, and for V
+    static constexpr int BYTES = KT * ROW;
+    // Where chunk c of a row lies in LDS: chunk c ^ k_turn(row) for K, so that 16 rows' same chunk are 16 different banks' groups; whole groups
+    // of four chunks (what a transposing read takes of a row) changed about for V.
+    static __device__ __forceinline__ int k_turn(int row) { return HD == 64 ? (row >> 1) & 7 : row & 15; }
+    static __device__ __forceinline__ int v_turn(int row) { return HD == 64 ? ((row >> 1) & 1) << 2 : (row & 3) << 2; }
+};
+
+template <int HD, int KT>
+__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kernel(DcPagedAttn a) {
+    using T = Tile<HD, KT>;
+    constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32;      // products of a tile's S; tiles of O and of S
+    __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2][T::BYTES];
+    const int n_units = (int)(gridDim.x / (unsigned)(a.tiles * a.n_splits));
+    // units first, so that a unit's blocks are on one XCD where their number divides by eight; late tokens first, they have the most rows
+    const int unit = (int)(blockIdx.x % (unsigned)n_units), rest = (int)(blockIdx.x / (unsigned)n_units);
+    const int split = rest % a.n_splits, tile = a.tiles - 1 - rest / a.n_splits;
+    const int b = unit / a.n_h, h = unit % a.n_h, G = a.group;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const DcSpan span = dc_span(a.t, b);
+    const int pairs = span.count * G, pair0 = tile * kChunkRows;
+    if (pair0 >= pairs) return;
+    const int t_lo = pair0 / G, t_hi = (pair0 + kChunkRows < pairs ? pair0 + kChunkRows : pairs) - 1;
+    const DcSteps steps = dc_steps<KT>(a, span.start + t_lo, span.start + t_hi / G);
+    const int per = (steps.steps + a.n_splits - 1) / a.n_splits;
+    const int begin = split * per, end = begin + per < steps.steps ? begin + per : steps.steps;
+
+    // the wave's pairs: lane's own, and the least and the largest row
+    const int first = pair0 + wave * kRowsOfWave;
+    const bool live = first < pairs;
+    const int own = first + (lane & 31), pair = own < pairs ? own : pairs - 1, token = pair / G;
+    const int p = span.start + token;
+    const int p_lo = span.start + (live ? first : pairs - 1) / G;
+    const int p_hi = span.start + (first + kRowsOfWave - 1 < pairs ? first + kRowsOfWave - 1 : pairs - 1) / G;
+    dc_u32x4 bq[KS];
+    {
+        const uint16_t *src = a.q + dc_token_at(a.t, a.qs, span, b, token) + (int64_t)(h * G + pair % G) * a.qs.h + 8 * half;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) bq[s] = *reinterpret_cast<const dc_u32x4 *>(src + 16 * s);
+    }
+    dc_f32x16 o[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = begin < end ? kNoLogit : -INFINITY, l = 0.f;
+
+    // staging: a wave's load n has rows (wave + 4 n) PER .., of one tile of 16 and so of one page
+    const uint16_t *kh = a.p.k + h * a.p.kh, *vh = a.p.v + h * a.p.vh;
+    const int32_t *table = a.p.table + (int64_t)b * a.p.table_stride;
+    const int last_page = (a.n_rows - 1) >> a.p.shift, mask = (1 << a.p.shift) - 1;
+    const int in_row = lane / T::CHUNKS, chunk = lane % T::CHUNKS;
+    dc_u32x4 kst[T::LOADS], vst[T::LOADS];
+    auto fetch = [&](int s) __attribute__((always_inline)) {  // returns a bit for each tile of 16 rows that has a page
+        const int row0 = steps.row(s, KT);
+        int have = 0, id[KT / 16];
+#pragma unroll
+        for (int t = 0; t < KT / 16; ++t) {
+            const int page = (row0 + 16 * t) >> a.p.shift;
+            id[t] = dc_page_id(a.p, table, page < last_page ? page : last_page);
+            have |= id[t] < 0 ? 0 : 1 << t;
+        }
+#pragma unroll
+        for (int n = 0; n < T::LOADS; ++n) {
+            const int row = (wave + 4 * n) * T::PER;
+            const int page_ = [&]() __attribute__((always_inline)) {
+                if constexpr (T::PER <= 4) return id[4 * n * T::PER / 16];  // (the four waves' loads n are one tile's, or a quarter of it)
+                else return wave * T::PER >= 16 ? id[2 * n + 1] : id[2 * n];
+            }();
+            const int64_t page = page_ < 0 ? 0 : page_;
+            const int64_t at = (int64_t)((row0 + row) & mask) * HD + in_row * HD + chunk * 8;
+            kst[n] = *reinterpret_cast<const dc_u32x4 *>(kh + page * a.p.kp + at);
+            vst[n] = *reinterpret_cast<const dc_u32x4 *>(vh + page * a.p.vp + at);
+        }
+        return have;
+    };
+    auto stage = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < T::LOADS; ++n) {
+            const int row = (wave + 4 * n) * T::PER + in_row;
+            *reinterpret_cast<dc_u32x4 *>(&s_kv[buf][0][row * T::ROW + ((chunk ^ T::k_turn(row)) << 4)]) = kst[n];
+            *reinterpret_cast<dc_u32x4 *>(&s_kv[buf][1][row * T::ROW + ((chunk ^ T::v_turn(row)) << 4)]) = vst[n];
+        }
+    };
+
+    int have = 0, next = 0;
+    if (begin < end) {
+        have = fetch(begin);
+        stage(0);
+    }
+    __syncthreads();
+    for (int s = begin; s < end; ++s) {
+        const int buf = (s - begin) & 1, row0 = steps.row(s, KT);
+        if (s + 1 < end) next = fetch(s + 1);
+        // rows that the wave has no use for: behind all its pairs, or between the sinks and all windows
+        const bool use = live && row0 <= p_hi && (a.window == 0 || row0 + KT - 1 > p_lo - a.window || row0 < a.n_sink);
+        if (use) {
+            const bool whole = have == (1 << (KT / 16)) - 1 && row0 + KT - 1 <= p_lo && row0 + KT <= a.n_rows &&
+                               (a.window == 0 || row0 > p_hi - a.window || row0 + KT <= a.n_sink);
+            // S^T: x[t][i] is row 32 t + 8 (i / 4) + 4 half + i % 4
+            dc_f32x16 x[ST];
+            const uint8_t *ks = s_kv[buf][0] + (lane & 31) * T::ROW;
+            const int turn = (half ^ T::k_turn(lane & 31)) << 4;
+#pragma unroll
+            for (int t = 0; t < ST; ++t) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    const dc_u32x4 w = *reinterpret_cast<const dc_u32x4 *>(ks + 32 * t * T::ROW + (turn ^ (j << 5)));
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, bq[j]), x[t], 0, 0, 0);
+                }
+            }
+            if (!whole) {
+#pragma unroll
+                for (int t = 0; t < ST; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (!((have >> (2 * t + i / 8)) & 1) || !dc_attends(a, p, row0 + 32 * t + 8 * (i / 4) + 4 * half + i % 4)) x[t][i] = -INFINITY;
+            }
+            float most = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < ST; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, x[t][i]);
+            most *= a.scale;
+            if (__any(most > m + 8.f)) {
+                const float to = fmaxf(m, dc_over32(most, [](float u, float v) { return fmaxf(u, v); }));
+                const float f = m > kNoLogit ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[d][i] *= f;
+                m = to;
+            }
+#pragma unroll
+            for (int t = 0; t < ST; ++t)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    x[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], a.scale, -m));
+                    l += x[t][i];
+                }
+            // O^T: rows 16 j + {0 .. 3, 8 .. 11} + 4 half at a time
+            const int in = (lane >> 2) & 3;  // a transposing read's row of four
+            const uint8_t *vs = s_kv[buf][1] + (4 * half + in) * T::ROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+            const int vturn = T::v_turn(4 * half + in) << 4;
+#pragma unroll
+            for (int j = 0; j < KT / 16; ++j) {
+                dc_u32x4 pw;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pw[i] = dc_pack_bf16(x[j / 2][8 * (j % 2) + 2 * i], x[j / 2][8 * (j % 2) + 2 * i + 1]);
+#pragma unroll
+                for (int d = 0; d < DT; ++d) {
+                    const uint8_t *at = vs + 16 * j * T::ROW + (vturn ^ (d << 6));
+                    const dc_u32x2 lo = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at)));
+                    const dc_u32x2 hi = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at + 8 * T::ROW)));
+                    const dc_u32x4 w = {lo.x, lo.y, hi.x, hi.y};
+                    auto mul = [&](dc_u32x4 v, dc_f32x16 acc) __attribute__((always_inline)) {
+                        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, v), __builtin_bit_cast(dc_bf16x8, pw), acc, 0, 0, 0);
+                    };
+                    if (whole) o[d] = mul(w, o[d]);
+                    else dc_careful<16>(w, o[d], mul);
+                }
+            }
+        }
+        if (s + 1 < end) stage(buf ^ 1);
+        have = next;
+        __syncthreads();
+    }
+
+    l = dc_over32(l, [](float u, float v) { return u + v; });
+    if (own >= pairs) return;
+    const int64_t dst = (int64_t)(span.first + token) * a.n_h * G + h * G + pair % G;
+    if (a.n_splits > 1) {
+        const int64_t slot = ((int64_t)(unit * a.tiles + tile) * a.n_splits + split) * kChunkRows + wave * kRowsOfWave + (lane & 31);
+        float *acc = a.ws_acc + slot * HD + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+                *reinterpret_cast<float4 *>(acc + 32 * d + 2 * i) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
+        if (half == 0) reinterpret_cast<float2 *>(a.ws_ml)[slot] = make_float2(m, l);
+        return;
+    }
+    const float inv = l == 0.f ? 1.f : l;
+    uint16_t *out = a.out + dst * HD + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<uint2 *>(out + 32 * d + 2 * i) =
+                make_uint2(dc_pack_bf16(o[d][i] / inv, o[d][i + 1] / inv), dc_pack_bf16(o[d][i + 2] / inv, o[d][i + 3] / inv));
+    if (a.lse && half == 0) a.lse[dst] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+}
+
+constexpr int step_rows(int hd) { return hd == 256 ? 32 : 64; }
+
+template <int HD>
+void launch(const DcPagedAttn &a, unsigned blocks, hipStream_t st) {
+    hipLaunchKernelGGL((paged_chunk_kernel<HD, step_rows(HD)>), dim3(blocks), dim3(kThreads), 0, st, a);
+}
+
+}  // namespace
+
+int dc_paged_chunk_splits(int64_t n_units, int64_t tiles, int hd, int64_t rows) {
+    const int64_t blocks = n_units * tiles, most = hd == 256 ? 256 : 512;
+    const int64_t parts = (rows + step_rows(hd) - 1) / step_rows(hd) / 4;   // four steps to a part or more
+    const int64_t want = blocks >= most ? 1 : most / blocks;
+    return (int)(want < parts ? want : parts > 1 ? parts : 1);
+}
+
+int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, int n_units, hipStream_t st) {
+    const unsigned blocks = (unsigned)((int64_t)n_units * a.tiles * a.n_splits);
+    if (hd == 64) launch<64>(a, blocks, st);
+    else if (hd == 128) launch<128>(a, blocks, st);
+    else launch<256>(a, blocks, st);
+    return DC_OK;
+}

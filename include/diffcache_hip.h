@@ -712,6 +712,99 @@ typedef struct dc_mx_attn_args {
 size_t dc_mx_attn_workspace_bytes(int n_units, int group, int hd, int n_rows);
 int dc_mx_attn_bf16(const dc_mx_attn_args *args, void *stream);
 
+/*
+ * K and V in pages, for callers that hold many sequences of unequal and growing lengths, or share the rows of a common beginning.
+ * The reference reserves max_length rows for every sequence (src/diffcache/kvcache/diffcache.py:48-66) and attends over them with
+ * flash_attn_with_kvcache (src/diffcache/base.py:134-142); here a sequence has the pages that it needs.
+ *
+ * dc_paged_store names the pages of a layer: head h's rows of page i, `page` of them, hd numbers each, one after another at
+ *   k + i * k_page_stride + h * k_head_stride
+ * and V's likewise; strides in elements, multiples of 8, pointers 16-byte aligned.  page: a power of two from 16 to 65536.  Pages or
+ * heads that share their rows may be read, not written.  hd: 64, 128 or 256.
+ *
+ * dc_paged_tokens says where sequences' rows and their new tokens are:
+ *   table    (n_b, table_pages) int32 on the device, rows table_stride apart: row r of sequence b is row r % page of page
+ *            table[b][r / page].  An id that the store does not have (-1, say) is no page: its rows are neither written nor
+ *            attended to
+ *   start    NULL (zeros), or (n_b) int32 on the device: the rows that the sequences hold before their new tokens.  Token i of sequence b
+ *            is its row start[b] + i.  A negative start counts as 0, one above 2^30 as 2^30
+ *   cu       NULL, or (n_b + 1) int32 on the device: tokens are packed, those of sequence b the rows cu[b] .. cu[b + 1] - 1 of tensors
+ *            of n_tokens rows; the batch strides are not used.  Of a sequence with more than max_new tokens the first max_new
+ *            count; what lies outside the tensors does not count
+ *   counts   with cu NULL, tensors of (n_b, max_new) tokens by strides: NULL (all of them), or (n_b) int32 on the device, the tokens
+ *            that sequence b has; those behind them are neither read nor written
+ *   max_new  the most new tokens of a sequence: sizes the launch
+ * Of a row that a call writes for two tokens (a page that two sequences share) it is not defined which one's numbers stay.
+ */
+typedef struct dc_paged_store {
+    void *k, *v;
+    int64_t k_page_stride, k_head_stride, v_page_stride, v_head_stride;
+    int n_pages, page;
+} dc_paged_store;
+typedef struct dc_paged_tokens {
+    const int32_t *table, *start, *cu, *counts;
+    int64_t table_stride;
+    int n_b, max_new, n_tokens, table_pages;
+} dc_paged_tokens;
+
+/*
+ * K and V of new tokens into their rows, K rotated by the tokens' positions on the way, and the queries rotated into q_out.
+ *   k_src, v_src  n_h heads of hd numbers of every token, by element strides (batch, token, head; hd contiguous)
+ *   q_src, q_out  NULL, or n_q heads likewise (n_q 0 without them); q_out contiguous, and q_src itself where that is contiguous
+ *            too.  A token's queries are rotated whether its row has a page or not
+ *   rot      rotated columns of a head, a multiple of 16 (0: none; then no queries); the others stay as they are
+ *   inv_freq (rot / 2) fp32: the angle of pair f is position * inv_freq[f], taken in 64 bits whatever the position
+ *   interleaved  0: pair f is columns f and f + rot / 2; else columns 2 f and 2 f + 1
+ *   pos      NULL (a token's position is its row), or n_axes int32 for every token on the device, contiguous
+ *   n_axes, section  1, or up to 4: the first section[0] frequencies go by a token's first position, the next section[1] by its
+ *            second, and so on (time, height and width of images and video); the sections' sum is rot / 2
+ * (x_a, x_b) becomes (x_a cos - x_b sin, x_b cos + x_a sin) in fp32, rounded once.  start is not changed.  Stands beside dc_append_kv_bf16
+ * and the rotation of the reference's layers (base.py:122-132).
+ */
+typedef struct dc_paged_append_args {
+    const void *k_src, *v_src, *q_src;
+    void *q_out;
+    const float *inv_freq;
+    const int32_t *pos;
+    dc_paged_store store;
+    dc_paged_tokens tokens;
+    int64_t k_batch_stride, k_token_stride, k_head_stride, v_batch_stride, v_token_stride, v_head_stride;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    int n_h, n_q, hd, rot, interleaved, n_axes, section[4];
+} dc_paged_append_args;
+int dc_paged_append_bf16(const dc_paged_append_args *args, void *stream);
+
+/*
+ * Attention of new tokens over the rows of their sequences, whose own rows are in their pages already: the token at row p attends to
+ * rows 0 .. p, or with window > 0 to the first n_sink and the last `window` of them (its own among these).
+ *   q        n_h * group heads of hd bf16 numbers of every token, by element strides (batch, token, head; hd contiguous)
+ *   out      as many, contiguous: softmax(scale q k^T) v; lse NULL, or (tokens, n_h * group) fp32, the log of the sum of
+ *            exp(scale q k^T).  Those of tokens that do not count stay as they were
+ *   n_rows   rows at or beyond it are not attended to (at most table_pages * page): sizes the launch
+ *   group    up to 16; scale: positive and finite
+ * A token that attends to no row has out 0 and lse -inf.  What a token does not attend to may hold anything, and leaves no trace.  Of what
+ * it does attend to, a number of K that is not finite makes the head's outputs and lse NaN where a logit becomes NaN or +inf; one of V the
+ * outputs of its column.  Logits are fp32, before the scale too: one that falls below its range is -inf, a weight of 0; one above
+ * it makes its head NaN.  Sums and statistics are fp32.
+ * The workspace (dc_paged_attn_workspace_bytes for the same sizes, 256-byte aligned; 0: none; with max_new * group up to 16, enough for
+ * more sequences, rows or tokens is enough for fewer) holds nothing between calls; calls that may overlap need one each.  Replaces
+ * flash_attn_with_kvcache (base.py:134-142) over such a cache.
+ */
+typedef struct dc_paged_attn_args {
+    const void *q;
+    void *out;
+    float *lse;
+    dc_paged_store store;
+    dc_paged_tokens tokens;
+    int64_t q_batch_stride, q_token_stride, q_head_stride;
+    void *workspace;
+    size_t workspace_bytes;
+    int n_h, group, hd, n_rows, n_sink, window;
+    float scale;
+} dc_paged_attn_args;
+size_t dc_paged_attn_workspace_bytes(int n_units, int group, int hd, int n_rows, int max_new);
+int dc_paged_attn_bf16(const dc_paged_attn_args *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
