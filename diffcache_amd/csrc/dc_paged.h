@@ -138,13 +138,20 @@ __device__ __forceinline__ float dc_over16(float x, F f) {
     return dc_over32(f(__uint_as_float(r.x), __uint_as_float(r.y)), f);
 }
 
-// Two bf16 numbers: whether one is not finite, and the parts that a product with weights of 0 can take.  Rows that some of a step's
-// heads attend to and others do not are multiplied by 0 for those: where V is not finite the product would be NaN.  So it is
-// taken of the finite numbers alone, and a sum of weights on what is +inf or NaN, and one on what is -inf or NaN, say where
-// the result is not finite.
-__device__ __forceinline__ uint32_t dc_unbounded(uint32_t w) {  // 0xffff in the halves that are not finite
-    const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u, hi = (w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u;
-    return lo | hi;
+// Rows that some of a step's pairs attend to and others do not are multiplied by 0 for those: where V is not finite the product would be
+// NaN.  A step that is not attended to as a whole is looked over for such numbers; where there are any, the product is taken of the
+// finite ones alone, and a sum of weights on what is +inf or NaN, and one on what is -inf or NaN, say where the result is not finite.
+typedef unsigned short dc_u16x2 __attribute__((ext_vector_type(2)));
+struct DcUnbounded {
+    dc_u16x2 most = {0, 0};
+    __device__ __forceinline__ void look(uint32_t w) {
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(dc_u16x2, w & 0x7f807f80u));
+    }
+    __device__ __forceinline__ bool any() const { return __any(most.x == 0x7f80 || most.y == 0x7f80); }
+};
+__device__ __forceinline__ uint32_t dc_finite(uint32_t w) {  // 0 in the halves that are not
+    const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0u : 0xffffu, hi = (w & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u;
+    return w & (lo | hi);
 }
 __device__ __forceinline__ uint32_t dc_unbounded_side(uint32_t w, bool negative) {  // 1 where a half is NaN or the infinity of that sign
     auto one = [&](uint32_t h) __attribute__((always_inline)) {
@@ -156,19 +163,9 @@ __device__ __forceinline__ uint32_t dc_unbounded_side(uint32_t w, bool negative)
 // acc += P V by mfma(V's operand, acc), V's operand in w
 template <int N, typename Acc, typename M>
 __device__ __forceinline__ void dc_careful(dc_u32x4 w, Acc &acc, M mfma) {
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) bad |= dc_unbounded(w[i]);
-    if (!__any(bad != 0u)) {
-        acc = mfma(w, acc);
-        return;
-    }
     dc_u32x4 fine, up, down;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        fine[i] = w[i] & ~dc_unbounded(w[i]);
-        up[i] = dc_unbounded_side(w[i], false), down[i] = dc_unbounded_side(w[i], true);
-    }
+    for (int i = 0; i < 4; ++i) fine[i] = dc_finite(w[i]), up[i] = dc_unbounded_side(w[i], false), down[i] = dc_unbounded_side(w[i], true);
     Acc zero;
 #pragma unroll
     for (int i = 0; i < N; ++i) zero[i] = 0.f;

@@ -118,8 +118,19 @@ struct Rows {
             }
     }
 
-    // acc += P V over the step that load_v brought; whole: every row is attended to by every pair
-    __device__ __forceinline__ void add(const float (&x)[TILES][4], bool whole) {
+    // whether a number of the step that load_v brought is not finite
+    __device__ __forceinline__ bool unbounded() const {
+        DcUnbounded u;
+#pragma unroll
+        for (int t = 0; t < TILES * 4; ++t)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) u.look(vw[t][i]);
+        return u.any();
+    }
+
+    // acc += P V over the step that load_v brought
+    template <bool CAREFUL>
+    __device__ __forceinline__ void add(const float (&x)[TILES][4]) {
 #pragma unroll
         for (int u = 0; u < TILES / 2; ++u) {
             dc_u32x4 hi, lo;
@@ -139,8 +150,8 @@ struct Rows {
                 dc_u32x4 w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(vw[8 * u + 2 * i + 1][j / 2], vw[8 * u + 2 * i][j / 2], sel);
-                if (whole) acc[j] = both(w, acc[j]);
-                else dc_careful<4>(w, acc[j], both);
+                if constexpr (CAREFUL) dc_careful<4>(w, acc[j], both);
+                else acc[j] = both(w, acc[j]);
             }
         }
     }
@@ -248,7 +259,8 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void paged_rows_kernel(DcPagedA
                     if (!((have >> t) & 1) || !dc_attends(a, p, r0 + 16 * t + 4 * i + w.q)) x[t][i] = -INFINITY;
         }
         w.weigh(x);
-        w.add(x, whole);
+        if (whole || !w.unbounded()) w.template add<false>(x);
+        else w.template add<true>(x);
         if (more) w.load_v(vt);
     }
 

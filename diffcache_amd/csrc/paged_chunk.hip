@@ -13,6 +13,7 @@
 // 1.7e-3 is the output's alone).  Softmax in powers of two, fp32; the maximum moves where a
 // logit passes it by more than 8.
 #include "dc_paged.h"
+#include <type_traits>
 
 namespace {
 
@@ -39,6 +40,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
     using T = Tile<HD, KT>;
     constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32;      // products of a tile's S; tiles of O and of S
     __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2][T::BYTES];
+    __shared__ __attribute__((aligned(16))) uint32_t s_unbounded[2][4];  // [buffer][wave]: of what the wave staged of V
     const int n_units = (int)(gridDim.x / (unsigned)(a.tiles * a.n_splits));
     // units first, so that a unit's blocks are on one XCD where their number divides by eight; late tokens first, they have the most rows
     const int unit = (int)(blockIdx.x % (unsigned)n_units), rest = (int)(blockIdx.x / (unsigned)n_units);
@@ -102,7 +104,21 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
         }
         return have;
     };
-    auto stage = [&](int buf) __attribute__((always_inline)) {
+    auto whole_for = [&](int lo, int hi, int row0, int have) __attribute__((always_inline)) {  // pairs at rows lo .. hi attend to all of a step
+        return have == (1 << (KT / 16)) - 1 && row0 + KT - 1 <= lo && row0 + KT <= a.n_rows &&
+               (a.window == 0 || row0 > hi - a.window || row0 + KT <= a.n_sink);
+    };
+    auto stage = [&](int buf, int s, int have) __attribute__((always_inline)) {
+        uint32_t unbounded = 0;
+        if (!whole_for(span.start + t_lo, span.start + t_hi / G, steps.row(s, KT), have)) {
+            DcUnbounded u;
+#pragma unroll
+            for (int n = 0; n < T::LOADS; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) u.look(vst[n][i]);
+            unbounded = u.any();
+        }
+        if (lane == 0) s_unbounded[buf][wave] = unbounded;
 #pragma unroll
         for (int n = 0; n < T::LOADS; ++n) {
             const int row = (wave + 4 * n) * T::PER + in_row;
@@ -114,7 +130,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
     int have = 0, next = 0;
     if (begin < end) {
         have = fetch(begin);
-        stage(0);
+        stage(0, begin, have);
     }
     __syncthreads();
     for (int s = begin; s < end; ++s) {
@@ -123,8 +139,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
         // rows that the wave has no use for: behind all its pairs, or between the sinks and all windows
         const bool use = live && row0 <= p_hi && (a.window == 0 || row0 + KT - 1 > p_lo - a.window || row0 < a.n_sink);
         if (use) {
-            const bool whole = have == (1 << (KT / 16)) - 1 && row0 + KT - 1 <= p_lo && row0 + KT <= a.n_rows &&
-                               (a.window == 0 || row0 > p_hi - a.window || row0 + KT <= a.n_sink);
+            const bool whole = whole_for(p_lo, p_hi, row0, have);
             // S^T: x[t][i] is row 32 t + 8 (i / 4) + 4 half + i % 4
             dc_f32x16 x[ST];
             const uint8_t *ks = s_kv[buf][0] + (lane & 31) * T::ROW;
@@ -173,26 +188,31 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
             const int in = (lane >> 2) & 3;  // a transposing read's row of four
             const uint8_t *vs = s_kv[buf][1] + (4 * half + in) * T::ROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
             const int vturn = T::v_turn(4 * half + in) << 4;
+            auto add = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < KT / 16; ++j) {
-                dc_u32x4 pw;
+                for (int j = 0; j < KT / 16; ++j) {
+                    dc_u32x4 pw;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) pw[i] = dc_pack_bf16(x[j / 2][8 * (j % 2) + 2 * i], x[j / 2][8 * (j % 2) + 2 * i + 1]);
+                    for (int i = 0; i < 4; ++i) pw[i] = dc_pack_bf16(x[j / 2][8 * (j % 2) + 2 * i], x[j / 2][8 * (j % 2) + 2 * i + 1]);
 #pragma unroll
-                for (int d = 0; d < DT; ++d) {
-                    const uint8_t *at = vs + 16 * j * T::ROW + (vturn ^ (d << 6));
-                    const dc_u32x2 lo = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at)));
-                    const dc_u32x2 hi = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at + 8 * T::ROW)));
-                    const dc_u32x4 w = {lo.x, lo.y, hi.x, hi.y};
-                    auto mul = [&](dc_u32x4 v, dc_f32x16 acc) __attribute__((always_inline)) {
-                        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, v), __builtin_bit_cast(dc_bf16x8, pw), acc, 0, 0, 0);
-                    };
-                    if (whole) o[d] = mul(w, o[d]);
-                    else dc_careful<16>(w, o[d], mul);
+                    for (int d = 0; d < DT; ++d) {
+                        const uint8_t *at = vs + 16 * j * T::ROW + (vturn ^ (d << 6));
+                        const dc_u32x2 lo = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at)));
+                        const dc_u32x2 hi = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at + 8 * T::ROW)));
+                        const dc_u32x4 w = {lo.x, lo.y, hi.x, hi.y};
+                        auto mul = [&](dc_u32x4 v, dc_f32x16 acc) __attribute__((always_inline)) {
+                            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, v), __builtin_bit_cast(dc_bf16x8, pw), acc, 0, 0, 0);
+                        };
+                        if constexpr (decltype(careful)::value) dc_careful<16>(w, o[d], mul);
+                        else o[d] = mul(w, o[d]);
+                    }
                 }
-            }
+            };
+            const uint4 bad = *reinterpret_cast<const uint4 *>(s_unbounded[buf]);
+            if (whole || __builtin_amdgcn_readfirstlane(bad.x | bad.y | bad.z | bad.w) == 0) add(std::false_type{});
+            else add(std::true_type{});
         }
-        if (s + 1 < end) stage(buf ^ 1);
+        if (s + 1 < end) stage(buf ^ 1, s + 1, next);
         have = next;
         __syncthreads();
     }
