@@ -72,9 +72,17 @@ struct DcPagedAttn {
     float scale;             // times log2(e)
 };
 
-// Which rows a token at row p attends to: those up to it, and with a window the first n_sink and the last `window` of them.
-__device__ __forceinline__ bool dc_attends(const DcPagedAttn &a, int p, int row) {
-    return row <= p && row < a.n_rows && (a.window == 0 || row > p - a.window || row < a.n_sink);
+// Which rows a token attends to: [0, hi] without those in [sink, lo].
+struct DcReach {
+    int hi, lo, sink;
+    __device__ __forceinline__ bool has(int row) const { return (row <= hi) & ((row > lo) | (row < sink)); }
+};
+__device__ __forceinline__ DcReach dc_reach(const DcPagedAttn &a, int p) {
+    return {p < a.n_rows ? p : a.n_rows - 1, a.window ? p - a.window : -1, a.window ? a.n_sink : 0};
+}
+// Whether tokens at rows p_lo .. p_hi attend to all of rows [row, row + n)
+__device__ __forceinline__ bool dc_whole(const DcPagedAttn &a, int p_lo, int p_hi, int row, int n) {
+    return row + n - 1 <= p_lo && row + n <= a.n_rows && (a.window == 0 || row > p_hi - a.window || row + n <= a.n_sink);
 }
 
 // The steps of STEP rows that tokens at rows [p_lo, p_hi] need: the first `sinks` of a sequence's, then those from `first` on.
@@ -139,8 +147,8 @@ __device__ __forceinline__ float dc_over16(float x, F f) {
 }
 
 // Rows that some of a step's pairs attend to and others do not are multiplied by 0 for those: where V is not finite the product would be
-// NaN.  A step that is not attended to as a whole is looked over for such numbers; where there are any, the product is taken of the
-// finite ones alone, and a sum of weights on what is +inf or NaN, and one on what is -inf or NaN, say where the result is not finite.
+// NaN.  A step that is not attended to as a whole is looked over for such numbers; where there are any, the product takes zeros in their
+// places, and they are added to the outputs of the pairs that attend to them afterwards, as they are.
 typedef unsigned short dc_u16x2 __attribute__((ext_vector_type(2)));
 struct DcUnbounded {
     dc_u16x2 most = {0, 0};
@@ -153,27 +161,4 @@ __device__ __forceinline__ uint32_t dc_finite(uint32_t w) {  // 0 in the halves 
     const uint32_t lo = (w & 0x7f80u) == 0x7f80u ? 0u : 0xffffu, hi = (w & 0x7f800000u) == 0x7f800000u ? 0u : 0xffff0000u;
     return w & (lo | hi);
 }
-__device__ __forceinline__ uint32_t dc_unbounded_side(uint32_t w, bool negative) {  // 1 where a half is NaN or the infinity of that sign
-    auto one = [&](uint32_t h) __attribute__((always_inline)) {
-        const bool nan = (h & 0x7fffu) > 0x7f80u, inf = (h & 0x7fffu) == 0x7f80u && ((h >> 15) != 0u) == negative;
-        return nan || inf ? 0x3f80u : 0u;
-    };
-    return one(w & 0xffffu) | (one(w >> 16) << 16);
-}
-// acc += P V by mfma(V's operand, acc), V's operand in w
-template <int N, typename Acc, typename M>
-__device__ __forceinline__ void dc_careful(dc_u32x4 w, Acc &acc, M mfma) {
-    dc_u32x4 fine, up, down;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fine[i] = dc_finite(w[i]), up[i] = dc_unbounded_side(w[i], false), down[i] = dc_unbounded_side(w[i], true);
-    Acc zero;
-#pragma unroll
-    for (int i = 0; i < N; ++i) zero[i] = 0.f;
-    const Acc a = mfma(up, zero), b = mfma(down, zero);
-    acc = mfma(fine, acc);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (a[i] > 0.f) acc[i] += INFINITY;
-        if (b[i] > 0.f) acc[i] -= INFINITY;
-    }
-}
+__device__ __forceinline__ float dc_only_unbounded(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? x : 0.f; }

@@ -128,8 +128,27 @@ struct Rows {
         return u.any();
     }
 
+    __device__ __forceinline__ void bound() {
+#pragma unroll
+        for (int t = 0; t < TILES * 4; ++t)
+#pragma unroll
+            for (int i = 0; i < VW; ++i) vw[t][i] = dc_finite(vw[t][i]);
+    }
+    // acc += what is not finite of one row of V (src, the row's column 0), for the pairs that attend to it
+    __device__ __forceinline__ void add_unbounded(const uint16_t *src, const bool (&in)[4]) {
+#pragma unroll
+        for (int j = 0; j < EPL; j += 4) {
+            const uint2 w = *reinterpret_cast<const uint2 *>(src + column(c, j));
+            const float x[4] = {dc_only_unbounded(dc_bf16_lo(w.x)), dc_only_unbounded(dc_bf16_hi(w.x)), dc_only_unbounded(dc_bf16_lo(w.y)),
+                                dc_only_unbounded(dc_bf16_hi(w.y))};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[j + e][i] += in[i] ? x[e] : 0.f;
+        }
+    }
+
     // acc += P V over the step that load_v brought
-    template <bool CAREFUL>
     __device__ __forceinline__ void add(const float (&x)[TILES][4]) {
 #pragma unroll
         for (int u = 0; u < TILES / 2; ++u) {
@@ -140,18 +159,14 @@ struct Rows {
                 hi[i] = dc_pack_bf16(x0, x1);
                 lo[i] = dc_pack_bf16(x0 - dc_bf16_lo(hi[i]), x1 - dc_bf16_hi(hi[i]));
             }
-            auto both = [&](dc_u32x4 w, dc_f32x4 o) __attribute__((always_inline)) {
-                o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, lo), __builtin_bit_cast(dc_bf16x8, w), o, 0, 0, 0);
-                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, hi), __builtin_bit_cast(dc_bf16x8, w), o, 0, 0, 0);
-            };
 #pragma unroll
             for (int j = 0; j < EPL; ++j) {
                 const uint32_t sel = j % 2 ? 0x07060302u : 0x05040100u;  // the high or the low halves of two words
                 dc_u32x4 w;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_perm(vw[8 * u + 2 * i + 1][j / 2], vw[8 * u + 2 * i][j / 2], sel);
-                if constexpr (CAREFUL) dc_careful<4>(w, acc[j], both);
-                else acc[j] = both(w, acc[j]);
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, lo), __builtin_bit_cast(dc_bf16x8, w), acc[j], 0, 0, 0);
+                acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, hi), __builtin_bit_cast(dc_bf16x8, w), acc[j], 0, 0, 0);
             }
         }
     }
@@ -199,7 +214,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void paged_rows_kernel(DcPagedA
     w.start(lane);
     const int pair = w.c < pairs ? w.c : pairs - 1, token = pair / G;  // (the last pair again in the place of one that does not exist)
     w.load_q(a.q + dc_token_at(a.t, a.qs, span, b, token) + (int64_t)(h * G + pair % G) * a.qs.h);
-    const int p = span.start + token;
+    const DcReach reach = dc_reach(a, span.start + token);
 
     const uint16_t *kh = a.p.k + h * a.p.kh, *vh = a.p.v + h * a.p.vh;
     const int32_t *table = a.p.table + (int64_t)b * a.p.table_stride;
@@ -248,19 +263,32 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void paged_rows_kernel(DcPagedA
             at = at + 1 < mine ? at + 1 : 0;
             look();
         }
-        // every row for every pair?
-        const bool whole = have == (1 << TILES) - 1 && r0 + STEP - 1 <= p_lo && r0 + STEP <= a.n_rows &&
-                           (a.window == 0 || r0 > p_hi - a.window || r0 + STEP <= a.n_sink);
+        const bool whole = have == (1 << TILES) - 1 && dc_whole(a, p_lo, p_hi, r0, STEP);  // every row for every pair
+        bool odd = false;
         if (!whole) {
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    if (!((have >> t) & 1) || !dc_attends(a, p, r0 + 16 * t + 4 * i + w.q)) x[t][i] = -INFINITY;
+                    if (!((have >> t) & 1) | !reach.has(r0 + 16 * t + 4 * i + w.q)) x[t][i] = -INFINITY;
+            odd = w.unbounded();
+            if (odd) w.bound();
         }
         w.weigh(x);
-        if (whole || !w.unbounded()) w.template add<false>(x);
-        else w.template add<true>(x);
+        w.add(x);
+        if (odd) {
+            DcReach of[4];  // of the pairs whose sums the lane has
+#pragma unroll
+            for (int i = 0; i < 4; ++i) of[i] = dc_reach(a, span.start + (4 * w.q + i < pairs ? 4 * w.q + i : pairs - 1) / G);
+            for (int r = 0; r < STEP; ++r) {
+                const int page = (r0 + r) >> a.p.shift, at_id = dc_page_id(a.p, table, page < last_page ? page : last_page);
+                if (at_id < 0) continue;
+                bool in[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) in[i] = of[i].has(r0 + r);
+                w.add_unbounded(vh + at_id * a.p.vp + (int64_t)((r0 + r) & mask) * HD, in);
+            }
+        }
         if (more) w.load_v(vt);
     }
 

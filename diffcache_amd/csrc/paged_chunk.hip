@@ -13,7 +13,6 @@
 // 1.7e-3 is the output's alone).  Softmax in powers of two, fp32; the maximum moves where a
 // logit passes it by more than 8.
 #include "dc_paged.h"
-#include <type_traits>
 
 namespace {
 
@@ -38,9 +37,9 @@ struct Tile {
 template <int HD, int KT>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kernel(DcPagedAttn a) {
     using T = Tile<HD, KT>;
-    constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32;      // products of a tile's S; tiles of O and of S
+    constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, TILES = KT / 16;  // products of a tile's S; tiles of O, of S, and of what a page holds whole
     __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2][T::BYTES];
-    __shared__ __attribute__((aligned(16))) uint32_t s_unbounded[2][4];  // [buffer][wave]: of what the wave staged of V
+    __shared__ __attribute__((aligned(16))) uint32_t s_odd[2][4];  // [buffer][wave]: whether the wave left out numbers of V that are not finite
     const int n_units = (int)(gridDim.x / (unsigned)(a.tiles * a.n_splits));
     // units first, so that a unit's blocks are on one XCD where their number divides by eight; late tokens first, they have the most rows
     const int unit = (int)(blockIdx.x % (unsigned)n_units), rest = (int)(blockIdx.x / (unsigned)n_units);
@@ -59,7 +58,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
     const int first = pair0 + wave * kRowsOfWave;
     const bool live = first < pairs;
     const int own = first + (lane & 31), pair = own < pairs ? own : pairs - 1, token = pair / G;
-    const int p = span.start + token;
+    const DcReach reach = dc_reach(a, span.start + token);
     const int p_lo = span.start + (live ? first : pairs - 1) / G;
     const int p_hi = span.start + (first + kRowsOfWave - 1 < pairs ? first + kRowsOfWave - 1 : pairs - 1) / G;
     dc_u32x4 bq[KS];
@@ -75,50 +74,55 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = begin < end ? kNoLogit : -INFINITY, l = 0.f;
 
-    // staging: a wave's load n has rows (wave + 4 n) PER .., of one tile of 16 and so of one page
+    // staging: a wave's load n has rows (wave + 4 n) PER .., of one tile of 16 and so of one page.  The step's page ids are one
+    // load of as many lanes, made a step before they are needed.
     const uint16_t *kh = a.p.k + h * a.p.kh, *vh = a.p.v + h * a.p.vh;
     const int32_t *table = a.p.table + (int64_t)b * a.p.table_stride;
     const int last_page = (a.n_rows - 1) >> a.p.shift, mask = (1 << a.p.shift) - 1;
-    const int in_row = lane / T::CHUNKS, chunk = lane % T::CHUNKS;
+    const int in_row = lane / T::CHUNKS, chunk = lane % T::CHUNKS, in_page = in_row * HD + chunk * 8;
     dc_u32x4 kst[T::LOADS], vst[T::LOADS];
-    auto fetch = [&](int s) __attribute__((always_inline)) {  // returns a bit for each tile of 16 rows that has a page
+    auto ids_of = [&](int s) __attribute__((always_inline)) {
+        const int page = (steps.row(s, KT) + 16 * (lane % TILES)) >> a.p.shift;
+        return table[page < last_page ? page : last_page];
+    };
+    auto fetch = [&](int s, int ids) __attribute__((always_inline)) {  // returns a bit for each tile of 16 rows that has a page
         const int row0 = steps.row(s, KT);
-        int have = 0, id[KT / 16];
+        int have = 0, id[TILES];
 #pragma unroll
-        for (int t = 0; t < KT / 16; ++t) {
-            const int page = (row0 + 16 * t) >> a.p.shift;
-            id[t] = dc_page_id(a.p, table, page < last_page ? page : last_page);
-            have |= id[t] < 0 ? 0 : 1 << t;
+        for (int t = 0; t < TILES; ++t) {
+            id[t] = __builtin_amdgcn_readlane(ids, t);
+            const bool is = (unsigned)id[t] < (unsigned)a.p.n_pages;
+            have |= is ? 1 << t : 0, id[t] = is ? id[t] : 0;  // (page 0 in the place of one that there is not)
         }
 #pragma unroll
         for (int n = 0; n < T::LOADS; ++n) {
             const int row = (wave + 4 * n) * T::PER;
-            const int page_ = [&]() __attribute__((always_inline)) {
-                if constexpr (T::PER <= 4) return id[4 * n * T::PER / 16];  // (the four waves' loads n are one tile's, or a quarter of it)
-                else return wave * T::PER >= 16 ? id[2 * n + 1] : id[2 * n];
-            }();
-            const int64_t page = page_ < 0 ? 0 : page_;
-            const int64_t at = (int64_t)((row0 + row) & mask) * HD + in_row * HD + chunk * 8;
-            kst[n] = *reinterpret_cast<const dc_u32x4 *>(kh + page * a.p.kp + at);
-            vst[n] = *reinterpret_cast<const dc_u32x4 *>(vh + page * a.p.vp + at);
+            int page = 0;
+            if constexpr (T::PER <= 4) page = id[4 * n * T::PER / 16];  // (the four waves' loads n are one tile's, or part of it)
+            else page = wave * T::PER >= 16 ? id[2 * n + 1] : id[2 * n];
+            const int64_t at = (int64_t)((row0 + row) & mask) * HD;
+            kst[n] = *reinterpret_cast<const dc_u32x4 *>(kh + (page * a.p.kp + at) + in_page);
+            vst[n] = *reinterpret_cast<const dc_u32x4 *>(vh + (page * a.p.vp + at) + in_page);
         }
         return have;
     };
-    auto whole_for = [&](int lo, int hi, int row0, int have) __attribute__((always_inline)) {  // pairs at rows lo .. hi attend to all of a step
-        return have == (1 << (KT / 16)) - 1 && row0 + KT - 1 <= lo && row0 + KT <= a.n_rows &&
-               (a.window == 0 || row0 > hi - a.window || row0 + KT <= a.n_sink);
-    };
     auto stage = [&](int buf, int s, int have) __attribute__((always_inline)) {
-        uint32_t unbounded = 0;
-        if (!whole_for(span.start + t_lo, span.start + t_hi / G, steps.row(s, KT), have)) {
+        uint32_t odd = 0;
+        if (have != (1 << TILES) - 1 || !dc_whole(a, span.start + t_lo, span.start + t_hi / G, steps.row(s, KT), KT)) {
             DcUnbounded u;
 #pragma unroll
             for (int n = 0; n < T::LOADS; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) u.look(vst[n][i]);
-            unbounded = u.any();
+            if (u.any()) {
+                odd = 1;
+#pragma unroll
+                for (int n = 0; n < T::LOADS; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vst[n][i] = dc_finite(vst[n][i]);
+            }
         }
-        if (lane == 0) s_unbounded[buf][wave] = unbounded;
+        if (lane == 0) s_odd[buf][wave] = odd;
 #pragma unroll
         for (int n = 0; n < T::LOADS; ++n) {
             const int row = (wave + 4 * n) * T::PER + in_row;
@@ -127,19 +131,22 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
         }
     };
 
-    int have = 0, next = 0;
+    int have = 0, next = 0, ids = 0;
     if (begin < end) {
-        have = fetch(begin);
+        have = fetch(begin, ids_of(begin));
+        if (begin + 1 < end) ids = ids_of(begin + 1);
         stage(0, begin, have);
     }
     __syncthreads();
     for (int s = begin; s < end; ++s) {
         const int buf = (s - begin) & 1, row0 = steps.row(s, KT);
-        if (s + 1 < end) next = fetch(s + 1);
+        if (s + 1 < end) {
+            next = fetch(s + 1, ids);
+            if (s + 2 < end) ids = ids_of(s + 2);
+        }
         // rows that the wave has no use for: behind all its pairs, or between the sinks and all windows
         const bool use = live && row0 <= p_hi && (a.window == 0 || row0 + KT - 1 > p_lo - a.window || row0 < a.n_sink);
         if (use) {
-            const bool whole = whole_for(p_lo, p_hi, row0, have);
             // S^T: x[t][i] is row 32 t + 8 (i / 4) + 4 half + i % 4
             dc_f32x16 x[ST];
             const uint8_t *ks = s_kv[buf][0] + (lane & 31) * T::ROW;
@@ -154,12 +161,12 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, bq[j]), x[t], 0, 0, 0);
                 }
             }
-            if (!whole) {
+            if (have != (1 << TILES) - 1 || !dc_whole(a, p_lo, p_hi, row0, KT)) {
 #pragma unroll
                 for (int t = 0; t < ST; ++t)
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
-                        if (!((have >> (2 * t + i / 8)) & 1) || !dc_attends(a, p, row0 + 32 * t + 8 * (i / 4) + 4 * half + i % 4)) x[t][i] = -INFINITY;
+                        if (!((have >> (2 * t + i / 8)) & 1) | !reach.has(row0 + 32 * t + 8 * (i / 4) + 4 * half + i % 4)) x[t][i] = -INFINITY;
             }
             float most = -INFINITY;
 #pragma unroll
@@ -188,29 +195,37 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
             const int in = (lane >> 2) & 3;  // a transposing read's row of four
             const uint8_t *vs = s_kv[buf][1] + (4 * half + in) * T::ROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
             const int vturn = T::v_turn(4 * half + in) << 4;
-            auto add = [&](auto careful) __attribute__((always_inline)) {
 #pragma unroll
-                for (int j = 0; j < KT / 16; ++j) {
-                    dc_u32x4 pw;
+            for (int j = 0; j < KT / 16; ++j) {
+                dc_u32x4 pw;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) pw[i] = dc_pack_bf16(x[j / 2][8 * (j % 2) + 2 * i], x[j / 2][8 * (j % 2) + 2 * i + 1]);
+                for (int i = 0; i < 4; ++i) pw[i] = dc_pack_bf16(x[j / 2][8 * (j % 2) + 2 * i], x[j / 2][8 * (j % 2) + 2 * i + 1]);
 #pragma unroll
-                    for (int d = 0; d < DT; ++d) {
-                        const uint8_t *at = vs + 16 * j * T::ROW + (vturn ^ (d << 6));
-                        const dc_u32x2 lo = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at)));
-                        const dc_u32x2 hi = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at + 8 * T::ROW)));
-                        const dc_u32x4 w = {lo.x, lo.y, hi.x, hi.y};
-                        auto mul = [&](dc_u32x4 v, dc_f32x16 acc) __attribute__((always_inline)) {
-                            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, v), __builtin_bit_cast(dc_bf16x8, pw), acc, 0, 0, 0);
-                        };
-                        if constexpr (decltype(careful)::value) dc_careful<16>(w, o[d], mul);
-                        else o[d] = mul(w, o[d]);
-                    }
+                for (int d = 0; d < DT; ++d) {
+                    const uint8_t *at = vs + 16 * j * T::ROW + (vturn ^ (d << 6));
+                    const dc_u32x2 lo = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at)));
+                    const dc_u32x2 hi = __builtin_bit_cast(dc_u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(s16x4 *)(at + 8 * T::ROW)));
+                    const dc_u32x4 w = {lo.x, lo.y, hi.x, hi.y};
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, pw), o[d], 0, 0, 0);
                 }
-            };
-            const uint4 bad = *reinterpret_cast<const uint4 *>(s_unbounded[buf]);
-            if (whole || __builtin_amdgcn_readfirstlane(bad.x | bad.y | bad.z | bad.w) == 0) add(std::false_type{});
-            else add(std::true_type{});
+            }
+            const uint4 odd = *reinterpret_cast<const uint4 *>(s_odd[buf]);
+            if (__builtin_amdgcn_readfirstlane(odd.x | odd.y | odd.z | odd.w)) {
+                for (int r = 0; r < KT; ++r) {
+                    const int page = (row0 + r) >> a.p.shift, id = dc_page_id(a.p, table, page < last_page ? page : last_page);
+                    if (id < 0) continue;
+                    const uint16_t *src = vh + id * a.p.vp + (int64_t)((row0 + r) & mask) * HD + 4 * half;
+                    const bool in = reach.has(row0 + r);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const uint2 w = *reinterpret_cast<const uint2 *>(src + 32 * d + 2 * i);
+                            o[d][i] += in ? dc_only_unbounded(dc_bf16_lo(w.x)) : 0.f, o[d][i + 1] += in ? dc_only_unbounded(dc_bf16_hi(w.x)) : 0.f;
+                            o[d][i + 2] += in ? dc_only_unbounded(dc_bf16_lo(w.y)) : 0.f, o[d][i + 3] += in ? dc_only_unbounded(dc_bf16_hi(w.y)) : 0.f;
+                        }
+                }
+            }
         }
         if (s + 1 < end) stage(buf ^ 1, s + 1, next);
         have = next;
