@@ -17,10 +17,11 @@
 namespace {
 
 constexpr int kThreads = 256, kRowsOfWave = 32;
+constexpr int kLoaded = 0x0f70;  // s_waitcnt vmcnt(0)
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-typedef __attribute__((address_space(3))) dc_u32x4 lds_u32x4;
-typedef __attribute__((address_space(3))) uint8_t lds_u8;
+typedef __attribute__((address_space(3))) uint32_t lds_u32;
+typedef __attribute__((address_space(1))) uint32_t glb_u32;
 
 template <int HD, int KT>
 struct Tile {
@@ -38,7 +39,8 @@ template <int HD, int KT>
 __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kernel(DcPagedAttn a) {
     using T = Tile<HD, KT>;
     constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, TILES = KT / 16;  // products of a tile's S; tiles of O, of S, and of what a page holds whole
-    __shared__ __attribute__((aligned(1024))) uint8_t s_kv[2][2][T::BYTES];
+    // (four arrays, not one of four: the reads of one are then known not to wait for the loads into another)
+    __shared__ __attribute__((aligned(1024))) uint8_t s_k0[T::BYTES], s_v0[T::BYTES], s_k1[T::BYTES], s_v1[T::BYTES];
     __shared__ __attribute__((aligned(16))) uint32_t s_odd[2][4];  // [buffer][wave]: whether the wave left out numbers of V that are not finite
     const int n_units = (int)(gridDim.x / (unsigned)(a.tiles * a.n_splits));
     // units first, so that a unit's blocks are on one XCD where their number divides by eight; late tokens first, they have the most rows
@@ -74,18 +76,18 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
         for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     float m = begin < end ? kNoLogit : -INFINITY, l = 0.f;
 
-    // staging: a wave's load n has rows (wave + 4 n) PER .., of one tile of 16 and so of one page.  The step's page ids are one
-    // load of as many lanes, made a step before they are needed.
+    // staging: a wave's load n has rows (wave + 4 n) PER .., of one tile of 16 and so of one page, and goes straight to LDS: lane i's 16 bytes to
+    // place i, so that which chunk it asks for is what turns the rows.  The step's page ids are one load of as many lanes, made a
+    // step before they are needed.
     const uint16_t *kh = a.p.k + h * a.p.kh, *vh = a.p.v + h * a.p.vh;
     const int32_t *table = a.p.table + (int64_t)b * a.p.table_stride;
     const int last_page = (a.n_rows - 1) >> a.p.shift, mask = (1 << a.p.shift) - 1;
-    const int in_row = lane / T::CHUNKS, chunk = lane % T::CHUNKS, in_page = in_row * HD + chunk * 8;
-    dc_u32x4 kst[T::LOADS], vst[T::LOADS];
+    const int in_row = lane / T::CHUNKS, chunk = lane % T::CHUNKS;
     auto ids_of = [&](int s) __attribute__((always_inline)) {
         const int page = (steps.row(s, KT) + 16 * (lane % TILES)) >> a.p.shift;
         return table[page < last_page ? page : last_page];
     };
-    auto fetch = [&](int s, int ids) __attribute__((always_inline)) {  // returns a bit for each tile of 16 rows that has a page
+    auto fetch = [&](uint8_t *k_lds, uint8_t *v_lds, int s, int ids) __attribute__((always_inline)) {  // returns a bit for each tile of 16 rows that has a page
         const int row0 = steps.row(s, KT);
         int have = 0, id[TILES];
 #pragma unroll
@@ -101,47 +103,52 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
             if constexpr (T::PER <= 4) page = id[4 * n * T::PER / 16];  // (the four waves' loads n are one tile's, or part of it)
             else page = wave * T::PER >= 16 ? id[2 * n + 1] : id[2 * n];
             const int64_t at = (int64_t)((row0 + row) & mask) * HD;
-            kst[n] = *reinterpret_cast<const dc_u32x4 *>(kh + (page * a.p.kp + at) + in_page);
-            vst[n] = *reinterpret_cast<const dc_u32x4 *>(vh + (page * a.p.vp + at) + in_page);
+            const int mine = row + in_row;
+            __builtin_amdgcn_global_load_lds((const glb_u32 *)(kh + (page * a.p.kp + at) + (in_row * HD + ((chunk ^ T::k_turn(mine)) << 3))),
+                                             (lds_u32 *)(k_lds + row * T::ROW), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const glb_u32 *)(vh + (page * a.p.vp + at) + (in_row * HD + ((chunk ^ T::v_turn(mine)) << 3))),
+                                             (lds_u32 *)(v_lds + row * T::ROW), 16, 0, 0);
         }
         return have;
     };
-    auto stage = [&](int buf, int s, int have) __attribute__((always_inline)) {
+    // what fetch brought is there, for the wave that asked for it
+    auto stage = [&](uint8_t *v_lds, int buf, int s, int have) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(kLoaded);
         uint32_t odd = 0;
         if (have != (1 << TILES) - 1 || !dc_whole(a, span.start + t_lo, span.start + t_hi / G, steps.row(s, KT), KT)) {
             DcUnbounded u;
+            dc_u32x4 w[T::LOADS];
 #pragma unroll
-            for (int n = 0; n < T::LOADS; ++n)
+            for (int n = 0; n < T::LOADS; ++n) {
+                w[n] = *reinterpret_cast<const dc_u32x4 *>(v_lds + (wave + 4 * n) * T::PER * T::ROW + lane * 16);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) u.look(vst[n][i]);
+                for (int i = 0; i < 4; ++i) u.look(w[n][i]);
+            }
             if (u.any()) {
                 odd = 1;
 #pragma unroll
-                for (int n = 0; n < T::LOADS; ++n)
+                for (int n = 0; n < T::LOADS; ++n) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) vst[n][i] = dc_finite(vst[n][i]);
+                    for (int i = 0; i < 4; ++i) w[n][i] = dc_finite(w[n][i]);
+                    *reinterpret_cast<dc_u32x4 *>(v_lds + (wave + 4 * n) * T::PER * T::ROW + lane * 16) = w[n];
+                }
             }
         }
         if (lane == 0) s_odd[buf][wave] = odd;
-#pragma unroll
-        for (int n = 0; n < T::LOADS; ++n) {
-            const int row = (wave + 4 * n) * T::PER + in_row;
-            *reinterpret_cast<dc_u32x4 *>(&s_kv[buf][0][row * T::ROW + ((chunk ^ T::k_turn(row)) << 4)]) = kst[n];
-            *reinterpret_cast<dc_u32x4 *>(&s_kv[buf][1][row * T::ROW + ((chunk ^ T::v_turn(row)) << 4)]) = vst[n];
-        }
     };
 
     int have = 0, next = 0, ids = 0;
     if (begin < end) {
-        have = fetch(begin, ids_of(begin));
+        have = fetch(s_k0, s_v0, begin, ids_of(begin));
         if (begin + 1 < end) ids = ids_of(begin + 1);
-        stage(0, begin, have);
+        stage(s_v0, 0, begin, have);
     }
+    __builtin_amdgcn_s_waitcnt(kLoaded);  // (Q too, on every way here: the loop would wait for it, and for all loads, in every step)
     __syncthreads();
-    for (int s = begin; s < end; ++s) {
-        const int buf = (s - begin) & 1, row0 = steps.row(s, KT);
+    auto step = [&](int s, int buf, const uint8_t *k_now, const uint8_t *v_now, uint8_t *k_next, uint8_t *v_next) __attribute__((always_inline)) {
+        const int row0 = steps.row(s, KT);
         if (s + 1 < end) {
-            next = fetch(s + 1, ids);
+            next = fetch(k_next, v_next, s + 1, ids);
             if (s + 2 < end) ids = ids_of(s + 2);
         }
         // rows that the wave has no use for: behind all its pairs, or between the sinks and all windows
@@ -149,14 +156,16 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
         if (use) {
             // S^T: x[t][i] is row 32 t + 8 (i / 4) + 4 half + i % 4
             dc_f32x16 x[ST];
-            const uint8_t *ks = s_kv[buf][0] + (lane & 31) * T::ROW;
+            const uint8_t *ks = k_now + (lane & 31) * T::ROW;
             const int turn = (half ^ T::k_turn(lane & 31)) << 4;
 #pragma unroll
-            for (int t = 0; t < ST; ++t) {
+            for (int t = 0; t < ST; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
 #pragma unroll
-                for (int j = 0; j < KS; ++j) {
+            for (int j = 0; j < KS; ++j) {
+#pragma unroll
+                for (int t = 0; t < ST; ++t) {
                     const dc_u32x4 w = *reinterpret_cast<const dc_u32x4 *>(ks + 32 * t * T::ROW + (turn ^ (j << 5)));
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, bq[j]), x[t], 0, 0, 0);
                 }
@@ -193,7 +202,7 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
                 }
             // O^T: rows 16 j + {0 .. 3, 8 .. 11} + 4 half at a time
             const int in = (lane >> 2) & 3;  // a transposing read's row of four
-            const uint8_t *vs = s_kv[buf][1] + (4 * half + in) * T::ROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+            const uint8_t *vs = v_now + (4 * half + in) * T::ROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
             const int vturn = T::v_turn(4 * half + in) << 4;
 #pragma unroll
             for (int j = 0; j < KT / 16; ++j) {
@@ -227,9 +236,13 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
                 }
             }
         }
-        if (s + 1 < end) stage(buf ^ 1, s + 1, next);
+        if (s + 1 < end) stage(v_next, buf ^ 1, s + 1, next);
         have = next;
         __syncthreads();
+    };
+    for (int s = begin; s < end; s += 2) {
+        step(s, 0, s_k0, s_v0, s_k1, s_v1);
+        if (s + 1 < end) step(s + 1, 1, s_k1, s_v1, s_k0, s_v0);
     }
 
     l = dc_over32(l, [](float u, float v) { return u + v; });
