@@ -10,9 +10,11 @@ tokens per second with the dense parts of the model in the loop.
 
     python -m diffcache_amd.harness --layers 32 --batch 8 --ctx 131072 --steps 20
     python -m diffcache_amd.harness --layers 32 --batch 8 --ctx 131072 --cache mx4
+    python -m diffcache_amd.harness --layers 32 --batch 8 --ctx 32768 --cache paged
 
 ``--cache mx4``, ``mx8`` and ``mx84`` (8-bit keys, 4-bit values) attend to the whole context in an ``MxCache`` instead of a
-selection of it in a ``DiffCache``.
+selection of it in a ``DiffCache``; ``--cache paged`` attends to the whole of a bf16 context in a ``PagedCache``, which rotates keys and
+queries itself.
 Everything dense is plain PyTorch (hipBLASLt GEMMs); only the cache calls go to
 the HIP library.
 """
@@ -28,9 +30,15 @@ import torch
 
 from .kvcache.diffcache import DiffCache
 from .kvcache.mxcache import MxCache
+from .kvcache.pagedcache import PagedCache
 
-Cache = Union[DiffCache, MxCache]
+Cache = Union[DiffCache, MxCache, PagedCache]
 MX_BITS = {"mx4": (4, 4), "mx8": (8, 8), "mx84": (8, 4)}
+
+
+def rotates(cache: Cache) -> bool:
+    """Whether the cache rotates keys and queries itself."""
+    return isinstance(cache, PagedCache) and cache.rotates
 
 
 class SyntheticLlama:
@@ -78,14 +86,16 @@ class SyntheticLlama:
         rot = torch.cat([-x[..., half:], x[..., :half]], dim=-1)
         return x * cos + rot * sin
 
-    def qkv(self, layer: int, x: torch.Tensor, pos):
-        """x (b, hidden) -> q (b, hq, hd), k (b, hkv, hd), v (b, hkv, hd) with RoPE on q and k."""
+    def qkv(self, layer: int, x: torch.Tensor, pos, rotated: bool = True):
+        """x (b, hidden) -> q (b, hq, hd), k (b, hkv, hd), v (b, hkv, hd) with RoPE on q and k, or as the projection leaves
+        them for a cache that rotates them itself."""
         b = x.shape[0]
         h = self.rmsnorm(x, self.norm1[layer])
         y = h @ self.wqkv[layer].t()
         q, k, v = torch.split(y, [self.hq * self.hd, self.hkv * self.hd, self.hkv * self.hd], dim=-1)
-        q = self.rope(q.view(b, self.hq, self.hd), pos)
-        k = self.rope(k.view(b, self.hkv, self.hd), pos)
+        q, k = q.view(b, self.hq, self.hd), k.view(b, self.hkv, self.hd)
+        if rotated:
+            q, k = self.rope(q, pos), self.rope(k, pos)
         return q.contiguous(), k.contiguous(), v.reshape(b, self.hkv, self.hd).contiguous()
 
     def post_attention(self, layer: int, x: torch.Tensor, attn: torch.Tensor) -> torch.Tensor:
@@ -101,7 +111,7 @@ class SyntheticLlama:
         """One token for every sequence of the batch: x (b, hidden) -> (b, hidden)."""
         pos = cache.seq_len(0)
         for layer in range(self.num_layers):
-            q, k, v = self.qkv(layer, x, pos)
+            q, k, v = self.qkv(layer, x, pos, rotated=not rotates(cache))
             attn = cache.decode_attention(layer, q, k.unsqueeze(1), v.unsqueeze(1))
             x = self.post_attention(layer, x, attn)
         return x
@@ -142,7 +152,7 @@ class GraphedDecoder:
         self.x.zero_()
 
     def _pre(self, layer: int) -> None:
-        q, k, v = self.model.qkv(layer, self.x, self.pos)
+        q, k, v = self.model.qkv(layer, self.x, self.pos, rotated=not rotates(self.cache))
         self.q.copy_(q)
         self.k.copy_(k.unsqueeze(1))
         self.v.copy_(v.unsqueeze(1))
@@ -183,6 +193,8 @@ def run(layers: int, batch: int, ctx: int, budget: int, steps: int, warmup: int,
     if cache_kind in MX_BITS:
         bits = MX_BITS[cache_kind]
         cache: Cache = MxCache(layers, batch, ctx + room, hkv, hq, hd, key_bits=bits[0], value_bits=bits[1])
+    elif cache_kind == "paged":
+        cache = PagedCache(layers, batch, ctx + room, hkv, hq, hd, inv_freq=model._inv_freq)
     else:
         cache = DiffCache(num_layers=layers, batch_size=batch, max_length=ctx + room, num_kv_heads=hkv,
                           num_q_heads=hq, head_dim=hd, retrieval_budget=budget, nsw_m=16, nsw_ef_cons=200,
@@ -229,8 +241,8 @@ def main(argv: Optional[List[str]] = None) -> int:
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--no-sketch", action="store_true", help="stream the bf16 keys instead of the 8-bit sketch")
     ap.add_argument("--eager", action="store_true", help="no captured graphs around the dense halves")
-    ap.add_argument("--cache", choices=["diffcache", *MX_BITS], default="diffcache",
-                    help="attend to a selection of bf16 rows, or to all rows held in 4 or 8 bits")
+    ap.add_argument("--cache", choices=["diffcache", *MX_BITS, "paged"], default="diffcache",
+                    help="attend to a selection of bf16 rows, or to all rows held in 4 or 8 bits or in pages of bf16")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
         print("harness: no GPU visible")
