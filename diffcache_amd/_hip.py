@@ -1342,7 +1342,7 @@ _PAGED_ATTN = struct.Struct("@3P2P4q2i4Pq4i3qPN6if0q")
 
 
 def _paged_store(k_pages: torch.Tensor, v_pages: torch.Tensor):
-    """The fields of a dc_paged_store, and (h, hd)."""
+    """The strides, page count and rows of a page of a dc_paged_store, and (h, hd)."""
     shape = k_pages.shape
     if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype is not _BF16 or v_pages.dtype is not _BF16:
         raise DiffCacheError("k_pages and v_pages must be (n_pages, h, page, hd) bf16 tensors of one shape")
@@ -1353,56 +1353,77 @@ def _paged_store(k_pages: torch.Tensor, v_pages: torch.Tensor):
         raise DiffCacheError("a page's rows must lie one after another")
     if n == 0 or h == 0:
         raise DiffCacheError("a store needs a page and a head")
-    return (_mx_dev(k_pages, "k_pages"), _mx_dev(v_pages, "v_pages"), k0, k1, v0, v1, n, page), h, hd
+    return k0, k1, v0, v1, n, page, h, hd
 
 
-def _paged_tokens(x: torch.Tensor, table: torch.Tensor, start: Optional[torch.Tensor], cu: Optional[torch.Tensor],
+def _paged_tokens(shape, table: torch.Tensor, start: Optional[torch.Tensor], cu: Optional[torch.Tensor],
                   counts: Optional[torch.Tensor], max_new: Optional[int], name: str):
-    """The fields of a dc_paged_tokens, and the leading dimensions of the tokens' tensors."""
-    if table.dim() != 2 or table.dtype is not _I32:
+    """(row stride of the table, b, max_new, n_tokens, table_pages) of a dc_paged_tokens for tokens' tensors of this shape."""
+    if table.dtype is not _I32 or table.dim() != 2:
         raise DiffCacheError("table must be an int32 tensor (b, pages)")
     b, pages = table.shape
     t0, t1 = table.stride()
     if pages == 0 or (t1 != 1 and pages > 1) or (t0 < pages and b > 1):
         raise DiffCacheError("table must have contiguous rows")
+    dims = len(shape)
     if cu is not None:
-        if x.dim() != 3 or counts is not None:
+        if dims != 3 or counts is not None:
             raise DiffCacheError(f"with cu, {name} holds packed tokens (tokens, heads, hd), and counts are not given")
         if cu.dtype is not _I32 or cu.numel() != b + 1 or not cu.is_contiguous():
             raise DiffCacheError(f"cu must be a contiguous int32 tensor of {b + 1} elements")
-        tokens = x.shape[0]
-        lead = (tokens,)
+        tokens = shape[0]
         if max_new is None:
             max_new = tokens
-        cu_ptr, counts_ptr = _mx_dev(cu, "cu"), 0
     else:
-        lead = tuple(x.shape[:-2])
-        if len(lead) not in (1, 2) or lead[0] != b:
+        if dims == 3:
+            new = 1
+        elif dims == 4:
+            new = shape[1]
+        else:
+            new = -1
+        if new < 0 or shape[0] != b:
             raise DiffCacheError(f"{name} must be ({b}, heads, hd), or ({b}, tokens, heads, hd), or packed with cu")
-        tokens = lead[1] if len(lead) == 2 else 1
-        if max_new is not None and max_new != tokens:
-            raise DiffCacheError(f"max_new is {max_new}, and {name} has {tokens} tokens to a sequence")
-        max_new, tokens = tokens, b * tokens
-        cu_ptr, counts_ptr = 0, _mx_lens(counts, b) if counts is not None else 0
-    start_ptr = 0
-    if start is not None:
-        if start.dtype is not _I32 or start.numel() != b or not start.is_contiguous():
-            raise DiffCacheError(f"start must be a contiguous int32 tensor of {b} elements")
-        start_ptr = _mx_dev(start, "start")
-    return (_mx_dev(table, "table"), start_ptr, cu_ptr, counts_ptr, t0 if b > 1 else pages, b, max_new, tokens, pages), lead
+        if max_new is not None and max_new != new:
+            raise DiffCacheError(f"max_new is {max_new}, and {name} has {new} tokens to a sequence")
+        max_new, tokens = new, b * new
+        if counts is not None and (counts.dtype is not _I32 or counts.numel() != b or not counts.is_contiguous()):
+            raise DiffCacheError(f"counts must be a contiguous int32 tensor of {b} elements")
+    if start is not None and (start.dtype is not _I32 or start.numel() != b or not start.is_contiguous()):
+        raise DiffCacheError(f"start must be a contiguous int32 tensor of {b} elements")
+    return t0 if b > 1 else pages, b, max_new, tokens, pages
 
 
-def _paged_src(t: torch.Tensor, lead, heads: Optional[int], hd: int, name: str):
-    """A tensor of tokens: itself or an aligned copy, and its (batch, token, head) strides."""
-    n = len(lead)
-    shape = t.shape
-    if t.dtype is not _BF16 or len(shape) != n + 2 or shape[:n] != lead or shape[n + 1] != hd or (heads is not None and shape[n] != heads):
-        raise DiffCacheError(f"{name} must be bf16 of {(*lead, 'heads' if heads is None else heads, hd)}, not {tuple(shape)} {t.dtype}")
+def _paged_src(t: torch.Tensor, shape, name: str):
+    """A tensor of tokens of this shape: itself or an aligned copy, its address, and its (batch, token, head) strides."""
+    if t.dtype is not _BF16 or t.shape != shape:
+        raise DiffCacheError(f"{name} must be bf16 of {tuple(shape)}, not {tuple(t.shape)} {t.dtype}")
+    at = t.data_ptr()
     strides = t.stride()
-    if strides[-1] != 1 or t.data_ptr() & 15 or any(s & 7 for s in strides[:-1]):
-        t = t.clone(memory_format=torch.contiguous_format)
-        strides = t.stride()
-    return t, strides[0], strides[-3], strides[-2]
+    if len(strides) == 3:
+        s0, s2, s3 = strides
+        s1 = s0
+    else:
+        s0, s1, s2, s3 = strides
+    if s3 != 1 or (at | s0 << 1 | s1 << 1 | s2 << 1) & 15:
+        return _paged_src(t.clone(memory_format=torch.contiguous_format), shape, name)
+    return t, at, s0, s1, s2
+
+
+def _paged_strides(shape):
+    """Those of a contiguous tensor of tokens.  (torch.empty_strided costs half of torch.empty's time.)"""
+    row = shape[-2] * shape[-1]
+    return (row, shape[-1], 1) if len(shape) == 3 else (shape[1] * row, row, shape[-1], 1)
+
+
+def _mx_opt(t: Optional[torch.Tensor], name: str) -> int:
+    return 0 if t is None else _mx_dev(t, name)
+
+
+def _paged_devices(*named) -> None:
+    """Raises for the first of the tensors that is not on the current device."""
+    for t, name in named:
+        if t is not None:
+            _mx_dev(t, name)
 
 
 def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -1421,44 +1442,54 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     position is its row, or ``pos`` (int32, as many as there are tokens); with ``sections``, up to four numbers of frequencies that add up to
     rot / 2, ``pos`` has a last dimension of as many and a section's frequencies go by its own.  ``q_out`` (contiguous, of q's
     shape) may be a contiguous ``q`` itself."""
-    store, h, hd = _paged_store(k_pages, v_pages)
-    tokens, lead = _paged_tokens(k, table, start, cu, counts, max_new, "k")
-    k, k0, k1, k2 = _paged_src(k, lead, h, hd, "k")
-    v, v0, v1, v2 = _paged_src(v, lead, h, hd, "v")
+    k0, k1, v0, v1, n_pages, page, h, hd = _paged_store(k_pages, v_pages)
+    shape = k.shape
+    stride, b, max_new, n_tokens, pages = _paged_tokens(shape, table, start, cu, counts, max_new, "k")
+    if shape[-2] != h or shape[-1] != hd:
+        raise DiffCacheError(f"k must be bf16 of (..., {h}, {hd}), not {tuple(shape)} {k.dtype}")
+    k, k_ptr, ks0, ks1, ks2 = _paged_src(k, shape, "k")
+    v, v_ptr, vs0, vs1, vs2 = _paged_src(v, shape, "v")
+    at = k_pages.get_device()
+    if (at < 0 or k.get_device() != at or v.get_device() != at or v_pages.get_device() != at or table.get_device() != at
+            or at != _device()):
+        _paged_devices((k_pages, "k_pages"), (v_pages, "v_pages"), (table, "table"), (k, "k"), (v, "v"))
     rot = n_q = q0 = q1 = q2 = inv_ptr = pos_ptr = q_ptr = out_ptr = 0
+    n_axes, section = 1, (0, 0, 0, 0)
     if inv_freq is not None:
         if inv_freq.dtype is not _F32 or not inv_freq.is_contiguous():
             raise DiffCacheError("inv_freq must be a contiguous fp32 tensor")
         rot, inv_ptr = 2 * inv_freq.numel(), _mx_dev(inv_freq, "inv_freq")
-    elif q is not None or pos is not None or sections is not None:
+        if sections is not None:
+            n_axes = len(sections)
+            if not 1 <= n_axes <= 4 or pos is None:
+                raise DiffCacheError("sections are one to four numbers of frequencies, and need pos")
+            section = tuple(sections) + (0,) * (4 - n_axes)
+        if pos is not None:
+            want = shape[:-2] if sections is None else (*shape[:-2], n_axes)
+            if pos.dtype is not _I32 or pos.shape != want or not pos.is_contiguous():
+                raise DiffCacheError(f"pos must be a contiguous int32 tensor of {tuple(want)}")
+            pos_ptr = _mx_dev(pos, "pos")
+        if q is not None:
+            n_q = q.shape[-2] if q.dim() == len(shape) else 0
+            of = (*shape[:-2], n_q, hd)
+            q, q_ptr, q0, q1, q2 = _paged_src(q, of, "q")
+            if q.get_device() != at:
+                _mx_dev(q, "q")
+            if q_out is None:
+                q_out = torch.empty_strided(of, _paged_strides(of), dtype=_BF16, device=q.device)
+                out_ptr = q_out.data_ptr()
+            elif q_out.dtype is not _BF16 or q_out.shape != of or not q_out.is_contiguous():
+                raise DiffCacheError("q_out must be a contiguous bf16 tensor of q's shape")
+            else:
+                out_ptr = _mx_dev(q_out, "q_out")
+        elif q_out is not None:
+            raise DiffCacheError("q_out is given without q")
+    elif q is not None or q_out is not None or pos is not None or sections is not None:
         raise DiffCacheError("q, pos and sections are for a rotation: inv_freq is missing")
-    n_axes, section = 1, (0, 0, 0, 0)
-    if sections is not None:
-        n_axes = len(sections)
-        if not 1 <= n_axes <= 4 or pos is None:
-            raise DiffCacheError("sections are one to four numbers of frequencies, and need pos")
-        section = tuple(sections) + (0,) * (4 - n_axes)
-    if pos is not None:
-        want = (*lead, n_axes) if sections is not None else lead
-        if pos.dtype is not _I32 or pos.shape != want or not pos.is_contiguous():
-            raise DiffCacheError(f"pos must be a contiguous int32 tensor of {tuple(want)}")
-        pos_ptr = _mx_dev(pos, "pos")
-    if q is not None:
-        given = q
-        q, q0, q1, q2 = _paged_src(q, lead, None, hd, "q")
-        n_q, q_ptr = q.shape[-2], _mx_dev(q, "q")
-        if q_out is None:
-            q_out = torch.empty(q.shape, dtype=_BF16, device=q.device)
-            out_ptr = q_out.data_ptr()
-        elif q_out.dtype is not _BF16 or q_out.shape != given.shape or not q_out.is_contiguous():
-            raise DiffCacheError("q_out must be a contiguous bf16 tensor of q's shape")
-        else:
-            out_ptr = _mx_dev(q_out, "q_out")
-    elif q_out is not None:
-        raise DiffCacheError("q_out is given without q")
     try:
-        args = _PAGED_APPEND.pack(_mx_dev(k, "k"), _mx_dev(v, "v"), q_ptr, out_ptr, inv_ptr, pos_ptr, *store, *tokens,
-                                  k0, k1, k2, v0, v1, v2, q0, q1, q2, h, n_q, hd, rot, bool(interleaved), n_axes, *section)
+        args = _PAGED_APPEND.pack(k_ptr, v_ptr, q_ptr, out_ptr, inv_ptr, pos_ptr, k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, v0, v1, n_pages, page,
+                                  table.data_ptr(), _mx_opt(start, "start"), _mx_opt(cu, "cu"), _mx_opt(counts, "counts"), stride, b, max_new,
+                                  n_tokens, pages, ks0, ks1, ks2, vs0, vs1, vs2, q0, q1, q2, h, n_q, hd, rot, 1 if interleaved else 0, n_axes, *section)
     except struct.error as e:
         raise DiffCacheError(f"a size or a section does not fit its type: {e}") from None
     _check(lib.dc_paged_append_bf16(args, _stream()))
@@ -1480,24 +1511,27 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, ta
     pages as in ``paged_append``.  ``n_rows``: no sequence has more rows, those of its new tokens among them (default: the table's); sizes the
     launch.  Returns out of q's shape, whose tokens that do not count stay as they were; with ``lse`` or ``want_lse`` (out, lse), lse
     (..., h * group) fp32 the log of the sum of exponentials.  A token without rows has out 0 and lse -inf."""
-    store, h, hd = _paged_store(k_pages, v_pages)
-    tokens, lead = _paged_tokens(q, table, start, cu, counts, max_new, "q")
-    q, q0, q1, q2 = _paged_src(q, lead, None, hd, "q")
-    hq = q.shape[-2]
+    k0, k1, v0, v1, n_pages, page, h, hd = _paged_store(k_pages, v_pages)
+    shape = q.shape
+    stride, b, max_new, n_tokens, pages = _paged_tokens(shape, table, start, cu, counts, max_new, "q")
+    hq = shape[-2]
     group = hq // h
-    if group * h != hq or group < 1:
-        raise DiffCacheError(f"q has {hq} heads, the store {h}")
+    if group * h != hq or group < 1 or shape[-1] != hd:
+        raise DiffCacheError(f"q has {hq} heads of {shape[-1]} numbers, the store {h} of {hd}")
     if group > PAGED_MAX_GROUP:
         raise DiffCacheError(f"more than {PAGED_MAX_GROUP} query heads to a KV head are not supported")
-    b, max_new, _, pages = tokens[5:]
-    room = pages * store[7]
+    q, q_ptr, q0, q1, q2 = _paged_src(q, shape, "q")
+    at = k_pages.get_device()
+    if at < 0 or q.get_device() != at or v_pages.get_device() != at or table.get_device() != at or at != _device():
+        _paged_devices((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"), (table, "table"))
+    room = pages * page
     if n_rows is None:
         n_rows = room
     elif not 1 <= n_rows <= room:
         raise DiffCacheError(f"{n_rows} rows outside the table of {room}")
     dev = q.device
     if out is None:
-        out = torch.empty(q.shape, dtype=_BF16, device=dev)
+        out = torch.empty_strided(shape, _paged_strides(shape), dtype=_BF16, device=dev)
         out_ptr = out.data_ptr()
     elif out.dtype is not _BF16 or out.numel() != q.numel() or not out.is_contiguous():
         raise DiffCacheError("out must be a contiguous bf16 tensor of the size of q")
@@ -1506,7 +1540,7 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, ta
     lse_ptr = ws_ptr = 0
     if lse is None:
         if want_lse:
-            lse = torch.empty(q.shape[:-1], dtype=_F32, device=dev)
+            lse = torch.empty_strided(shape[:-1], (hq, 1) if len(shape) == 3 else (shape[1] * hq, hq, 1), dtype=_F32, device=dev)
             lse_ptr = lse.data_ptr()
     elif lse.dtype is not _F32 or lse.numel() * hd != q.numel() or not lse.is_contiguous():
         raise DiffCacheError("lse must be a contiguous fp32 tensor of (..., h * group) elements")
@@ -1522,8 +1556,10 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, ta
             workspace = torch.empty(ws_bytes, dtype=_U8, device=dev)
             ws_ptr = workspace.data_ptr()
     try:
-        args = _PAGED_ATTN.pack(_mx_dev(q, "q"), out_ptr, lse_ptr, *store, *tokens, q0, q1, q2, ws_ptr, ws_bytes, h, group, hd,
-                                n_rows, n_sink, window, hd ** -0.5 if scale is None else scale)
+        args = _PAGED_ATTN.pack(q_ptr, out_ptr, lse_ptr, k_pages.data_ptr(), v_pages.data_ptr(), k0, k1, v0, v1, n_pages, page,
+                                table.data_ptr(), _mx_opt(start, "start"), _mx_opt(cu, "cu"), _mx_opt(counts, "counts"), stride, b, max_new,
+                                n_tokens, pages, q0, q1, q2, ws_ptr, ws_bytes, h, group, hd, n_rows, n_sink, window,
+                                hd ** -0.5 if scale is None else scale)
     except struct.error as e:
         raise DiffCacheError(f"n_sink, window, max_new or scale does not fit its type: {e}") from None
     _check(lib.dc_paged_attn_bf16(args, _stream()))

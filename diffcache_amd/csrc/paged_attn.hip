@@ -25,7 +25,8 @@ template <int HD, int TILES>
 struct Rows {
     static constexpr int STEP = 16 * TILES, CH = HD / 32, EPL = HD / 16, VW = EPL / 2;
 
-    dc_u32x4 bq[CH];
+    static constexpr bool kQueryInLds = HD == 256;  // (its registers are 25 too many there)
+    dc_u32x4 bq[kQueryInLds ? 1 : CH];
     dc_u32x4 kw[TILES][CH];
     uint32_t vw[TILES * 4][VW];
     dc_f32x4 acc[EPL];
@@ -38,9 +39,23 @@ struct Rows {
         for (int j = 0; j < EPL; ++j) acc[j] = dc_f32x4{0.f, 0.f, 0.f, 0.f};
         m = -INFINITY, l = 0.f;
     }
-    __device__ __forceinline__ void load_q(const uint16_t *src) {
+    // columns 32 s + 8 q .. of the queries of pair c: src its column 0, lds 16 HD numbers for all waves
+    __device__ __forceinline__ void load_q(const uint16_t *src, dc_u32x4 *lds, int wave) {
+        if constexpr (kQueryInLds) {
+            if (wave == 0) {
 #pragma unroll
-        for (int s = 0; s < CH; ++s) bq[s] = *reinterpret_cast<const dc_u32x4 *>(src + 32 * s + 8 * q);
+                for (int s = 0; s < CH; ++s) lds[place(s)] = *reinterpret_cast<const dc_u32x4 *>(src + 32 * s + 8 * q);
+            }
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int s = 0; s < CH; ++s) bq[s] = *reinterpret_cast<const dc_u32x4 *>(src + 32 * s + 8 * q);
+        }
+    }
+    __device__ __forceinline__ int place(int s) const { return c * (HD / 8) + ((4 * s + q) ^ c); }  // (16 pairs' same chunk in 16 places)
+    __device__ __forceinline__ dc_u32x4 query(const dc_u32x4 *lds, int s) const {
+        if constexpr (kQueryInLds) return lds[place(s)];  // (every step anew, for what the barrier in logits() tells the compiler)
+        else return bq[s];
     }
     // lane (q, c) has columns 32 s + 8 q .. of row 4 (c % 4) + c / 4 of every tile
     __device__ __forceinline__ void load_k(const uint16_t *const (&tile)[TILES]) {
@@ -75,16 +90,21 @@ struct Rows {
     }
 
     // x[t][i]: tile t, row 4 i + q, pair c
-    __device__ __forceinline__ void logits(float scale, float (&x)[TILES][4]) const {
+    __device__ __forceinline__ void logits(float scale, const dc_u32x4 *lds, float (&x)[TILES][4]) const {
+        if constexpr (kQueryInLds) asm volatile("" ::: "memory");
+        dc_f32x4 s[TILES];
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            dc_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < TILES; ++t) s[t] = dc_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < CH; ++j)
-                s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, kw[t][j]), __builtin_bit_cast(dc_bf16x8, bq[j]), s, 0, 0, 0);
+        for (int j = 0; j < CH; ++j) {
+            const dc_bf16x8 w = __builtin_bit_cast(dc_bf16x8, query(lds, j));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[t][i] = s[i] * scale;
+            for (int t = 0; t < TILES; ++t) s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(dc_bf16x8, kw[t][j]), w, s[t], 0, 0, 0);
         }
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[t][i] = s[t][i] * scale;
     }
 
     // a new maximum for every pair, and what was summed so far brought to it
@@ -190,11 +210,12 @@ __device__ __forceinline__ float share(float m, float l, float top) { return l =
 __device__ __forceinline__ float log_sum(float top, float total) { return total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f; }
 
 template <int HD, int TILES>
-__global__ __launch_bounds__(kMostWaves * 64, 2) void paged_rows_kernel(DcPagedAttn a) {
+__global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows_kernel(DcPagedAttn a) {
     using T = Rows<HD, TILES>;
     constexpr int STEP = T::STEP;
     extern __shared__ float s_dyn[];
     const int waves = a.waves;
+    __shared__ dc_u32x4 s_q[T::kQueryInLds ? kRows * HD / 8 : 1];
     float *s_m = s_dyn, *s_l = s_dyn + waves * kRows, *s_acc = s_dyn + 2 * waves * kRows;  // [wave][16], [wave][16], [wave][pairs * HD]
     const int b = blockIdx.x, h = blockIdx.y, split = blockIdx.z, unit = b * a.n_h + h, G = a.group;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -213,7 +234,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void paged_rows_kernel(DcPagedA
     T w;
     w.start(lane);
     const int pair = w.c < pairs ? w.c : pairs - 1, token = pair / G;  // (the last pair again in the place of one that does not exist)
-    w.load_q(a.q + dc_token_at(a.t, a.qs, span, b, token) + (int64_t)(h * G + pair % G) * a.qs.h);
+    w.load_q(a.q + dc_token_at(a.t, a.qs, span, b, token) + (int64_t)(h * G + pair % G) * a.qs.h, s_q, wave);
     const DcReach reach = dc_reach(a, span.start + token);
 
     const uint16_t *kh = a.p.k + h * a.p.kh, *vh = a.p.v + h * a.p.vh;
@@ -254,7 +275,7 @@ __global__ __launch_bounds__(kMostWaves * 64, 2) void paged_rows_kernel(DcPagedA
     }
     for (int n = 0; n < mine; ++n) {
         float x[TILES][4];
-        w.logits(a.scale, x);
+        w.logits(a.scale, s_q, x);
         const bool more = n + 1 < mine;
         const int r0 = held_row, have = live;
         if (more) {
@@ -426,8 +447,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(DcPagedAttn a
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
-constexpr int row_tiles(int hd) { return hd == 256 ? 2 : 4; }
-constexpr int kBlocks = 512;  // two to a CU
+constexpr int row_tiles(int hd) { return hd == 64 ? 4 : 2; }
+constexpr int blocks_of(int hd) { return hd == 256 ? 512 : 768; }  // as many as run at once, two or three to a CU
 // Steps of a wave up to which a unit is one block of eight waves, which writes the output itself.
 constexpr int kAlone = 2;
 
@@ -450,7 +471,7 @@ Cut cut_of(int64_t n_units, int group, int hd, int64_t rows, int max_new) {
         c.n_splits = 1, c.waves = steps <= kWaves ? kWaves : kMostWaves;
         return c;
     }
-    const int64_t parts = (steps + kWaves - 1) / kWaves, most = kBlocks / n_units > 1 ? kBlocks / n_units : 1;
+    const int64_t parts = (steps + kWaves - 1) / kWaves, most = blocks_of(hd) / n_units > 1 ? blocks_of(hd) / n_units : 1;
     c.n_splits = (int)(parts < most ? parts : most), c.waves = kWaves;
     return c;
 }

@@ -146,6 +146,7 @@ def i32(*shape):
 
 def test_wrappers_refuse_what_does_not_fit(monkeypatch):
     monkeypatch.setattr(hip, "_mx_dev", lambda t, name: t.data_ptr())       # so that the checks behind the first tensor's place are reached
+    monkeypatch.setattr(hip, "_device", lambda: -1)
     pool, table = bf(4, 2, 16, 64), i32(3, 5)
     k, q = bf(3, 2, 64), bf(3, 4, 64)
     bad = pytest.raises(hip.DiffCacheError)
@@ -184,7 +185,7 @@ def test_wrappers_refuse_what_does_not_fit(monkeypatch):
     no("q_out must be", append(pool, pool, table, k, k, inv_freq=torch.zeros(32), q=q, q_out=bf(3, 4, 32)))
     no("without q", append(pool, pool, table, k, k, inv_freq=torch.zeros(32), q_out=q))
     no("does not fit its type", append(pool, pool, table, k, k, inv_freq=torch.zeros(32), sections=(1 << 40, 16), pos=i32(3, 2)))
-    no("4 heads, the store 3", attn(q, bf(4, 3, 16, 64), bf(4, 3, 16, 64), table))
+    no("4 heads of 64 numbers, the store 3", attn(q, bf(4, 3, 16, 64), bf(4, 3, 16, 64), table))
     no("more than 16", attn(bf(3, 34, 64), pool, pool, table))
     no("outside the table", attn(q, pool, pool, table, n_rows=81))
     no("outside the table", attn(q, pool, pool, table, n_rows=0))
