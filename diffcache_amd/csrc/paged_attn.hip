@@ -420,26 +420,44 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(DcPagedAttn a) {
     if (a.lse && tid == 0) a.lse[row.dst] = log_sum(top, total);
 }
 
-// The same for many rows of few parts: HD / 4 threads to a row, its parts one after another.
+// The same for many rows of few parts: HD / 4 threads to a row, four parts asked for at once, before anything is known of the row.
 template <int HD>
 __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(DcPagedAttn a) {
-    constexpr int kLanes = HD / 4, kPer = kThreads / kLanes;
+    constexpr int kLanes = HD / 4, kPer = kThreads / kLanes, kBatch = 4;
     const int at = (int)(blockIdx.x * kPer) + (int)threadIdx.x / kLanes, c = threadIdx.x % kLanes;  // (tile_rows is a multiple of kPer)
-    const Row row = row_of(a, at / a.tile_rows, at % a.tile_rows);
-    if (!row.live) return;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + row.slot0;
-    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + row.slot0 * kLanes + c;
+    const int group = at / a.tile_rows, r = at % a.tile_rows, n = a.n_splits;
+    const int64_t slot0 = (int64_t)group * n * a.tile_rows + r;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0;
+    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + slot0 * kLanes + c;
     float top = -INFINITY, total = 0.f;
-    for (int s = 0; s < a.n_splits; ++s) top = fmaxf(top, ml[s * (int64_t)a.tile_rows].x);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.n_splits; ++s) {
-        const float2 o = ml[s * (int64_t)a.tile_rows];
-        total += share(o.x, o.y, top);
-        if (!(o.x > -INFINITY)) continue;
-        const float4 v = pa[s * (int64_t)a.tile_rows * kLanes];
-        const float f = weight(o.x, top);
-        acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+    for (int s0 = 0; s0 < n; s0 += kBatch) {
+        float2 o[kBatch];
+        float4 v[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {  // (the last part again where there are no more; what a row without a token reads is not used)
+            const int64_t s = (int64_t)(s0 + i < n ? s0 + i : n - 1) * a.tile_rows;
+            o[i] = ml[s], v[i] = pa[s * kLanes];
+        }
+        float to = top;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) to = fmaxf(to, o[i].x);
+        const float f = weight(top, to);
+        acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+        total = share(top, total, to);
+        top = to;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            // (a part without rows has no sums in the workspace)
+            const bool in = s0 + i < n && o[i].x > -INFINITY;
+            const float g = in ? weight(o[i].x, top) : 0.f;
+            total += in ? share(o[i].x, o[i].y, top) : 0.f;
+            acc.x = fmaf(g, in ? v[i].x : 0.f, acc.x), acc.y = fmaf(g, in ? v[i].y : 0.f, acc.y);
+            acc.z = fmaf(g, in ? v[i].z : 0.f, acc.z), acc.w = fmaf(g, in ? v[i].w : 0.f, acc.w);
+        }
     }
+    const Row row = row_of(a, group, r);
+    if (!row.live) return;
     const float d = total == 0.f ? 1.f : total;
     *reinterpret_cast<uint2 *>(a.out + row.dst * HD + 4 * c) = make_uint2(dc_pack_bf16(acc.x / d, acc.y / d), dc_pack_bf16(acc.z / d, acc.w / d));
     if (a.lse && c == 0) a.lse[row.dst] = log_sum(top, total);
@@ -449,8 +467,10 @@ __global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(DcPagedAttn a
 
 constexpr int row_tiles(int hd) { return hd == 64 ? 4 : 2; }
 constexpr int blocks_of(int hd) { return hd == 256 ? 512 : 768; }  // as many as run at once, two or three to a CU
-// Steps of a wave up to which a unit is one block of eight waves, which writes the output itself.
-constexpr int kAlone = 2;
+// Rows times columns up to which a unit is one block of eight waves, which writes the output itself: 384 KB of K and V, some 2 us of what a CU
+// can read more, but less than a second kernel that joins parts where the host waits for its launches (one sequence of 8 heads x
+// 128: 700 rows 10.7 us, in parts 8.9, called one after another 11.0 and 15.4; 32 sequences 17.2 and 22.7 us).
+constexpr int64_t kAlone = 768 * 128;
 
 struct Cut {
     bool chunk;
@@ -467,7 +487,7 @@ Cut cut_of(int64_t n_units, int group, int hd, int64_t rows, int max_new) {
     }
     c.tiles = 1, c.tile_rows = max_new * group;
     const int64_t step = 16 * row_tiles(hd), steps = (rows + step - 1) / step;
-    if (steps <= kAlone * kMostWaves) {
+    if (steps * step * hd <= kAlone) {
         c.n_splits = 1, c.waves = steps <= kWaves ? kWaves : kMostWaves;
         return c;
     }
@@ -546,7 +566,7 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
         const int64_t rows = (int64_t)n_units * c.tiles * c.tile_rows;
 #define DC_JOIN(HD)                                                                                                                        \
     do {                                                                                                                                   \
-        if (c.chunk) hipLaunchKernelGGL(paged_join_rows_kernel<HD>, dim3((unsigned)(rows / (kThreads / (HD / 4)))), dim3(kThreads), 0, st, a); \
+        if (c.chunk && c.n_splits <= 8) hipLaunchKernelGGL(paged_join_rows_kernel<HD>, dim3((unsigned)(rows / (kThreads / (HD / 4)))), dim3(kThreads), 0, st, a); \
         else hipLaunchKernelGGL(paged_join_kernel<HD>, dim3((unsigned)rows), dim3(kThreads), 0, st, a);                                    \
     } while (0)
         if (x->hd == 64) DC_JOIN(64);

@@ -280,9 +280,12 @@ void launch(const DcPagedAttn &a, unsigned blocks, hipStream_t st) {
 }  // namespace
 
 int dc_paged_chunk_splits(int64_t n_units, int64_t tiles, int hd, int64_t rows) {
-    const int64_t blocks = n_units * tiles, most = hd == 256 ? 256 : 512;
-    const int64_t parts = (rows + step_rows(hd) - 1) / step_rows(hd) / 4;   // four steps to a part or more
-    const int64_t want = blocks >= most ? 1 : most / blocks;
+    const int64_t blocks = n_units * tiles, want = (hd == 256 ? 256 : 512) / blocks, steps = (rows + step_rows(hd) - 1) / step_rows(hd);
+    if (want < 2) return 1;
+    // Parts of four steps where the blocks alone leave most CUs idle (16 tokens of 8 heads behind 4080 rows: 16 us, of eight steps 21);
+    // where they do not, a part has to save more than the join takes (a prompt of 517 tokens, 136 blocks: 19.6 us, in two parts 26.7; a step of
+    // 256 columns takes longer: 700 tokens of 4 heads, 88 blocks, 47 us, in two parts 41).
+    const int64_t parts = steps / (want >= 4 ? 4 : hd == 256 ? 8 : 16);
     return (int)(want < parts ? want : parts > 1 ? parts : 1);
 }
 
