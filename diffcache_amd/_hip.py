@@ -230,7 +230,7 @@ def _load() -> C.CDLL:
         "dc_mx_attn_workspace_bytes": (sz, [i, i, i, i]),
         "dc_mx_attn_bf16": (i, [mx, p]),
         "dc_paged_append_bf16": (i, [mx, p]),
-        "dc_paged_attn_workspace_bytes": (sz, [i, i, i, i, i]),
+        "dc_paged_attn_workspace_bytes": (sz, [i, i, i, i, i, i, i]),
         "dc_paged_attn_bf16": (i, [mx, p]),
     })
     for name, (res, args) in sigs.items():
@@ -1496,8 +1496,9 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
     return q_out
 
 
-def paged_attn_workspace_bytes(n_units: int, group: int, hd: int, n_rows: int, max_new: int = 1) -> int:
-    return int(lib.dc_paged_attn_workspace_bytes(n_units, group, hd, n_rows, max_new))
+def paged_attn_workspace_bytes(b: int, h: int, group: int, hd: int, n_rows: int, max_new: int = 1, n_tokens: int = 0) -> int:
+    """Of ``paged_attn``'s workspace; ``n_tokens``: of all sequences together where they are packed."""
+    return int(lib.dc_paged_attn_workspace_bytes(b, h, group, hd, n_rows, max_new, n_tokens))
 
 
 def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -1551,7 +1552,7 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, ta
             raise DiffCacheError("workspace must be contiguous")
         ws_ptr, ws_bytes = _mx_dev(workspace, "workspace"), workspace.numel() * workspace.element_size()
     else:
-        ws_bytes = lib.dc_paged_attn_workspace_bytes(b * h, group, hd, n_rows, max_new)
+        ws_bytes = lib.dc_paged_attn_workspace_bytes(b, h, group, hd, n_rows, max_new, 0 if cu is None else n_tokens)
         if ws_bytes:
             workspace = torch.empty(ws_bytes, dtype=_U8, device=dev)
             ws_ptr = workspace.data_ptr()

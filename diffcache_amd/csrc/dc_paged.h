@@ -1,6 +1,7 @@
 // What the kernels of the paged cache share (paged.hip, paged_attn.hip, paged_chunk.hip): where a sequence's rows and its new tokens lie.
 #pragma once
 #include "dc_common.h"
+#include <type_traits>
 
 // K and V in pages, as the kernels see them: row r of sequence b is row r % page of page table[b * table_stride + r / page].
 struct DcPages {
@@ -25,18 +26,23 @@ struct DcSpan {
 constexpr int kMostRows = 1 << 30;
 
 __device__ __forceinline__ int dc_clamp(int x, int lo, int hi) { return x < lo ? lo : (x < hi ? x : hi); }
-__device__ __forceinline__ DcSpan dc_span(const DcNew &t, int b) {
+// word(p): the number at p, which no block changes
+template <typename F>
+__device__ __forceinline__ DcSpan dc_span_by(const DcNew &t, int b, F word) {
     DcSpan s;
     if (t.cu) {  // (whatever cu holds, no token lies outside the tensors)
-        s.first = dc_clamp(dc_step_word(t.cu + b), 0, t.n_tokens);
-        s.count = dc_clamp(dc_step_word(t.cu + b + 1), s.first, t.n_tokens) - s.first;
+        s.first = dc_clamp(word(t.cu + b), 0, t.n_tokens);
+        s.count = dc_clamp(word(t.cu + b + 1), s.first, t.n_tokens) - s.first;
         s.count = s.count < t.max_new ? s.count : t.max_new;
     } else {
         s.first = b * t.max_new;
-        s.count = t.counts ? dc_clamp(dc_step_word(t.counts + b), 0, t.max_new) : t.max_new;
+        s.count = t.counts ? dc_clamp(word(t.counts + b), 0, t.max_new) : t.max_new;
     }
-    s.start = t.start ? dc_clamp(dc_step_word(t.start + b), 0, kMostRows) : 0;
+    s.start = t.start ? dc_clamp(word(t.start + b), 0, kMostRows) : 0;
     return s;
+}
+__device__ __forceinline__ DcSpan dc_span(const DcNew &t, int b) {  // the same b in the whole wave
+    return dc_span_by(t, b, [](const int32_t *p) { return dc_step_word(p); });
 }
 
 // Tensors of tokens by strides (batch, token, head); the batch's is not used where tokens are packed.
@@ -67,8 +73,10 @@ struct DcPagedAttn {
     DcNew t;
     DcTokenStrides qs;
     int n_h, group, n_rows, n_sink, window;
-    int n_splits, waves;     // parts of a unit's steps; waves of a block (paged_attn.hip)
-    int tiles, tile_rows;    // of a unit's (token, head) rows: blocks, and rows of one
+    int n_b, waves;          // waves of a block (paged_attn.hip)
+    int tiles, tile_rows;    // of a unit's (token, head) pairs: at most so many tiles of so many
+    int at_once, least, items;  // blocks that the GPU runs at once, the fewest steps of a part, and the items that there is room for; at_once 0: nothing is dealt out
+    float of_all;            // 1.0001 / at_once: a little more steps to a part than come of the division, so that rounding makes no more of them
     float scale;             // times log2(e)
 };
 
@@ -105,15 +113,135 @@ __device__ __forceinline__ DcSteps dc_steps(const DcPagedAttn &a, int p_lo, int 
     return s;
 }
 
+// ---- how the steps are dealt out ------------------------------------------------------------------------------------
+//
+// Sequences differ in length, and the host does not know by how much: with as many blocks to each, the longest one's end last (8 x 131072
+// rows of 8 heads x 128 attended to by one token 625 us; one such sequence and seven of 8192 would take as long).  So the blocks count the steps of all
+// sequences themselves, divide them by the blocks that run at once, and cut every tile of a sequence's pairs into as many parts as come nearest to
+// that.  Block x of the grid takes item x / n_h of KV head x % n_h; the items are those of sequence 0, then those of sequence 1, ...; a sequence
+// has for each of its tiles the parts of its last one, which has the most steps (others may leave some of them empty).  A part's results stand in
+// the workspace at the item's own place; a tile of one part goes to the outputs at once.
+//
+// A part has at least half of steps / at_once steps or is a tile's only one, and a sequence's tiles have at most twice the steps that the mean
+// of its first and last suggests: there are never more items than 2 at_once / n_h and one for each tile (at_once / n_h and one for each sequence
+// where those have one tile).
+struct DcItem {
+    int b, tile, part, parts;  // parts of this tile; 0: nothing to do
+    int64_t slot;              // of part 0; the next part is n_h slots on
+};
+
+// the sum over the wave's lanes up to each lane's own
+template <typename T>
+__device__ __forceinline__ T dc_lane_sums(T x) {
+    auto moved = [](T v, auto ctrl, auto rows) __attribute__((always_inline)) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value, 0xf, false));
+    };
+    using std::integral_constant;
+    const integral_constant<int, 0xf> all;
+    x += moved(x, integral_constant<int, 0x111>{}, all);                               // row_shr:1
+    x += moved(x, integral_constant<int, 0x112>{}, all);                               // row_shr:2
+    x += moved(x, integral_constant<int, 0x114>{}, all);                               // row_shr:4
+    x += moved(x, integral_constant<int, 0x118>{}, all);                               // row_shr:8
+    x += moved(x, integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});     // row_bcast:15
+    x += moved(x, integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});     // row_bcast:31
+    return x;
+}
+template <typename T>
+__device__ __forceinline__ T dc_of_lane(T x, int lane) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), lane));
+}
+
+struct DcTiles {
+    int tiles, first, last;  // of a sequence: how many, and the steps of the first and of the last
+};
+// TILED: a sequence's pairs may be several tiles
+template <int STEP, bool TILED>
+__device__ __forceinline__ DcTiles dc_tiles_of(const DcPagedAttn &a, const DcSpan &s) {
+    if (s.count == 0) return {0, 0, 0};
+    if constexpr (!TILED) {
+        const int steps = dc_steps<STEP>(a, s.start, s.start + s.count - 1).steps;
+        return {1, steps, steps};
+    }
+    const int pairs = s.count * a.group, tiles = (int)((unsigned)(pairs + a.tile_rows - 1) / (unsigned)a.tile_rows);
+    const int hi = (int)((unsigned)((a.tile_rows < pairs ? a.tile_rows : pairs) - 1) / (unsigned)a.group), lo = (int)((unsigned)((tiles - 1) * a.tile_rows) / (unsigned)a.group);
+    return {tiles, dc_steps<STEP>(a, s.start, s.start + hi).steps, dc_steps<STEP>(a, s.start + lo, s.start + s.count - 1).steps};
+}
+// steps / per to the nearest number, 1 at least.  (In fp32: what it loses, 1e-7 of the number, is little beside the 1e-4 below.)
+__device__ __forceinline__ int dc_parts_of(int steps, float by) {
+    const int n = (int)fmaf((float)steps, by, 0.5f);
+    return n > 1 ? n : 1;
+}
+// 1 / the steps of a part, for the work of all sequences
+__device__ __forceinline__ float dc_per(const DcPagedAttn &a, float work) {
+    const float even = work * (float)a.n_h * a.of_all;  // (of_all is 1.0001 / at_once)
+    return __builtin_amdgcn_rcpf(even > (float)a.least ? even : (float)a.least);
+}
+
+// Item x, or with OF_SEQUENCE the first one of sequence x (x is the same in the whole wave, all of whose lanes are here).
+template <int STEP, bool TILED, bool OF_SEQUENCE = false>
+__device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane) {
+    DcItem d = {0, 0, 0, 0, 0};
+    float by = 0.f;
+    // x is item `in` of sequence b, whose first is at; its last tile has `most` parts
+    auto found = [&](const DcSpan &s, int b, int at, int in, int tiles, int most) __attribute__((always_inline)) {
+        d.b = b;
+        if constexpr (TILED) {
+            d.tile = tiles - 1 - (int)((unsigned)in / (unsigned)most), d.part = (int)((unsigned)in % (unsigned)most);  // (late tokens first: they have the most rows)
+            const int pairs = s.count * a.group, lo = d.tile * a.tile_rows, hi = (lo + a.tile_rows < pairs ? lo + a.tile_rows : pairs) - 1;
+            const int own = dc_parts_of(dc_steps<STEP>(a, s.start + (int)((unsigned)lo / (unsigned)a.group), s.start + (int)((unsigned)hi / (unsigned)a.group)).steps, by);
+            d.parts = own < most ? own : most;
+        } else {
+            d.part = in, d.parts = most;
+        }
+        if (at + in - d.part + most > a.items) d.parts = 1;  // (never, but for numbers of tokens that say more than there are)
+        d.slot = (int64_t)(at + in - d.part) * a.n_h;
+    };
+    if (a.n_b == 1) {
+        const DcSpan s = dc_span(a.t, 0);
+        const DcTiles t = dc_tiles_of<STEP, TILED>(a, s);
+        by = dc_per(a, 0.5f * (float)t.tiles * (float)(t.first + t.last));
+        const int most = dc_parts_of(t.last, by);
+        if (x < t.tiles * most) found(s, 0, 0, x, t.tiles, most);
+        return d;
+    }
+    auto tiles_of = [&](int b) __attribute__((always_inline)) {
+        if (b >= a.n_b) return DcTiles{0, 0, 0};
+        return dc_tiles_of<STEP, TILED>(a, dc_span_by(a.t, b, [](const int32_t *p) { return *p; }));
+    };
+    const DcTiles mine = tiles_of(lane);  // of sequence lane; those from 64 on are read again when it is their turn
+    float work = 0.f;
+    for (int b0 = 0; b0 < a.n_b; b0 += 64) {
+        const DcTiles t = b0 == 0 ? mine : tiles_of(b0 + lane);
+        work += dc_of_lane(dc_lane_sums(0.5f * (float)t.tiles * (float)(t.first + t.last)), 63);
+    }
+    by = dc_per(a, work);
+    int base = 0;
+    for (int b0 = 0; b0 < a.n_b; b0 += 64) {
+        const DcTiles t = b0 == 0 ? mine : tiles_of(b0 + lane);
+        const int parts = dc_parts_of(t.last, by), items = t.tiles * parts, upto = dc_lane_sums(items);
+        const uint64_t past = OF_SEQUENCE ? (x < b0 + 64 ? 1ull << (x - b0) : 0) : __ballot(base + upto > x);
+        if (past) {
+            const int k = __builtin_ctzll(past), at = base + dc_of_lane(upto, k) - dc_of_lane(items, k);  // the sequence's first item
+            const int tiles = dc_of_lane(t.tiles, k);
+            if (tiles) found(dc_span(a.t, b0 + k), b0 + k, at, OF_SEQUENCE ? 0 : x - at, tiles, dc_of_lane(parts, k));
+            return d;
+        }
+        base += dc_of_lane(upto, 63);
+    }
+    return d;
+}
+
 // A page's id, or -1 where the table names none that there is.
 __device__ __forceinline__ int dc_page_id(const DcPages &p, const int32_t *table, int index) {
     const int id = dc_step_word(table + index);
     return (unsigned)id < (unsigned)p.n_pages ? id : -1;
 }
 
-int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, int n_units, hipStream_t st);
-// Parts that a chunk's blocks are cut into.
-int dc_paged_chunk_splits(int64_t n_units, int64_t tiles, int hd, int64_t rows);
+// paged_chunk.hip
+int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, unsigned blocks, bool join, hipStream_t st);
+// Rows of a step; blocks that run at once.
+constexpr int dc_chunk_step(int hd) { return hd == 256 ? 32 : 64; }
+constexpr int dc_chunk_at_once(int hd) { return hd == 64 ? 1024 : hd == 128 ? 512 : 256; }
 constexpr int kChunkRows = 128;
 
 typedef __bf16 dc_bf16x2 __attribute__((ext_vector_type(2)));
@@ -162,3 +290,9 @@ __device__ __forceinline__ uint32_t dc_finite(uint32_t w) {  // 0 in the halves 
     return w & (lo | hi);
 }
 __device__ __forceinline__ float dc_only_unbounded(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? x : 0.f; }
+
+// ---- joining parts --------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float dc_weight(float m, float top) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f; }
+// a part's share of the sum (one that is no number stays none, whatever its maximum)
+__device__ __forceinline__ float dc_share(float m, float l, float top) { return l == l ? dc_weight(m, top) * l : l; }
+__device__ __forceinline__ float dc_log_sum(float top, float total) { return total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f; }

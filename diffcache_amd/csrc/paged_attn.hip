@@ -8,7 +8,7 @@ namespace {
 constexpr int kThreads = 256, kWaves = 4, kMostWaves = 8, kRows = 16;
 
 // out = sum_r p_r v_r / sum_r p_r with p_r = exp(scale q k_r - m), over the rows that a token attends to.  A unit's (one sequence's, one KV
-// head's) rows are cut into steps of 16 TILES, its steps into n_splits parts, a block each, whose waves take them in turn; a wave
+// head's) rows are cut into steps of 16 TILES, its steps into parts, a block each, whose waves take them in turn; a wave
 // keeps its running maximum, sum and weighted rows in registers, so K and V are read once and nothing is written but the parts' results.
 //
 //   S = K Q^T   v_mfma_f32_16x16x32_bf16 over 16 rows (M), 16 (token, head) pairs (N) and 32 columns.  Lane (q, c) = (lane / 16, lane % 16)
@@ -204,11 +204,6 @@ struct Rows {
     }
 };
 
-__device__ __forceinline__ float weight(float m, float top) { return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : 0.f; }
-// a part's share of the sum (one that is no number stays none, whatever its maximum)
-__device__ __forceinline__ float share(float m, float l, float top) { return l == l ? weight(m, top) * l : l; }
-__device__ __forceinline__ float log_sum(float top, float total) { return total == 0.f ? -INFINITY : (top + log2f(total)) * 0.693147180559945309f; }
-
 template <int HD, int TILES>
 __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows_kernel(DcPagedAttn a) {
     using T = Rows<HD, TILES>;
@@ -217,17 +212,21 @@ __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows
     const int waves = a.waves;
     __shared__ dc_u32x4 s_q[T::kQueryInLds ? kRows * HD / 8 : 1];
     float *s_m = s_dyn, *s_l = s_dyn + waves * kRows, *s_acc = s_dyn + 2 * waves * kRows;  // [wave][16], [wave][16], [wave][pairs * HD]
-    const int b = blockIdx.x, h = blockIdx.y, split = blockIdx.z, unit = b * a.n_h + h, G = a.group;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), G = a.group;
+    int b = blockIdx.x, h = blockIdx.y, part_ = 0, parts = 1;
+    int64_t slot = 0;
+    if (a.at_once) {
+        const int x = (int)(blockIdx.x / (unsigned)a.n_h);
+        const DcItem d = dc_deal<STEP, false>(a, x, lane);
+        if (d.parts == 0) return;
+        b = d.b, h = (int)(blockIdx.x % (unsigned)a.n_h), part_ = d.part, parts = d.parts, slot = d.slot + (int64_t)part_ * a.n_h + h;
+    }
     const DcSpan span = dc_span(a.t, b);
     if (span.count == 0) return;
     const int pairs = span.count * G, p_lo = span.start, p_hi = span.start + span.count - 1;
     const DcSteps st = dc_steps<STEP>(a, p_lo, p_hi);
-    const int64_t slot = (int64_t)unit * a.n_splits + split;
-    int per = a.n_splits == 1 ? st.steps : (int)((uint32_t)(st.steps + a.n_splits - 1) / (uint32_t)a.n_splits);
-    per = per < waves ? waves : per;
-    const int begin = split * per, end = begin + per < st.steps ? begin + per : st.steps;
-    if (begin >= end && a.n_splits > 1) {  // a part without rows: the join takes nothing of it
+    const int per = (st.steps + parts - 1) / parts, begin = part_ * per, end = begin + per < st.steps ? begin + per : st.steps;
+    if (begin >= end && parts > 1) {  // a part without rows: the join takes nothing of it
         if (tid < pairs) reinterpret_cast<float2 *>(a.ws_ml)[slot * a.tile_rows + tid] = make_float2(-INFINITY, 0.f);
         return;
     }
@@ -242,7 +241,7 @@ __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows
     const int last_page = (a.n_rows - 1) >> a.p.shift, mask = (1 << a.p.shift) - 1;
     // a wave's steps are every waves-th of the block's, from a start of its block's own on
     const int mine = end > begin + wave ? (end - begin - wave + waves - 1) / waves : 0;
-    int at = (int)(((uint64_t)((uint32_t)slot * 0x9e3779b9u) * (uint32_t)mine) >> 32);
+    int at = (int)(((uint64_t)((uint32_t)blockIdx.x * 0x9e3779b9u) * (uint32_t)mine) >> 32);
     int id[TILES], row = 0;
     auto look = [&]() __attribute__((always_inline)) {
         row = st.row(begin + wave + at * waves, STEP);
@@ -333,44 +332,35 @@ __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows
         float sum = 0.f, total = 0.f;
 #pragma unroll
         for (int i = 0; i < kMostWaves; ++i) {
-            sum = fmaf(i < waves ? weight(m[i], top) : 0.f, i < waves ? part[i] : 0.f, sum);
-            total += i < waves ? share(m[i], ls[i], top) : 0.f;
+            sum = fmaf(i < waves ? dc_weight(m[i], top) : 0.f, i < waves ? part[i] : 0.f, sum);
+            total += i < waves ? dc_share(m[i], ls[i], top) : 0.f;
         }
-        if (a.n_splits > 1) {
+        if (parts > 1) {
             a.ws_acc[(slot * a.tile_rows + r) * HD + o % HD] = sum;
             if (o % HD == 0) reinterpret_cast<float2 *>(a.ws_ml)[slot * a.tile_rows + r] = make_float2(top, total);
         } else {
             const int64_t dst = (int64_t)(span.first + r / G) * a.n_h * G + h * G + r % G;
             a.out[dst * HD + o % HD] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
-            if (a.lse && o % HD == 0) a.lse[dst] = log_sum(top, total);
+            if (a.lse && o % HD == 0) a.lse[dst] = dc_log_sum(top, total);
         }
     }
 }
 
-// What a join's block has to know of its row of a unit: where the parts are, and where the result goes.
-struct Row {
-    int64_t slot0, dst;  // the row's place in part 0; the (token, head) of the outputs
-    bool live;
-};
-__device__ __forceinline__ Row row_of(const DcPagedAttn &a, int group, int r) {
-    const int unit = group / a.tiles, b = unit / a.n_h, h = unit % a.n_h;
-    const int pair = (group % a.tiles) * a.tile_rows + r, token = pair / a.group;
-    const DcSpan span = dc_span(a.t, b);
-    return {(int64_t)group * a.n_splits * a.tile_rows + r, (int64_t)(span.first + token) * a.n_h * a.group + h * a.group + pair % a.group,
-            token < span.count};
-}
-
 // The parts of one row joined by a block: HD / 4 threads to a part, all of a round's parts asked for before any weight is known.
-template <int HD>
+template <int HD, int STEP>
 __global__ __launch_bounds__(kThreads) void paged_join_kernel(DcPagedAttn a) {
     constexpr int kLanes = HD / 4, kParts = kThreads / kLanes, kBatch = HD == 256 ? 8 : 4;
     __shared__ float4 s_acc[kThreads];
-    const int tid = threadIdx.x, lane = tid & 63, n = a.n_splits;
-    const Row row = row_of(a, (int)(blockIdx.x / (unsigned)a.tile_rows), (int)(blockIdx.x % (unsigned)a.tile_rows));
-    if (!row.live) return;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + row.slot0;
-    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + row.slot0 * kLanes + tid % kLanes;
-    const int64_t step = a.tile_rows;
+    const int tid = threadIdx.x, lane = tid & 63, h = (int)(blockIdx.x % (unsigned)a.n_h), r = blockIdx.y;
+    const DcItem d = dc_deal<STEP, false, true>(a, (int)(blockIdx.x / (unsigned)a.n_h), lane);
+    if (d.parts < 2) return;
+    const DcSpan span = dc_span(a.t, d.b);
+    const int token = r / a.group, n = d.parts;
+    if (token >= span.count) return;
+    const int64_t dst = (int64_t)(span.first + token) * a.n_h * a.group + h * a.group + r % a.group;
+    const int64_t slot0 = (d.slot + h) * a.tile_rows + r, step = (int64_t)a.n_h * a.tile_rows;
+    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0;
+    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + slot0 * kLanes + tid % kLanes;
     float4 v[kBatch];
     float2 o[kBatch];
     auto load = [&](int s0) __attribute__((always_inline)) {
@@ -391,8 +381,8 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(DcPagedAttn a) {
     float top = own.x;
     for (int s = lane + 64; s < n; s += 64) top = fmaxf(top, ml[s * step].x);
     top = all(top, [](float x, float y) { return fmaxf(x, y); });
-    float total = share(own.x, own.y, top);
-    for (int s = lane + 64; s < n; s += 64) total += share(ml[s * step].x, ml[s * step].y, top);
+    float total = dc_share(own.x, own.y, top);
+    for (int s = lane + 64; s < n; s += 64) total += dc_share(ml[s * step].x, ml[s * step].y, top);
     total = all(total, [](float x, float y) { return x + y; });
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int s0 = tid / kLanes;;) {
@@ -400,7 +390,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(DcPagedAttn a) {
         for (int i = 0; i < kBatch; ++i) {
             // (a part without rows has no sums in the workspace)
             const bool in = s0 + i * kParts < n && o[i].x > -INFINITY;
-            const float f = in ? weight(o[i].x, top) : 0.f;
+            const float f = in ? dc_weight(o[i].x, top) : 0.f;
             acc.x = fmaf(f, in ? v[i].x : 0.f, acc.x), acc.y = fmaf(f, in ? v[i].y : 0.f, acc.y);
             acc.z = fmaf(f, in ? v[i].z : 0.f, acc.z), acc.w = fmaf(f, in ? v[i].w : 0.f, acc.w);
         }
@@ -415,104 +405,75 @@ __global__ __launch_bounds__(kThreads) void paged_join_kernel(DcPagedAttn a) {
         float sum = x[0];
 #pragma unroll
         for (int i = 1; i < kParts; ++i) sum += x[i * HD];
-        a.out[row.dst * HD + tid] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
+        a.out[dst * HD + tid] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
     }
-    if (a.lse && tid == 0) a.lse[row.dst] = log_sum(top, total);
-}
-
-// The same for many rows of few parts: HD / 4 threads to a row, four parts asked for at once, before anything is known of the row.
-template <int HD>
-__global__ __launch_bounds__(kThreads) void paged_join_rows_kernel(DcPagedAttn a) {
-    constexpr int kLanes = HD / 4, kPer = kThreads / kLanes, kBatch = 4;
-    const int at = (int)(blockIdx.x * kPer) + (int)threadIdx.x / kLanes, c = threadIdx.x % kLanes;  // (tile_rows is a multiple of kPer)
-    const int group = at / a.tile_rows, r = at % a.tile_rows, n = a.n_splits;
-    const int64_t slot0 = (int64_t)group * n * a.tile_rows + r;
-    const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0;
-    const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + slot0 * kLanes + c;
-    float top = -INFINITY, total = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < n; s0 += kBatch) {
-        float2 o[kBatch];
-        float4 v[kBatch];
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {  // (the last part again where there are no more; what a row without a token reads is not used)
-            const int64_t s = (int64_t)(s0 + i < n ? s0 + i : n - 1) * a.tile_rows;
-            o[i] = ml[s], v[i] = pa[s * kLanes];
-        }
-        float to = top;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) to = fmaxf(to, o[i].x);
-        const float f = weight(top, to);
-        acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-        total = share(top, total, to);
-        top = to;
-#pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-            // (a part without rows has no sums in the workspace)
-            const bool in = s0 + i < n && o[i].x > -INFINITY;
-            const float g = in ? weight(o[i].x, top) : 0.f;
-            total += in ? share(o[i].x, o[i].y, top) : 0.f;
-            acc.x = fmaf(g, in ? v[i].x : 0.f, acc.x), acc.y = fmaf(g, in ? v[i].y : 0.f, acc.y);
-            acc.z = fmaf(g, in ? v[i].z : 0.f, acc.z), acc.w = fmaf(g, in ? v[i].w : 0.f, acc.w);
-        }
-    }
-    const Row row = row_of(a, group, r);
-    if (!row.live) return;
-    const float d = total == 0.f ? 1.f : total;
-    *reinterpret_cast<uint2 *>(a.out + row.dst * HD + 4 * c) = make_uint2(dc_pack_bf16(acc.x / d, acc.y / d), dc_pack_bf16(acc.z / d, acc.w / d));
-    if (a.lse && c == 0) a.lse[row.dst] = log_sum(top, total);
+    if (a.lse && tid == 0) a.lse[dst] = dc_log_sum(top, total);
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 
 constexpr int row_tiles(int hd) { return hd == 64 ? 4 : 2; }
-constexpr int blocks_of(int hd) { return hd == 256 ? 512 : 768; }  // as many as run at once, two or three to a CU
+constexpr int rows_at_once(int hd) { return hd == 256 ? 512 : 768; }  // two or three blocks to a CU
 // Rows times columns up to which a unit is one block of eight waves, which writes the output itself: 384 KB of K and V, some 2 us of what a CU
 // can read more, but less than a second kernel that joins parts where the host waits for its launches (one sequence of 8 heads x
 // 128: 700 rows 10.7 us, in parts 8.9, called one after another 11.0 and 15.4; 32 sequences 17.2 and 22.7 us).
 constexpr int64_t kAlone = 768 * 128;
 
 struct Cut {
-    bool chunk;
-    int n_splits, waves, tiles, tile_rows;
+    bool chunk, deal, join;   // deal: blocks find their items; join: some may be parts
+    int waves, tiles, tile_rows, at_once, least;
+    int64_t blocks;
 };
-Cut cut_of(int64_t n_units, int group, int hd, int64_t rows, int max_new) {
+// tokens: of all sequences together, where they are packed; else 0
+Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, int64_t tokens) {
     Cut c;
+    const int64_t n_units = n_b * n_h;
     c.chunk = (int64_t)max_new * group > kRows;
     if (c.chunk) {
-        c.tile_rows = kChunkRows, c.waves = 4;
+        c.tile_rows = kChunkRows, c.waves = 4, c.at_once = dc_chunk_at_once(hd);
         c.tiles = (int)(((int64_t)max_new * group + kChunkRows - 1) / kChunkRows);
-        c.n_splits = dc_paged_chunk_splits(n_units, c.tiles, hd, rows);
+        int64_t all = n_b * c.tiles;
+        if (tokens && tokens * group / kChunkRows + n_b < all) all = tokens * group / kChunkRows + n_b;
+        // Parts of four steps where the tiles alone leave most CUs idle (16 tokens of 8 heads behind 4080 rows: 16 us, of eight steps 21).
+        // Where they do not, a part has to save more than the join takes (a prompt of 517 tokens, 136 tiles: 19.6 us, in two parts
+        // 26.7; of 2048, 512 tiles: 63 us, the longer half of them in two parts of 16 steps 84).
+        const int64_t steps = (rows + dc_chunk_step(hd) - 1) / dc_chunk_step(hd);
+        c.least = all * n_h <= (hd == 256 ? 64 : 128) ? 4 : hd == 256 ? 16 : 32;
+        c.join = all * n_h <= (n_b == 1 ? c.at_once / 2 : 2 * c.at_once) && 2 * steps >= 3 * c.least;
+        c.deal = c.join || (tokens && n_b > 1);
+        if (!c.join) c.least = kMostRows;
+        if (!c.deal && c.tiles > all) c.tiles = (int)all;  // (one sequence of fewer packed tokens than max_new)
+        c.blocks = c.deal ? n_h * (all + (c.join ? 2 * c.at_once / n_h + 1 : 0)) : n_b * c.tiles * n_h;
         return c;
     }
-    c.tiles = 1, c.tile_rows = max_new * group;
+    c.tiles = 1, c.tile_rows = max_new * group, c.at_once = rows_at_once(hd), c.least = kWaves;
     const int64_t step = 16 * row_tiles(hd), steps = (rows + step - 1) / step;
-    if (steps * step * hd <= kAlone) {
-        c.n_splits = 1, c.waves = steps <= kWaves ? kWaves : kMostWaves;
-        return c;
-    }
-    const int64_t parts = (steps + kWaves - 1) / kWaves, most = blocks_of(hd) / n_units > 1 ? blocks_of(hd) / n_units : 1;
-    c.n_splits = (int)(parts < most ? parts : most), c.waves = kWaves;
+    c.deal = c.join = steps * step * hd > kAlone && n_units <= 2 * c.at_once;
+    c.waves = steps * step * hd > kAlone || steps <= kWaves ? kWaves : kMostWaves;
+    c.blocks = c.deal ? n_h * (n_b + c.at_once / n_h + 1) : n_units;
     return c;
 }
 size_t acc_bytes(int64_t slots, int rows, int hd) { return dc_align_up((size_t)slots * rows * hd * 4, 256); }
 size_t ml_bytes(int64_t slots, int rows) { return dc_align_up((size_t)slots * rows * 8, 256); }
 
 template <int HD>
-void launch_rows(const DcPagedAttn &a, int n_units, hipStream_t st) {
+void launch_rows(const DcPagedAttn &a, const Cut &c, hipStream_t st) {
+    constexpr int TILES = row_tiles(HD);
     const size_t lds = (size_t)a.waves * (2 * kRows + a.tile_rows * HD) * sizeof(float);
-    hipLaunchKernelGGL((paged_rows_kernel<HD, row_tiles(HD)>), dim3((unsigned)(n_units / a.n_h), (unsigned)a.n_h, (unsigned)a.n_splits),
-                       dim3(a.waves * 64), lds, st, a);
+    const dim3 grid = c.deal ? dim3((unsigned)c.blocks) : dim3((unsigned)a.n_b, (unsigned)a.n_h);
+    hipLaunchKernelGGL((paged_rows_kernel<HD, TILES>), grid, dim3(a.waves * 64), lds, st, a);
+    if (c.join) hipLaunchKernelGGL((paged_join_kernel<HD, 16 * TILES>), dim3((unsigned)(a.n_b * a.n_h), (unsigned)a.tile_rows), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace
 
-extern "C" size_t dc_paged_attn_workspace_bytes(int n_units, int group, int hd, int n_rows, int max_new) {
-    if (n_units <= 0 || n_units >= (1 << 24) || group <= 0 || group > 16 || hd < 64 || n_rows < 0 || max_new <= 0) return 0;
-    const Cut c = cut_of(n_units, group, hd, n_rows, max_new);
-    if (c.n_splits == 1) return 0;
-    const int64_t slots = (int64_t)n_units * c.tiles * c.n_splits;
-    return acc_bytes(slots, c.tile_rows, hd) + ml_bytes(slots, c.tile_rows);
+extern "C" size_t dc_paged_attn_workspace_bytes(int n_b, int n_h, int group, int hd, int n_rows, int max_new, int n_tokens) {
+    if (n_b <= 0 || n_h <= 0 || (int64_t)n_b * n_h >= (1 << 24) || group <= 0 || group > 16 || hd < 64 || n_rows < 0 || max_new <= 0 || n_tokens < 0) return 0;
+    // (so many sequences that nothing is dealt out: enough for fewer, where it is)
+    const int64_t most = 2 * rows_at_once(hd) / n_h;
+    const bool few = (int64_t)max_new * group <= kRows;
+    const Cut c = cut_of(few && most > 0 && n_b > most ? most : n_b, n_h, group, hd, n_rows, max_new, n_tokens);
+    return c.join ? acc_bytes(c.blocks, c.tile_rows, hd) + ml_bytes(c.blocks, c.tile_rows) : 0;
 }
 
 extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
@@ -530,14 +491,12 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
     DC_REQUIRE(x->scale > 0.f && x->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
     DC_REQUIRE((int64_t)t.max_new * x->group < (1ll << 30), "%s: too many tokens", who);
-    const int n_units = t.n_b * x->n_h;
-    const Cut c = cut_of(n_units, x->group, x->hd, x->n_rows, t.max_new);
-    const int64_t slots = (int64_t)n_units * c.tiles * c.n_splits;
-    DC_REQUIRE(dc_grid_fits(c.chunk ? slots : t.n_b, c.waves * 64), "%s: grid too large", who);
+    const Cut c = cut_of(t.n_b, x->n_h, x->group, x->hd, x->n_rows, t.max_new, t.cu ? t.n_tokens : 0);
+    DC_REQUIRE(dc_grid_fits(c.chunk || c.deal ? c.blocks : t.n_b, c.waves * 64), "%s: grid too large", who);
     DcPagedAttn a;
     a.ws_acc = a.ws_ml = nullptr;
-    if (c.n_splits > 1) {
-        const size_t acc = acc_bytes(slots, c.tile_rows, x->hd), need = acc + ml_bytes(slots, c.tile_rows);
+    if (c.join) {
+        const size_t acc = acc_bytes(c.blocks, c.tile_rows, x->hd), need = acc + ml_bytes(c.blocks, c.tile_rows);
         DC_REQUIRE(x->workspace && ((uintptr_t)x->workspace & 255u) == 0, "%s: workspace must be non-null and 256-byte aligned", who);
         if (x->workspace_bytes < need) {
             dc_set_error("%s: workspace %zu bytes < %zu needed", who, x->workspace_bytes, need);
@@ -549,31 +508,14 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     a.p = dc_pages_of(x->store, t), a.t = dc_new_of(t);
     a.qs = {x->q_batch_stride, x->q_token_stride, x->q_head_stride};
     a.n_h = x->n_h, a.group = x->group, a.n_rows = x->n_rows, a.n_sink = x->n_sink, a.window = x->window;
-    a.n_splits = c.n_splits, a.waves = c.waves, a.tiles = c.tiles, a.tile_rows = c.tile_rows;
+    a.n_b = t.n_b, a.waves = c.waves, a.tiles = c.tiles, a.tile_rows = c.tile_rows;
+    a.at_once = c.deal ? c.at_once : 0, a.least = c.least, a.items = (int)(c.blocks / x->n_h), a.of_all = 1.0001f / (float)c.at_once;
     a.scale = x->scale * 1.44269504088896341f;
     hipStream_t st = (hipStream_t)stream;
-    if (c.chunk) {
-        if (const int rc = dc_paged_chunk_launch(a, x->hd, n_units, st)) return rc;
-    } else if (x->hd == 64) {
-        launch_rows<64>(a, n_units, st);
-    } else if (x->hd == 128) {
-        launch_rows<128>(a, n_units, st);
-    } else {
-        launch_rows<256>(a, n_units, st);
-    }
+    if (c.chunk) return dc_paged_chunk_launch(a, x->hd, (unsigned)c.blocks, c.join, st);
+    if (x->hd == 64) launch_rows<64>(a, c, st);
+    else if (x->hd == 128) launch_rows<128>(a, c, st);
+    else launch_rows<256>(a, c, st);
     DC_CHECK_LAUNCH(who);
-    if (c.n_splits > 1) {
-        const int64_t rows = (int64_t)n_units * c.tiles * c.tile_rows;
-#define DC_JOIN(HD)                                                                                                                        \
-    do {                                                                                                                                   \
-        if (c.chunk && c.n_splits <= 8) hipLaunchKernelGGL(paged_join_rows_kernel<HD>, dim3((unsigned)(rows / (kThreads / (HD / 4)))), dim3(kThreads), 0, st, a); \
-        else hipLaunchKernelGGL(paged_join_kernel<HD>, dim3((unsigned)rows), dim3(kThreads), 0, st, a);                                    \
-    } while (0)
-        if (x->hd == 64) DC_JOIN(64);
-        else if (x->hd == 128) DC_JOIN(128);
-        else DC_JOIN(256);
-#undef DC_JOIN
-        DC_CHECK_LAUNCH(who);
-    }
     return DC_OK;
 }

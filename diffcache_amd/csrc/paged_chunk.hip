@@ -42,19 +42,20 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
     // (four arrays, not one of four: the reads of one are then known not to wait for the loads into another)
     __shared__ __attribute__((aligned(1024))) uint8_t s_k0[T::BYTES], s_v0[T::BYTES], s_k1[T::BYTES], s_v1[T::BYTES];
     __shared__ __attribute__((aligned(16))) uint32_t s_odd[2][4];  // [buffer][wave]: whether the wave left out numbers of V that are not finite
-    const int n_units = (int)(gridDim.x / (unsigned)(a.tiles * a.n_splits));
-    // units first, so that a unit's blocks are on one XCD where their number divides by eight; late tokens first, they have the most rows
-    const int unit = (int)(blockIdx.x % (unsigned)n_units), rest = (int)(blockIdx.x / (unsigned)n_units);
-    const int split = rest % a.n_splits, tile = a.tiles - 1 - rest / a.n_splits;
-    const int b = unit / a.n_h, h = unit % a.n_h, G = a.group;
+    // heads first, so that a sequence's blocks of one head are on one XCD where their number divides by eight; late tokens first
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
+    const int h = (int)(blockIdx.x % (unsigned)a.n_h), x_ = (int)(blockIdx.x / (unsigned)a.n_h), G = a.group;
+    DcItem d = {x_ % a.n_b, a.tiles - 1 - x_ / a.n_b, 0, 1, 0};
+    if (a.at_once) d = dc_deal<KT, true>(a, x_, lane);
+    if (d.part >= d.parts) return;  // (its tile has fewer parts than the sequence's last one)
+    const int b = d.b;
     const DcSpan span = dc_span(a.t, b);
-    const int pairs = span.count * G, pair0 = tile * kChunkRows;
+    const int pairs = span.count * G, pair0 = d.tile * kChunkRows;
     if (pair0 >= pairs) return;
     const int t_lo = pair0 / G, t_hi = (pair0 + kChunkRows < pairs ? pair0 + kChunkRows : pairs) - 1;
     const DcSteps steps = dc_steps<KT>(a, span.start + t_lo, span.start + t_hi / G);
-    const int per = (steps.steps + a.n_splits - 1) / a.n_splits;
-    const int begin = split * per, end = begin + per < steps.steps ? begin + per : steps.steps;
+    const int per = (steps.steps + d.parts - 1) / d.parts;
+    const int begin = d.part * per, end = begin + per < steps.steps ? begin + per : steps.steps;
 
     // the wave's pairs: lane's own, and the least and the largest row
     const int first = pair0 + wave * kRowsOfWave;
@@ -248,8 +249,8 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
     l = dc_over32(l, [](float u, float v) { return u + v; });
     if (own >= pairs) return;
     const int64_t dst = (int64_t)(span.first + token) * a.n_h * G + h * G + pair % G;
-    if (a.n_splits > 1) {
-        const int64_t slot = ((int64_t)(unit * a.tiles + tile) * a.n_splits + split) * kChunkRows + wave * kRowsOfWave + (lane & 31);
+    if (d.parts > 1) {
+        const int64_t slot = (d.slot + (int64_t)d.part * a.n_h + h) * kChunkRows + wave * kRowsOfWave + (lane & 31);
         float *acc = a.ws_acc + slot * HD + 4 * half;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
@@ -267,32 +268,72 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
         for (int i = 0; i < 16; i += 4)
             *reinterpret_cast<uint2 *>(out + 32 * d + 2 * i) =
                 make_uint2(dc_pack_bf16(o[d][i] / inv, o[d][i + 1] / inv), dc_pack_bf16(o[d][i + 2] / inv, o[d][i + 3] / inv));
-    if (a.lse && half == 0) a.lse[dst] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945309f;
+    if (a.lse && half == 0) a.lse[dst] = dc_log_sum(m, l);
 }
 
-constexpr int step_rows(int hd) { return hd == 256 ? 32 : 64; }
+// The parts of a tile joined: its blocks share its rows, every parts-th of them each, HD / 4 threads to a row, four parts asked for at
+// once.
+template <int HD, int KT>
+__global__ __launch_bounds__(kThreads) void paged_chunk_join_kernel(DcPagedAttn a) {
+    constexpr int kLanes = HD / 4, kPer = kThreads / kLanes, kBatch = 4;
+    const int tid = threadIdx.x, c = tid % kLanes, h = (int)(blockIdx.x % (unsigned)a.n_h), G = a.group;
+    const DcItem d = dc_deal<KT, true>(a, (int)(blockIdx.x / (unsigned)a.n_h), tid & 63);
+    if (d.parts < 2 || d.part >= d.parts) return;
+    const DcSpan span = dc_span(a.t, d.b);
+    const int n = d.parts, pair0 = d.tile * kChunkRows, left = span.count * G - pair0, rows = left < kChunkRows ? left : kChunkRows;
+    const int64_t step = (int64_t)a.n_h * kChunkRows;
+    for (int r = d.part + tid / kLanes * n; r < rows; r += kPer * n) {
+        const int64_t slot0 = (d.slot + h) * kChunkRows + r;
+        const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0;
+        const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + slot0 * kLanes + c;
+        float top = -INFINITY, total = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < n; s0 += kBatch) {
+            float2 o[kBatch];
+            float4 v[kBatch];
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {  // (the last part again where there are no more)
+                const int64_t s = (int64_t)(s0 + i < n ? s0 + i : n - 1) * step;
+                o[i] = ml[s], v[i] = pa[s * kLanes];
+            }
+            float to = top;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) to = fmaxf(to, o[i].x);
+            const float f = dc_weight(top, to);
+            acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+            total = dc_share(top, total, to);
+            top = to;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                // (a part without rows has nothing to add)
+                const bool in = s0 + i < n && o[i].x > -INFINITY;
+                const float g = in ? dc_weight(o[i].x, top) : 0.f;
+                total += in ? dc_share(o[i].x, o[i].y, top) : 0.f;
+                acc.x = fmaf(g, in ? v[i].x : 0.f, acc.x), acc.y = fmaf(g, in ? v[i].y : 0.f, acc.y);
+                acc.z = fmaf(g, in ? v[i].z : 0.f, acc.z), acc.w = fmaf(g, in ? v[i].w : 0.f, acc.w);
+            }
+        }
+        const int pair = pair0 + r;
+        const int64_t dst = (int64_t)(span.first + pair / G) * a.n_h * G + h * G + pair % G;
+        const float by = total == 0.f ? 1.f : total;
+        *reinterpret_cast<uint2 *>(a.out + dst * HD + 4 * c) = make_uint2(dc_pack_bf16(acc.x / by, acc.y / by), dc_pack_bf16(acc.z / by, acc.w / by));
+        if (a.lse && c == 0) a.lse[dst] = dc_log_sum(top, total);
+    }
+}
 
 template <int HD>
-void launch(const DcPagedAttn &a, unsigned blocks, hipStream_t st) {
-    hipLaunchKernelGGL((paged_chunk_kernel<HD, step_rows(HD)>), dim3(blocks), dim3(kThreads), 0, st, a);
+void launch(const DcPagedAttn &a, unsigned blocks, bool join, hipStream_t st) {
+    constexpr int KT = dc_chunk_step(HD);
+    hipLaunchKernelGGL((paged_chunk_kernel<HD, KT>), dim3(blocks), dim3(kThreads), 0, st, a);
+    if (join) hipLaunchKernelGGL((paged_chunk_join_kernel<HD, KT>), dim3(blocks), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace
 
-int dc_paged_chunk_splits(int64_t n_units, int64_t tiles, int hd, int64_t rows) {
-    const int64_t blocks = n_units * tiles, want = (hd == 256 ? 256 : 512) / blocks, steps = (rows + step_rows(hd) - 1) / step_rows(hd);
-    if (want < 2) return 1;
-    // Parts of four steps where the blocks alone leave most CUs idle (16 tokens of 8 heads behind 4080 rows: 16 us, of eight steps 21);
-    // where they do not, a part has to save more than the join takes (a prompt of 517 tokens, 136 blocks: 19.6 us, in two parts 26.7; a step of
-    // 256 columns takes longer: 700 tokens of 4 heads, 88 blocks, 47 us, in two parts 41).
-    const int64_t parts = steps / (want >= 4 ? 4 : hd == 256 ? 8 : 16);
-    return (int)(want < parts ? want : parts > 1 ? parts : 1);
-}
-
-int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, int n_units, hipStream_t st) {
-    const unsigned blocks = (unsigned)((int64_t)n_units * a.tiles * a.n_splits);
-    if (hd == 64) launch<64>(a, blocks, st);
-    else if (hd == 128) launch<128>(a, blocks, st);
-    else launch<256>(a, blocks, st);
+int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, unsigned blocks, bool join, hipStream_t st) {
+    if (hd == 64) launch<64>(a, blocks, join, st);
+    else if (hd == 128) launch<128>(a, blocks, join, st);
+    else launch<256>(a, blocks, join, st);
+    DC_CHECK_LAUNCH("dc_paged_attn_bf16");
     return DC_OK;
 }

@@ -66,7 +66,7 @@ class PagedCache:
         self._holders = [0] * self.num_pages                         # sequences that hold a page
         self._room = 0                                               # tokens that every sequence has pages for
         self._workspace = torch.empty(
-            (hip.paged_attn_workspace_bytes(batch_size * num_kv_heads, num_q_heads // num_kv_heads, head_dim, max_length),),
+            (hip.paged_attn_workspace_bytes(batch_size, num_kv_heads, num_q_heads // num_kv_heads, head_dim, max_length),),
             dtype=torch.uint8, device=self.device)
         self._q = self._attn_out = None
 

@@ -728,7 +728,7 @@ int dc_mx_attn_bf16(const dc_mx_attn_args *args, void *stream);
  *            attended to
  *   start    NULL (zeros), or (n_b) int32 on the device: the rows that the sequences hold before their new tokens.  Token i of sequence b
  *            is its row start[b] + i.  A negative start counts as 0, one above 2^30 as 2^30
- *   cu       NULL, or (n_b + 1) int32 on the device: tokens are packed, those of sequence b the rows cu[b] .. cu[b + 1] - 1 of tensors
+ *   cu       NULL, or (n_b + 1) int32 on the device, none less than the one before: tokens are packed, those of sequence b the rows cu[b] .. cu[b + 1] - 1 of tensors
  *            of n_tokens rows; the batch strides are not used.  Of a sequence with more than max_new tokens the first max_new
  *            count; what lies outside the tensors does not count
  *   counts   with cu NULL, tensors of (n_b, max_new) tokens by strides: NULL (all of them), or (n_b) int32 on the device, the tokens
@@ -786,8 +786,8 @@ int dc_paged_append_bf16(const dc_paged_append_args *args, void *stream);
  * it does attend to, a number of K that is not finite makes the head's outputs and lse NaN where a logit becomes NaN or +inf; one of V the
  * outputs of its column.  Logits are fp32, before the scale too: one that falls below its range is -inf, a weight of 0; one above
  * it makes its head NaN.  Sums and statistics are fp32.
- * The workspace (dc_paged_attn_workspace_bytes for the same sizes, 256-byte aligned; 0: none; with max_new * group up to 16, enough for
- * more sequences, rows or tokens is enough for fewer) holds nothing between calls; calls that may overlap need one each.  Replaces
+ * The workspace (dc_paged_attn_workspace_bytes for the same sizes, n_tokens 0 without cu, 256-byte aligned; 0: none; with max_new *
+ * group up to 16, enough for more sequences, rows or tokens is enough for fewer) holds nothing between calls; calls that may overlap need one each.  Replaces
  * flash_attn_with_kvcache (base.py:134-142) over such a cache.
  */
 typedef struct dc_paged_attn_args {
@@ -802,7 +802,7 @@ typedef struct dc_paged_attn_args {
     int n_h, group, hd, n_rows, n_sink, window;
     float scale;
 } dc_paged_attn_args;
-size_t dc_paged_attn_workspace_bytes(int n_units, int group, int hd, int n_rows, int max_new);
+size_t dc_paged_attn_workspace_bytes(int n_b, int n_h, int group, int hd, int n_rows, int max_new, int n_tokens);
 int dc_paged_attn_bf16(const dc_paged_attn_args *args, void *stream);
 
 #ifdef __cplusplus

@@ -1,0 +1,97 @@
+"""How attention over pages deals its steps out: sequences of very unequal lengths, more of them than lanes, packed tokens, no row twice and none left out."""
+import pytest
+import torch
+
+from oracle import paged as ref
+from test_gpu_paged_attn import DEV, bf, build, check, i32
+
+pytestmark = pytest.mark.gpu
+
+
+def lengths_of(b, most, seed):
+    g = torch.Generator().manual_seed(seed)
+    n = (most ** torch.rand((b,), generator=g)).int().tolist()
+    n[b // 2] = most
+    return [max(x, 1) for x in n]
+
+
+@pytest.mark.parametrize("b,most,hd,h,group", [(1, 9000, 128, 1, 4), (3, 9000, 64, 2, 7), (8, 5000, 256, 2, 4), (64, 4000, 128, 2, 2), (65, 4000, 64, 1, 4), (130, 2500, 128, 3, 1),
+                                               (300, 1800, 64, 1, 16), (800, 900, 128, 2, 1)])
+def test_one_token_of_unequal_sequences(b, most, hd, h, group):
+    from diffcache_amd import _hip as hip
+    lengths = lengths_of(b, most, b)
+    k, v, table, g = build(b, h, hd, 32, lengths, seed=b)
+    q = bf((b, h * group, hd), g)
+    out, lse = hip.paged_attn(q, k, v, table, i32([n - 1 for n in lengths]), want_lse=True)
+    want = ref.attend(q, k, v, table, [(i, 1, n - 1) for i, n in enumerate(lengths)], table.shape[1] * 32, hd ** -0.5)
+    check(out, lse, want, 2.0 ** -15, hd)
+
+
+@pytest.mark.parametrize("b,most,new,hd,h,group", [(2, 3000, 40, 128, 1, 4), (5, 4000, 90, 64, 2, 7), (70, 1500, 30, 128, 1, 4), (3, 2500, 60, 256, 1, 4), (1, 6000, 33, 128, 2, 4)])
+def test_packed_tokens_of_unequal_sequences(b, most, new, hd, h, group):
+    from diffcache_amd import _hip as hip
+    lengths = lengths_of(b, most, b + 1)
+    g0 = torch.Generator().manual_seed(b)
+    counts = [min(n, int(x)) for n, x in zip(lengths, torch.randint(0, new + 1, (b,), generator=g0))]
+    counts[b // 2] = new
+    k, v, table, g = build(b, h, hd, 16, lengths, seed=b)
+    ends = [3]
+    for c in counts:
+        ends.append(ends[-1] + c)
+    total = ends[-1] + 5
+    q = bf((total, h * group, hd), g)
+    out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 9.0, device=DEV)
+    starts = [n - c for n, c in zip(lengths, counts)]
+    hip.paged_attn(q, k, v, table, i32(starts), cu=i32(ends), max_new=new, out=out, lse=lse)
+    span = ref.spans(b, starts, ends, None, new, total)
+    want = ref.attend(q, k, v, table, span, table.shape[1] * 16, hd ** -0.5)
+    check(out, lse, want, 2.0 ** -8, hd)
+    # what is no sequence's stays
+    assert (out[:3] == 3).all() and (out[-5:] == 3).all() and (lse[:3] == 9).all() and (lse[-5:] == 9).all()
+
+
+def counted(b, h, hd, page, lengths, seed):
+    """Values that count: column c of row r is 1 where r % hd == c, else 0.  With queries of zeros every row weighs the same, so the
+    outputs are the numbers of a token's rows of each remainder over that of its rows, exactly, but for their own rounding."""
+    k, v, table, g = build(b, h, hd, page, lengths, seed)
+    v.zero_()
+    for i, n in enumerate(lengths):
+        r = torch.arange(n, device=DEV)
+        v[table[i].long()[r // page], :, r % page] = torch.nn.functional.one_hot(r % hd, hd).to(torch.bfloat16)[:, None]
+    return k.nan_to_num_(0), v, table, g
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 128])
+@pytest.mark.parametrize("sink,window", [(0, 0), (5, 33), (70, 500), (0, 1), (300, 64)])
+@pytest.mark.parametrize("new", [1, 2, 70])
+def test_every_row_counts_once(hd, page, sink, window, new):
+    from diffcache_amd import _hip as hip
+    lengths = [new, 63 + new, 64 + new, 777 + new, 5003]
+    b, h, group = len(lengths), 1, 3
+    k, v, table, g = counted(b, h, hd, page, lengths, 1)
+    q = torch.zeros((b, new, h * group, hd), dtype=torch.bfloat16, device=DEV)
+    out, lse = hip.paged_attn(q, k, v, table, i32([n - new for n in lengths]), n_sink=sink, window=window, want_lse=True)
+    for i, n in enumerate(lengths):
+        for t in range(new):
+            p = n - new + t
+            r = torch.arange(p + 1, device=DEV)
+            if window:
+                r = r[(r > p - window) | (r < sink)]
+            share = torch.bincount(r % hd, minlength=hd).double() / r.numel()
+            # sums of ones up to 5003 are exact; a division, and for parts two products and a sum, in fp32
+            got = out[i, t].double()
+            assert ((got - share).abs() <= 2.0 ** -8 * share * (1 + 2.0 ** -12)).all()
+            assert ((lse[i, t].double() - torch.tensor(r.numel(), dtype=torch.float64).log()).abs() <= 1e-5).all()
+
+
+def test_a_long_and_many_short_sequences_take_little_more_than_their_rows():
+    """One of 4000 rows among seven of 16 gets most of the blocks: its item alone would be one of its parts' time many times over.  (That no
+    item is lost shows in the results; here only that two layouts of one call agree to rounding.)"""
+    from diffcache_amd import _hip as hip
+    lengths = [16] * 3 + [4000] + [16] * 4
+    k, v, table, g = build(8, 2, 128, 16, lengths, 7)
+    q = bf((8, 8, 128), g)
+    a = hip.paged_attn(q, k, v, table, i32([n - 1 for n in lengths]))
+    one = hip.paged_attn(q[3:4], k, v, table[3:4], i32([3999]))
+    assert ((a[3].double() - one[0].double()).abs() <= 2.0 ** -7 * one[0].double().abs() + 1e-6).all()

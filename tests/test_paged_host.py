@@ -122,18 +122,21 @@ def test_nothing_to_do_is_no_error():
 
 
 def test_enough_workspace_for_more_is_enough_for_fewer():
+    rows = (0, 1, 64, 65, 1000, 100000, 2**30)
     for hd in (64, 128, 256):
         for group in (1, 4, 16):
             for new in range(1, 16 // group + 1):
-                last = [0] * 7
-                for units in (1, 2, 7, 64, 300, 512, 513, 5000):
-                    sizes = [hip.paged_attn_workspace_bytes(units, group, hd, n, new) for n in (0, 1, 64, 65, 1000, 100000, 2**30)]
-                    assert sizes == sorted(sizes), (units, sizes)
-                    if new > 1:
-                        assert all(x >= y for x, y in zip(sizes, [hip.paged_attn_workspace_bytes(units, group, hd, n, new - 1)
-                                                                  for n in (0, 1, 64, 65, 1000, 100000, 2**30)]))
-    assert hip.paged_attn_workspace_bytes(0, 4, 128, 100) == hip.paged_attn_workspace_bytes(4, 17, 128, 100) == 0
-    assert hip.paged_attn_workspace_bytes(4, 4, 128, -1) == hip.paged_attn_workspace_bytes(4, 4, 128, 100, 0) == 0
+                for h in (1, 3, 8, 2000):
+                    last = [0] * len(rows)
+                    for b in (1, 2, 7, 64, 65, 192, 193, 300, 512, 513, 5000):
+                        sizes = [hip.paged_attn_workspace_bytes(b, h, group, hd, n, new) for n in rows]
+                        assert sizes == sorted(sizes) and all(x >= y for x, y in zip(sizes, last)), (b, h, sizes)
+                        last = sizes
+                        if new > 1:
+                            assert all(x >= y for x, y in zip(sizes, [hip.paged_attn_workspace_bytes(b, h, group, hd, n, new - 1) for n in rows]))
+    assert hip.paged_attn_workspace_bytes(0, 1, 4, 128, 100) == hip.paged_attn_workspace_bytes(4, 1, 17, 128, 100) == 0
+    assert hip.paged_attn_workspace_bytes(4, 1, 4, 128, -1) == hip.paged_attn_workspace_bytes(4, 1, 4, 128, 100, 0) == 0
+    assert hip.paged_attn_workspace_bytes(1 << 20, 1 << 5, 4, 128, 1 << 20) == 0
 
 
 def bf(*shape):
