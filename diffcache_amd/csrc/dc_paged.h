@@ -241,7 +241,7 @@ __device__ __forceinline__ int dc_page_id(const DcPages &p, const int32_t *table
 int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, unsigned blocks, bool join, hipStream_t st);
 // Rows of a step; blocks that run at once.
 constexpr int dc_chunk_step(int hd) { return hd == 256 ? 32 : 64; }
-constexpr int dc_chunk_at_once(int hd) { return hd == 64 ? 1024 : hd == 128 ? 512 : 256; }
+constexpr int dc_chunk_at_once(int hd) { return hd == 64 ? 1024 : hd == 128 ? 512 : 512; }
 constexpr int kChunkRows = 128;
 
 typedef __bf16 dc_bf16x2 __attribute__((ext_vector_type(2)));

@@ -36,12 +36,15 @@ struct Tile {
 };
 
 template <int HD, int KT>
-__global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kernel(DcPagedAttn a) {
+__global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a) {
     using T = Tile<HD, KT>;
     constexpr int KS = HD / 16, DT = HD / 32, ST = KT / 32, TILES = KT / 16;  // products of a tile's S; tiles of O, of S, and of what a page holds whole
     // (four arrays, not one of four: the reads of one are then known not to wait for the loads into another)
     __shared__ __attribute__((aligned(1024))) uint8_t s_k0[T::BYTES], s_v0[T::BYTES], s_k1[T::BYTES], s_v1[T::BYTES];
     __shared__ __attribute__((aligned(16))) uint32_t s_odd[2][4];  // [buffer][wave]: whether the wave left out numbers of V that are not finite
+    // (at 256 columns three of a lane's sixteen pieces of Q stand in LDS: with them its registers would be 16 too many for two blocks to a CU)
+    constexpr int QL = HD == 256 ? 3 : 0;
+    __shared__ dc_u32x4 s_q[QL ? QL : 1][QL ? kThreads : 1];
     // heads first, so that a sequence's blocks of one head are on one XCD where their number divides by eight; late tokens first
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
     const int h = (int)(blockIdx.x % (unsigned)a.n_h), x_ = (int)(blockIdx.x / (unsigned)a.n_h), G = a.group;
@@ -64,11 +67,13 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
     const DcReach reach = dc_reach(a, span.start + token);
     const int p_lo = span.start + (live ? first : pairs - 1) / G;
     const int p_hi = span.start + (first + kRowsOfWave - 1 < pairs ? first + kRowsOfWave - 1 : pairs - 1) / G;
-    dc_u32x4 bq[KS];
+    dc_u32x4 bq[KS - QL];
     {
         const uint16_t *src = a.q + dc_token_at(a.t, a.qs, span, b, token) + (int64_t)(h * G + pair % G) * a.qs.h + 8 * half;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) bq[s] = *reinterpret_cast<const dc_u32x4 *>(src + 16 * s);
+        for (int s = 0; s < KS - QL; ++s) bq[s] = *reinterpret_cast<const dc_u32x4 *>(src + 16 * s);
+#pragma unroll
+        for (int s = KS - QL; s < KS; ++s) s_q[s - KS + QL][tid] = *reinterpret_cast<const dc_u32x4 *>(src + 16 * s);
     }
     dc_f32x16 o[DT];
 #pragma unroll
@@ -165,10 +170,11 @@ __global__ __launch_bounds__(kThreads, HD == 256 ? 1 : 2) void paged_chunk_kerne
                 for (int i = 0; i < 16; ++i) x[t][i] = 0.f;
 #pragma unroll
             for (int j = 0; j < KS; ++j) {
+                const dc_u32x4 qw = j < KS - QL ? bq[j < KS - QL ? j : 0] : s_q[j < KS - QL ? 0 : j - KS + QL][QL ? tid : 0];
 #pragma unroll
                 for (int t = 0; t < ST; ++t) {
                     const dc_u32x4 w = *reinterpret_cast<const dc_u32x4 *>(ks + 32 * t * T::ROW + (turn ^ (j << 5)));
-                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, bq[j]), x[t], 0, 0, 0);
+                    x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, qw), x[t], 0, 0, 0);
                 }
             }
             if (have != (1 << TILES) - 1 || !dc_whole(a, p_lo, p_hi, row0, KT)) {
