@@ -10,6 +10,10 @@
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kMany = 1024;  // tokens, from which a block takes several
+// Bytes read and written that no cache holds: beyond the last one's 256 MB the hints save (801 MB 157 -> 143 us, 604 MB 122 -> 109), below they cost
+// what the caches would keep (151 MB 27 -> 36 us).
+constexpr int64_t kStream = 256ll << 20;
 
 struct AppendArgs {
     DcPages p;
@@ -25,10 +29,14 @@ struct AppendArgs {
 
 // A block has 256 / (HD / 16) places for heads: `side` of one token, the rest for more tokens.  A thread has 16 numbers of a head, the
 // two eights that are turned with each other, and takes the same of every side-th head, so that it needs eight angles in
-// all.
-template <int HD, bool ADJACENT>
+// all.  ADJACENT: pairs of adjacent columns.  STREAM: what is read and written passes through the caches.
+//
+// What bounds it: HBM, from some 1000 tokens on.  32601 tokens of 32 + 2 x 8 heads x 128, 801 MB: 143 us = 5.6 TB/s (a large copy 4.9);
+// without the hints of STREAM 157, and then with four heads at a time for three 158 and eight heads or more to a thread for four 163.  Eight tokens of as many sequences:
+// 4.1 us, a kernel's start and the chain of start, page and row; the host takes 8 us more.
+template <int HD, bool ADJACENT, bool STREAM>
 __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs a) {
-    constexpr int J = HD / 16, kPlaces = kThreads / J, kBatch = 4;
+    constexpr int J = HD / 16, kPlaces = kThreads / J, kBatch = 3;
     const int b = (int)(blockIdx.x / (unsigned)a.chunks), chunk = (int)(blockIdx.x % (unsigned)a.chunks);
     const int j = threadIdx.x % J, place = threadIdx.x / J;
     const DcSpan span = dc_span(a.t, b);
@@ -47,7 +55,8 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs a) {
             int at = h + n * a.side;
             if (at >= heads) continue;
             const uint16_t *src = at < a.n_q ? q_src + at * a.qs.h : at < a.n_q + a.n_h ? k_src + (at - a.n_q) * a.ks.h : v_src + (at - a.n_q - a.n_h) * a.vs.h;
-            x[n][0] = *reinterpret_cast<const uint4 *>(src + c0), x[n][1] = *reinterpret_cast<const uint4 *>(src + c1);
+            if constexpr (STREAM) x[n][0] = dc_load_stream16(src + c0), x[n][1] = dc_load_stream16(src + c1);
+            else x[n][0] = *reinterpret_cast<const uint4 *>(src + c0), x[n][1] = *reinterpret_cast<const uint4 *>(src + c1);
         }
     };
     load(h0);
@@ -98,7 +107,9 @@ __global__ __launch_bounds__(kThreads) void paged_append_kernel(AppendArgs a) {
                 turn(x[n][0].z, x[n][1].z, 2), turn(x[n][0].w, x[n][1].w, 3);
             }
             uint16_t *dst = at < a.n_q ? q_dst + at * HD : at < a.n_q + a.n_h ? k_dst + (at - a.n_q) * a.p.kh : v_dst + (at - a.n_q - a.n_h) * a.p.vh;
-            if (at < a.n_q || held) *reinterpret_cast<uint4 *>(dst + c0) = x[n][0], *reinterpret_cast<uint4 *>(dst + c1) = x[n][1];
+            if (at >= a.n_q && !held) continue;
+            if constexpr (STREAM) dc_store_stream16(dst + c0, x[n][0]), dc_store_stream16(dst + c1, x[n][1]);
+            else *reinterpret_cast<uint4 *>(dst + c0) = x[n][0], *reinterpret_cast<uint4 *>(dst + c1) = x[n][1];
         }
         load(h + kBatch * a.side);
     }
@@ -168,22 +179,25 @@ extern "C" int dc_paged_append_bf16(const dc_paged_append_args *x, void *stream)
     a.inv_freq = x->inv_freq, a.pos = x->pos;
     a.ks = {strides[0], strides[1], strides[2]}, a.vs = {strides[3], strides[4], strides[5]}, a.qs = {strides[6], strides[7], strides[8]};
     a.n_h = x->n_h, a.n_q = x->n_q, a.rot16 = x->rot / 16, a.n_axes = x->n_axes, a.table_pages = t.table_pages;
-    // few tokens: a block each; many: as many to a block as give a thread eight heads or more
+    // few tokens: a block each; many: as many to a block as give a thread four heads or more
     const int places = kThreads / (x->hd / 16), heads = x->n_q + 2 * x->n_h;
     const int64_t tokens = t.cu ? t.n_tokens : (int64_t)t.n_b * t.max_new;
     a.side = places;
-    if (tokens > 1024)
-        while (a.side > 2 && heads < 8 * a.side) a.side /= 2;
+    if (tokens > kMany)
+        while (a.side > 2 && heads < 4 * a.side) a.side /= 2;
+    const bool through = tokens * heads * x->hd * 4 > kStream;
     const int per = places / a.side;
     const int64_t chunks = ((int64_t)t.max_new + per - 1) / per;
     DC_REQUIRE(dc_grid_fits((int64_t)t.n_b * chunks, kThreads), "%s: grid too large", who);
     a.chunks = (int)chunks;
     const dim3 grid((unsigned)(t.n_b * chunks)), block(kThreads);
     hipStream_t st = (hipStream_t)stream;
-#define DC_APPEND(HD)                                                                                \
-    do {                                                                                             \
-        if (x->interleaved) hipLaunchKernelGGL((paged_append_kernel<HD, true>), grid, block, 0, st, a); \
-        else hipLaunchKernelGGL((paged_append_kernel<HD, false>), grid, block, 0, st, a);            \
+#define DC_APPEND(HD)                                                                                             \
+    do {                                                                                                          \
+        if (x->interleaved && through) hipLaunchKernelGGL((paged_append_kernel<HD, true, true>), grid, block, 0, st, a); \
+        else if (x->interleaved) hipLaunchKernelGGL((paged_append_kernel<HD, true, false>), grid, block, 0, st, a);   \
+        else if (through) hipLaunchKernelGGL((paged_append_kernel<HD, false, true>), grid, block, 0, st, a);             \
+        else hipLaunchKernelGGL((paged_append_kernel<HD, false, false>), grid, block, 0, st, a);                      \
     } while (0)
     if (x->hd == 64) DC_APPEND(64);
     else if (x->hd == 128) DC_APPEND(128);

@@ -434,11 +434,12 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
         c.tiles = (int)(((int64_t)max_new * group + kChunkRows - 1) / kChunkRows);
         int64_t all = n_b * c.tiles;
         if (tokens && tokens * group / kChunkRows + n_b < all) all = tokens * group / kChunkRows + n_b;
-        // Parts of four steps where the tiles alone leave most CUs idle (16 tokens of 8 heads behind 4080 rows: 16 us, of eight steps 21).
-        // Where they do not, a part has to save more than the join takes (a prompt of 517 tokens, 136 tiles: 19.6 us, in two parts
-        // 26.7; of 2048, 512 tiles: 63 us, the longer half of them in two parts of 16 steps 84).
+        // Parts of seven steps where the tiles alone leave most CUs idle (16 tokens of 8 heads behind 4083 rows: 21.9 us of eight steps, 18.8 of
+        // four; a prompt of 517 of one head in groups of 8: 19.0 and 24.7).  Where they do not, a part has to save more than the join
+        // takes (a prompt of 517 tokens of 8 heads, 136 tiles: 19.6 us, in two parts 26.7; of 2048, 512 tiles: 63 us, the longer half of
+        // them in two parts of 16 steps 84).
         const int64_t steps = (rows + dc_chunk_step(hd) - 1) / dc_chunk_step(hd);
-        c.least = all * n_h <= (hd == 256 ? 64 : 128) ? 4 : hd == 256 ? 16 : 32;
+        c.least = all * n_h <= 128 ? 7 : 24;
         c.join = all * n_h <= (n_b == 1 ? c.at_once / 2 : 2 * c.at_once) && 2 * steps >= 3 * c.least;
         c.deal = c.join || (tokens && n_b > 1);
         if (!c.join) c.least = kMostRows;
