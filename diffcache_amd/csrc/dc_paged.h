@@ -231,6 +231,26 @@ __device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane)
     return d;
 }
 
+// Packed tokens of which no tile is cut: block x / n_h is place x of the tiles' places, of which sequence b has those from
+// floor(cu[b] group / tile_rows) + b on, as many as its tiles or one more.  The sequence is found 64 at a time.
+__device__ __forceinline__ DcItem dc_packed(const DcPagedAttn &a, int x, int lane) {
+    auto place = [&](int b) __attribute__((always_inline)) {
+        return (int)((unsigned)(dc_clamp(a.t.cu[b], 0, a.t.n_tokens) * a.group) / (unsigned)a.tile_rows) + b;
+    };
+    int lo = 0, n = a.n_b;  // the last sequence of [lo, lo + n) whose place is not past x
+    while (n > 1) {
+        const int step = (n + 63) / 64, b = lo + lane * step;
+        const int k = __popcll(__ballot(lane * step < n && place(b) <= x));  // (they do not decrease, so these are the first k lanes)
+        const int at = k > 1 ? (k - 1) * step : 0;
+        lo += at, n = n - at < step ? n - at : step;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const DcSpan s = dc_span(a.t, lo);
+    const int tiles = (int)((unsigned)(s.count * a.group + a.tile_rows - 1) / (unsigned)a.tile_rows), in = x - __builtin_amdgcn_readfirstlane(place(lo));
+    if (in < 0 || in >= tiles) return {0, 0, 0, 0, 0};
+    return {lo, tiles - 1 - in, 0, 1, 0};
+}
+
 // A page's id, or -1 where the table names none that there is.
 __device__ __forceinline__ int dc_page_id(const DcPages &p, const int32_t *table, int index) {
     const int id = dc_step_word(table + index);
@@ -254,6 +274,12 @@ typedef uint32_t dc_u32x2 __attribute__((ext_vector_type(2)));
 // A head's maximum before any logit passed it: finite, so that a logit of -inf has the weight 0 then too, where -inf - -inf
 // would be NaN.  -inf stands for no rows.
 constexpr float kNoLogit = -3.402823466e+38f;
+
+// x - y of x as it was rounded: a product that the compiler takes into the subtraction would not be, and the largest logit's weight not 1
+__device__ __forceinline__ float dc_less(float x, float y) {
+    asm("" : "+v"(x));
+    return x - y;
+}
 
 __device__ __forceinline__ uint32_t dc_pack_bf16(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, dc_bf16x2{(__bf16)lo, (__bf16)hi});

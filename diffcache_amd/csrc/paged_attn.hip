@@ -133,7 +133,7 @@ struct Rows {
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                x[t][i] = __builtin_amdgcn_exp2f(x[t][i] - m);
+                x[t][i] = __builtin_amdgcn_exp2f(dc_less(x[t][i], m));
                 l += x[t][i];
             }
     }
@@ -284,16 +284,16 @@ __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows
             look();
         }
         const bool whole = have == (1 << TILES) - 1 && dc_whole(a, p_lo, p_hi, r0, STEP);  // every row for every pair
-        bool odd = false;
         if (!whole) {
 #pragma unroll
             for (int t = 0; t < TILES; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     if (!((have >> t) & 1) | !reach.has(r0 + 16 * t + 4 * i + w.q)) x[t][i] = -INFINITY;
-            odd = w.unbounded();
-            if (odd) w.bound();
         }
+        // (in every step, for P's second part may be negative: the sum of its products with an infinity would be NaN)
+        const bool odd = w.unbounded();
+        if (odd) w.bound();
         w.weigh(x);
         w.add(x);
         if (odd) {
@@ -432,8 +432,9 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
     if (c.chunk) {
         c.tile_rows = kChunkRows, c.waves = 4, c.at_once = dc_chunk_at_once(hd);
         c.tiles = (int)(((int64_t)max_new * group + kChunkRows - 1) / kChunkRows);
+        const int64_t places = tokens * group / kChunkRows + n_b;  // of packed tokens' tiles (dc_packed)
         int64_t all = n_b * c.tiles;
-        if (tokens && tokens * group / kChunkRows + n_b < all) all = tokens * group / kChunkRows + n_b;
+        if (tokens && places < all) all = places;
         // Parts of seven steps where the tiles alone leave most CUs idle (16 tokens of 8 heads behind 4083 rows: 21.9 us of eight steps, 18.8 of
         // four; a prompt of 517 of one head in groups of 8: 19.0 and 24.7).  Where they do not, a part has to save more than the join
         // takes (a prompt of 517 tokens of 8 heads, 136 tiles: 19.6 us, in two parts 26.7; of 2048, 512 tiles: 63 us, the longer half of
@@ -441,10 +442,10 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
         const int64_t steps = (rows + dc_chunk_step(hd) - 1) / dc_chunk_step(hd);
         c.least = all * n_h <= 128 ? 7 : 24;
         c.join = all * n_h <= (n_b == 1 ? c.at_once / 2 : 2 * c.at_once) && 2 * steps >= 3 * c.least;
-        c.deal = c.join || (tokens && n_b > 1);
-        if (!c.join) c.least = kMostRows;
-        if (!c.deal && c.tiles > all) c.tiles = (int)all;  // (one sequence of fewer packed tokens than max_new)
-        c.blocks = c.deal ? n_h * (all + (c.join ? 2 * c.at_once / n_h + 1 : 0)) : n_b * c.tiles * n_h;
+        c.deal = c.join;
+        if (c.tiles > all) c.tiles = (int)all;  // (one sequence of fewer packed tokens than max_new)
+        if (!c.join && tokens && n_b > 1) all = places;
+        c.blocks = n_h * (all + (c.join ? 2 * c.at_once / n_h + 1 : 0));
         return c;
     }
     c.tiles = 1, c.tile_rows = max_new * group, c.at_once = rows_at_once(hd), c.least = kWaves;
@@ -491,7 +492,7 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     DC_REQUIRE(x->n_rows >= 1 && x->n_rows <= (int64_t)t.table_pages * x->store.page, "%s: %d rows outside the table", who, x->n_rows);
     DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
     DC_REQUIRE(x->scale > 0.f && x->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
-    DC_REQUIRE((int64_t)t.max_new * x->group < (1ll << 30), "%s: too many tokens", who);
+    DC_REQUIRE((int64_t)t.max_new * x->group < (1ll << 30) && (int64_t)t.n_tokens * x->group < (1ll << 31), "%s: too many tokens", who);
     const Cut c = cut_of(t.n_b, x->n_h, x->group, x->hd, x->n_rows, t.max_new, t.cu ? t.n_tokens : 0);
     DC_REQUIRE(dc_grid_fits(c.chunk || c.deal ? c.blocks : t.n_b, c.waves * 64), "%s: grid too large", who);
     DcPagedAttn a;

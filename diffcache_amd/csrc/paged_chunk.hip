@@ -50,6 +50,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
     const int h = (int)(blockIdx.x % (unsigned)a.n_h), x_ = (int)(blockIdx.x / (unsigned)a.n_h), G = a.group;
     DcItem d = {x_ % a.n_b, a.tiles - 1 - x_ / a.n_b, 0, 1, 0};
     if (a.at_once) d = dc_deal<KT, true>(a, x_, lane);
+    else if (a.t.cu && a.n_b > 1) d = dc_packed(a, x_, lane);
     if (d.part >= d.parts) return;  // (its tile has fewer parts than the sequence's last one)
     const int b = d.b;
     const DcSpan span = dc_span(a.t, b);
@@ -200,11 +201,20 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                     for (int i = 0; i < 16; ++i) o[d][i] *= f;
                 m = to;
             }
+            // The product below is exact and m is not: of logits so large that would be more than a weight can grow.
+            const bool huge = __any(fabsf(m) > 0x1p24f);
+            if (huge) {
+#pragma unroll
+                for (int t = 0; t < ST; ++t)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[t][i] = dc_less(x[t][i] * a.scale, m);
+            }
+            const float by = huge ? 1.f : a.scale, less = huge ? 0.f : -m;
 #pragma unroll
             for (int t = 0; t < ST; ++t)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    x[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], a.scale, -m));
+                    x[t][i] = __builtin_amdgcn_exp2f(fmaf(x[t][i], by, less));
                     l += x[t][i];
                 }
             // O^T: rows 16 j + {0 .. 3, 8 .. 11} + 4 half at a time
