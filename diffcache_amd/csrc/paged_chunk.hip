@@ -65,7 +65,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
     const int first = pair0 + wave * kRowsOfWave;
     const bool live = first < pairs;
     const int own = first + (lane & 31), pair = own < pairs ? own : pairs - 1, token = pair / G;
-    const DcReach reach = dc_reach(a, span.start + token);
+    const int p = span.start + token;
     const int p_lo = span.start + (live ? first : pairs - 1) / G;
     const int p_hi = span.start + (first + kRowsOfWave - 1 < pairs ? first + kRowsOfWave - 1 : pairs - 1) / G;
     dc_u32x4 bq[KS - QL];
@@ -144,6 +144,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
         if (lane == 0) s_odd[buf][wave] = odd;
     };
 
+    bool huge = true;  // (as kNoLogit is)
     int have = 0, next = 0, ids = 0;
     if (begin < end) {
         have = fetch(s_k0, s_v0, begin, ids_of(begin));
@@ -179,6 +180,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                 }
             }
             if (have != (1 << TILES) - 1 || !dc_whole(a, p_lo, p_hi, row0, KT)) {
+                const DcReach reach = dc_reach(a, p);
 #pragma unroll
                 for (int t = 0; t < ST; ++t)
 #pragma unroll
@@ -191,7 +193,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) most = fmaxf(most, x[t][i]);
             most *= a.scale;
-            if (__any(most > m + 8.f)) {
+            if (__builtin_expect(__any(most > m + 8.f), 0)) {
                 const float to = fmaxf(m, dc_over32(most, [](float u, float v) { return fmaxf(u, v); }));
                 const float f = m > kNoLogit ? __builtin_amdgcn_exp2f(m - to) : 1.f;  // (nothing was summed, or what is no number)
                 l *= f;
@@ -200,10 +202,10 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[d][i] *= f;
                 m = to;
+                huge = __any(fabsf(m) > 0x1p24f);
             }
             // The product below is exact and m is not: of logits so large that would be more than a weight can grow.
-            const bool huge = __any(fabsf(m) > 0x1p24f);
-            if (huge) {
+            if (__builtin_expect(huge, 0)) {
 #pragma unroll
                 for (int t = 0; t < ST; ++t)
 #pragma unroll
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                     const int page = (row0 + r) >> a.p.shift, id = dc_page_id(a.p, table, page < last_page ? page : last_page);
                     if (id < 0) continue;
                     const uint16_t *src = vh + id * a.p.vp + (int64_t)((row0 + r) & mask) * HD + 4 * half;
-                    const bool in = reach.has(row0 + r);
+                    const bool in = dc_reach(a, p).has(row0 + r);
 #pragma unroll
                     for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -263,28 +265,30 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
     }
 
     l = dc_over32(l, [](float u, float v) { return u + v; });
-    if (own >= pairs) return;
-    const int64_t dst = (int64_t)(span.first + token) * a.n_h * G + h * G + pair % G;
+    // (the lane's number and its pair again, from nothing: no register has to keep them through the loop)
+    const int lane_ = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), half_ = lane_ >> 5, mine = first + (lane_ & 31);
+    if (mine >= pairs) return;
+    const int64_t dst = (int64_t)(span.first + mine / G) * a.n_h * G + h * G + mine % G;
     if (d.parts > 1) {
-        const int64_t slot = (d.slot + (int64_t)d.part * a.n_h + h) * kChunkRows + wave * kRowsOfWave + (lane & 31);
-        float *acc = a.ws_acc + slot * HD + 4 * half;
+        const int64_t slot = (d.slot + (int64_t)d.part * a.n_h + h) * kChunkRows + wave * kRowsOfWave + (lane_ & 31);
+        float *acc = a.ws_acc + slot * HD + 4 * half_;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
                 *reinterpret_cast<float4 *>(acc + 32 * d + 2 * i) = make_float4(o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]);
-        if (half == 0) reinterpret_cast<float2 *>(a.ws_ml)[slot] = make_float2(m, l);
+        if (half_ == 0) reinterpret_cast<float2 *>(a.ws_ml)[slot] = make_float2(m, l);
         return;
     }
     const float inv = l == 0.f ? 1.f : l;
-    uint16_t *out = a.out + dst * HD + 4 * half;
+    uint16_t *out = a.out + dst * HD + 4 * half_;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
             *reinterpret_cast<uint2 *>(out + 32 * d + 2 * i) =
                 make_uint2(dc_pack_bf16(o[d][i] / inv, o[d][i + 1] / inv), dc_pack_bf16(o[d][i + 2] / inv, o[d][i + 3] / inv));
-    if (a.lse && half == 0) a.lse[dst] = dc_log_sum(m, l);
+    if (a.lse && half_ == 0) a.lse[dst] = dc_log_sum(m, l);
 }
 
 // The parts of a tile joined: its blocks share its rows, every parts-th of them each, HD / 4 threads to a row, four parts asked for at

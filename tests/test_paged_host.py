@@ -298,3 +298,11 @@ def test_the_plain_rows_and_spans():
     assert ref.attended(6, [0, 1], 4, 2, 8, n_sink=1, window=3) == [0, 4, 5, 6]
     assert ref.spans(2, [-3, 1 << 31], None, [9, -1], 4, 8) == [(0, 4, 0), (4, 0, 1 << 30)]
     assert ref.spans(3, None, [-2, 3, 1, 99], None, 2, 8) == [(0, 2, 0), (3, 0, 0), (1, 2, 0)]
+
+
+@pytest.mark.parametrize("source,kernels", [("paged.hip", ["paged_append_kernel"]), ("paged_attn.hip", ["paged_rows_kernel", "paged_join_kernel"]),
+                                            ("paged_chunk.hip", ["paged_chunk_kernel", "paged_chunk_join_kernel"])])
+def test_kernels_do_not_spill(source, kernels):
+    """The 256-column kernels stand at the 256 registers that two waves to a SIMD leave: 16 spilled ones made a chunk's take 1.4 times as long."""
+    from test_host_logic import test_scan_kernels_do_not_spill as check
+    check(source, kernels)
