@@ -493,7 +493,9 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
     DC_REQUIRE(x->scale > 0.f && x->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
     DC_REQUIRE((int64_t)t.max_new * x->group < (1ll << 30) && (int64_t)t.n_tokens * x->group < (1ll << 31), "%s: too many tokens", who);
-    const Cut c = cut_of(t.n_b, x->n_h, x->group, x->hd, x->n_rows, t.max_new, t.cu ? t.n_tokens : 0);
+    // rows that a window's tokens can need at most, and a step more at its two ends
+    const int64_t in_window = (int64_t)x->n_sink + x->window + t.max_new + 256, rows = x->window && in_window < x->n_rows ? in_window : x->n_rows;
+    const Cut c = cut_of(t.n_b, x->n_h, x->group, x->hd, rows, t.max_new, t.cu ? t.n_tokens : 0);
     DC_REQUIRE(dc_grid_fits(c.chunk || c.deal ? c.blocks : t.n_b, c.waves * 64), "%s: grid too large", who);
     DcPagedAttn a;
     a.ws_acc = a.ws_ml = nullptr;
