@@ -21,6 +21,13 @@ constexpr int kThreads = 256, kWaves = 4, kMostWaves = 8, kRows = 16;
 //
 // Which row of a tile is which row of M is free as long as K and V agree: M row 4 q + i is the tile's row 4 i + q, so that every
 // load takes whole lines.  A tile of 16 rows lies in one page, so its address is the scalar unit's; page ids are read a step ahead.
+//
+// What bounds it: HBM from some 300 MB on.  8 x 131072 rows of 8 heads x 128 with groups of 4, 4.29 GB: 626 us = 6.9 TB/s (pages of 16 rows 647);
+// 8 x 65536 of 4 heads x 256 321 us = 6.7 TB/s; 16 x 65536 of 8 heads x 64 343 us = 6.3; four drafted tokens of 8 x 32601 rows 171 us = 6.2.  A step of
+// 32 rows x 128 columns is 50 vector, 6 matrix and 4 load instructions for each 4 KB; the vector unit issues a fifth of the time.  Below, the chain of start,
+// page ids, rows, products and the join: 32601 rows of 8 units 24.7 + 3.9 us (the bytes 19), 517 rows in one kernel 10 us, 64 rows 5.6.
+// Steps of 64 rows at 128 columns (two blocks to a CU) took 10.8 us for 517 rows and 279 for 48 x 8192 (242 now), the large ones the same.
+// At 256 columns 25 registers spilled cost 447 us for 321.
 template <int HD, int TILES>
 struct Rows {
     static constexpr int STEP = 16 * TILES, CH = HD / 32, EPL = HD / 16, VW = EPL / 2;

@@ -12,6 +12,15 @@
 // much matrix work again, for an error no larger than that of the output's own rounding (against 64 bits 2.1e-3 of the result with both,
 // 1.7e-3 is the output's alone).  Softmax in powers of two, fp32; the maximum moves where a
 // logit passes it by more than 8.
+//
+// What bounds it: the matrix and the vector unit one after the other.  2048 tokens of 32 heads x 128 behind 30553 rows: 1060 us warm, 1086 with inputs in
+// turn = 976 TFLOP/s (a large library product: 1160); the matrix unit works in 43 % of the cycles, the vector unit (half of it the exponentials) in
+// 39 %, LDS reads in 22 % without a conflict; two waves to a SIMD leave little of that side by side.  A prompt of 8195 tokens 568-645 us = 850-970 TFLOP/s; 1024
+// tokens at 256 columns 1030-1110 us = 970-1040; at 64 columns, where a row has half the products for the same exponentials, 330-360 us for 224 GFLOP =
+// 620-680.  One step takes some 1.1 us where a CU has one block, 2.1 where it has two; a prompt of 517 tokens (nine steps) 20 us.
+// Kept: K and V straight to LDS instead of through registers (1163 -> 1060), page ids a step ahead and masks without branches (1348 -> 1163), at 256
+// columns two blocks to a CU (1781 -> 1068).  Tried and dropped: wave priorities (the same), three blocks of 32-row steps to a CU at 128
+// columns (1293 for 1116), a zero operand kept for the first product (1222 for 1172).
 #include "dc_paged.h"
 
 namespace {
