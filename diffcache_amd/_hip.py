@@ -1347,6 +1347,8 @@ def _paged_store(k_pages: torch.Tensor, v_pages: torch.Tensor):
     if len(shape) != 4 or v_pages.shape != shape or k_pages.dtype is not _BF16 or v_pages.dtype is not _BF16:
         raise DiffCacheError("k_pages and v_pages must be (n_pages, h, page, hd) bf16 tensors of one shape")
     n, h, page, hd = shape
+    if hd not in (64, 128, 256):
+        raise DiffCacheError(f"head_dim {hd} is not supported (64, 128 or 256)")
     k0, k1, k2, k3 = k_pages.stride()
     v0, v1, v2, v3 = v_pages.stride()
     if k3 != 1 or v3 != 1 or (page > 1 and (k2 != hd or v2 != hd)):
@@ -1372,7 +1374,7 @@ def _paged_tokens(shape, table: torch.Tensor, start: Optional[torch.Tensor], cu:
         if cu.dtype is not _I32 or cu.numel() != b + 1 or not cu.is_contiguous():
             raise DiffCacheError(f"cu must be a contiguous int32 tensor of {b + 1} elements")
         tokens = shape[0]
-        if max_new is None:
+        if max_new is None or max_new > tokens:
             max_new = tokens
     else:
         if dims == 3:

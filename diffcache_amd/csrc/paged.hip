@@ -130,7 +130,7 @@ int dc_check_paged(const char *who, const dc_paged_store &s, const dc_paged_toke
     DC_REQUIRE(t.table && t.table_pages >= 1 && t.table_stride >= t.table_pages, "%s: bad table", who);
     DC_REQUIRE((int64_t)t.table_pages * s.page <= kMostRows, "%s: a table of more than 2^30 rows", who);
     DC_REQUIRE(!(t.cu && t.counts), "%s: cu and counts are for tokens laid out in different ways", who);
-    DC_REQUIRE(t.max_new < kMostRows && (int64_t)t.n_b * t.max_new < (1ll << 31), "%s: too many tokens", who);
+    DC_REQUIRE(t.max_new < kMostRows && (t.cu || (int64_t)t.n_b * t.max_new < (1ll << 31)), "%s: too many tokens", who);
     if (written) {
         // a page's heads, and all pages of a head, each with its rows alone
         const int64_t rows = (int64_t)s.page * hd;

@@ -225,7 +225,7 @@ __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows
     if (a.at_once) {
         const int x = (int)(blockIdx.x / (unsigned)a.n_h);
         const DcItem d = dc_deal<STEP, false>(a, x, lane);
-        if (d.parts == 0) return;
+        if (d.part >= d.parts) return;
         b = d.b, h = (int)(blockIdx.x % (unsigned)a.n_h), part_ = d.part, parts = d.parts, slot = d.slot + (int64_t)part_ * a.n_h + h;
     }
     const DcSpan span = dc_span(a.t, b);

@@ -12,7 +12,7 @@ tokens at a time:
     seq_len / seq_len_gpu, advance_host_step
     reserve, share_prefix, free
 
-With ``inv_freq`` the cache rotates keys and queries by their positions on their way (``base.py:122-132``), so a model hands them over as its
+With ``inv_freq`` the cache rotates keys and queries by their positions on their way (``base.py:121-125``), so a model hands them over as its
 projections leave them.
 
 ``lens`` (int32, on the device) holds the lengths of the sequences and ``table`` their pages, the same for all layers.  A captured
@@ -68,7 +68,9 @@ class PagedCache:
         self._workspace = torch.empty(
             (hip.paged_attn_workspace_bytes(batch_size, num_kv_heads, num_q_heads // num_kv_heads, head_dim, max_length),),
             dtype=torch.uint8, device=self.device)
-        self._q = self._attn_out = None
+        # (made here: one that a captured step made would be the graph's)
+        self._attn_out = torch.empty((batch_size, num_q_heads, head_dim), device=self.device, dtype=torch.bfloat16)
+        self._q = torch.empty_like(self._attn_out) if self.rotates else None
 
     @property
     def rotates(self) -> bool:
@@ -188,8 +190,15 @@ class PagedCache:
         # pages that others hold too stay theirs
         dropped = [i for i, p in enumerate(self._pages) if any(self._holders[x] > 1 for x in p)]
         need = [max((n + self.page_size - 1) // self.page_size - (0 if i in dropped else len(self._pages[i])), 0) for i, n in enumerate(at)]
+        before = [list(p) for p in self._pages], list(self._holders), list(self._free)
         self._hand_out(need, dropped)
-        self._append(layer_idx, key_states, value_states, None, counts, None, None, pos)
+        try:
+            self._append(layer_idx, key_states, value_states, None, counts, None, None, pos)
+        except Exception:
+            if dropped:    # the pages that were given back hold rows yet
+                self._pages, self._holders, self._free = before
+                self._upload()
+            raise
         # only now: a call that was refused leaves the lengths of what the cache holds
         if counts is None:
             self.lens.fill_(seq)
@@ -248,11 +257,7 @@ class PagedCache:
         sequences grow by one after the last layer."""
         b, hq, h, hd = self.batch_size, self.num_q_heads, self.num_kv_heads, self.head_dim
         if out is None:
-            if self._attn_out is None:
-                self._attn_out = torch.empty((b, hq, hd), device=self.device, dtype=torch.bfloat16)
             out = self._attn_out
-        if self.rotates and self._q is None:
-            self._q = torch.empty((b, hq, hd), device=self.device, dtype=torch.bfloat16)
         return self._attend(layer_idx, queries.reshape(b, hq, hd), key_states.reshape(b, h, hd), value_states.reshape(b, h, hd),
                             [1] * b, None, out, lse, pos, self._workspace, self._q)
 

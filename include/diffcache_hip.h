@@ -759,7 +759,7 @@ typedef struct dc_paged_tokens {
  *   n_axes, section  1, or up to 4: the first section[0] frequencies go by a token's first position, the next section[1] by its
  *            second, and so on (time, height and width of images and video); the sections' sum is rot / 2
  * (x_a, x_b) becomes (x_a cos - x_b sin, x_b cos + x_a sin) in fp32, rounded once.  start is not changed.  Stands beside dc_append_kv_bf16
- * and the rotation of the reference's layers (base.py:122-132).
+ * and the rotation of the reference's layers (base.py:121-125).
  */
 typedef struct dc_paged_append_args {
     const void *k_src, *v_src, *q_src;

@@ -56,6 +56,9 @@ def test_lengths_that_are_none(new):
     none = hip.paged_attn(q[:0], k, v, table[:0], i32([]))
     assert none.shape == (0, new, h * group, hd)
     assert hip.paged_attn(q[:, :0], k, v, table, i32(starts)).numel() == 0
+    empty, cu = q.flatten(0, 1)[:0], i32([0] * 5)
+    assert hip.paged_attn(empty, k, v, table, i32(starts), cu=cu, max_new=7).shape == (0, h * group, hd)
+    assert hip.paged_append(k, v, table, empty[:, :h], empty[:, :h], i32(starts), cu=cu, max_new=7) is None
 
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])

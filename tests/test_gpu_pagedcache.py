@@ -202,6 +202,27 @@ def test_a_prompt_of_one_sequence_leaves_shared_pages_alone():
     assert not set(cache._pages[0]) & set(cache._pages[1]) and kept != cache._pages[0]
 
 
+def test_a_refused_prompt_leaves_shared_pages_where_they_were():
+    from diffcache_amd import _hip as hip
+    cache = make(1, 2, 64, 1, 2, 64, page_size=16)
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    k, v = bf((2, 40, 1, 64), gen), bf((2, 40, 1, 64), gen)
+    cache.prefill_update_kv_cache(k, v, 0, lens=[40, 0])
+    cache.share_prefix(1, 0, 32)
+    rows, table, free = cache.get_kvcache(0), cache.table.clone(), sorted(cache._free)
+    for bad in (lambda: cache.prefill_update_kv_cache(k.float(), v.float(), 0), lambda: cache.prefill_update_kv_cache(k, v, 0, pos=torch.zeros((2, 40), device=DEV)),
+                lambda: cache.prefill_update_kv_cache(k.cpu(), v.cpu(), 0)):
+        with pytest.raises(hip.DiffCacheError):
+            bad()
+        assert torch.equal(cache.table, table) and sorted(cache._free) == free and cache.lens.tolist() == [40, 32] and cache._lens == [40, 32]
+        assert all(torch.equal(a, b) for a, b in zip(cache.get_kvcache(0), rows))
+    q = bf((2, 2, 64), gen)
+    for bad in (lambda: cache.decode_attention(0, q.float(), k[:, :1], v[:, :1]), lambda: cache.decode_attention(0, q, k[:, :1].float(), v[:, :1])):
+        with pytest.raises(hip.DiffCacheError):
+            bad()
+        assert cache.lens.tolist() == [40, 32] and cache._lens == [40, 32]
+
+
 def test_a_copied_cache_has_memory_of_its_own():
     cache = make(1, 1, 64, 1, 2, 64, page_size=16)
     gen = torch.Generator(device=DEV).manual_seed(4)

@@ -164,6 +164,8 @@ def test_wrappers_refuse_what_does_not_fit(monkeypatch):
     no("one shape", append(pool, bf(4, 2, 32, 64), table, k, k))
     no("one shape", append(pool.float(), pool.float(), table, k, k))
     no("one after another", append(pool.transpose(1, 2), pool.transpose(1, 2), table, bf(3, 16, 64), bf(3, 16, 64)))
+    no("head_dim 32", append(bf(4, 2, 16, 32), bf(4, 2, 16, 32), table, bf(3, 2, 32), bf(3, 2, 32)))
+    no("head_dim 4", attn(bf(3, 4, 4), bf(4, 2, 16, 4), bf(4, 2, 16, 4), table))
     no("needs a page", append(pool[:0], pool[:0], table, k, k))
     no("int32 tensor", append(pool, pool, table.long(), k, k))
     no("int32 tensor", append(pool, pool, table[0], k, k))
