@@ -13,20 +13,24 @@
 // 1.7e-3 is the output's alone).  Softmax in powers of two, fp32; the maximum moves where a
 // logit passes it by more than 8.
 //
-// What bounds it: the matrix and the vector unit one after the other.  2048 tokens of 32 heads x 128 behind 30553 rows: 1060 us warm, 1086 with inputs in
-// turn = 976 TFLOP/s (a large library product: 1160); the matrix unit works in 43 % of the cycles, the vector unit (half of it the exponentials) in
-// 39 %, LDS reads in 22 % without a conflict; two waves to a SIMD leave little of that side by side.  A prompt of 8195 tokens 568-645 us = 850-970 TFLOP/s; 1024
-// tokens at 256 columns 1030-1110 us = 970-1040; at 64 columns, where a row has half the products for the same exponentials, 330-360 us for 224 GFLOP =
-// 620-680.  One step takes some 1.1 us where a CU has one block, 2.1 where it has two; a prompt of 517 tokens (nine steps) 20 us.
+// What bounds it: the power that the products take, and the matrix and the vector unit side by side only in part.  2048 tokens of 32 heads x 128
+// behind 30553 rows: 1017-1066 us = 990-1040 TFLOP/s, by the card (a large library product: 1160); on Q, K and V of one value, where the clock
+// stays up, 881 us.  A prompt of 8195 tokens 551-581 us = 950-1000 TFLOP/s; 1024 tokens at 256 columns 1060-1095 us = 980-1020; at 64 columns,
+// where a row has half the products for the same exponentials, 325-330 us for 224 GFLOP = 690.  A prompt of 517 tokens (nine steps) 19 us.
 // Kept: K and V straight to LDS instead of through registers (1163 -> 1060), page ids a step ahead and masks without branches (1348 -> 1163), at 256
-// columns two blocks to a CU (1781 -> 1068).  Tried and dropped: wave priorities (the same), three blocks of 32-row steps to a CU at 128
-// columns (1293 for 1116), a zero operand kept for the first product (1222 for 1172).
+// columns two blocks to a CU (1781 -> 1068); a wave that is at S ahead of the one it shares its SIMD with, so that the two do not stand at the same unit at once
+// (1125 -> 1073 on one card), and K read from LDS three products ahead at 128 columns (1026 -> 1017 on another).  At 64 columns it stays ahead to the step's
+// end (337 -> 328), which is slower at 128 (1017 -> 1035).
+// Tried and dropped: S of a step beside the exponentials of the one before (1105 -> 1145, and slower on equal values too), the weights' products ahead as well
+// (1073 -> 1149), blocks started half a step apart (the same), three blocks of 32-row steps to a CU at 128 columns (1293 for 1116), a zero operand kept for
+// the first product (1222 for 1172).
 #include "dc_paged.h"
 
 namespace {
 
 constexpr int kThreads = 256, kRowsOfWave = 32;
 constexpr int kLoaded = 0x0f70;  // s_waitcnt vmcnt(0)
+constexpr int kMatrix = 0x008, kLdsRead = 0x100;  // (kinds of instruction, to the scheduler)
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) uint32_t lds_u32;
@@ -171,6 +175,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
         // rows that the wave has no use for: behind all its pairs, or between the sinks and all windows
         const bool use = live && row0 <= p_hi && (a.window == 0 || row0 + KT - 1 > p_lo - a.window || row0 < a.n_sink);
         if (use) {
+            __builtin_amdgcn_s_setprio(1);  // (among waves of the SIMD)
             // S^T: x[t][i] is row 32 t + 8 (i / 4) + 4 half + i % 4
             dc_f32x16 x[ST];
             const uint8_t *ks = k_now + (lane & 31) * T::ROW;
@@ -188,6 +193,15 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                     x[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, qw), x[t], 0, 0, 0);
                 }
             }
+            if constexpr (HD == 128) {  // K's reads three products' ahead
+                __builtin_amdgcn_sched_group_barrier(kLdsRead, 6, 0);
+#pragma unroll
+                for (int j = 0; j < KS; ++j) {
+                    __builtin_amdgcn_sched_group_barrier(kMatrix, 2, 0);
+                    __builtin_amdgcn_sched_group_barrier(kLdsRead, 2, 0);
+                }
+            }
+            if constexpr (HD > 64) __builtin_amdgcn_s_setprio(0);
             if (have != (1 << TILES) - 1 || !dc_whole(a, p_lo, p_hi, row0, KT)) {
                 const DcReach reach = dc_reach(a, p);
 #pragma unroll
@@ -264,6 +278,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                 }
             }
         }
+        if constexpr (HD == 64) __builtin_amdgcn_s_setprio(0);
         if (s + 1 < end) stage(v_next, buf ^ 1, s + 1, next);
         have = next;
         __syncthreads();
