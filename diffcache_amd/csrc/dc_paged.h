@@ -117,14 +117,17 @@ __device__ __forceinline__ DcSteps dc_steps(const DcPagedAttn &a, int p_lo, int 
 //
 // Sequences differ in length, and the host does not know by how much: with as many blocks to each, the longest one's end last (8 x 131072
 // rows of 8 heads x 128 attended to by one token 625 us; one such sequence and seven of 8192 would take as long).  So the blocks count the steps of all
-// sequences themselves, divide them by the blocks that run at once, and cut every tile of a sequence's pairs into as many parts as come nearest to
-// that.  Block x of the grid takes item x / n_h of KV head x % n_h; the items are those of sequence 0, then those of sequence 1, ...; a sequence
+// sequences themselves, divide them by the blocks that run at once, and cut every tile of a sequence's pairs by that: to the nearest number of parts, or
+// rounded up with a share so large that all items run at once, if up to a fifth more does for that; or else, of tiles, that they run in two rounds.
+// To the nearest alone a last few blocks often run by themselves (up to 512 tokens of 4 sequences of up to 32601 rows, 8 heads x 128: 528 items
+// for 512 places took 712 us, 984 take 508; 1021 tokens of 5 sequences, 4 heads x 64: 319 and 262; a token of 7 sequences of 32601 rows 176
+// and 154).  Block x of the grid takes item x / n_h of KV head x % n_h; the items are those of sequence 0, then those of sequence 1, ...; a sequence
 // has for each of its tiles the parts of its last one, which has the most steps (others may leave some of them empty).  A part's results stand in
 // the workspace at the item's own place; a tile of one part goes to the outputs at once.
 //
-// A part has at least half of steps / at_once steps or is a tile's only one, and a sequence's tiles have at most twice the steps that the mean
-// of its first and last suggests: there are never more items than 2 at_once / n_h and one for each tile (at_once / n_h and one for each sequence
-// where those have one tile).
+// Rounded to the nearest, a part has at least half of steps / at_once steps or is a tile's only one, and a sequence's tiles have at most twice the steps
+// that the mean of its first and last suggests: there are never more items than 2 at_once / n_h and one for each tile (at_once / n_h and one for each
+// sequence where those have one tile); rounded up, the items are counted first.
 struct DcItem {
     int b, tile, part, parts;  // parts of this tile; 0: nothing to do
     int64_t slot;              // of part 0; the next part is n_h slots on
@@ -166,29 +169,28 @@ __device__ __forceinline__ DcTiles dc_tiles_of(const DcPagedAttn &a, const DcSpa
     const int hi = (int)((unsigned)((a.tile_rows < pairs ? a.tile_rows : pairs) - 1) / (unsigned)a.group), lo = (int)((unsigned)((tiles - 1) * a.tile_rows) / (unsigned)a.group);
     return {tiles, dc_steps<STEP>(a, s.start, s.start + hi).steps, dc_steps<STEP>(a, s.start + lo, s.start + s.count - 1).steps};
 }
-// steps / per to the nearest number, 1 at least.  (In fp32: what it loses, 1e-7 of the number, is little beside the 1e-4 below.)
-__device__ __forceinline__ int dc_parts_of(int steps, float by) {
-    const int n = (int)fmaf((float)steps, by, 0.5f);
-    return n > 1 ? n : 1;
-}
-// 1 / the steps of a part, for the work of all sequences
-__device__ __forceinline__ float dc_per(const DcPagedAttn &a, float work) {
-    const float even = work * (float)a.n_h * a.of_all;  // (of_all is 1.0001 / at_once)
-    return __builtin_amdgcn_rcpf(even > (float)a.least ? even : (float)a.least);
-}
+// A tile's parts: its steps times by (1 / those of a part), up added and the fraction dropped, 1 at least.  (In fp32: what it loses, 1e-7 of the
+// number, is little beside the 1e-4 below.)
+struct DcParts {
+    float by, up;
+    __device__ __forceinline__ int of(int steps) const {
+        const int n = (int)fmaf((float)steps, by, up);
+        return n > 1 ? n : 1;
+    }
+};
 
 // Item x, or with OF_SEQUENCE the first one of sequence x (x is the same in the whole wave, all of whose lanes are here).
 template <int STEP, bool TILED, bool OF_SEQUENCE = false>
 __device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane) {
     DcItem d = {0, 0, 0, 0, 0};
-    float by = 0.f;
+    DcParts cut = {0.f, 0.5f};
     // x is item `in` of sequence b, whose first is at; its last tile has `most` parts
     auto found = [&](const DcSpan &s, int b, int at, int in, int tiles, int most) __attribute__((always_inline)) {
         d.b = b;
         if constexpr (TILED) {
             d.tile = tiles - 1 - (int)((unsigned)in / (unsigned)most), d.part = (int)((unsigned)in % (unsigned)most);  // (late tokens first: they have the most rows)
             const int pairs = s.count * a.group, lo = d.tile * a.tile_rows, hi = (lo + a.tile_rows < pairs ? lo + a.tile_rows : pairs) - 1;
-            const int own = dc_parts_of(dc_steps<STEP>(a, s.start + (int)((unsigned)lo / (unsigned)a.group), s.start + (int)((unsigned)hi / (unsigned)a.group)).steps, by);
+            const int own = cut.of(dc_steps<STEP>(a, s.start + (int)((unsigned)lo / (unsigned)a.group), s.start + (int)((unsigned)hi / (unsigned)a.group)).steps);
             d.parts = own < most ? own : most;
         } else {
             d.part = in, d.parts = most;
@@ -196,11 +198,26 @@ __device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane)
         if (at + in - d.part + most > a.items) d.parts = 1;  // (never, but for numbers of tokens that say more than there are)
         d.slot = (int64_t)(at + in - d.part) * a.n_h;
     };
+    // How the tiles are cut, for the work of all sequences.  Each lane counts the items of a share of its own: lanes 0 .. 31 one part's work for
+    // each block that runs at once and up to a fifth more, the others half of it and up to all of it (the first that fits is the least).  Where the
+    // least part is what counts, and of sequences so many that it all evens out or that counting takes longer than it saves (60 sequences of one tile: 697 us
+    // and 706), the nearest number.
+    auto plan = [&](float work, auto &&each) __attribute__((always_inline)) {
+        const float even = work * (float)a.n_h * a.of_all, least = (float)a.least;  // (of_all is 1.0001 / at_once)
+        cut.by = __builtin_amdgcn_rcpf(even > least ? even : least);
+        if (!(even > least) || a.n_b > (TILED ? 64 : 16)) return;
+        const float base = lane < 32 ? even : fmaxf(0.5f * even, least), rise = lane < 32 ? 0.2f / 32 : 1.f / 32;
+        const DcParts mine = {__builtin_amdgcn_rcpf(fmaf(base * rise, (float)(lane & 31), base)), 0.999f};
+        float n = 0.f;
+        each([&](float tiles, float last) __attribute__((always_inline)) { n = fmaf(tiles, fmaxf(floorf(fmaf(last, mine.by, mine.up)), 1.f), n); });
+        const uint64_t fits = __ballot(n * (float)a.n_h <= (float)(lane < 32 ? a.at_once : TILED ? 2 * a.at_once : 0));
+        if (fits) cut = {dc_of_lane(mine.by, __builtin_ctzll(fits)), 0.999f};
+    };
     if (a.n_b == 1) {
         const DcSpan s = dc_span(a.t, 0);
         const DcTiles t = dc_tiles_of<STEP, TILED>(a, s);
-        by = dc_per(a, 0.5f * (float)t.tiles * (float)(t.first + t.last));
-        const int most = dc_parts_of(t.last, by);
+        plan(0.5f * (float)t.tiles * (float)(t.first + t.last), [&](auto &&f) { f((float)t.tiles, (float)t.last); });
+        const int most = cut.of(t.last);
         if (x < t.tiles * most) found(s, 0, 0, x, t.tiles, most);
         return d;
     }
@@ -214,11 +231,15 @@ __device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane)
         const DcTiles t = b0 == 0 ? mine : tiles_of(b0 + lane);
         work += dc_of_lane(dc_lane_sums(0.5f * (float)t.tiles * (float)(t.first + t.last)), 63);
     }
-    by = dc_per(a, work);
+    const float tiles_f = (float)mine.tiles, last_f = (float)mine.last;
+    plan(work, [&](auto &&f) {
+#pragma unroll 4
+        for (int b = 0; b < a.n_b; ++b) f(dc_of_lane(tiles_f, b), dc_of_lane(last_f, b));
+    });
     int base = 0;
     for (int b0 = 0; b0 < a.n_b; b0 += 64) {
         const DcTiles t = b0 == 0 ? mine : tiles_of(b0 + lane);
-        const int parts = dc_parts_of(t.last, by), items = t.tiles * parts, upto = dc_lane_sums(items);
+        const int parts = cut.of(t.last), items = t.tiles * parts, upto = dc_lane_sums(items);
         const uint64_t past = OF_SEQUENCE ? (x < b0 + 64 ? 1ull << (x - b0) : 0) : __ballot(base + upto > x);
         if (past) {
             const int k = __builtin_ctzll(past), at = base + dc_of_lane(upto, k) - dc_of_lane(items, k);  // the sequence's first item

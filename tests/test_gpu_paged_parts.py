@@ -95,3 +95,24 @@ def test_a_long_and_many_short_sequences_take_little_more_than_their_rows():
     a = hip.paged_attn(q, k, v, table, i32([n - 1 for n in lengths]))
     one = hip.paged_attn(q[3:4], k, v, table[3:4], i32([3999]))
     assert ((a[3].double() - one[0].double()).abs() <= 2.0 ** -7 * one[0].double().abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("lengths,new,hd,h,group", [
+    ([5589] * 11, 37, 128, 4, 1),                                                          # 44 tiles: 11 parts each where 12 are nearer, 484 items for 512 places
+    ([1500, 1471, 1441, 1501, 1483] * 10, 20, 256, 6, 4),                                  # 300 tiles of a share and a half each: two parts, 600 items in two rounds
+    ([6000, 9000, 7000, 8000, 8500], 120, 128, 2, 4),                                      # four tiles of each sequence, cut differently
+    ([2100] * 66, 30, 256, 3, 4),                                                          # more sequences than lanes: the nearest number
+    ([4099] * 7, 1, 128, 8, 4), ([4099, 3000, 100, 4000, 3500], 1, 128, 8, 4),              # of one token: fewer parts than the nearest number, and as many
+    ([3600, 3000, 2500, 4000, 3500, 2800] * 3, 1, 128, 4, 4),                              # more than 16 sequences
+])
+def test_every_row_counts_once_however_tiles_are_cut(lengths, new, hd, h, group):
+    from diffcache_amd import _hip as hip
+    k, v, table, g = counted(len(lengths), h, hd, 64, lengths, 2)
+    q = torch.zeros((len(lengths), new, h * group, hd), dtype=torch.bfloat16, device=DEV)
+    out, lse = hip.paged_attn(q, k, v, table, i32([n - new for n in lengths]), want_lse=True)
+    for i, n in enumerate(lengths):
+        r = torch.arange(1, n + 1, device=DEV)[-new:, None]                                # rows of each token
+        share = ((r - torch.arange(hd, device=DEV) + hd - 1).div(hd, rounding_mode="floor").double() / r)[:, None]
+        # (the bounds as above, of counts that are exact in fp32)
+        assert ((out[i].double() - share).abs() <= 2.0 ** -8 * share * (1 + 2.0 ** -12)).all()
+        assert ((lse[i].double() - r.double().log()).abs() <= 1e-5).all()
