@@ -75,7 +75,8 @@ struct DcPagedAttn {
     int n_h, group, n_rows, n_sink, window;
     int n_b, waves;          // waves of a block (paged_attn.hip)
     int tiles, tile_rows;    // of a unit's (token, head) pairs: at most so many tiles of so many
-    int at_once, least, items;  // blocks that the GPU runs at once, the fewest steps of a part, and the items that there is room for; at_once 0: nothing is dealt out
+    int at_once, round;      // blocks that the GPU runs at once, and those of a KV head among them; at_once 0: nothing is dealt out
+    int least, places;       // the fewest steps of a part; the cut tiles' parts that there is room for
     float of_all;            // 1.0001 / at_once: a little more steps to a part than come of the division, so that rounding makes no more of them
     float scale;             // times log2(e)
 };
@@ -119,6 +120,7 @@ __device__ __forceinline__ DcSteps dc_steps(const DcPagedAttn &a, int p_lo, int 
 // rows of 8 heads x 128 attended to by one token 625 us; one such sequence and seven of 8192 would take as long).  So the blocks count the steps of all
 // sequences themselves, divide them by the blocks that run at once, and cut every tile of a sequence's pairs by that: to the nearest number of parts, or
 // rounded up with a share so large that all items run at once, if up to a fifth more does for that; or else, of tiles, that they run in two rounds.
+// Of more tiles than run at once, none much longer than a share, whole rounds stay uncut, and the rest is cut for one round more.
 // To the nearest alone a last few blocks often run by themselves (up to 512 tokens of 4 sequences of up to 32601 rows, 8 heads x 128: 528 items
 // for 512 places took 712 us, 984 take 508; 1021 tokens of 5 sequences, 4 heads x 64: 319 and 262; a token of 7 sequences of 32601 rows 176
 // and 154).  Block x of the grid takes item x / n_h of KV head x % n_h; the items are those of sequence 0, then those of sequence 1, ...; a sequence
@@ -173,9 +175,10 @@ __device__ __forceinline__ DcTiles dc_tiles_of(const DcPagedAttn &a, const DcSpa
 // number, is little beside the 1e-4 below.)
 struct DcParts {
     float by, up;
+    int most;
     __device__ __forceinline__ int of(int steps) const {
         const int n = (int)fmaf((float)steps, by, up);
-        return n > 1 ? n : 1;
+        return n <= 1 ? 1 : n < most ? n : most;
     }
 };
 
@@ -183,42 +186,74 @@ struct DcParts {
 template <int STEP, bool TILED, bool OF_SEQUENCE = false>
 __device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane) {
     DcItem d = {0, 0, 0, 0, 0};
-    DcParts cut = {0.f, 0.5f};
-    // x is item `in` of sequence b, whose first is at; its last tile has `most` parts
-    auto found = [&](const DcSpan &s, int b, int at, int in, int tiles, int most) __attribute__((always_inline)) {
+    DcParts cut = {0.f, 0.5f, INT32_MAX};
+    int whole = 0;  // so many tiles, from the first sequence's last tile on, are not cut
+    // x is item `in` of sequence b, whose first is at; `uncut` of its tiles are, and its last tile would have `most` parts
+    auto found = [&](const DcSpan &s, int b, int at, int in, int tiles, int uncut, int most) __attribute__((always_inline)) {
         d.b = b;
         if constexpr (TILED) {
-            d.tile = tiles - 1 - (int)((unsigned)in / (unsigned)most), d.part = (int)((unsigned)in % (unsigned)most);  // (late tokens first: they have the most rows)
+            // (late tokens first: they have the most rows)
+            if (in < uncut) {
+                d.tile = tiles - 1 - in, d.parts = 1;
+                return;
+            }
+            const unsigned of_cut = (unsigned)(in - uncut);
+            d.tile = tiles - uncut - 1 - (int)(of_cut / (unsigned)most), d.part = (int)(of_cut % (unsigned)most);
             const int pairs = s.count * a.group, lo = d.tile * a.tile_rows, hi = (lo + a.tile_rows < pairs ? lo + a.tile_rows : pairs) - 1;
             const int own = cut.of(dc_steps<STEP>(a, s.start + (int)((unsigned)lo / (unsigned)a.group), s.start + (int)((unsigned)hi / (unsigned)a.group)).steps);
             d.parts = own < most ? own : most;
         } else {
             d.part = in, d.parts = most;
         }
-        if (at + in - d.part + most > a.items) d.parts = 1;  // (never, but for numbers of tokens that say more than there are)
-        d.slot = (int64_t)(at + in - d.part) * a.n_h;
+        const int first = at + in - d.part - whole;  // (places of uncut tiles are not kept)
+        if (first + most > a.places) d.parts = 1;    // (never, but for numbers of tokens that say more than there are)
+        d.slot = (int64_t)first * a.n_h;
     };
-    // How the tiles are cut, for the work of all sequences.  Each lane counts the items of a share of its own: lanes 0 .. 31 one part's work for
-    // each block that runs at once and up to a fifth more, the others half of it and up to all of it (the first that fits is the least).  Where the
-    // least part is what counts, and of sequences so many that it all evens out or that counting takes longer than it saves (60 sequences of one tile: 697 us
-    // and 706), the nearest number.
+    // How the tiles are cut, for the work of all sequences.
     auto plan = [&](float work, auto &&each) __attribute__((always_inline)) {
         const float even = work * (float)a.n_h * a.of_all, least = (float)a.least;  // (of_all is 1.0001 / at_once)
         cut.by = __builtin_amdgcn_rcpf(even > least ? even : least);
+        // (a part's least steps are what counts, or so many sequences that it all evens out and counting takes longer than it saves: 60 of one
+        // tile 697 us and 706)
         if (!(even > least) || a.n_b > (TILED ? 64 : 16)) return;
+        // Each lane counts the items of a share of its own: lanes 0 .. 31 one part's work for each block that runs at once and up to a fifth
+        // more, the others half of it and up to all of it.
         const float base = lane < 32 ? even : fmaxf(0.5f * even, least), rise = lane < 32 ? 0.2f / 32 : 1.f / 32;
-        const DcParts mine = {__builtin_amdgcn_rcpf(fmaf(base * rise, (float)(lane & 31), base)), 0.999f};
-        float n = 0.f;
-        each([&](float tiles, float last) __attribute__((always_inline)) { n = fmaf(tiles, fmaxf(floorf(fmaf(last, mine.by, mine.up)), 1.f), n); });
+        const DcParts mine = {__builtin_amdgcn_rcpf(fmaf(base * rise, (float)(lane & 31), base)), 0.999f, INT32_MAX};
+        float n = 0.f, all = 0.f, longest = 0.f;
+        each([&](float tiles, float last) __attribute__((always_inline)) {
+            n = fmaf(tiles, fmaxf(floorf(fmaf(last, mine.by, mine.up)), 1.f), n);
+            if constexpr (TILED) all += tiles, longest = fmaxf(longest, last);
+        });
+        if constexpr (TILED) {
+            const int tiles = (int)dc_of_lane(all, 0), over = tiles * a.n_h - a.at_once;
+            if (over > 0 && dc_of_lane(longest, 0) <= 1.3f * even) {
+                // whole rounds, and what is left cut for one more
+                const unsigned left = (unsigned)tiles % (unsigned)a.round;
+                const int parts = left ? (int)((unsigned)a.round / left) : 1;
+                if (parts > 1) whole = tiles - (int)left, cut = {__builtin_amdgcn_rcpf(least), 0.f, parts};
+                else whole = INT32_MAX;
+                return;
+            }
+            if (over > a.at_once) {
+                whole = INT32_MAX;
+                return;
+            }
+        }
         const uint64_t fits = __ballot(n * (float)a.n_h <= (float)(lane < 32 ? a.at_once : TILED ? 2 * a.at_once : 0));
-        if (fits) cut = {dc_of_lane(mine.by, __builtin_ctzll(fits)), 0.999f};
+        if (!fits) return;
+        const int k = __builtin_ctzll(fits);  // (the least share that does)
+        cut = {dc_of_lane(mine.by, k), 0.999f, INT32_MAX};
+        // (two rounds that are not shorter than the longest tile)
+        if constexpr (TILED)
+            if (k >= 32 && dc_of_lane(longest, 0) * cut.by < 2.1f) whole = INT32_MAX;
     };
     if (a.n_b == 1) {
         const DcSpan s = dc_span(a.t, 0);
         const DcTiles t = dc_tiles_of<STEP, TILED>(a, s);
         plan(0.5f * (float)t.tiles * (float)(t.first + t.last), [&](auto &&f) { f((float)t.tiles, (float)t.last); });
-        const int most = cut.of(t.last);
-        if (x < t.tiles * most) found(s, 0, 0, x, t.tiles, most);
+        const int most = cut.of(t.last), uncut = whole < t.tiles ? whole : t.tiles;
+        if (x < uncut + (t.tiles - uncut) * most) found(s, 0, 0, x, t.tiles, uncut, most);
         return d;
     }
     auto tiles_of = [&](int b) __attribute__((always_inline)) {
@@ -239,12 +274,18 @@ __device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane)
     int base = 0;
     for (int b0 = 0; b0 < a.n_b; b0 += 64) {
         const DcTiles t = b0 == 0 ? mine : tiles_of(b0 + lane);
-        const int parts = cut.of(t.last), items = t.tiles * parts, upto = dc_lane_sums(items);
+        const int parts = cut.of(t.last);
+        int uncut = whole == 0 ? 0 : t.tiles;
+        if (TILED && whole > 0 && whole < INT32_MAX) {  // (of 64 sequences at most)
+            uncut = whole - (dc_lane_sums(t.tiles) - t.tiles);
+            uncut = uncut < 0 ? 0 : uncut < t.tiles ? uncut : t.tiles;
+        }
+        const int items = uncut + (t.tiles - uncut) * parts, upto = dc_lane_sums(items);
         const uint64_t past = OF_SEQUENCE ? (x < b0 + 64 ? 1ull << (x - b0) : 0) : __ballot(base + upto > x);
         if (past) {
             const int k = __builtin_ctzll(past), at = base + dc_of_lane(upto, k) - dc_of_lane(items, k);  // the sequence's first item
             const int tiles = dc_of_lane(t.tiles, k);
-            if (tiles) found(dc_span(a.t, b0 + k), b0 + k, at, OF_SEQUENCE ? 0 : x - at, tiles, dc_of_lane(parts, k));
+            if (tiles) found(dc_span(a.t, b0 + k), b0 + k, at, OF_SEQUENCE ? 0 : x - at, tiles, dc_of_lane(uncut, k), dc_of_lane(parts, k));
             return d;
         }
         base += dc_of_lane(upto, 63);

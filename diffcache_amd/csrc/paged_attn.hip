@@ -429,7 +429,7 @@ constexpr int64_t kAlone = 768 * 128;
 struct Cut {
     bool chunk, deal, join;   // deal: blocks find their items; join: some may be parts
     int waves, tiles, tile_rows, at_once, least;
-    int64_t blocks;
+    int64_t blocks, places;   // places: of parts, in the workspace
 };
 // tokens: of all sequences together, where they are packed; else 0
 Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, int64_t tokens) {
@@ -448,18 +448,25 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
         // them in two parts of 16 steps 84).
         const int64_t steps = (rows + dc_chunk_step(hd) - 1) / dc_chunk_step(hd);
         c.least = all * n_h <= 128 ? 7 : 24;
-        c.join = all * n_h <= (n_b == 1 ? c.at_once / 2 : 2 * c.at_once) && 2 * steps >= 3 * c.least;
+        // Of more tiles than that, where tokens have rows before them and there are few rounds, the last round's are cut if they are at most half of
+        // what runs at once, or two thirds where they are all (dc_deal; 2048 tokens of 8 heads x 128 behind some 30000 rows, 512 tiles: 1036 us; 2100
+        // 1697 and 1081, 2600 1688 and 1340, 1100 873 and 658).  At 64 columns, four blocks to a CU, the others of a CU gain more by one that ends.
+        const bool few = all * n_h <= (n_b == 1 ? c.at_once / 2 : 2 * c.at_once);
+        const int64_t left = all * n_h % c.at_once, cut = all * n_h < c.at_once ? c.at_once * 2 / 3 : hd == 64 ? c.at_once * 3 / 10 : c.at_once / 2;
+        const bool tail = all * n_h <= 4 * c.at_once && n_b <= 64 && rows >= 2 * (int64_t)max_new && left > 0 && left <= cut;
+        c.join = (few || tail) && 2 * steps >= 3 * c.least;
         c.deal = c.join;
         if (c.tiles > all) c.tiles = (int)all;  // (one sequence of fewer packed tokens than max_new)
         if (!c.join && tokens && n_b > 1) all = places;
-        c.blocks = n_h * (all + (c.join ? 2 * c.at_once / n_h + 1 : 0));
+        const int64_t parts = c.join ? 2 * c.at_once / n_h + 1 : 0;
+        c.blocks = n_h * (all + parts), c.places = n_h * ((all < parts ? all : parts) + parts);
         return c;
     }
     c.tiles = 1, c.tile_rows = max_new * group, c.at_once = rows_at_once(hd), c.least = kWaves;
     const int64_t step = 16 * row_tiles(hd), steps = (rows + step - 1) / step;
     c.deal = c.join = steps * step * hd > kAlone && n_units <= 2 * c.at_once;
     c.waves = steps * step * hd > kAlone || steps <= kWaves ? kWaves : kMostWaves;
-    c.blocks = c.deal ? n_h * (n_b + c.at_once / n_h + 1) : n_units;
+    c.blocks = c.places = c.deal ? n_h * (n_b + c.at_once / n_h + 1) : n_units;
     return c;
 }
 size_t acc_bytes(int64_t slots, int rows, int hd) { return dc_align_up((size_t)slots * rows * hd * 4, 256); }
@@ -482,7 +489,7 @@ extern "C" size_t dc_paged_attn_workspace_bytes(int n_b, int n_h, int group, int
     const int64_t most = 2 * rows_at_once(hd) / n_h;
     const bool few = (int64_t)max_new * group <= kRows;
     const Cut c = cut_of(few && most > 0 && n_b > most ? most : n_b, n_h, group, hd, n_rows, max_new, n_tokens);
-    return c.join ? acc_bytes(c.blocks, c.tile_rows, hd) + ml_bytes(c.blocks, c.tile_rows) : 0;
+    return c.join ? acc_bytes(c.places, c.tile_rows, hd) + ml_bytes(c.places, c.tile_rows) : 0;
 }
 
 extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
@@ -507,7 +514,7 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     DcPagedAttn a;
     a.ws_acc = a.ws_ml = nullptr;
     if (c.join) {
-        const size_t acc = acc_bytes(c.blocks, c.tile_rows, x->hd), need = acc + ml_bytes(c.blocks, c.tile_rows);
+        const size_t acc = acc_bytes(c.places, c.tile_rows, x->hd), need = acc + ml_bytes(c.places, c.tile_rows);
         DC_REQUIRE(x->workspace && ((uintptr_t)x->workspace & 255u) == 0, "%s: workspace must be non-null and 256-byte aligned", who);
         if (x->workspace_bytes < need) {
             dc_set_error("%s: workspace %zu bytes < %zu needed", who, x->workspace_bytes, need);
@@ -520,7 +527,7 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     a.qs = {x->q_batch_stride, x->q_token_stride, x->q_head_stride};
     a.n_h = x->n_h, a.group = x->group, a.n_rows = x->n_rows, a.n_sink = x->n_sink, a.window = x->window;
     a.n_b = t.n_b, a.waves = c.waves, a.tiles = c.tiles, a.tile_rows = c.tile_rows;
-    a.at_once = c.deal ? c.at_once : 0, a.least = c.least, a.items = (int)(c.blocks / x->n_h), a.of_all = 1.0001f / (float)c.at_once;
+    a.at_once = c.deal ? c.at_once : 0, a.round = c.at_once > x->n_h ? c.at_once / x->n_h : 1, a.least = c.least, a.places = (int)(c.places / x->n_h), a.of_all = 1.0001f / (float)c.at_once;
     a.scale = x->scale * 1.44269504088896341f;
     hipStream_t st = (hipStream_t)stream;
     if (c.chunk) return dc_paged_chunk_launch(a, x->hd, (unsigned)c.blocks, c.join, st);

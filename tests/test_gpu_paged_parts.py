@@ -104,6 +104,11 @@ def test_a_long_and_many_short_sequences_take_little_more_than_their_rows():
     ([2100] * 66, 30, 256, 3, 4),                                                          # more sequences than lanes: the nearest number
     ([4099] * 7, 1, 128, 8, 4), ([4099, 3000, 100, 4000, 3500], 1, 128, 8, 4),              # of one token: fewer parts than the nearest number, and as many
     ([3600, 3000, 2500, 4000, 3500, 2800] * 3, 1, 128, 4, 4),                              # more than 16 sequences
+    ([2900], 1100, 256, 8, 8),                                                             # 552 tiles for 512 places: 512 whole, 40 cut
+    ([3000, 2900, 2950, 2800, 2990], 1000, 256, 4, 4),                                     # 640 of five sequences: the last one's all, and none of the others'
+    ([3000, 2900, 2950, 2800, 2990], 900, 256, 4, 4),                                      # 580: some of the last one's
+    ([700] * 8 + [5000], 240, 256, 8, 8),                                                  # 1080, one sequence's much longer: none cut
+    ([2000] * 10, 160, 256, 8, 4),                                                         # 400: two rounds would be no shorter than one
 ])
 def test_every_row_counts_once_however_tiles_are_cut(lengths, new, hd, h, group):
     from diffcache_amd import _hip as hip
