@@ -319,8 +319,8 @@ __device__ __forceinline__ int dc_page_id(const DcPages &p, const int32_t *table
     return (unsigned)id < (unsigned)p.n_pages ? id : -1;
 }
 
-// paged_chunk.hip
-int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, unsigned blocks, bool join, hipStream_t st);
+// paged_chunk.hip; join: 0, or the y of the join's grid
+int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, unsigned blocks, unsigned join, hipStream_t st);
 // Rows of a step; blocks that run at once.
 constexpr int dc_chunk_step(int hd) { return hd == 256 ? 32 : 64; }
 constexpr int dc_chunk_at_once(int hd) { return hd == 64 ? 1024 : hd == 128 ? 512 : 512; }

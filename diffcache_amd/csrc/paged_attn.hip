@@ -324,31 +324,38 @@ __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows
     if (lane < kRows) s_m[wave * kRows + lane] = w.m, s_l[wave * kRows + lane] = l;
     w.finish(s_acc + wave * pairs * HD, pairs);
     __syncthreads();
-    for (int o = tid; o < pairs * HD; o += waves * 64) {
-        const int r = o / HD;
+    constexpr int kLanes = HD / 4;
+    for (int o = tid; o < pairs * kLanes; o += waves * 64) {
+        const int r = o / kLanes, column = 4 * (o % kLanes);
         // (without a branch to a wave: the first one again in the place of those that a block of four does not have)
-        float m[kMostWaves], ls[kMostWaves], part[kMostWaves];
+        float m[kMostWaves], ls[kMostWaves];
+        float4 part[kMostWaves];
 #pragma unroll
         for (int i = 0; i < kMostWaves; ++i) {
             const int x = i < waves ? i : 0;
-            m[i] = s_m[x * kRows + r], ls[i] = s_l[x * kRows + r], part[i] = s_acc[x * pairs * HD + o];
+            m[i] = s_m[x * kRows + r], ls[i] = s_l[x * kRows + r], part[i] = reinterpret_cast<const float4 *>(s_acc)[x * pairs * kLanes + o];
         }
         float top = m[0];
 #pragma unroll
         for (int i = 1; i < kMostWaves; ++i) top = fmaxf(top, m[i]);
-        float sum = 0.f, total = 0.f;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        float total = 0.f;
 #pragma unroll
         for (int i = 0; i < kMostWaves; ++i) {
-            sum = fmaf(i < waves ? dc_weight(m[i], top) : 0.f, i < waves ? part[i] : 0.f, sum);
-            total += i < waves ? dc_share(m[i], ls[i], top) : 0.f;
+            const bool is = i < waves;
+            const float f = is ? dc_weight(m[i], top) : 0.f;
+            sum.x = fmaf(f, is ? part[i].x : 0.f, sum.x), sum.y = fmaf(f, is ? part[i].y : 0.f, sum.y);
+            sum.z = fmaf(f, is ? part[i].z : 0.f, sum.z), sum.w = fmaf(f, is ? part[i].w : 0.f, sum.w);
+            total += is ? dc_share(m[i], ls[i], top) : 0.f;
         }
         if (parts > 1) {
-            a.ws_acc[(slot * a.tile_rows + r) * HD + o % HD] = sum;
-            if (o % HD == 0) reinterpret_cast<float2 *>(a.ws_ml)[slot * a.tile_rows + r] = make_float2(top, total);
+            *reinterpret_cast<float4 *>(a.ws_acc + (slot * a.tile_rows + r) * HD + column) = sum;
+            if (column == 0) reinterpret_cast<float2 *>(a.ws_ml)[slot * a.tile_rows + r] = make_float2(top, total);
         } else {
             const int64_t dst = (int64_t)(span.first + r / G) * a.n_h * G + h * G + r % G;
-            a.out[dst * HD + o % HD] = dc_f32_to_bf16(sum / (total == 0.f ? 1.f : total));
-            if (a.lse && o % HD == 0) a.lse[dst] = dc_log_sum(top, total);
+            const float by = total == 0.f ? 1.f : total;
+            *reinterpret_cast<uint2 *>(a.out + dst * HD + column) = make_uint2(dc_pack_bf16(sum.x / by, sum.y / by), dc_pack_bf16(sum.z / by, sum.w / by));
+            if (a.lse && column == 0) a.lse[dst] = dc_log_sum(top, total);
         }
     }
 }
@@ -429,6 +436,7 @@ constexpr int64_t kAlone = 768 * 128;
 struct Cut {
     bool chunk, deal, join;   // deal: blocks find their items; join: some may be parts
     int waves, tiles, tile_rows, at_once, least;
+    unsigned sharers;         // blocks of the chunks' join to each part
     int64_t blocks, places;   // places: of parts, in the workspace
 };
 // tokens: of all sequences together, where they are packed; else 0
@@ -458,15 +466,19 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
         c.deal = c.join;
         if (c.tiles > all) c.tiles = (int)all;  // (one sequence of fewer packed tokens than max_new)
         if (!c.join && tokens && n_b > 1) all = places;
-        const int64_t parts = c.join ? 2 * c.at_once / n_h + 1 : 0;
-        c.blocks = n_h * (all + parts), c.places = n_h * ((all < parts ? all : parts) + parts);
+        // (items: see dc_deal; and no tile has more parts than its steps allow.  A thousand blocks that find none cost 1-2 us in each kernel)
+        const int64_t parts = c.join ? 2 * c.at_once / n_h + 1 : 0, most = all * (c.join ? steps / c.least + 1 : 1);
+        c.blocks = n_h * (all + parts < most ? all + parts : most), c.places = n_h * ((all < parts ? all : parts) + parts);
+        if (c.places > c.blocks) c.places = c.blocks;
+        c.sharers = c.blocks <= 128 ? 4 : c.blocks <= 256 ? 2 : 1;  // (38 tokens of 12 units over 1575 rows of 256 columns, 96 blocks: 36 us, four times as many to join 31)
         return c;
     }
     c.tiles = 1, c.tile_rows = max_new * group, c.at_once = rows_at_once(hd), c.least = kWaves;
     const int64_t step = 16 * row_tiles(hd), steps = (rows + step - 1) / step;
     c.deal = c.join = steps * step * hd > kAlone && n_units <= 2 * c.at_once;
     c.waves = steps * step * hd > kAlone || steps <= kWaves ? kWaves : kMostWaves;
-    c.blocks = c.places = c.deal ? n_h * (n_b + c.at_once / n_h + 1) : n_units;
+    const int64_t items = n_b + c.at_once / n_h + 1, most = n_b * (steps / c.least + 1);
+    c.blocks = c.places = c.deal ? n_h * (items < most ? items : most) : n_units;
     return c;
 }
 size_t acc_bytes(int64_t slots, int rows, int hd) { return dc_align_up((size_t)slots * rows * hd * 4, 256); }
@@ -530,7 +542,7 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     a.at_once = c.deal ? c.at_once : 0, a.round = c.at_once > x->n_h ? c.at_once / x->n_h : 1, a.least = c.least, a.places = (int)(c.places / x->n_h), a.of_all = 1.0001f / (float)c.at_once;
     a.scale = x->scale * 1.44269504088896341f;
     hipStream_t st = (hipStream_t)stream;
-    if (c.chunk) return dc_paged_chunk_launch(a, x->hd, (unsigned)c.blocks, c.join, st);
+    if (c.chunk) return dc_paged_chunk_launch(a, x->hd, (unsigned)c.blocks, c.join ? c.sharers : 0, st);
     if (x->hd == 64) launch_rows<64>(a, c, st);
     else if (x->hd == 128) launch_rows<128>(a, c, st);
     else launch_rows<256>(a, c, st);

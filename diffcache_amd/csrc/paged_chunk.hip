@@ -315,8 +315,8 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
     if (a.lse && half_ == 0) a.lse[dst] = dc_log_sum(m, l);
 }
 
-// The parts of a tile joined: its blocks share its rows, every parts-th of them each, HD / 4 threads to a row, four parts asked for at
-// once.
+// The parts of a tile joined: as many blocks as it has parts, times the grid's y, share its rows, every so many-th of them each, HD / 4 threads to a row, four
+// parts asked for at once.
 template <int HD, int KT>
 __global__ __launch_bounds__(kThreads) void paged_chunk_join_kernel(DcPagedAttn a) {
     constexpr int kLanes = HD / 4, kPer = kThreads / kLanes, kBatch = 4;
@@ -325,8 +325,9 @@ __global__ __launch_bounds__(kThreads) void paged_chunk_join_kernel(DcPagedAttn 
     if (d.parts < 2 || d.part >= d.parts) return;
     const DcSpan span = dc_span(a.t, d.b);
     const int n = d.parts, pair0 = d.tile * kChunkRows, left = span.count * G - pair0, rows = left < kChunkRows ? left : kChunkRows;
+    const int sharers = n * (int)gridDim.y;
     const int64_t step = (int64_t)a.n_h * kChunkRows;
-    for (int r = d.part + tid / kLanes * n; r < rows; r += kPer * n) {
+    for (int r = d.part + n * (int)blockIdx.y + tid / kLanes * sharers; r < rows; r += kPer * sharers) {
         const int64_t slot0 = (d.slot + h) * kChunkRows + r;
         const float2 *ml = reinterpret_cast<const float2 *>(a.ws_ml) + slot0;
         const float4 *pa = reinterpret_cast<const float4 *>(a.ws_acc) + slot0 * kLanes + c;
@@ -366,15 +367,15 @@ __global__ __launch_bounds__(kThreads) void paged_chunk_join_kernel(DcPagedAttn 
 }
 
 template <int HD>
-void launch(const DcPagedAttn &a, unsigned blocks, bool join, hipStream_t st) {
+void launch(const DcPagedAttn &a, unsigned blocks, unsigned join, hipStream_t st) {
     constexpr int KT = dc_chunk_step(HD);
     hipLaunchKernelGGL((paged_chunk_kernel<HD, KT>), dim3(blocks), dim3(kThreads), 0, st, a);
-    if (join) hipLaunchKernelGGL((paged_chunk_join_kernel<HD, KT>), dim3(blocks), dim3(kThreads), 0, st, a);
+    if (join) hipLaunchKernelGGL((paged_chunk_join_kernel<HD, KT>), dim3(blocks, join), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace
 
-int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, unsigned blocks, bool join, hipStream_t st) {
+int dc_paged_chunk_launch(const DcPagedAttn &a, int hd, unsigned blocks, unsigned join, hipStream_t st) {
     if (hd == 64) launch<64>(a, blocks, join, st);
     else if (hd == 128) launch<128>(a, blocks, join, st);
     else launch<256>(a, blocks, join, st);
