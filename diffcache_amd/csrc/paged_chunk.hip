@@ -13,17 +13,20 @@
 // 1.7e-3 is the output's alone).  Softmax in powers of two, fp32; the maximum moves where a
 // logit passes it by more than 8.
 //
-// What bounds it: the power that the products take, and the matrix and the vector unit side by side only in part.  2048 tokens of 32 heads x 128
-// behind 30553 rows: 1017-1066 us = 990-1040 TFLOP/s, by the card (a large library product: 1160); on Q, K and V of one value, where the clock
-// stays up, 881 us.  A prompt of 8195 tokens 551-581 us = 950-1000 TFLOP/s; 1024 tokens at 256 columns 1060-1095 us = 980-1020; at 64 columns,
-// where a row has half the products for the same exponentials, 325-330 us for 224 GFLOP = 690.  A prompt of 517 tokens (nine steps) 19 us.
-// Kept: K and V straight to LDS instead of through registers (1163 -> 1060), page ids a step ahead and masks without branches (1348 -> 1163), at 256
-// columns two blocks to a CU (1781 -> 1068); a wave that is at S ahead of the one it shares its SIMD with, so that the two do not stand at the same unit at once
-// (1125 -> 1073 on one card), and K read from LDS three products ahead at 128 columns (1026 -> 1017 on another).  At 64 columns it stays ahead to the step's
-// end (337 -> 328), which is slower at 128 (1017 -> 1035).
-// Tried and dropped: S of a step beside the exponentials of the one before (1105 -> 1145, and slower on equal values too), the weights' products ahead as well
-// (1073 -> 1149), blocks started half a step apart (the same), three blocks of 32-row steps to a CU at 128 columns (1293 for 1116), a zero operand kept for
-// the first product (1222 for 1172).
+// What bounds it: the power that the products take, and the matrix and the vector unit side by side only in part.  2048 tokens of 32 heads x
+// 128 behind 30553 rows: 1017-1066 us = 990-1040 TFLOP/s, by the card (a large library product: 1160); on Q, K and V of one value, where the
+// clock stays up, 881 us.  A prompt of 8195 tokens 551-581 us = 950-1000 TFLOP/s; 1024 tokens at 256 columns 1050-1095 us = 980-1030; at 64
+// columns, where a row has half the products for the same exponentials, 325-330 us for 224 GFLOP = 690.  A prompt of 517 tokens (nine steps)
+// 18 us, of 1024 29: there a step is a chain that nothing else fills, 1.26 us where a CU has one block.
+// Kept: K and V straight to LDS instead of through registers (1163 -> 1060), page ids a step ahead and masks without branches (1348 -> 1163),
+// at 256 columns two blocks to a CU (1781 -> 1068); a wave that is at S ahead of the one it shares its SIMD with, so that the two do not stand
+// at the same unit at once (1125 -> 1073 on one card; at 64 columns to the step's end, 337 -> 328, which is slower at 128, 1017 -> 1035), and K
+// read from LDS three products ahead at 128 columns (1026 -> 1017 on another); the loads' addresses made by lanes, and steps without masks known
+// as such by the block (517 tokens 19.0 -> 17.7).
+// Tried and dropped: S of a step beside the exponentials of the one before (1105 -> 1145, and slower on equal values too), the weights'
+// products ahead as well (1073 -> 1149), the next step's loads between this one's products or V's behind them (one block alone 1.26 -> 1.34 a
+// step; 1049 -> 1037 and 1084), blocks started half a step apart (the same), three blocks of 32-row steps to a CU at 128 columns (1293 for
+// 1116), a zero operand kept for the first product (1222 for 1172).
 #include "dc_paged.h"
 
 namespace {
@@ -107,35 +110,33 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
         const int page = (steps.row(s, KT) + 16 * (lane % TILES)) >> a.p.shift;
         return table[page < last_page ? page : last_page];
     };
+    const uint32_t in_tile = (uint32_t)(wave * T::PER % 16 + in_row);  // of a load's rows, for those n that begin a tile
     auto fetch = [&](uint8_t *k_lds, uint8_t *v_lds, int s, int ids) __attribute__((always_inline)) {  // returns a bit for each tile of 16 rows that has a page
-        const int row0 = steps.row(s, KT);
-        int have = 0, id[TILES];
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-            id[t] = __builtin_amdgcn_readlane(ids, t);
-            const bool is = (unsigned)id[t] < (unsigned)a.p.n_pages;
-            have |= is ? 1 << t : 0, id[t] = is ? id[t] : 0;  // (page 0 in the place of one that there is not)
-        }
+        // (lane t makes tile t's addresses, page 0's in the place of one that there is not: some 30 vector instructions for 150 of the scalar unit)
+        const bool is = (unsigned)ids < (unsigned)a.p.n_pages;
+        const int64_t id = is ? ids : 0;
+        const int first = ((steps.row(s, KT) + 16 * (lane % TILES)) & mask) * HD;
+        const uint64_t kb = (uint64_t)(kh + (id * a.p.kp + first)), vb = (uint64_t)(vh + (id * a.p.vp + first));
+        auto of_tile = [](uint64_t x, int t) __attribute__((always_inline)) {
+            return (uint64_t)dc_of_lane((uint32_t)(x >> 32), t) << 32 | dc_of_lane((uint32_t)x, t);
+        };
 #pragma unroll
         for (int n = 0; n < T::LOADS; ++n) {
-            const int row = (wave + 4 * n) * T::PER;
-            int page = 0;
-            if constexpr (T::PER <= 4) page = id[4 * n * T::PER / 16];  // (the four waves' loads n are one tile's, or part of it)
-            else page = wave * T::PER >= 16 ? id[2 * n + 1] : id[2 * n];
-            const int64_t at = (int64_t)((row0 + row) & mask) * HD;
-            const int mine = row + in_row;
-            __builtin_amdgcn_global_load_lds((const glb_u32 *)(kh + (page * a.p.kp + at) + (in_row * HD + ((chunk ^ T::k_turn(mine)) << 3))),
-                                             (lds_u32 *)(k_lds + row * T::ROW), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const glb_u32 *)(vh + (page * a.p.vp + at) + (in_row * HD + ((chunk ^ T::v_turn(mine)) << 3))),
-                                             (lds_u32 *)(v_lds + row * T::ROW), 16, 0, 0);
+            const int row = (wave + 4 * n) * T::PER, tile = T::PER == 8 ? 2 * n + (wave >> 1) : 4 * n * T::PER / 16;
+            const uint32_t mine = in_tile + 4 * n * T::PER % 16;
+            const uint32_t k_at = mine * T::ROW + ((chunk ^ T::k_turn(mine)) << 4), v_at = mine * T::ROW + ((chunk ^ T::v_turn(mine)) << 4);
+            __builtin_amdgcn_global_load_lds((const glb_u32 *)(of_tile(kb, tile) + k_at), (lds_u32 *)(k_lds + row * T::ROW), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const glb_u32 *)(of_tile(vb, tile) + v_at), (lds_u32 *)(v_lds + row * T::ROW), 16, 0, 0);
         }
-        return have;
+        return (int)__ballot(is) & ((1 << TILES) - 1);
     };
-    // what fetch brought is there, for the wave that asked for it
+    // what fetch brought is there, for the wave that asked for it; returns whether all of the rows have pages and all of the block's pairs attend to
+    // them (as every wave finds: then no one has to look for numbers that are not finite, nor at masks)
     auto stage = [&](uint8_t *v_lds, int buf, int s, int have) __attribute__((always_inline)) {
         __builtin_amdgcn_s_waitcnt(kLoaded);
-        uint32_t odd = 0;
-        if (have != (1 << TILES) - 1 || !dc_whole(a, span.start + t_lo, span.start + t_hi / G, steps.row(s, KT), KT)) {
+        const bool plain = have == (1 << TILES) - 1 && dc_whole(a, span.start + t_lo, span.start + t_hi / G, steps.row(s, KT), KT);
+        if (!plain) {
+            uint32_t odd = 0;
             DcUnbounded u;
             dc_u32x4 w[T::LOADS];
 #pragma unroll
@@ -153,16 +154,22 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                     *reinterpret_cast<dc_u32x4 *>(v_lds + (wave + 4 * n) * T::PER * T::ROW + lane * 16) = w[n];
                 }
             }
+            if (lane == 0) s_odd[buf][wave] = odd;
         }
-        if (lane == 0) s_odd[buf][wave] = odd;
+        return plain;
     };
 
+    auto any_odd = [&](int buf) __attribute__((always_inline)) {
+        const uint4 odd = *reinterpret_cast<const uint4 *>(s_odd[buf]);
+        return __builtin_amdgcn_readfirstlane(odd.x | odd.y | odd.z | odd.w) != 0;
+    };
     bool huge = true;  // (as kNoLogit is)
     int have = 0, next = 0, ids = 0;
+    bool plain = true;  // a step whose rows are there and attended to by all of the block's pairs
     if (begin < end) {
         have = fetch(s_k0, s_v0, begin, ids_of(begin));
         if (begin + 1 < end) ids = ids_of(begin + 1);
-        stage(s_v0, 0, begin, have);
+        plain = stage(s_v0, 0, begin, have);
     }
     __builtin_amdgcn_s_waitcnt(kLoaded);  // (Q too, on every way here: the loop would wait for it, and for all loads, in every step)
     __syncthreads();
@@ -173,7 +180,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
             if (s + 2 < end) ids = ids_of(s + 2);
         }
         // rows that the wave has no use for: behind all its pairs, or between the sinks and all windows
-        const bool use = live && row0 <= p_hi && (a.window == 0 || row0 + KT - 1 > p_lo - a.window || row0 < a.n_sink);
+        const bool use = live && (plain || (row0 <= p_hi && (a.window == 0 || row0 + KT - 1 > p_lo - a.window || row0 < a.n_sink)));
         if (use) {
             __builtin_amdgcn_s_setprio(1);  // (among waves of the SIMD)
             // S^T: x[t][i] is row 32 t + 8 (i / 4) + 4 half + i % 4
@@ -202,7 +209,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                 }
             }
             if constexpr (HD > 64) __builtin_amdgcn_s_setprio(0);
-            if (have != (1 << TILES) - 1 || !dc_whole(a, p_lo, p_hi, row0, KT)) {
+            if (!plain && (have != (1 << TILES) - 1 || !dc_whole(a, p_lo, p_hi, row0, KT))) {
                 const DcReach reach = dc_reach(a, p);
 #pragma unroll
                 for (int t = 0; t < ST; ++t)
@@ -260,8 +267,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(dc_bf16x8, w), __builtin_bit_cast(dc_bf16x8, pw), o[d], 0, 0, 0);
                 }
             }
-            const uint4 odd = *reinterpret_cast<const uint4 *>(s_odd[buf]);
-            if (__builtin_amdgcn_readfirstlane(odd.x | odd.y | odd.z | odd.w)) {
+            if (!plain && any_odd(buf)) {
                 for (int r = 0; r < KT; ++r) {
                     const int page = (row0 + r) >> a.p.shift, id = dc_page_id(a.p, table, page < last_page ? page : last_page);
                     if (id < 0) continue;
@@ -279,7 +285,7 @@ __global__ __launch_bounds__(kThreads, 2) void paged_chunk_kernel(DcPagedAttn a)
             }
         }
         if constexpr (HD == 64) __builtin_amdgcn_s_setprio(0);
-        if (s + 1 < end) stage(v_next, buf ^ 1, s + 1, next);
+        if (s + 1 < end) plain = stage(v_next, buf ^ 1, s + 1, next);
         have = next;
         __syncthreads();
     };
