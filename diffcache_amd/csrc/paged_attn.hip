@@ -25,7 +25,7 @@ constexpr int kThreads = 256, kWaves = 4, kMostWaves = 8, kRows = 16;
 // What bounds it: HBM from some 300 MB on.  8 x 131072 rows of 8 heads x 128 with groups of 4, 4.29 GB: 626 us = 6.9 TB/s (pages of 16 rows 647);
 // 8 x 65536 of 4 heads x 256 321 us = 6.7 TB/s; 16 x 65536 of 8 heads x 64 343 us = 6.3; four drafted tokens of 8 x 32601 rows 171 us = 6.2.  A step of
 // 32 rows x 128 columns is 50 vector, 6 matrix and 4 load instructions for each 4 KB; the vector unit issues a fifth of the time.  Below, the chain of start,
-// page ids, rows, products and the join: 32601 rows of 8 units 24.7 + 3.9 us (the bytes 19), 517 rows in one kernel 10 us, 64 rows 5.6.
+// page ids, rows, products and the join: 32601 rows of 8 units 23.9 + 4.0 us (the bytes 19), 517 rows in one kernel 9.7 us, 64 rows 5.
 // Steps of 64 rows at 128 columns (two blocks to a CU) took 10.8 us for 517 rows and 279 for 48 x 8192 (242 now), the large ones the same.
 // At 256 columns 25 registers spilled cost 447 us for 321.
 template <int HD, int TILES>
@@ -324,6 +324,7 @@ __global__ __launch_bounds__(kMostWaves * 64, HD == 128 ? 3 : 2) void paged_rows
     if (lane < kRows) s_m[wave * kRows + lane] = w.m, s_l[wave * kRows + lane] = l;
     w.finish(s_acc + wave * pairs * HD, pairs);
     __syncthreads();
+    // (four columns at a time: the weights are made again for every one of a thread's pieces, 16 heads of 256 columns 16.1 us by single numbers, 8.5 so)
     constexpr int kLanes = HD / 4;
     for (int o = tid; o < pairs * kLanes; o += waves * 64) {
         const int r = o / kLanes, column = 4 * (o % kLanes);
