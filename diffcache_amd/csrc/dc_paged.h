@@ -76,7 +76,8 @@ struct DcPagedAttn {
     int n_b, waves;          // waves of a block (paged_attn.hip)
     int tiles, tile_rows;    // of a unit's (token, head) pairs: at most so many tiles of so many
     int at_once, round;      // blocks that the GPU runs at once, and those of a KV head among them; at_once 0: nothing is dealt out
-    int least, places;       // the fewest steps of a part; the cut tiles' parts that there is room for
+    int least, fewest;       // steps of a part, at least; down to the fewest as long as there is no more than one block to a CU
+    int places;              // the cut tiles' parts that there is room for
     float of_all;            // 1.0001 / at_once: a little more steps to a part than come of the division, so that rounding makes no more of them
     float scale;             // times log2(e)
 };
@@ -211,7 +212,8 @@ __device__ __forceinline__ DcItem dc_deal(const DcPagedAttn &a, int x, int lane)
     };
     // How the tiles are cut, for the work of all sequences.
     auto plan = [&](float work, auto &&each) __attribute__((always_inline)) {
-        const float even = work * (float)a.n_h * a.of_all, least = (float)a.least;  // (of_all is 1.0001 / at_once)
+        const float even = work * (float)a.n_h * a.of_all;  // (of_all is 1.0001 / at_once)
+        const float least = fminf(fmaxf(even * (float)a.at_once * (1.f / 256), (float)a.fewest), (float)a.least);
         cut.by = __builtin_amdgcn_rcpf(even > least ? even : least);
         // (a part's least steps are what counts, or so many sequences that it all evens out and counting takes longer than it saves: 60 of one
         // tile 697 us and 706)

@@ -436,7 +436,7 @@ constexpr int64_t kAlone = 768 * 128;
 
 struct Cut {
     bool chunk, deal, join;   // deal: blocks find their items; join: some may be parts
-    int waves, tiles, tile_rows, at_once, least;
+    int waves, tiles, tile_rows, at_once, least, fewest;
     unsigned sharers;         // blocks of the chunks' join to each part
     int64_t blocks, places;   // places: of parts, in the workspace
 };
@@ -451,12 +451,13 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
         const int64_t places = tokens * group / kChunkRows + n_b;  // of packed tokens' tiles (dc_packed)
         int64_t all = n_b * c.tiles;
         if (tokens && places < all) all = places;
-        // Parts of seven steps where the tiles alone leave most CUs idle (16 tokens of 8 heads behind 4083 rows: 21.9 us of eight steps, 18.8 of
-        // four; a prompt of 517 of one head in groups of 8: 19.0 and 24.7).  Where they do not, a part has to save more than the join
-        // takes (a prompt of 517 tokens of 8 heads, 136 tiles: 19.6 us, in two parts 26.7; of 2048, 512 tiles: 63 us, the longer half of
-        // them in two parts of 16 steps 84).
+        // Short parts where the tiles alone leave most CUs idle: three steps at least, four of the smaller ones of 256 columns, and up to seven as
+        // long as CUs are left without a block (38 tokens of 12 units of 128 columns over 700 rows 20.2 us in parts of seven steps, 15.4 of
+        // three; over 8195 rows 29.0 and 33.6, as few as CUs 27), and none of ten steps or fewer (a prompt of 517 of one head in groups of 8: 17.6
+        // and 19.3).  Where they do not, a part has to save more than the join takes (a prompt of 517 tokens of 8 heads, 136 tiles: 19.6 us, in two
+        // parts 26.7; of 2048, 512 tiles: 63 us, the longer half of them in two parts of 16 steps 84).
         const int64_t steps = (rows + dc_chunk_step(hd) - 1) / dc_chunk_step(hd);
-        c.least = all * n_h <= 128 ? 7 : 24;
+        c.least = all * n_h <= 128 ? 7 : 24, c.fewest = all * n_h > 128 ? 24 : hd == 256 ? 4 : 3;
         // Of more tiles than that, where tokens have rows before them and there are few rounds, the last round's are cut if they are at most half of
         // what runs at once, or two thirds where they are all (dc_deal; 2048 tokens of 8 heads x 128 behind some 30000 rows, 512 tiles: 1036 us; 2100
         // 1697 and 1081, 2600 1688 and 1340, 1100 873 and 658).  At 64 columns, four blocks to a CU, the others of a CU gain more by one that ends.
@@ -468,13 +469,13 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
         if (c.tiles > all) c.tiles = (int)all;  // (one sequence of fewer packed tokens than max_new)
         if (!c.join && tokens && n_b > 1) all = places;
         // (items: see dc_deal; and no tile has more parts than its steps allow.  A thousand blocks that find none cost 1-2 us in each kernel)
-        const int64_t parts = c.join ? 2 * c.at_once / n_h + 1 : 0, most = all * (c.join ? steps / c.least + 1 : 1);
+        const int64_t parts = c.join ? 2 * c.at_once / n_h + 1 : 0, most = all * (c.join ? steps / c.fewest + 1 : 1);
         c.blocks = n_h * (all + parts < most ? all + parts : most), c.places = n_h * ((all < parts ? all : parts) + parts);
         if (c.places > c.blocks) c.places = c.blocks;
         c.sharers = c.blocks <= 128 ? 4 : c.blocks <= 256 ? 2 : 1;  // (38 tokens of 12 units over 1575 rows of 256 columns, 96 blocks: 36 us, four times as many to join 31)
         return c;
     }
-    c.tiles = 1, c.tile_rows = max_new * group, c.at_once = rows_at_once(hd), c.least = kWaves;
+    c.tiles = 1, c.tile_rows = max_new * group, c.at_once = rows_at_once(hd), c.least = c.fewest = kWaves;
     const int64_t step = 16 * row_tiles(hd), steps = (rows + step - 1) / step;
     c.deal = c.join = steps * step * hd > kAlone && n_units <= 2 * c.at_once;
     c.waves = steps * step * hd > kAlone || steps <= kWaves ? kWaves : kMostWaves;
@@ -540,7 +541,7 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     a.qs = {x->q_batch_stride, x->q_token_stride, x->q_head_stride};
     a.n_h = x->n_h, a.group = x->group, a.n_rows = x->n_rows, a.n_sink = x->n_sink, a.window = x->window;
     a.n_b = t.n_b, a.waves = c.waves, a.tiles = c.tiles, a.tile_rows = c.tile_rows;
-    a.at_once = c.deal ? c.at_once : 0, a.round = c.at_once > x->n_h ? c.at_once / x->n_h : 1, a.least = c.least, a.places = (int)(c.places / x->n_h), a.of_all = 1.0001f / (float)c.at_once;
+    a.at_once = c.deal ? c.at_once : 0, a.round = c.at_once > x->n_h ? c.at_once / x->n_h : 1, a.least = c.least, a.fewest = c.fewest, a.places = (int)(c.places / x->n_h), a.of_all = 1.0001f / (float)c.at_once;
     a.scale = x->scale * 1.44269504088896341f;
     hipStream_t st = (hipStream_t)stream;
     if (c.chunk) return dc_paged_chunk_launch(a, x->hd, (unsigned)c.blocks, c.join ? c.sharers : 0, st);
