@@ -472,7 +472,7 @@ Cut cut_of(int64_t n_b, int n_h, int group, int hd, int64_t rows, int max_new, i
         const int64_t parts = c.join ? 2 * c.at_once / n_h + 1 : 0, most = all * (c.join ? steps / c.fewest + 1 : 1);
         c.blocks = n_h * (all + parts < most ? all + parts : most), c.places = n_h * ((all < parts ? all : parts) + parts);
         if (c.places > c.blocks) c.places = c.blocks;
-        c.sharers = c.blocks <= 128 ? 4 : c.blocks <= 256 ? 2 : 1;  // (38 tokens of 12 units over 1575 rows of 256 columns, 96 blocks: 36 us, four times as many to join 31)
+        c.sharers = c.blocks <= 128 ? 4 : c.blocks <= 512 ? 2 : 1;  // (38 tokens of 12 units over 1575 rows of 256 columns, 96 blocks: 36 us, four times as many to join 31)
         return c;
     }
     c.tiles = 1, c.tile_rows = max_new * group, c.at_once = rows_at_once(hd), c.least = c.fewest = kWaves;
@@ -521,8 +521,10 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
     DC_REQUIRE(x->scale > 0.f && x->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
     DC_REQUIRE((int64_t)t.max_new * x->group < (1ll << 30) && (int64_t)t.n_tokens * x->group < (1ll << 31), "%s: too many tokens", who);
-    // rows that a window's tokens can need at most, and a step more at its two ends
-    const int64_t in_window = (int64_t)x->n_sink + x->window + t.max_new + 256, rows = x->window && in_window < x->n_rows ? in_window : x->n_rows;
+    // rows that a window's tokens, or those of a tile, can need at most, and a step more at its two ends
+    const int64_t of_tile = (int64_t)t.max_new * x->group > kRows ? kChunkRows / x->group + 2 : t.max_new;
+    const int64_t in_window = (int64_t)x->n_sink + x->window + (of_tile < t.max_new ? of_tile : t.max_new) + 256;
+    const int64_t rows = x->window && in_window < x->n_rows ? in_window : x->n_rows;
     const Cut c = cut_of(t.n_b, x->n_h, x->group, x->hd, rows, t.max_new, t.cu ? t.n_tokens : 0);
     DC_REQUIRE(dc_grid_fits(c.chunk || c.deal ? c.blocks : t.n_b, c.waves * 64), "%s: grid too large", who);
     DcPagedAttn a;
