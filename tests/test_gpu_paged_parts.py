@@ -121,3 +121,32 @@ def test_every_row_counts_once_however_tiles_are_cut(lengths, new, hd, h, group)
         # (the bounds as above, of counts that are exact in fp32)
         assert ((out[i].double() - share).abs() <= 2.0 ** -8 * share * (1 + 2.0 ** -12)).all()
         assert ((lse[i].double() - r.double().log()).abs() <= 1e-5).all()
+
+
+@pytest.mark.parametrize("sink,window", [(0, 0), (64, 900), (0, 1500)])
+@pytest.mark.parametrize("counts", [[700, 0, 1000, 999, 1, 1000], [1000, 1000, 130, 1000, 1000, 1]])
+def test_packed_tokens_whose_last_tiles_are_cut(counts, sink, window):
+    """More tiles than run at once: whole ones first, the rest in parts, across sequences with and without tokens."""
+    from diffcache_amd import _hip as hip
+    lengths, hd, h, group = [2600, 2500, 2700, 2650, 2400, 2550], 256, 4, 4
+    k, v, table, g = counted(len(lengths), h, hd, 64, lengths, 3)
+    ends = [2]
+    for c in counts:
+        ends.append(ends[-1] + c)
+    total = ends[-1] + 3
+    q = torch.zeros((total, h * group, hd), dtype=torch.bfloat16, device=DEV)
+    out, lse = torch.full_like(q, 3.0), torch.full(q.shape[:2], 9.0, device=DEV)
+    hip.paged_attn(q, k, v, table, i32([n - c for n, c in zip(lengths, counts)]), cu=i32(ends), max_new=1000, n_sink=sink, window=window, out=out, lse=lse)
+    assert (out[:2] == 3).all() and (out[-3:] == 3).all() and (lse[:2] == 9).all() and (lse[-3:] == 9).all()
+    below = lambda n: (n[:, None] - torch.arange(hd, device=DEV) + hd - 1).div(hd, rounding_mode="floor").clamp(min=0)  # noqa: E731 (rows 0 .. n - 1 of each remainder)
+    for i, (n, c) in enumerate(zip(lengths, counts)):
+        p = torch.arange(n - c, n, device=DEV)
+        first = (p - window + 1).clamp(min=0) if window else torch.zeros_like(p)
+        sinks = torch.minimum(first, torch.full_like(p, sink if window else 0))
+        have = below(p + 1) - below(first) + below(sinks)
+        rows = (p + 1 - first + sinks).double()
+        share = (have.double() / rows[:, None])[:, None]
+        got = out[ends[i]:ends[i + 1]].double()
+        # (the bounds as above)
+        assert ((got - share).abs() <= 2.0 ** -8 * share * (1 + 2.0 ** -12)).all()
+        assert ((lse[ends[i]:ends[i + 1]].double() - rows.log()[:, None]).abs() <= 1e-5).all()
