@@ -265,8 +265,9 @@ class PagedCache:
         """After ``steps`` replays of a captured decode step: bring the host's mirror of the lengths up to the device's (no
         synchronisation).  Negative: tokens taken back, which ``lens.sub_`` takes off the device's."""
         grown = [n + steps for n in self._lens]
-        hip.require(min(grown) >= 0 and all(n <= len(p) * self.page_size for n, p in zip(grown, self._pages)),
-                    "more steps were replayed than the sequences have pages")
+        # (a step is captured for max_length rows: of one behind them in the last page a token would be written and never attended to)
+        hip.require(min(grown) >= 0 and max(grown) <= self.max_length and all(n <= len(p) * self.page_size for n, p in zip(grown, self._pages)),
+                    "more steps were replayed than the sequences have pages, or rows up to max_length")
         hip.require(all(n >= self.page_size * sum(1 for x in p if self._holders[x] > 1) for n, p in zip(grown, self._pages)),
                     "rows of pages that two sequences hold cannot be taken back")
         self._lens = grown
