@@ -17,8 +17,9 @@ projections leave them.
 
 ``lens`` (int32, on the device) holds the lengths of the sequences and ``table`` their pages, the same for all layers.  A captured
 ``decode_attention`` goes by both when it is replayed; pages are handed out on the host, so ``reserve`` has to give the sequences
-room for the replays first.  All layers share one workspace: calls and replays of one cache go one after another (two caches
-may run side by side).
+room for the replays first.  A sequence that was given up (``free``) holds nothing and takes no part in decode steps, captured ones
+among them, until a prompt or a shared beginning takes its place: ``live`` (int32, on the device) is 0 for it, else 1.  All layers share one
+workspace: calls and replays of one cache go one after another (two caches may run side by side).
 """
 from __future__ import annotations
 
@@ -60,16 +61,18 @@ class PagedCache:
         self.interleaved, self.sections = interleaved, sections
         self.lens = torch.zeros((batch_size,), dtype=torch.int32, device=self.device)
         self.table = torch.full((batch_size, wide), -1, dtype=torch.int32, device=self.device)
+        self.live = torch.ones((batch_size,), dtype=torch.int32, device=self.device)
         self._lens: List[int] = [0] * batch_size                     # the host's mirror of lens
+        self._live: List[int] = [1] * batch_size                     # and of live
         self._pages: List[List[int]] = [[] for _ in range(batch_size)]
         self._free = list(range(self.num_pages - 1, -1, -1))
         self._holders = [0] * self.num_pages                         # sequences that hold a page
-        self._room = 0                                               # tokens that every sequence has pages for
+        self._room = 0                                               # tokens that every live sequence has pages for
         self._workspace = torch.empty(
             (hip.paged_attn_workspace_bytes(batch_size, num_kv_heads, num_q_heads // num_kv_heads, head_dim, max_length),),
             dtype=torch.uint8, device=self.device)
-        # (made here: one that a captured step made would be the graph's)
-        self._attn_out = torch.empty((batch_size, num_q_heads, head_dim), device=self.device, dtype=torch.bfloat16)
+        # (made here: one that a captured step made would be the graph's; zeros, for what stays there of sequences that are not live)
+        self._attn_out = torch.zeros((batch_size, num_q_heads, head_dim), device=self.device, dtype=torch.bfloat16)
         self._q = torch.empty_like(self._attn_out) if self.rotates else None
 
     @property
@@ -80,9 +83,9 @@ class PagedCache:
     # ---- pages, on the host ----
 
     def reserve(self, lengths: Union[int, Sequence[int]]) -> None:
-        """Pages for rows 0 .. lengths[i] - 1 of every sequence (an int: of each of them).  A call that the pool has too few pages for
-        changes nothing."""
-        lengths = [lengths] * self.batch_size if isinstance(lengths, int) else [int(n) for n in lengths]
+        """Pages for rows 0 .. lengths[i] - 1 of every sequence (an int: of each of them that is live).  A call that the pool has too
+        few pages for changes nothing."""
+        lengths = [lengths * x for x in self._live] if isinstance(lengths, int) else [int(n) for n in lengths]
         hip.require(len(lengths) == self.batch_size and all(0 <= n <= self.max_length for n in lengths),
                     "lengths must be one for every sequence, up to max_length")
         need = [max((n + self.page_size - 1) // self.page_size - len(p), 0) for n, p in zip(lengths, self._pages)]
@@ -131,7 +134,16 @@ class PagedCache:
         return torch.tensor(numbers, dtype=torch.int32, pin_memory=self.device.type == "cuda")
 
     def _count_room(self) -> None:
-        self._room = min(len(p) * self.page_size - n for p, n in zip(self._pages, self._lens))
+        self._room = min((len(p) * self.page_size - n for p, n, x in zip(self._pages, self._lens, self._live) if x), default=0)
+
+    def _set_live(self, live: Sequence[int]) -> None:
+        if list(live) != self._live:
+            self._live = list(live)
+            self.live.copy_(self._pinned(self._live), non_blocking=True)
+
+    def _with(self, counts: Sequence[int]) -> List[int]:
+        """live, with the sequences that these tokens are of."""
+        return [1 if n else x for n, x in zip(counts, self._live)]
 
     @staticmethod
     def _capturing() -> bool:
@@ -150,15 +162,18 @@ class PagedCache:
         self._pages[sequence] = list(pages)
         self._lens[sequence] = rows
         self.lens[sequence:sequence + 1].fill_(rows)
+        self._set_live([1 if i == sequence else x for i, x in enumerate(self._live)])
         self._upload()
 
     def free(self, sequence: int) -> None:
-        """Sequence ``sequence`` holds nothing any more; its pages are others' to take."""
+        """Sequence ``sequence`` holds nothing any more; its pages are others' to take.  Decode steps leave it alone until
+        ``extend_attention`` or ``prefill_update_kv_cache`` has tokens of it or ``share_prefix`` begins it anew."""
         hip.require(0 <= sequence < self.batch_size, "no such sequence")
         hip.require(not self._capturing(), "pages cannot be given back while a graph is captured")
         self._give_back(sequence)
         self._lens[sequence] = 0
         self.lens[sequence:sequence + 1].zero_()
+        self._set_live([0 if i == sequence else x for i, x in enumerate(self._live)])
         self._upload()
 
     # ---- the decoder's hooks ----
@@ -205,6 +220,7 @@ class PagedCache:
         else:
             self.lens.copy_(counts)
         self._lens = at
+        self._set_live(self._with(at))
         self._count_room()
         return key_states, value_states
 
@@ -218,7 +234,8 @@ class PagedCache:
         capturing = self._capturing()
         grown = [n + c for n, c in zip(self._lens, at)]
         hip.require(max(grown) <= self.max_length, "the cache is full (max_length)")
-        if max(at) > self._room:
+        live = self._with(at)
+        if max(at) > self._room or live != self._live:
             self.reserve(grown)
         turned = self._append(layer_idx, k, v, self.lens, counts, q if self.rotates else None, q_out, pos)
         got = hip.paged_attn(q if turned is None else turned, self.k_pages[layer_idx], self.v_pages[layer_idx], self.table, self.lens,
@@ -230,6 +247,7 @@ class PagedCache:
             self.lens.add_(q.shape[1] if q.dim() == 4 else 1) if counts is None else self.lens.add_(counts)
             if not capturing:   # a captured step is counted when it is replayed (advance_host_step)
                 self._lens = grown
+                self._set_live(live)
                 self._count_room()
         return got if lse is None else got[0]
 
@@ -254,17 +272,17 @@ class PagedCache:
         """One layer of a decode step: write the token's k/v behind each sequence and attend to all of it (or to its sinks and
         window).  queries (bsz, 1, Hq*hd) or (bsz, Hq, hd); key/value_states (bsz, 1, Hkv, hd); ``pos`` (bsz) int32, or (bsz, axes).  Returns
         (bsz, Hq, hd) bf16; ``lse`` (bsz, Hq) fp32 receives the log of the sum of exponentials.  Call it for every layer of a step; the
-        sequences grow by one after the last layer."""
+        sequences grow by one after the last layer.  Those that are not live are left alone: their rows of ``out`` and ``lse`` stay what they were."""
         b, hq, h, hd = self.batch_size, self.num_q_heads, self.num_kv_heads, self.head_dim
         if out is None:
             out = self._attn_out
         return self._attend(layer_idx, queries.reshape(b, hq, hd), key_states.reshape(b, h, hd), value_states.reshape(b, h, hd),
-                            [1] * b, None, out, lse, pos, self._workspace, self._q)
+                            list(self._live), self.live, out, lse, pos, self._workspace, self._q)
 
     def advance_host_step(self, steps: int = 1) -> None:
         """After ``steps`` replays of a captured decode step: bring the host's mirror of the lengths up to the device's (no
         synchronisation).  Negative: tokens taken back, which ``lens.sub_`` takes off the device's."""
-        grown = [n + steps for n in self._lens]
+        grown = [n + steps * x for n, x in zip(self._lens, self._live)]
         # (a step is captured for max_length rows: of one behind them in the last page a token would be written and never attended to)
         hip.require(min(grown) >= 0 and max(grown) <= self.max_length and all(n <= len(p) * self.page_size for n, p in zip(grown, self._pages)),
                     "more steps were replayed than the sequences have pages, or rows up to max_length")

@@ -61,3 +61,99 @@ def test_no_replay_is_counted_past_max_length(cache, page):
     with pytest.raises(AssertionError, match="max_length"):
         c.advance_host_step(2)
     assert c._lens == [99] * 3
+
+
+def test_a_freed_sequence_is_left_alone_by_decode_steps(cache):
+    c = cache(num_pages=14)
+    prefill(c, 90, lens=[90, 50, 20])
+    c.free(1)
+    for step in range(10):
+        decode(c)
+        assert all(a["counts"] == [1, 0, 1] for a in cache.appended[-2:] + cache.attended[-2:])
+        assert c._lens == c.lens.tolist() == [91 + step, 0, 21 + step]
+    assert c._pages[1] == [] and (c.table[1] == -1).all() and len(c._free) == 14 - 7 - 2
+    with pytest.raises(AssertionError, match="full"):
+        decode(c)
+    c.free(0)                                                      # (the one that is full)
+    decode(c)
+    assert c._lens == c.lens.tolist() == [0, 0, 31]
+    c.free(2)
+    decode(c)                                                      # nothing to do
+    assert c._lens == c.lens.tolist() == [0, 0, 0] and sorted(c._free) == list(range(14)) and cache.attended[-1]["counts"] == [0, 0, 0]
+
+
+def test_a_freed_sequence_does_not_count_in_replays(cache):
+    c = cache()
+    prefill(c, 40, lens=[40, 33, 8])
+    c.free(1)
+    c.reserve(60)                                                  # (of the sequences that there are)
+    assert [len(p) for p in c._pages] == [4, 0, 4]
+    c.advance_host_step(20)
+    assert c._lens == [60, 0, 28]
+    c.advance_host_step(-3)
+    assert c._lens == [57, 0, 25]
+    with pytest.raises(AssertionError, match="more steps"):
+        c.advance_host_step(8)
+    with pytest.raises(AssertionError, match="more steps"):
+        c.advance_host_step(-26)
+    assert c._lens == [57, 0, 25]
+
+
+@pytest.mark.parametrize("how", ["extend", "whole extend", "prefill", "share", "share nothing"])
+def test_a_freed_sequence_begins_anew(cache, how):
+    c = cache()
+    prefill(c, 40, lens=[40, 33, 8])
+    c.free(1)
+    c.reserve([90, 0, 90])                                         # room enough for the others
+    decode(c)
+    want = [41, 0, 9]
+    if how == "extend":
+        for layer in range(2):
+            c.extend_attention(layer, bf(3, 5, 2, 64), bf(3, 5, 1, 64), bf(3, 5, 1, 64), lens=[0, 5, 0])
+            assert len(c._pages[1]) == 1 and (cache.appended[-1]["table"][1] >= 0).sum() == 1
+        want = [41, 5, 9]
+    elif how == "whole extend":
+        for layer in range(2):
+            c.extend_attention(layer, bf(3, 20, 2, 64), bf(3, 20, 1, 64), bf(3, 20, 1, 64))
+            assert len(c._pages[1]) == 2
+        want = [61, 20, 29]
+    elif how == "prefill":
+        prefill(c, 7, lens=[3, 7, 0])
+        want = [3, 7, 0]
+    else:
+        c.share_prefix(1, 0, 32 if how == "share" else 0)
+        want = [41, 32 if how == "share" else 0, 9]
+    assert c._lens == c.lens.tolist() == want
+    decode(c)
+    assert c._lens == c.lens.tolist() == [n + 1 for n in want]
+    assert all(len(p) * 16 >= n for n, p in zip(c._lens, c._pages))
+    c.reserve(96)
+    c.advance_host_step()
+    assert c._lens == [n + 2 for n in want]
+
+
+def test_an_empty_prompt_begins_a_sequence_that_was_not_freed(cache):
+    c = cache()
+    prefill(c, 7, lens=[7, 0, 3])
+    decode(c)
+    assert c._lens == c.lens.tolist() == [8, 1, 4]
+    c.free(2)
+    prefill(c, 5, lens=[5, 0, 0])
+    decode(c)
+    assert c._lens == c.lens.tolist() == [6, 1, 0]
+
+
+def test_steps_go_by_what_is_freed_and_filled_when_they_run(cache):
+    """One tensor, made with the cache, says which sequences a step counts: a captured step reads it at every replay."""
+    c = cache()
+    prefill(c, 7)
+    live = c.live
+    at = live.data_ptr()
+    c.free(0)
+    c.free(2)
+    assert live.tolist() == [0, 1, 0]
+    c.share_prefix(2, 1, 0)
+    for layer in range(2):
+        assert live.tolist() == [0, 1, 1]
+        c.extend_attention(layer, bf(3, 2, 2, 64), bf(3, 2, 1, 64), bf(3, 2, 1, 64), lens=[2, 0, 0])
+    assert c.live is live and live.tolist() == [1, 1, 1] and live.data_ptr() == at and live.dtype == torch.int32
