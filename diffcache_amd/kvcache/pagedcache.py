@@ -197,6 +197,7 @@ class PagedCache:
         ``lens``: the prompts' lengths where they are padded to a common one (behind their tokens); the same for every layer.  ``pos``: positions
         of the tokens, (bsz, seq_len) int32, or (bsz, seq_len, axes) with sections; their rows without it."""
         seq = key_states.size(1)
+        hip.require(0 <= layer_idx < self.num_layers, "no such layer")
         hip.require(0 < seq <= self.max_length, "the prompt is empty or longer than max_length")
         # a replay would move the rows and leave the host's lengths as they are
         hip.require(not self._capturing(), "a prefill cannot be captured in a graph")

@@ -157,3 +157,18 @@ def test_steps_go_by_what_is_freed_and_filled_when_they_run(cache):
         assert live.tolist() == [0, 1, 1]
         c.extend_attention(layer, bf(3, 2, 2, 64), bf(3, 2, 1, 64), bf(3, 2, 1, 64), lens=[2, 0, 0])
     assert c.live is live and live.tolist() == [1, 1, 1] and live.data_ptr() == at and live.dtype == torch.int32
+
+
+def state(c):
+    return [list(p) for p in c._pages], sorted(c._free), list(c._holders), list(c._lens), list(c._live), c._room, c.table.tolist(), c.lens.tolist(), c.live.tolist()
+
+
+@pytest.mark.parametrize("layer", [-1, -2, 2, 7])
+def test_prompts_for_layers_that_there_are_not_are_refused(cache, layer):
+    c = cache()
+    for lens in ([40, 33, 8], None):
+        before = state(c)
+        with pytest.raises(AssertionError, match="no such layer"):
+            c.prefill_update_kv_cache(bf(3, 40, 1, 64), bf(3, 40, 1, 64), layer, lens=lens)
+        assert state(c) == before and not cache.appended
+        c.reserve(20)
