@@ -85,11 +85,15 @@ class PagedCache:
     def reserve(self, lengths: Union[int, Sequence[int]]) -> None:
         """Pages for rows 0 .. lengths[i] - 1 of every sequence (an int: of each of them that is live).  A call that the pool has too
         few pages for changes nothing."""
-        lengths = [lengths * x for x in self._live] if isinstance(lengths, int) else [int(n) for n in lengths]
+        self._reserve([lengths * x for x in self._live] if isinstance(lengths, int) else [int(n) for n in lengths])
+
+    def _reserve(self, lengths: Sequence[int]) -> List[int]:
+        """The pages that every sequence got, for _take_back."""
         hip.require(len(lengths) == self.batch_size and all(0 <= n <= self.max_length for n in lengths),
                     "lengths must be one for every sequence, up to max_length")
         need = [max((n + self.page_size - 1) // self.page_size - len(p), 0) for n, p in zip(lengths, self._pages)]
         self._hand_out(need, [])
+        return need
 
     def _hand_out(self, need: Sequence[int], dropped: Sequence[int]) -> None:
         """need[i] more pages for sequence i, after the sequences in ``dropped`` gave theirs back."""
@@ -106,6 +110,17 @@ class PagedCache:
                 page = self._free.pop()
                 self._holders[page] = 1
                 pages.append(page)
+        self._upload()
+
+    def _take_back(self, need: Sequence[int]) -> None:
+        """The last need[i] pages of every sequence, as they were before _hand_out."""
+        if not any(need):
+            return
+        for pages, n in reversed(list(zip(self._pages, need))):
+            for _ in range(n):
+                page = pages.pop()
+                self._holders[page] = 0
+                self._free.append(page)
         self._upload()
 
     def _held_by(self, sequences: Sequence[int]) -> List[int]:
@@ -206,12 +221,14 @@ class PagedCache:
         # pages that others hold too stay theirs
         dropped = [i for i, p in enumerate(self._pages) if any(self._holders[x] > 1 for x in p)]
         need = [max((n + self.page_size - 1) // self.page_size - (0 if i in dropped else len(self._pages[i])), 0) for i, n in enumerate(at)]
-        before = [list(p) for p in self._pages], list(self._holders), list(self._free)
+        before = ([list(p) for p in self._pages], list(self._holders), list(self._free)) if dropped else None
         self._hand_out(need, dropped)
         try:
             self._append(layer_idx, key_states, value_states, None, counts, None, None, pos)
         except Exception:
-            if dropped:    # the pages that were given back hold rows yet
+            if before is None:
+                self._take_back(need)
+            else:          # the pages that were given back hold rows yet
                 self._pages, self._holders, self._free = before
                 self._upload()
             raise
@@ -236,14 +253,17 @@ class PagedCache:
         grown = [n + c for n, c in zip(self._lens, at)]
         hip.require(max(grown) <= self.max_length, "the cache is full (max_length)")
         live = self._with(at)
-        if max(at) > self._room or live != self._live:
-            self.reserve(grown)
-        turned = self._append(layer_idx, k, v, self.lens, counts, q if self.rotates else None, q_out, pos)
-        got = hip.paged_attn(q if turned is None else turned, self.k_pages[layer_idx], self.v_pages[layer_idx], self.table, self.lens,
-                             counts=counts,
-                             # a captured launch is laid out for the longest sequences that the cache holds, and goes by lens when it runs
-                             n_rows=self.max_length if capturing else max(max(grown), 1),
-                             n_sink=self.sink_len, window=self.window, out=out, lse=lse, workspace=workspace)
+        need = self._reserve(grown) if max(at) > self._room or live != self._live else []
+        try:
+            turned = self._append(layer_idx, k, v, self.lens, counts, q if self.rotates else None, q_out, pos)
+            got = hip.paged_attn(q if turned is None else turned, self.k_pages[layer_idx], self.v_pages[layer_idx], self.table, self.lens,
+                                 counts=counts,
+                                 # a captured launch is laid out for the longest sequences that the cache holds, and goes by lens when it runs
+                                 n_rows=self.max_length if capturing else max(max(grown), 1),
+                                 n_sink=self.sink_len, window=self.window, out=out, lse=lse, workspace=workspace)
+        except Exception:
+            self._take_back(need)
+            raise
         if layer_idx == self.num_layers - 1:
             self.lens.add_(q.shape[1] if q.dim() == 4 else 1) if counts is None else self.lens.add_(counts)
             if not capturing:   # a captured step is counted when it is replayed (advance_host_step)

@@ -172,3 +172,35 @@ def test_prompts_for_layers_that_there_are_not_are_refused(cache, layer):
             c.prefill_update_kv_cache(bf(3, 40, 1, 64), bf(3, 40, 1, 64), layer, lens=lens)
         assert state(c) == before and not cache.appended
         c.reserve(20)
+
+
+@pytest.mark.parametrize("call,refuses", [(call, "append") for call in ("prefill", "padded prefill", "extend", "padded extend", "decode")]
+                         + [(call, "attn") for call in ("extend", "padded extend", "decode")])
+@pytest.mark.parametrize("shared", [False, True])
+def test_a_refused_call_gives_back_the_pages_that_it_took(cache, monkeypatch, call, shared, refuses):
+    c = cache()
+    prefill(c, 16, lens=[16, 16, 3])
+    if shared:
+        c.share_prefix(1, 0, 16)
+    c.free(2)
+    before = state(c)
+
+    def refuse(*a, **kw):
+        raise hip.DiffCacheError("k must be bf16")
+
+    calls = {"prefill": lambda: c.prefill_update_kv_cache(bf(3, 50, 1, 64), bf(3, 50, 1, 64), 1),
+             "padded prefill": lambda: c.prefill_update_kv_cache(bf(3, 50, 1, 64), bf(3, 50, 1, 64), 1, lens=[50, 0, 20]),
+             "extend": lambda: c.extend_attention(1, bf(3, 40, 2, 64), bf(3, 40, 1, 64), bf(3, 40, 1, 64)),
+             "padded extend": lambda: c.extend_attention(1, bf(3, 40, 2, 64), bf(3, 40, 1, 64), bf(3, 40, 1, 64), lens=[0, 17, 40]),
+             "decode": lambda: decode(c, [1])}
+    with monkeypatch.context() as m:
+        m.setattr(hip, "paged_" + refuses, refuse)
+        for _ in range(2):
+            with pytest.raises(hip.DiffCacheError, match="bf16"):
+                calls[call]()
+            assert state(c) == before
+    free = list(c._free)
+    calls[call]()                                                  # and goes as if there had been no refused one
+    taken = [p for pages, old in zip(c._pages, before[0]) for p in pages if p not in old]
+    assert taken and set(taken) <= set(free + sum(before[0], []))
+    assert sorted(c._free + list({p for pages in c._pages for p in pages})) == list(range(c.num_pages))
