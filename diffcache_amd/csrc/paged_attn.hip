@@ -519,7 +519,8 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     DC_REQUIRE(x->group >= 1 && x->group <= 16, "%s: group %d not in [1,16]", who, x->group);
     DC_REQUIRE(x->n_rows >= 1 && x->n_rows <= (int64_t)t.table_pages * x->store.page, "%s: %d rows outside the table", who, x->n_rows);
     DC_REQUIRE(x->n_sink >= 0 && x->window >= 0, "%s: negative n_sink or window", who);
-    DC_REQUIRE(x->scale > 0.f && x->scale <= 3.0e38f, "%s: scale must be positive and finite", who);
+    const float scale = x->scale * 1.44269504088896341f;  // in powers of two
+    DC_REQUIRE(x->scale > 0.f && scale < INFINITY, "%s: scale must be positive and at most 2.35e38", who);
     DC_REQUIRE((int64_t)t.max_new * x->group < (1ll << 30) && (int64_t)t.n_tokens * x->group < (1ll << 31), "%s: too many tokens", who);
     // rows that a window's tokens, or those of a tile, can need at most, and a step more at its two ends
     const int64_t of_tile = (int64_t)t.max_new * x->group > kRows ? kChunkRows / x->group + 2 : t.max_new;
@@ -544,7 +545,7 @@ extern "C" int dc_paged_attn_bf16(const dc_paged_attn_args *x, void *stream) {
     a.n_h = x->n_h, a.group = x->group, a.n_rows = x->n_rows, a.n_sink = x->n_sink, a.window = x->window;
     a.n_b = t.n_b, a.waves = c.waves, a.tiles = c.tiles, a.tile_rows = c.tile_rows;
     a.at_once = c.deal ? c.at_once : 0, a.round = c.at_once > x->n_h ? c.at_once / x->n_h : 1, a.least = c.least, a.fewest = c.fewest, a.places = (int)(c.places / x->n_h), a.of_all = 1.0001f / (float)c.at_once;
-    a.scale = x->scale * 1.44269504088896341f;
+    a.scale = scale;
     hipStream_t st = (hipStream_t)stream;
     if (c.chunk) return dc_paged_chunk_launch(a, x->hd, (unsigned)c.blocks, c.join ? c.sharers : 0, st);
     if (x->hd == 64) launch_rows<64>(a, c, st);

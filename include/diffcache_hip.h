@@ -781,7 +781,7 @@ int dc_paged_append_bf16(const dc_paged_append_args *args, void *stream);
  *   out      as many, contiguous: softmax(scale q k^T) v; lse NULL, or (tokens, n_h * group) fp32, the log of the sum of
  *            exp(scale q k^T).  Those of tokens that do not count stay as they were
  *   n_rows   rows at or beyond it are not attended to (at most table_pages * page): sizes the launch
- *   group    up to 16; scale: positive and finite
+ *   group    up to 16; scale: positive, up to 2.35e38 (times log2(e) it has to be finite)
  * A token that attends to no row has out 0 and lse -inf.  What a token does not attend to may hold anything, and leaves no trace.  Of what
  * it does attend to, a number of K that is not finite makes the head's outputs and lse NaN where a logit becomes NaN or +inf; an infinity in V
  * makes the outputs of its column that infinity (NaN where there are both, or where the row's weight is below fp32), a NaN makes them NaN.  Logits are fp32, before the scale too: one that falls below its range is -inf, a weight of 0; one above
