@@ -1466,6 +1466,8 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tens
             if not 1 <= n_axes <= 4 or pos is None:
                 raise DiffCacheError("sections are one to four numbers of frequencies, and need pos")
             section = tuple(sections) + (0,) * (4 - n_axes)
+            if n_axes == 1 and section[0] != rot // 2:
+                raise DiffCacheError(f"the sections hold {section[0]} frequencies, not {rot // 2}")
         if pos is not None:
             want = shape[:-2] if sections is None else (*shape[:-2], n_axes)
             if pos.dtype is not _I32 or pos.shape != want or not pos.is_contiguous():

@@ -172,7 +172,7 @@ extern "C" int dc_paged_append_bf16(const dc_paged_append_args *x, void *stream)
         }
         if (i < 3) a.bound[i] = i + 1 < x->n_axes ? upto : x->hd;
     }
-    DC_REQUIRE(x->n_axes == 1 || upto == x->rot / 2, "%s: the sections hold %d frequencies, not %d", who, upto, x->rot / 2);
+    DC_REQUIRE((x->n_axes == 1 && upto == 0) || upto == x->rot / 2, "%s: the sections hold %d frequencies, not %d", who, upto, x->rot / 2);
     a.p = dc_pages_of(x->store, t);
     a.t = dc_new_of(t);
     a.k = (const uint16_t *)x->k_src, a.v = (const uint16_t *)x->v_src, a.q = (const uint16_t *)x->q_src, a.q_out = (uint16_t *)x->q_out;

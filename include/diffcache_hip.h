@@ -757,7 +757,8 @@ typedef struct dc_paged_tokens {
  *   interleaved  0: pair f is columns f and f + rot / 2; else columns 2 f and 2 f + 1
  *   pos      NULL (a token's position is its row), or n_axes int32 for every token on the device, contiguous
  *   n_axes, section  1, or up to 4: the first section[0] frequencies go by a token's first position, the next section[1] by its
- *            second, and so on (time, height and width of images and video); the sections' sum is rot / 2
+ *            second, and so on (time, height and width of images and video); the sections' sum is rot / 2 (with 1 axis section[0]
+ *            may be 0: all of them)
  * (x_a, x_b) becomes (x_a cos - x_b sin, x_b cos + x_a sin) in fp32, rounded once.  start is not changed.  Stands beside dc_append_kv_bf16
  * and the rotation of the reference's layers (base.py:121-125).
  */
