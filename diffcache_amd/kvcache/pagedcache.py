@@ -188,6 +188,7 @@ class PagedCache:
         self._give_back(sequence)
         self._lens[sequence] = 0
         self.lens[sequence:sequence + 1].zero_()
+        self._attn_out[sequence].zero_()        # (no step writes it until the sequence begins anew)
         self._set_live([0 if i == sequence else x for i, x in enumerate(self._live)])
         self._upload()
 
@@ -292,8 +293,9 @@ class PagedCache:
                          pos: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One layer of a decode step: write the token's k/v behind each sequence and attend to all of it (or to its sinks and
         window).  queries (bsz, 1, Hq*hd) or (bsz, Hq, hd); key/value_states (bsz, 1, Hkv, hd); ``pos`` (bsz) int32, or (bsz, axes).  Returns
-        (bsz, Hq, hd) bf16; ``lse`` (bsz, Hq) fp32 receives the log of the sum of exponentials.  Call it for every layer of a step; the
-        sequences grow by one after the last layer.  Those that are not live are left alone: their rows of ``out`` and ``lse`` stay what they were."""
+        (bsz, Hq, hd) bf16, ``out`` or a tensor of the cache's that the next call writes again; ``lse`` (bsz, Hq) fp32 receives the log of the sum of exponentials.  Call it for every layer of a step; the
+        sequences grow by one after the last layer.  Those that are not live are left alone: their rows of ``out`` and ``lse`` stay what they were (those of the
+        cache's own tensor are zeros)."""
         b, hq, h, hd = self.batch_size, self.num_q_heads, self.num_kv_heads, self.head_dim
         if out is None:
             out = self._attn_out

@@ -204,3 +204,13 @@ def test_a_refused_call_gives_back_the_pages_that_it_took(cache, monkeypatch, ca
     taken = [p for pages, old in zip(c._pages, before[0]) for p in pages if p not in old]
     assert taken and set(taken) <= set(free + sum(before[0], []))
     assert sorted(c._free + list({p for pages in c._pages for p in pages})) == list(range(c.num_pages))
+
+
+def test_nothing_of_a_freed_sequence_is_handed_out_again(cache):
+    """Without `out` a step returns the cache's own tensor: a sequence that is not live has zeros there, not its last outputs."""
+    c = cache()
+    prefill(c, 7)
+    c._attn_out.fill_(3)                                           # (what a step would leave)
+    c.free(1)
+    got = c.decode_attention(0, bf(3, 2, 64), bf(3, 1, 1, 64), bf(3, 1, 1, 64))
+    assert got is c._attn_out and (got[1] == 0).all() and (got[0] == 3).all() and (got[2] == 3).all()
