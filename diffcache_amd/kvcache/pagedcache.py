@@ -255,6 +255,9 @@ class PagedCache:
         hip.require(max(grown) <= self.max_length, "the cache is full (max_length)")
         live = self._with(at)
         need = self._reserve(grown) if max(at) > self._room or live != self._live else []
+        for i, (x, y) in enumerate(zip(live, self._live)):
+            if x > y:                               # (tokens that were taken back of all sequences may have gone off a freed one's too)
+                self.lens[i:i + 1].zero_()
         try:
             turned = self._append(layer_idx, k, v, self.lens, counts, q if self.rotates else None, q_out, pos)
             got = hip.paged_attn(q if turned is None else turned, self.k_pages[layer_idx], self.v_pages[layer_idx], self.table, self.lens,
@@ -304,7 +307,7 @@ class PagedCache:
 
     def advance_host_step(self, steps: int = 1) -> None:
         """After ``steps`` replays of a captured decode step: bring the host's mirror of the lengths up to the device's (no
-        synchronisation).  Negative: tokens taken back, which ``lens.sub_`` takes off the device's."""
+        synchronisation).  Negative: tokens taken back of the live sequences, which ``lens.sub_`` takes off the device's."""
         grown = [n + steps * x for n, x in zip(self._lens, self._live)]
         # (a step is captured for max_length rows: of one behind them in the last page a token would be written and never attended to)
         hip.require(min(grown) >= 0 and max(grown) <= self.max_length and all(n <= len(p) * self.page_size for n, p in zip(grown, self._pages)),

@@ -214,3 +214,19 @@ def test_nothing_of_a_freed_sequence_is_handed_out_again(cache):
     c.free(1)
     got = c.decode_attention(0, bf(3, 2, 64), bf(3, 1, 1, 64), bf(3, 1, 1, 64))
     assert got is c._attn_out and (got[1] == 0).all() and (got[0] == 3).all() and (got[2] == 3).all()
+
+
+def test_tokens_taken_back_of_all_sequences_leave_a_freed_one_empty(cache):
+    c = cache()
+    prefill(c, 7)
+    c.free(1)
+    decode(c)
+    c.lens.sub_(1)                                                 # (of the freed one too)
+    c.advance_host_step(-1)
+    assert c._lens == [7, 0, 7]
+    for layer in range(2):
+        c.extend_attention(layer, bf(3, 5, 2, 64), bf(3, 5, 1, 64), bf(3, 5, 1, 64), lens=[0, 5, 1])
+        assert cache.attended[-1]["start"] == [7, 0, 7]
+    assert c._lens == c.lens.tolist() == [7, 5, 8]
+    decode(c)
+    assert c._lens == c.lens.tolist() == [8, 6, 9]
