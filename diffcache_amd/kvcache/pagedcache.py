@@ -253,11 +253,12 @@ class PagedCache:
         capturing = self._capturing()
         grown = [n + c for n, c in zip(self._lens, at)]
         hip.require(max(grown) <= self.max_length, "the cache is full (max_length)")
-        live = self._with(at)
+        live = at if at is self._live else self._with(at)       # (a decode step has one token of each)
         need = self._reserve(grown) if max(at) > self._room or live != self._live else []
-        for i, (x, y) in enumerate(zip(live, self._live)):
-            if x > y:                               # (tokens that were taken back of all sequences may have gone off a freed one's too)
-                self.lens[i:i + 1].zero_()
+        if live != self._live:
+            for i, (x, y) in enumerate(zip(live, self._live)):
+                if x > y:   # (tokens that were taken back of all sequences may have gone off a freed one's too)
+                    self.lens[i:i + 1].zero_()
         try:
             turned = self._append(layer_idx, k, v, self.lens, counts, q if self.rotates else None, q_out, pos)
             got = hip.paged_attn(q if turned is None else turned, self.k_pages[layer_idx], self.v_pages[layer_idx], self.table, self.lens,
@@ -303,7 +304,7 @@ class PagedCache:
         if out is None:
             out = self._attn_out
         return self._attend(layer_idx, queries.reshape(b, hq, hd), key_states.reshape(b, h, hd), value_states.reshape(b, h, hd),
-                            list(self._live), self.live, out, lse, pos, self._workspace, self._q)
+                            self._live, self.live, out, lse, pos, self._workspace, self._q)
 
     def advance_host_step(self, steps: int = 1) -> None:
         """After ``steps`` replays of a captured decode step: bring the host's mirror of the lengths up to the device's (no
