@@ -785,8 +785,10 @@ int dc_paged_append_bf16(const dc_paged_append_args *args, void *stream);
  *   group    up to 16; scale: positive, up to 2.35e38 (times log2(e) it has to be finite)
  * A token that attends to no row has out 0 and lse -inf.  What a token does not attend to may hold anything, and leaves no trace.  Of what
  * it does attend to, a number of K that is not finite makes the head's outputs and lse NaN where a logit becomes NaN or +inf; an infinity in V
- * makes the outputs of its column that infinity (NaN where there are both, or where the row's weight is below fp32), a NaN makes them NaN.  Logits are fp32, before the scale too: one that falls below its range is -inf, a weight of 0; one above
- * it makes its head NaN.  Sums and statistics are fp32.
+ * makes the outputs of its column that infinity (NaN where there are both; that infinity or NaN where the row's weight is below fp32), a NaN
+ * makes them NaN.  Logits are fp32, before the scale and times log2(e) too: one that falls below its range is -inf, a weight of 0; one above
+ * it makes its head NaN.  Sums and statistics are fp32.  A weight counts in the product with V as the sum of two bf16 numbers with max_new * group
+ * up to 16 (2^-16 of it lost at most), and is rounded to one with more (2^-8 at most; the sum of the weights is that before the rounding).
  * The workspace (dc_paged_attn_workspace_bytes for the same sizes, n_tokens 0 without cu, 256-byte aligned; 0: none; with max_new *
  * group up to 16, enough for more sequences, rows or tokens is enough for fewer) holds nothing between calls; calls that may overlap need one each.  Replaces
  * flash_attn_with_kvcache (base.py:134-142) over such a cache.

@@ -28,3 +28,25 @@ def test_the_largest_scale(hd, new):
     assert torch.equal(out, want[0]) and torch.equal(lse, want[1]) and out.isfinite().all() and lse.isfinite().all()
     with pytest.raises(hip.DiffCacheError, match="scale"):
         hip.paged_attn(q, k, v, table, i32([n]), scale=2.4e38)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf")])
+@pytest.mark.parametrize("low", [3, 100, 348, 399])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", NEW)
+def test_an_infinity_whose_weight_is_below_fp32(new, hd, low, bad):
+    """An infinity in V of a row whose weight, exp(-1600), fp32 does not hold: its column is that infinity or NaN (which one goes by the steps' order),
+    never a number, and the other columns know nothing of it."""
+    from diffcache_amd import _hip as hip
+    n, page = 400, 16
+    k, v, table, g = build(1, 1, hd, page, [n + new], 33)
+    k[..., 1:], k[..., 0] = 0, 8
+    k[int(table[0, low // page]), 0, low % page, 0] = -8
+    q = torch.zeros((1, new, 2, hd), dtype=torch.bfloat16, device=DEV)
+    q[..., 0] = 100
+    clean = hip.paged_attn(q, k, v, table, i32([n]), scale=1.0, want_lse=True)
+    v[int(table[0, low // page]), 0, low % page, 7] = bad
+    out, lse = hip.paged_attn(q, k, v, table, i32([n]), scale=1.0, want_lse=True)
+    assert ((out[..., 7] == bad) | out[..., 7].isnan()).all()
+    rest = [c for c in range(hd) if c != 7]
+    assert torch.equal(out[..., rest], clean[0][..., rest]) and torch.equal(lse, clean[1]) and out[..., rest].isfinite().all()
